@@ -358,6 +358,67 @@ MR_API int mr_rglru_step(const void* a, const void* x, int dtype, int64_t batch,
 MR_API int mr_rotlru_step(const void* a, const void* cs, const void* sn, const void* x, int dtype,
                           int64_t batch, int64_t Dp, float* state, float* y, void* stream);
 
+/* ------------------------------------------------------- packed batches ---
+ * No counterpart in the reference, whose scans take one length per batch.
+ * cu_seqlens [S+1] int32 (device, nondecreasing, from 0 to at most T): sequence
+ * s holds the rows cu_seqlens[s] .. cu_seqlens[s+1]-1 of the packed tensors;
+ * lengths of zero and one are fine. Rows outside every sequence come out as
+ * zeros, in outputs and gradients. T may be 0.
+ *
+ * RG-LRU recurrence h_t = a_t h_{t-1} + x_t per sequence: a, x [T,D] in `dtype`
+ * (any T, D >= 1; element-aligned pointers), y [T,D] f32, h0 [S,D] f32 or NULL
+ * (zero), final_state [S,D] f32 or NULL (h0 for an empty sequence). ckpt
+ * [ceil(T / mr_rglru_packed_chunk()), D] f32 receives what the backward needs
+ * (NULL when none follows). grad_final [S,D] and grad_h0 [S,D] may be NULL. */
+MR_API int64_t mr_rglru_packed_chunk(void);
+MR_API size_t mr_rglru_packed_workspace_bytes(int64_t T, int64_t D);
+MR_API int mr_rglru_packed_fwd(const void* a, const void* x, const int32_t* cu_seqlens, int64_t S, int dtype,
+                               int64_t T, int64_t D, const float* h0, float* y, float* ckpt, float* final_state,
+                               void* workspace, size_t workspace_bytes, void* stream);
+MR_API int mr_rglru_packed_bwd(const float* grad_y, const float* grad_final, const float* ckpt, const void* a,
+                               const void* x, const int32_t* cu_seqlens, int64_t S, int dtype, int64_t T, int64_t D,
+                               const float* h0, void* grad_a, void* grad_x, float* grad_h0, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* Sliding-window attention with sinks (causal): query i of a sequence sees key
+ * j when j <= i and (i - j < window or j < sinks), both counted from the
+ * sequence's start; y_i = sum_j softmax_j(scale q_i.k_j) v_j. q, y [T,Hq,Dh],
+ * k, v [T,Hkv,Dh], Hq a multiple of Hkv (consecutive query heads share a
+ * key/value head), Dh 32, 64, 96 or 128, sinks 0..64. *_ts, *_hs: token and
+ * head strides in elements (multiples of 16 bytes; the last axis is dense).
+ * cu_seqlens NULL: S sequences of L tokens (T = S L). y and the gradients are
+ * dense and in `dtype`; lse [Hq,T] f32 (NULL when no backward follows) holds
+ * what the backward needs. */
+MR_API int mr_window_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ts, int64_t q_hs, int64_t k_ts,
+                              int64_t k_hs, int64_t v_ts, int64_t v_hs, const int32_t* cu_seqlens, int64_t S,
+                              int64_t L, int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t window,
+                              int64_t sinks, float scale, void* y, float* lse, void* stream);
+MR_API size_t mr_window_attn_bwd_workspace_bytes(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t Dh,
+                                                 int64_t sinks);
+MR_API int mr_window_attn_bwd(const void* grad_y, const void* y, const float* lse, const void* q, const void* k,
+                              const void* v, int64_t q_ts, int64_t q_hs, int64_t k_ts, int64_t k_hs, int64_t v_ts,
+                              int64_t v_hs, const int32_t* cu_seqlens, int64_t S, int64_t L, int dtype, int64_t T,
+                              int64_t Hq, int64_t Hkv, int64_t Dh, int64_t window, int64_t sinks, float scale,
+                              void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* The caches a decode loop starts from: cache_k, cache_v [S,slots,Hkv,Dh]
+ * (slots = sinks + window) receive, for every sequence, token t at slot t
+ * (t < sinks) or sinks + (t - sinks) % window, the newest token of each slot;
+ * slots that no token reached are zeroed. */
+MR_API int mr_window_cache(const void* k, const void* v, int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs,
+                           const int32_t* cu_seqlens, int64_t S, int64_t L, int dtype, int64_t T, int64_t Hkv,
+                           int64_t Dh, int64_t slots, int64_t sinks, void* cache_k, void* cache_v, void* stream);
+
+/* One decode step: the token at position pos[b] (from 0; int64 or int32 by
+ * pos_is_int64) of every batch row is written to its slot of the caches and
+ * attends to every visible token. q, y [B,Hq,Dh], k, v [B,Hkv,Dh] dense in
+ * `dtype`, the caches too. Rows with pos[b] < 0 are free: their caches stay as
+ * they are and their y is zero. */
+MR_API int mr_window_step(const void* q, const void* k, const void* v, void* cache_k, void* cache_v, const void* pos,
+                          int pos_is_int64, int dtype, int64_t batch, int64_t Hq, int64_t Hkv, int64_t Dh,
+                          int64_t slots, int64_t sinks, float scale, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

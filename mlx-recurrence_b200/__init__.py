@@ -15,6 +15,10 @@ Beyond the reference: an optional initial state ``h0=`` on every scan
 ``gated_deltanet_scan``, the recurrence the reference carries as a design
 (``docs/DESIGN_gated_deltanet.md``).
 
+For packed batches (sequences of different lengths back to back) and hybrid
+models: ``rglru_scan_packed`` and sliding-window attention with sinks
+(``window_attention``, ``window_attention_packed``, ``window_attention_step``).
+
 Import with ``importlib.import_module("mlx-recurrence_b200")`` (the directory
 name carries a hyphen); after that the package is also registered as
 ``mlx_recurrence_b200``.
@@ -26,11 +30,14 @@ from ._chassis import DEFAULT_SEG, check_segment_shape, get_or_build_kernel, par
 from .gdn import (gated_deltanet_scan, gated_deltanet_scan_reference, gated_deltanet_scan_with_state,
                   gated_deltanet_step)
 from .gla import gla_scan, gla_scan_reference, gla_scan_with_state, gla_step
-from .rglru import (rglru_scan, rglru_scan_gated, rglru_scan_gated_with_state, rglru_scan_reference,
+from .rglru import (rglru_scan, rglru_scan_gated, rglru_scan_gated_with_state, rglru_scan_packed,
+                    rglru_scan_packed_reference, rglru_scan_packed_with_state, rglru_scan_reference,
                     rglru_scan_with_state, rglru_step)
 from .rotlru import (rotlru_scan, rotlru_scan_angle, rotlru_scan_angle_with_state, rotlru_scan_reference,
                      rotlru_scan_with_state, rotlru_step)
 from .ssd import ssd_scan, ssd_scan_reference, ssd_scan_with_state, ssd_step
+from .window import (window_attention, window_attention_packed, window_attention_packed_with_state,
+                     window_attention_reference, window_attention_step, window_attention_with_state)
 
 __all__ = [
     "ssd_scan",
@@ -60,6 +67,17 @@ __all__ = [
     "rglru_step",
     "rotlru_step",
     "gated_deltanet_step",
+    # packed batches: sequences of different lengths back to back (not in the reference)
+    "rglru_scan_packed",
+    "rglru_scan_packed_with_state",
+    "rglru_scan_packed_reference",
+    # sliding-window attention with sinks (not in the reference)
+    "window_attention",
+    "window_attention_with_state",
+    "window_attention_packed",
+    "window_attention_packed_with_state",
+    "window_attention_reference",
+    "window_attention_step",
     "DEFAULT_SEG",
     "get_or_build_kernel",
     "check_segment_shape",

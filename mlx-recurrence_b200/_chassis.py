@@ -93,6 +93,18 @@ def step_state(state, shape, device):
     return state
 
 
+def prep_cu(cu_seqlens, device):
+    """Sequence borders [S + 1] as int32 on ``device``. Their values stay on the
+    device (checking them would synchronise)."""
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+        raise ValueError("cu_seqlens must be a 1-D tensor of S + 1 sequence borders")
+    if cu_seqlens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"cu_seqlens must be int32 or int64, got {cu_seqlens.dtype}")
+    if cu_seqlens.device != device:
+        raise ValueError(f"cu_seqlens must be on {device}, got {cu_seqlens.device}")
+    return cu_seqlens.to(torch.int32).contiguous()
+
+
 def grad_out(g, shape, device):
     """fp32 contiguous cotangent (zeros when autograd passes None)."""
     if g is None:

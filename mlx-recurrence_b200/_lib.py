@@ -96,6 +96,20 @@ SIGNATURES = {
     "mr_gla_step": (_int, [_p, _p, _p, _p, _int, _i64, _i64, _i64, _p, _p, _p]),
     "mr_rglru_step": (_int, [_p, _p, _int, _i64, _i64, _p, _p, _p]),
     "mr_rotlru_step": (_int, [_p, _p, _p, _p, _int, _i64, _i64, _p, _p, _p]),
+    # packed batches: the RG-LRU scan and sliding-window attention
+    "mr_rglru_packed_chunk": (_i64, []),
+    "mr_rglru_packed_workspace_bytes": (_sz, [_i64, _i64]),
+    "mr_rglru_packed_fwd": (_int, [_p, _p, _p, _i64, _int, _i64, _i64, _p, _p, _p, _p, _p, _sz, _p]),
+    "mr_rglru_packed_bwd": (_int, [_p, _p, _p, _p, _p, _p, _i64, _int, _i64, _i64, _p, _p, _p, _p, _p, _sz, _p]),
+    "mr_window_attn_fwd": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64,
+                                  _i64, _i64, _i64, _i64, ctypes.c_float, _p, _p, _p]),
+    "mr_window_attn_bwd_workspace_bytes": (_sz, [_int, _i64, _i64, _i64, _i64, _i64]),
+    "mr_window_attn_bwd": (_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _int,
+                                  _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _p, _p, _p, _p, _sz, _p]),
+    "mr_window_cache": (_int, [_p, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, _i64, _i64, _p,
+                               _p, _p]),
+    "mr_window_step": (_int, [_p, _p, _p, _p, _p, _p, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float,
+                              _p, _p]),
 }
 
 _lib = None
@@ -148,6 +162,15 @@ def ptr(t):
 
 def stream_of(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def call_on(dev, name, *args):
+    """:func:`call` on ``dev``, with its current stream as the last argument."""
+    if torch.cuda.current_device() == dev.index:
+        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
 
 
 def require_cuda(*tensors):

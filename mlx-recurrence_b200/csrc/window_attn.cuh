@@ -1,0 +1,209 @@
+// Sliding-window attention with sinks: arguments, masks and the exact
+// row-by-row forms shared by the attention kernels.
+//
+// A batch is T tokens in a row, [T, H, Dh]; sequences are the ranges
+// cu[s] .. cu[s+1]-1, or (cu == NULL) consecutive runs of L tokens. Query i
+// sees key j of its own sequence when
+//   j <= i  and  (i - j < window  or  j - start < sinks).
+// Tokens outside every sequence are nobody's key; their rows are zero.
+#pragma once
+
+#include "common.cuh"
+
+namespace mr {
+
+struct AttnArgs {
+  const void *q, *k, *v;            // [T, H, Dh], rows dense, strides in elements
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
+  const int* cu;                    // [S + 1] or NULL
+  int S, L;                         // L: sequence length when cu is NULL
+  int T, Hq, Hkv, Dh;
+  int window, sinks;                // window <= T
+  float scale;                      // > 0
+  void* y;                          // [T, Hq, Dh] dense
+  float* lse;                       // [Hq, T]: log2 of the row's sum of exponentials; NULL when not wanted
+  // backward
+  const void* gy;                   // [T, Hq, Dh] dense
+  float* delta;                     // [Hq, T]: sum_d gy y
+  void *gq, *gk, *gv;               // [T, Hq, Dh], [T, Hkv, Dh] dense
+};
+
+struct SeqRange {
+  int start, end;  // end <= start: no sequence
+};
+
+// The sequence that holds token t. Entries of cu are only compared and clamped
+// to [0, T], so a malformed cu cannot lead an access out of range.
+__device__ __forceinline__ SeqRange seq_of(const AttnArgs& A, int t) {
+  if (t < 0 || t >= A.T) return {0, 0};
+  if (A.cu == nullptr) {
+    const int s = t / A.L * A.L;
+    return {s, min(s + A.L, A.T)};
+  }
+  int lo = 0, hi = A.S;  // the last s with cu[s] <= t
+  while (lo < hi) {
+    const int m = (lo + hi + 1) >> 1;
+    if (A.cu[m] <= t) lo = m; else hi = m - 1;
+  }
+  const int s = A.cu[lo];
+  if (lo >= A.S || s > t) return {0, 0};
+  return {max(s, 0), min(A.cu[lo + 1], A.T)};
+}
+
+__device__ __forceinline__ int first_token(const AttnArgs& A) { return A.cu ? min(max(A.cu[0], 0), A.T) : 0; }
+__device__ __forceinline__ int end_token(const AttnArgs& A) { return A.cu ? min(max(A.cu[A.S], 0), A.T) : A.T; }
+
+// What a query sees: keys [lo, i] and sinks [start, sink_end).
+struct RowMask {
+  int i, lo, start, sink_end;
+  __device__ bool sees(int j) const { return (j >= lo && j <= i) || (j >= start && j < sink_end && j <= i); }
+};
+__device__ __forceinline__ RowMask row_mask(const AttnArgs& A, int i) {
+  const SeqRange s = seq_of(A, i);
+  if (s.end <= i) return {-1, INT32_MAX, INT32_MAX, -1};
+  return {i, max(s.start, i - A.window + 1), s.start, s.start + min(A.sinks, A.T)};
+}
+
+// Keys that the queries [q0, q1) may see: the band [kmin, kend) and the sinks
+// before it, [s0, send), which belong to the first query's sequence (any later
+// sequence starts inside the band). Nothing when kend <= kmin.
+struct KeyRange {
+  int kmin, kend, s0, send;
+};
+__device__ __forceinline__ KeyRange keys_of(const AttnArgs& A, int q0, int q1) {
+  const int f = max(q0, first_token(A)), e = min(q1, end_token(A));
+  if (f >= e) return {0, 0, 0, 0};
+  const SeqRange s = seq_of(A, f);
+  const int kmin = max(min(s.start, f), f - A.window + 1);
+  return {kmin, e, s.start, min(s.start + min(A.sinks, A.T), kmin)};
+}
+
+// The first query that no longer sees key j (0: j is nobody's key); queries
+// j .. hi-1 see it.
+__device__ __forceinline__ int key_limit(const AttnArgs& A, int j) {
+  const SeqRange s = seq_of(A, j);
+  if (s.end <= j) return 0;
+  return j - s.start < A.sinks ? s.end : min(s.end, j + A.window);
+}
+
+// Queries [qbeg, qend) that may see the keys [k0, k1).
+struct QueryRange {
+  int qbeg, qend;
+};
+__device__ __forceinline__ QueryRange queries_of(const AttnArgs& A, int k0, int k1) {
+  const int f = max(k0, first_token(A)), e = min(k1, end_token(A));
+  if (f >= e) return {0, 0};
+  const SeqRange s = seq_of(A, e - 1);
+  const bool sink = max(f, s.start) - s.start < A.sinks;
+  return {f, max(sink ? s.end : min(s.end, e - 1 + A.window), e)};
+}
+
+// ---- exact rows --------------------------------------------------------------
+// The tiled kernels multiply masked terms by zero, which an infinity or a NaN
+// that a row must not see (another sequence's, a later token's) turns into a
+// NaN. A row whose results are not finite is therefore computed again here, one
+// warp per row, from its visible keys (queries) alone: whatever non-finite value
+// then remains is the row's own. Slow (a shuffle reduction per pair), and only
+// ever reached by inputs that hold infinities or NaN.
+
+constexpr float kAttnLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float attn_warp_sum(float v) {
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
+  return v;
+}
+
+struct RowVec {
+  float v[4];  // elements lane + 32 n of one head's row, Dh <= 128
+};
+template <typename T> __device__ __forceinline__ RowVec row_load(const T* p, int Dh, int lane) {
+  RowVec r;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) r.v[n] = 32 * n < Dh ? to_f(p[lane + 32 * n]) : 0.f;
+  return r;
+}
+template <typename T> __device__ __forceinline__ void row_store(T* p, const RowVec& r, float f, int Dh, int lane) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+    if (32 * n < Dh) p[lane + 32 * n] = from_f<T>(r.v[n] * f);
+}
+__device__ __forceinline__ float row_dot(const RowVec& a, const RowVec& b, int Dh) {
+  float s = 0.f;
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+    if (32 * n < Dh) s = fmaf(a.v[n], b.v[n], s);
+  return attn_warp_sum(s);
+}
+__device__ __forceinline__ void row_axpy(RowVec& a, float f, const RowVec& b) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n) a.v[n] = fmaf(f, b.v[n], a.v[n]);
+}
+
+template <typename T> __device__ __noinline__ void exact_fwd_row(const AttnArgs& A, int h, int i) {
+  const int lane = threadIdx.x & 31, hk = h / (A.Hq / A.Hkv);
+  const RowMask w = row_mask(A, i);
+  if (w.i < 0) return;
+  const T* k = (const T*)A.k + hk * A.k_hs;
+  const T* v = (const T*)A.v + hk * A.v_hs;
+  const RowVec q = row_load((const T*)A.q + i * A.q_ts + h * A.q_hs, A.Dh, lane);
+  RowVec o = {};
+  float m = -INFINITY, l = 0.f;
+  int j = w.start < min(w.sink_end, w.lo) ? w.start : w.lo;
+  while (j <= i) {
+    const float s = row_dot(q, row_load(k + j * A.k_ts, A.Dh, lane), A.Dh) * (A.scale * kAttnLog2e);
+    const float mx = fmaxf(m, s), base = mx == -INFINITY ? 0.f : mx, keep = exp2f(m - base), e = exp2f(s - base);
+    m = mx;
+    l = l * keep + e;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) o.v[n] *= keep;
+    row_axpy(o, e, row_load(v + j * A.v_ts, A.Dh, lane));
+    ++j;
+    if (j >= w.sink_end && j < w.lo) j = w.lo;
+  }
+  row_store((T*)A.y + ((int64_t)i * A.Hq + h) * A.Dh, o, 1.f / l, A.Dh, lane);
+  if (A.lse != nullptr && lane == 0) A.lse[(int64_t)h * A.T + i] = m + log2f(l);
+}
+
+template <typename T> __device__ __noinline__ void exact_gq_row(const AttnArgs& A, int h, int i) {
+  const int lane = threadIdx.x & 31, hk = h / (A.Hq / A.Hkv);
+  const RowMask w = row_mask(A, i);
+  if (w.i < 0) return;
+  const T* k = (const T*)A.k + hk * A.k_hs;
+  const T* v = (const T*)A.v + hk * A.v_hs;
+  const int64_t at = ((int64_t)i * A.Hq + h) * A.Dh;
+  const RowVec q = row_load((const T*)A.q + i * A.q_ts + h * A.q_hs, A.Dh, lane);
+  const RowVec g = row_load((const T*)A.gy + at, A.Dh, lane);
+  const float lse = A.lse[(int64_t)h * A.T + i], delta = A.delta[(int64_t)h * A.T + i];
+  RowVec o = {};
+  int j = w.start < min(w.sink_end, w.lo) ? w.start : w.lo;
+  while (j <= i) {
+    const RowVec kj = row_load(k + j * A.k_ts, A.Dh, lane);
+    const float p = exp2f(row_dot(q, kj, A.Dh) * (A.scale * kAttnLog2e) - lse);
+    row_axpy(o, p * (row_dot(g, row_load(v + j * A.v_ts, A.Dh, lane), A.Dh) - delta), kj);
+    ++j;
+    if (j >= w.sink_end && j < w.lo) j = w.lo;
+  }
+  row_store((T*)A.gq + at, o, A.scale, A.Dh, lane);
+}
+
+template <typename T> __device__ __noinline__ void exact_gkv_row(const AttnArgs& A, int hk, int j) {
+  const int lane = threadIdx.x & 31, G = A.Hq / A.Hkv, end = key_limit(A, j);
+  if (end == 0) return;
+  const RowVec k = row_load((const T*)A.k + j * A.k_ts + hk * A.k_hs, A.Dh, lane);
+  const RowVec v = row_load((const T*)A.v + j * A.v_ts + hk * A.v_hs, A.Dh, lane);
+  RowVec gk = {}, gv = {};
+  for (int h = hk * G; h < (hk + 1) * G; ++h)
+    for (int i = j; i < end; ++i) {
+      const RowVec q = row_load((const T*)A.q + i * A.q_ts + h * A.q_hs, A.Dh, lane);
+      const RowVec g = row_load((const T*)A.gy + ((int64_t)i * A.Hq + h) * A.Dh, A.Dh, lane);
+      const float p = exp2f(row_dot(q, k, A.Dh) * (A.scale * kAttnLog2e) - A.lse[(int64_t)h * A.T + i]);
+      row_axpy(gv, p, g);
+      row_axpy(gk, p * (row_dot(g, v, A.Dh) - A.delta[(int64_t)h * A.T + i]), q);
+    }
+  const int64_t at = ((int64_t)j * A.Hkv + hk) * A.Dh;
+  row_store((T*)A.gk + at, gk, A.scale, A.Dh, lane);
+  row_store((T*)A.gv + at, gv, 1.f, A.Dh, lane);
+}
+
+}  // namespace mr

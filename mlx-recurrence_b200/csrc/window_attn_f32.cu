@@ -1,0 +1,341 @@
+// Sliding-window attention with sinks on the CUDA cores, in float32: forward,
+// and the backward as one pass over key tiles per query tile (grad_q) and one
+// pass over query tiles per key tile (grad_k, grad_v; a shared key/value head
+// sums its query heads in a fixed order, so results do not vary).
+//
+//   s_ij = scale q_i.k_j,  p = softmax over the visible j,  y_i = sum_j p_ij v_j
+//   ds_ij = p_ij (gy_i.v_j - delta_i),  delta_i = gy_i.y_i
+//   grad_q_i = scale sum_j ds_ij k_j,  grad_k_j = scale sum_i ds_ij q_i,  grad_v_j = sum_i p_ij gy_i
+//
+// Tiles are 64 x 64; 128 threads own 8 x 4 results of a tile and 8 rows x Dh/16
+// columns of the products that follow. Operands lie transposed ([d][64 + 4]) in
+// shared memory, so a thread's rows and columns come as 16-byte reads.
+#include "window_attn.cuh"
+
+namespace mr {
+
+constexpr int kBT = 64;        // tile edge
+constexpr int kPitch = kBT + 4;
+constexpr int kThreads = 128;
+
+// rows r0 .. r0+63 of one head as [d][kPitch] float32, zeros outside [lo, hi)
+template <typename T, int DH>
+__device__ __forceinline__ void load_t(float* dst, const T* src, int64_t ts, int r0, int lo, int hi) {
+  for (int e = threadIdx.x; e < kBT * DH; e += kThreads) {
+    const int r = e / DH, d = e % DH, t = r0 + r;
+    dst[d * kPitch + r] = (t >= lo && t < hi) ? to_f(src[t * ts + d]) : 0.f;
+  }
+}
+
+// acc[8][4] = sum_d R[d][8 rows of ty] C[d][4 columns of tx]
+template <int DH>
+__device__ __forceinline__ void tile_dot(float (&acc)[8][4], const float* R, const float* C, int ty, int tx) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+#pragma unroll 4
+  for (int d = 0; d < DH; ++d) {
+    float r[8], c[4];
+    *reinterpret_cast<float4*>(r) = *reinterpret_cast<const float4*>(R + d * kPitch + ty * 8);
+    *reinterpret_cast<float4*>(r + 4) = *reinterpret_cast<const float4*>(R + d * kPitch + ty * 8 + 4);
+    *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(C + d * kPitch + tx * 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(r[i], c[j], acc[i][j]);
+  }
+}
+
+// out[8][DH/16] += sum_n P[n][8 rows of ty] C[tx + 16 m][n]
+template <int DH>
+__device__ __forceinline__ void tile_acc(float (&out)[8][DH / 16], const float* P, const float* C, int ty, int tx) {
+#pragma unroll 2
+  for (int n = 0; n < kBT; ++n) {
+    float r[8];
+    *reinterpret_cast<float4*>(r) = *reinterpret_cast<const float4*>(P + n * kPitch + ty * 8);
+    *reinterpret_cast<float4*>(r + 4) = *reinterpret_cast<const float4*>(P + n * kPitch + ty * 8 + 4);
+#pragma unroll
+    for (int m = 0; m < DH / 16; ++m) {
+      const float c = C[(tx + 16 * m) * kPitch + n];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out[i][m] = fmaf(r[i], c, out[i][m]);
+    }
+  }
+}
+
+// P[column][row] <- a thread's 8 x 4 block
+__device__ __forceinline__ void put_block(float* P, const float (&v)[8][4], int ty, int tx) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float* p = P + (tx * 4 + j) * kPitch + ty * 8;
+    *reinterpret_cast<float4*>(p) = make_float4(v[0][j], v[1][j], v[2][j], v[3][j]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4][j], v[5][j], v[6][j], v[7][j]);
+  }
+}
+
+template <typename T, int DH>
+__global__ void __launch_bounds__(kThreads) attn_fwd_f32(const __grid_constant__ AttnArgs A) {
+  extern __shared__ float sm[];
+  float *sQ = sm, *sK = sQ + DH * kPitch, *sV = sK + DH * kPitch, *sP = sV + DH * kPitch;
+  __shared__ RowMask rows[kBT];
+  __shared__ int again[kBT];
+  const int q0 = blockIdx.x * kBT, h = blockIdx.y, hk = h / (A.Hq / A.Hkv);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const T* q = (const T*)A.q + h * A.q_hs;
+  const T* k = (const T*)A.k + hk * A.k_hs;
+  const T* v = (const T*)A.v + hk * A.v_hs;
+  const KeyRange R = keys_of(A, q0, q0 + kBT);
+  const int first = first_token(A), last = end_token(A);
+  if (threadIdx.x < kBT) rows[threadIdx.x] = row_mask(A, q0 + threadIdx.x), again[threadIdx.x] = 0;
+  load_t<T, DH>(sQ, q, A.q_ts, q0, first, last);
+  const float c = A.scale * kAttnLog2e;
+  float m[8], l[8], o[8][DH / 16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    m[i] = -INFINITY, l[i] = 0.f;
+#pragma unroll
+    for (int n = 0; n < DH / 16; ++n) o[i][n] = 0.f;
+  }
+  const int nsink = R.send > R.s0 ? (R.send - R.s0 + kBT - 1) / kBT : 0;
+  const int nband = R.kend > R.kmin ? (R.kend - R.kmin + kBT - 1) / kBT : 0;
+  for (int it = 0; it < nsink + nband; ++it) {
+    const int k0 = it < nsink ? R.s0 + it * kBT : R.kmin + (it - nsink) * kBT;
+    const int k1 = min(k0 + kBT, it < nsink ? R.send : R.kend);
+    __syncthreads();
+    load_t<T, DH>(sK, k, A.k_ts, k0, first, k1);
+    load_t<T, DH>(sV, v, A.v_ts, k0, first, k1);
+    __syncthreads();
+    float s[8][4];
+    tile_dot<DH>(s, sQ, sK, ty, tx);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const RowMask w = rows[ty * 8 + i];
+      float mx = m[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = k0 + tx * 4 + j;
+        s[i][j] = key < k1 && w.sees(key) ? s[i][j] * c : -INFINITY;
+        mx = fmaxf(mx, s[i][j]);
+      }
+#pragma unroll
+      for (int x = 8; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x, 16));
+      const float base = mx == -INFINITY ? 0.f : mx;  // nothing visible so far: every term is exp2(-inf)
+      const float keep = exp2f(m[i] - base);
+      m[i] = mx;
+      l[i] *= keep;
+#pragma unroll
+      for (int n = 0; n < DH / 16; ++n) o[i][n] *= keep;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = exp2f(s[i][j] - base);
+        l[i] += s[i][j];
+      }
+    }
+    put_block(sP, s, ty, tx);
+    __syncthreads();
+    tile_acc<DH>(o, sP, sV, ty, tx);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x, 16);
+    const int t = q0 + ty * 8 + i;
+    if (t >= A.T) continue;
+    const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
+    T* y = (T*)A.y + ((int64_t)t * A.Hq + h) * A.Dh;
+    float odd = 0.f;  // NaN as soon as one element is not finite
+#pragma unroll
+    for (int n = 0; n < DH / 16; ++n) {
+      y[tx + 16 * n] = from_f<T>(o[i][n] * inv);
+      odd = fmaf(o[i][n], 0.f, odd);
+    }
+    if (A.lse != nullptr && tx == 0) A.lse[(int64_t)h * A.T + t] = l[i] == 0.f ? INFINITY : m[i] + log2f(l[i]);
+    if (odd != 0.f) again[ty * 8 + i] = 1;
+  }
+  __syncthreads();
+  for (int r = threadIdx.x >> 5; r < kBT; r += kThreads / 32)
+    if (again[r]) exact_fwd_row<T>(A, h, q0 + r);
+}
+
+// delta[h][t] = sum_d gy y: one warp per row
+template <typename T>
+__global__ void __launch_bounds__(256) attn_delta(const __grid_constant__ AttnArgs A) {
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= (int64_t)A.T * A.Hq) return;
+  const T* g = (const T*)A.gy + row * A.Dh;
+  const T* y = (const T*)A.y + row * A.Dh;
+  float s = 0.f;
+  for (int d = lane; d < A.Dh; d += 32) s = fmaf(to_f(g[d]), to_f(y[d]), s);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+  if (lane == 0) A.delta[(row % A.Hq) * A.T + row / A.Hq] = s;
+}
+
+// KV = false: rows are queries, columns keys, out1 = grad_q.
+// KV = true: rows are keys, columns queries, out1 = grad_k, out2 = grad_v.
+template <typename T, int DH, bool KV>
+__global__ void __launch_bounds__(kThreads) attn_bwd_f32(const __grid_constant__ AttnArgs A) {
+  extern __shared__ float sm[];
+  float *sR1 = sm, *sR2 = sR1 + DH * kPitch, *sC1 = sR2 + DH * kPitch, *sC2 = sC1 + DH * kPitch, *sP = sC2 + DH * kPitch;
+  __shared__ RowMask rows[kBT];
+  __shared__ int limit[kBT], again[kBT];
+  __shared__ float lse[kBT], delta[kBT];
+  const int r0 = blockIdx.x * kBT, G = A.Hq / A.Hkv;
+  const int hk = KV ? blockIdx.y : blockIdx.y / G;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int first = first_token(A), last = end_token(A);
+  const T* k = (const T*)A.k + hk * A.k_hs;
+  const T* v = (const T*)A.v + hk * A.v_hs;
+  const int64_t gts = (int64_t)A.Hq * A.Dh;
+  const float c = A.scale * kAttnLog2e;
+  float o1[8][DH / 16], o2[KV ? 8 : 1][DH / 16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int n = 0; n < DH / 16; ++n) o1[i][n] = o2[KV ? i : 0][n] = 0.f;
+
+  const KeyRange R = keys_of(A, r0, r0 + kBT);
+  const QueryRange Q = queries_of(A, r0, r0 + kBT);
+  const int nsink = !KV && R.send > R.s0 ? (R.send - R.s0 + kBT - 1) / kBT : 0;
+  const int nband = KV ? (Q.qend > Q.qbeg ? (Q.qend - Q.qbeg + kBT - 1) / kBT : 0)
+                       : (R.kend > R.kmin ? (R.kend - R.kmin + kBT - 1) / kBT : 0);
+  if (threadIdx.x < kBT) {
+    const int t = r0 + threadIdx.x;
+    again[threadIdx.x] = 0;
+    if (KV) {
+      limit[threadIdx.x] = key_limit(A, t);
+    } else {
+      rows[threadIdx.x] = row_mask(A, t);
+      lse[threadIdx.x] = t < A.T ? A.lse[(int64_t)blockIdx.y * A.T + t] : INFINITY;
+      delta[threadIdx.x] = t < A.T ? A.delta[(int64_t)blockIdx.y * A.T + t] : 0.f;
+    }
+  }
+  if (KV) {
+    load_t<T, DH>(sR1, k, A.k_ts, r0, first, last);
+    load_t<T, DH>(sR2, v, A.v_ts, r0, first, last);
+  } else {
+    load_t<T, DH>(sR1, (const T*)A.q + blockIdx.y * A.q_hs, A.q_ts, r0, first, last);
+    load_t<T, DH>(sR2, (const T*)A.gy + (int64_t)blockIdx.y * A.Dh, gts, r0, first, last);
+  }
+  for (int it = 0; it < (KV ? G : 1) * (nsink + nband); ++it) {
+    const int h = KV ? hk * G + it / nband : blockIdx.y;
+    const int n = KV ? it % nband : it;
+    const int c0 = KV ? Q.qbeg + n * kBT : n < nsink ? R.s0 + n * kBT : R.kmin + (n - nsink) * kBT;
+    const int c1 = min(c0 + kBT, KV ? Q.qend : n < nsink ? R.send : R.kend);
+    __syncthreads();
+    if (KV) {
+      load_t<T, DH>(sC1, (const T*)A.q + h * A.q_hs, A.q_ts, c0, first, c1);
+      load_t<T, DH>(sC2, (const T*)A.gy + (int64_t)h * A.Dh, gts, c0, first, c1);
+      if (threadIdx.x < kBT) {
+        const int t = c0 + threadIdx.x;
+        lse[threadIdx.x] = t < c1 ? A.lse[(int64_t)h * A.T + t] : INFINITY;
+        delta[threadIdx.x] = t < c1 ? A.delta[(int64_t)h * A.T + t] : 0.f;
+      }
+    } else {
+      load_t<T, DH>(sC1, k, A.k_ts, c0, first, c1);
+      load_t<T, DH>(sC2, v, A.v_ts, c0, first, c1);
+    }
+    __syncthreads();
+    float s[8][4], dp[8][4];
+    tile_dot<DH>(s, sR1, sC1, ty, tx);
+    tile_dot<DH>(dp, sR2, sC2, ty, tx);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = ty * 8 + i, col = tx * 4 + j;
+        const bool see = c0 + col < c1 && (KV ? (c0 + col >= r0 + r && c0 + col < limit[r]) : rows[r].sees(c0 + col));
+        const int qi = KV ? col : r;
+        const float p = see ? exp2f(s[i][j] * c - lse[qi]) : 0.f;
+        dp[i][j] = see ? p * (dp[i][j] - delta[qi]) : 0.f;
+        s[i][j] = p;
+      }
+    if (KV) {
+      put_block(sP, s, ty, tx);
+      __syncthreads();
+      tile_acc<DH>(reinterpret_cast<float(&)[8][DH / 16]>(o2), sP, sC2, ty, tx);
+      __syncthreads();
+    }
+    put_block(sP, dp, ty, tx);
+    __syncthreads();
+    tile_acc<DH>(o1, sP, sC1, ty, tx);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int t = r0 + ty * 8 + i;
+    if (t >= A.T) continue;
+    const int H = KV ? A.Hkv : A.Hq;
+    const int64_t at = ((int64_t)t * H + blockIdx.y) * A.Dh;
+    T* g1 = (T*)(KV ? A.gk : A.gq) + at;
+    float odd = 0.f;  // NaN as soon as one element is not finite
+#pragma unroll
+    for (int n = 0; n < DH / 16; ++n) {
+      g1[tx + 16 * n] = from_f<T>(o1[i][n] * A.scale);
+      if (KV) ((T*)A.gv + at)[tx + 16 * n] = from_f<T>(o2[KV ? i : 0][n]);
+      odd = fmaf(o1[i][n], 0.f, fmaf(o2[KV ? i : 0][n], 0.f, odd));
+    }
+    if (odd != 0.f) again[ty * 8 + i] = 1;
+  }
+  __syncthreads();
+  for (int r = threadIdx.x >> 5; r < kBT; r += kThreads / 32)
+    if (again[r]) {
+      if (KV) exact_gkv_row<T>(A, blockIdx.y, r0 + r);
+      else exact_gq_row<T>(A, blockIdx.y, r0 + r);
+    }
+}
+
+template <typename K>
+static int launch(K kernel, dim3 grid, size_t smem, const AttnArgs& A, cudaStream_t st, const char* what) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return set_error(MR_E_LAUNCH, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
+  }
+  kernel<<<grid, kThreads, smem, st>>>(A);
+  return check_launch(what);
+}
+
+template <typename T, int DH> static int fwd_dh(const AttnArgs& A, cudaStream_t st) {
+  return launch(attn_fwd_f32<T, DH>, dim3((A.T + kBT - 1) / kBT, A.Hq), (3 * DH + kBT) * kPitch * 4, A, st, "attn_fwd_f32");
+}
+template <typename T, int DH> static int bwd_dh(const AttnArgs& A, cudaStream_t st) {
+  const size_t sm = (4 * DH + kBT) * kPitch * 4;
+  const unsigned n = (A.T + kBT - 1) / kBT;
+  if (int rc = launch(attn_bwd_f32<T, DH, false>, dim3(n, A.Hq), sm, A, st, "attn_bwd_f32 (grad_q)")) return rc;
+  return launch(attn_bwd_f32<T, DH, true>, dim3(n, A.Hkv), sm, A, st, "attn_bwd_f32 (grad_k, grad_v)");
+}
+
+template <typename T> int attn_delta_launch(const AttnArgs& A, cudaStream_t st) {
+  attn_delta<T><<<(unsigned)(((int64_t)A.T * A.Hq + 7) / 8), 256, 0, st>>>(A);
+  return check_launch("attn_delta");
+}
+
+template <typename T> int attn_fwd_simt(const AttnArgs& A, cudaStream_t st) {
+  switch (A.Dh) {
+    case 32: return fwd_dh<T, 32>(A, st);
+    case 64: return fwd_dh<T, 64>(A, st);
+    case 96: return fwd_dh<T, 96>(A, st);
+    default: return fwd_dh<T, 128>(A, st);
+  }
+}
+template <typename T> int attn_bwd_simt(const AttnArgs& A, cudaStream_t st) {
+  if (int rc = attn_delta_launch<T>(A, st)) return rc;
+  switch (A.Dh) {
+    case 32: return bwd_dh<T, 32>(A, st);
+    case 64: return bwd_dh<T, 64>(A, st);
+    case 96: return bwd_dh<T, 96>(A, st);
+    default: return bwd_dh<T, 128>(A, st);
+  }
+}
+
+#define MR_INST(T)                                                   \
+  template int attn_delta_launch<T>(const AttnArgs&, cudaStream_t);  \
+  template int attn_fwd_simt<T>(const AttnArgs&, cudaStream_t);      \
+  template int attn_bwd_simt<T>(const AttnArgs&, cudaStream_t);
+MR_INST(float)
+MR_INST(__nv_bfloat16)
+MR_INST(__half)
+#undef MR_INST
+
+}  // namespace mr

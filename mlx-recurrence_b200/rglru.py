@@ -15,9 +15,11 @@ drops it, ``rglru.py:226``; its pure loop does not).
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._chassis import DEFAULT_SEG, check_segment_shape, common_dtype, grad_out, prep, prep_h0, step_state
+from ._chassis import (DEFAULT_SEG, check_segment_shape, common_dtype, grad_out, prep, prep_cu, prep_h0,
+                       step_state)
 
 
 class _RGLRUScan(torch.autograd.Function):
@@ -196,3 +198,90 @@ def rglru_scan_gated(x, r, i, lam, c=8.0, seg=DEFAULT_SEG, h0=None):
 def rglru_scan_gated_with_state(x, r, i, lam, c=8.0, seg=DEFAULT_SEG, h0=None):
     """:func:`rglru_scan_gated` that also returns the final state [B, D]."""
     return _RGLRUGatedScan.apply(x, r, i, lam, c, seg, h0, True)
+
+
+class _RGLRUPacked(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, a, x, cu_seqlens, h0, want_final):
+        ctx.set_materialize_grads(False)
+        if a.dim() != 2 or x.shape != a.shape or a.shape[1] == 0:
+            raise ValueError(f"a and x must both be [T, D] with D > 0, got {tuple(a.shape)} and {tuple(x.shape)}")
+        T, D = a.shape
+        dev = _lib.require_cuda(a, x)
+        dt = common_dtype(a, x)
+        cu = prep_cu(cu_seqlens, dev)
+        S = cu.numel() - 1
+        a_, x_ = prep(a, dt), prep(x, dt)
+        h0_ = prep_h0(h0, (S, D), dev)
+        lib = _lib.load()
+        y = torch.empty((T, D), dtype=torch.float32, device=dev)
+        final = torch.empty((S, D), dtype=torch.float32, device=dev) if want_final else None
+        ckpt = None
+        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or ctx.needs_input_grad[3]:
+            ckpt = torch.empty((-(-T // lib.mr_rglru_packed_chunk()), D), dtype=torch.float32, device=dev)
+        nws = lib.mr_rglru_packed_workspace_bytes(T, D)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+        _lib.call_on(dev, "mr_rglru_packed_fwd", a_.data_ptr(), x_.data_ptr(), cu.data_ptr(), S, _lib.DTYPE_CODE[dt],
+                     T, D, _lib.ptr(h0_), y.data_ptr(), _lib.ptr(ckpt), _lib.ptr(final), _lib.ptr(ws), nws)
+        ctx.save_for_backward(a_, x_, cu, ckpt, h0_)
+        return y, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, gfinal):
+        a_, x_, cu, ckpt, h0_ = ctx.saved_tensors
+        T, D = a_.shape
+        dev, dt = a_.device, a_.dtype
+        gy = grad_out(gy, (T, D), dev)
+        gf = None if gfinal is None else gfinal.to(torch.float32).contiguous()
+        ga, gx = torch.empty_like(a_), torch.empty_like(x_)
+        gh0 = torch.empty_like(h0_) if (h0_ is not None and ctx.needs_input_grad[3]) else None
+        nws = _lib.load().mr_rglru_packed_workspace_bytes(T, D)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+        _lib.call_on(dev, "mr_rglru_packed_bwd", gy.data_ptr(), _lib.ptr(gf), ckpt.data_ptr(), a_.data_ptr(),
+                     x_.data_ptr(), cu.data_ptr(), cu.numel() - 1, _lib.DTYPE_CODE[dt], T, D, _lib.ptr(h0_),
+                     ga.data_ptr(), gx.data_ptr(), _lib.ptr(gh0), _lib.ptr(ws), nws)
+        return ga, gx, None, gh0, None
+
+
+def rglru_scan_packed(a, x, cu_seqlens, h0=None):
+    """RG-LRU scan over a packed batch: sequences of different lengths back to back.
+
+    No counterpart in the reference, whose scan takes one length per batch.
+    Unlike :func:`rglru_scan` there is no segment rule: lengths may be zero,
+    one or anything else, and D may be any size.
+
+    Args:
+        a:   [T, D] per-channel recurrent gate (any real value).
+        x:   [T, D] the already-gated input.
+        cu_seqlens: [S + 1] int32 or int64 borders on the same device,
+             nondecreasing, starting at 0: sequence s holds the rows
+             cu_seqlens[s] .. cu_seqlens[s+1]-1. Rows behind the last border
+             (padding) belong to no sequence: their y and gradients are zero,
+             whatever they hold.
+        h0:  optional initial states [S, D] (float32 state; differentiable).
+
+    Returns:
+        y:   [T, D] float32. State and accumulation are float32; gradients
+             come in the inputs' dtype.
+    """
+    return _RGLRUPacked.apply(a, x, cu_seqlens, h0, False)[0]
+
+
+def rglru_scan_packed_with_state(a, x, cu_seqlens, h0=None):
+    """:func:`rglru_scan_packed` that also returns the final states [S, D] (an
+    empty sequence's is its h0). Passed back as ``h0`` they continue the scan;
+    passed to :func:`rglru_step` they start decoding."""
+    return _RGLRUPacked.apply(a, x, cu_seqlens, h0, True)
+
+
+def rglru_scan_packed_reference(a, x, cu_seqlens, h0=None):
+    """Per-step torch loop of :func:`rglru_scan_packed`. Differentiable, any device."""
+    cu = cu_seqlens.tolist()
+    ys = []
+    for s, (lo, hi) in enumerate(zip(cu[:-1], cu[1:])):
+        if hi > lo:
+            ys.append(rglru_scan_reference(a[None, lo:hi], x[None, lo:hi], None if h0 is None else h0[s:s + 1])[0])
+    ft = torch.promote_types(a.dtype, torch.float32)
+    ys.append(torch.zeros((a.shape[0] - cu[-1], a.shape[1]), dtype=ft, device=a.device))
+    return torch.cat(ys)
