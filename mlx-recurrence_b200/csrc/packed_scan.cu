@@ -71,25 +71,36 @@ __device__ __forceinline__ Rec rec_wait(const Rec* p) {
 struct Borders {
   int start[kChunk], end[kChunk];
   int lo, hi;
+  uint32_t starts, ends;  // bit w: a sequence starts (ends) in warp w's steps
+  // no border in warp w's steps, and all of them in a sequence: the short loops serve
+  __device__ bool plain(int w) const {
+    return !((starts | ends) >> w & 1) && w * kSteps >= lo && (w + 1) * kSteps <= hi;
+  }
 };
 
+// All threads call it; the result is there after the next barrier.
 __device__ __forceinline__ void find_borders(Borders& b, const int* __restrict__ cu, int S, int64_t t0, int n) {
   for (int i = threadIdx.x; i < kChunk; i += kWarps * 32) b.start[i] = b.end[i] = -1;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
   int l = 0, r = S;  // the first s with cu[s] >= t0
   while (l < r) {
     const int m = (l + r) >> 1;
     if (cu[m] < t0) l = m + 1; else r = m;
   }
-  __syncthreads();
-  for (int s = l + threadIdx.x; s <= S; s += kWarps * 32) {
+  uint32_t starts = 0, ends = 0;
+  for (int s = l + threadIdx.x; s <= S; s += 32) {
     const int64_t at = cu[s] - t0;
     if (at > n) break;
-    if (at >= 0 && at < n && s < S && cu[s + 1] > cu[s]) b.start[at] = s;
-    if (at >= 1 && s > 0 && cu[s] > cu[s - 1]) b.end[at - 1] = s - 1;
+    if (at >= 0 && at < n && s < S && cu[s + 1] > cu[s]) b.start[at] = s, starts |= 1u << (at / kSteps);
+    if (at >= 1 && s > 0 && cu[s] > cu[s - 1]) b.end[at - 1] = s - 1, ends |= 1u << ((at - 1) / kSteps);
   }
+  starts = __reduce_or_sync(0xffffffffu, starts);
+  ends = __reduce_or_sync(0xffffffffu, ends);
   if (threadIdx.x == 0) {
     b.lo = (int)min(max((int64_t)cu[0] - t0, (int64_t)0), (int64_t)n);
     b.hi = (int)min(max((int64_t)cu[S] - t0, (int64_t)0), (int64_t)n);
+    b.starts = starts, b.ends = ends;
   }
 }
 
@@ -141,7 +152,7 @@ __device__ __forceinline__ void look_back(Chain& sh, Rec* recs, int64_t stride, 
       __syncthreads();
       bool open = false;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
+      for (int v = 0; w == 0 && v < V; ++v) {
         for (int i = 0; i < kWarps && !known[v]; ++i) {
           const Rec r = sh.back[i][lane * V + v];
           b[v] = fmaf(a[v], r.B, b[v]);
@@ -196,10 +207,20 @@ packed_fwd_kernel(const T* __restrict__ a, const T* __restrict__ x, const int* _
   }
   find_borders(bd, cu, S, t0, n);
   __syncthreads();
+  const bool plain = bd.plain(w);
   {
     float A[V], B[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
+    if (plain) {
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          B[v] = fmaf(to_f(av[k].v[v]), B[v], to_f(xv[k].v[v]));
+          A[v] *= to_f(av[k].v[v]);
+        }
+    } else {
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
       const int i = k0 + k, s = bd.start[i];
@@ -211,16 +232,12 @@ packed_fwd_kernel(const T* __restrict__ a, const T* __restrict__ x, const int* _
         A[v] *= to_f(av[k].v[v]);
       }
     }
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) sh.A[w][lane * V + v] = A[v], sh.B[w][lane * V + v] = B[v];
   }
-  const int mine = threadIdx.x < kChunk ? bd.start[threadIdx.x] : -1;
-  __shared__ uint32_t cuts;  // bit w: warp w's steps hold a start
-  if (threadIdx.x == 0) cuts = 0;
   __syncthreads();
-  if (mine >= 0) atomicOr(&cuts, 1u << (threadIdx.x / kSteps));
-  __syncthreads();
-  const uint32_t cut = cuts;
+  const uint32_t cut = bd.starts;
   // the state after warps 0 .. e-1, given the one before them
   auto through = [&](int c, int e, float& A, float& B) {
     for (int i = 0; i < e; ++i) {
@@ -246,6 +263,14 @@ packed_fwd_kernel(const T* __restrict__ a, const T* __restrict__ x, const int* _
     if (ckpt != nullptr && w == 0 && live && n > 0) ckpt[chunk * D + ch + v] = h[v];
     through(lane * V + v, w, A, h[v]);
   }
+  if (plain) {
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = fmaf(to_f(av[k].v[v]), h[v], to_f(xv[k].v[v]));
+      if (live) st_stream_f32<V>(y + (t0 + k0 + k) * D + ch, h);
+    }
+  } else {
 #pragma unroll
   for (int k = 0; k < kSteps; ++k) {
     const int i = k0 + k;
@@ -261,6 +286,7 @@ packed_fwd_kernel(const T* __restrict__ a, const T* __restrict__ x, const int* _
       if (fin != nullptr && in && e >= 0 && live) fin[e * D + ch + v] = h[v];
     }
     if (live) st_stream_f32<V>(y + (t0 + i) * D + ch, out);
+  }
   }
   if (fin != nullptr && live)  // empty sequences, spread over the chunks
     for (int s = (int)((int64_t)chunk * S / nchunk) + w; s < (int)((int64_t)(chunk + 1) * S / nchunk); s += kWarps)
@@ -295,10 +321,26 @@ packed_bwd_kernel(const float* __restrict__ gy, const float* __restrict__ gf, co
   }
   find_borders(bd, cu, S, t0, n);
   __syncthreads();
+  const bool plain = bd.plain(w);
   {
     float A[V], B[V], P[V], Q[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) A[v] = P[v] = 1.f, B[v] = Q[v] = 0.f;
+    if (plain) {
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          B[v] = fmaf(to_f(av[k].v[v]), B[v], to_f(xv[k].v[v]));
+          A[v] *= to_f(av[k].v[v]);
+        }
+#pragma unroll
+      for (int k = kSteps - 1; k >= 0; --k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) Q[v] = to_f(av[k].v[v]) * (gv[k].v[v] + Q[v]);
+#pragma unroll
+      for (int v = 0; v < V; ++v) P[v] = A[v];
+    } else {
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
       const int i = k0 + k, s = bd.start[i];
@@ -321,21 +363,15 @@ packed_bwd_kernel(const float* __restrict__ gy, const float* __restrict__ gf, co
         P[v] *= to_f(av[k].v[v]);
       }
     }
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       fA[w][lane * V + v] = A[v], fB[w][lane * V + v] = B[v];
       sh.A[w][lane * V + v] = P[v], sh.B[w][lane * V + v] = Q[v];
     }
   }
-  __shared__ uint32_t cuts, ends;
-  if (threadIdx.x == 0) cuts = ends = 0;
   __syncthreads();
-  if (threadIdx.x < kChunk) {
-    if (bd.start[threadIdx.x] >= 0) atomicOr(&cuts, 1u << (threadIdx.x / kSteps));
-    if (bd.end[threadIdx.x] >= 0) atomicOr(&ends, 1u << (threadIdx.x / kSteps));
-  }
-  __syncthreads();
-  const uint32_t cut = cuts, end = ends;
+  const uint32_t cut = bd.starts, end = bd.ends;
   // r left of warps 7 .. e, given the one right of them
   auto through = [&](int c, int e, float& P, float& Q) {
     for (int i = kWarps - 1; i >= e; --i) {
@@ -363,6 +399,29 @@ packed_bwd_kernel(const float* __restrict__ gy, const float* __restrict__ gf, co
     for (int i = 0; i < w; ++i)
       h[v] = cut >> i & 1 ? fB[i][lane * V + v] : fmaf(fA[i][lane * V + v], h[v], fB[i][lane * V + v]);
   }
+  if (plain) {
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        before[k][v] = h[v];
+        h[v] = fmaf(to_f(av[k].v[v]), h[v], to_f(xv[k].v[v]));
+      }
+#pragma unroll
+    for (int k = kSteps - 1; k >= 0; --k) {
+      float oa[V], ox[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        ox[v] = gv[k].v[v] + r[v];
+        oa[v] = ox[v] * before[k][v];
+        r[v] = to_f(av[k].v[v]) * ox[v];
+      }
+      if (live) {
+        st_vec<T, V>(ga + (t0 + k0 + k) * D + ch, oa);
+        st_vec<T, V>(gx + (t0 + k0 + k) * D + ch, ox);
+      }
+    }
+  } else {
 #pragma unroll
   for (int k = 0; k < kSteps; ++k) {
     const int i = k0 + k, s = bd.start[i];
@@ -393,6 +452,7 @@ packed_bwd_kernel(const float* __restrict__ gy, const float* __restrict__ gf, co
       st_vec<T, V>(ga + (t0 + i) * D + ch, oa);
       st_vec<T, V>(gx + (t0 + i) * D + ch, ox);
     }
+  }
   }
   if (gh0 != nullptr && live)
     for (int s = (int)((int64_t)chunk * S / nchunk) + w; s < (int)((int64_t)(chunk + 1) * S / nchunk); s += kWarps)
