@@ -7,23 +7,27 @@
 // the sequence's last token; grad_x = adj, grad_a[t] = adj_t h_{t-1},
 // grad_h0[s] = r left of its first token (gf_s for an empty sequence).
 //
-// One pass over the data, HBM-bound: a CTA takes kChunk steps of 32 V channels,
-// 8 warps x kSteps steps each, and holds them in registers. A step is the affine
-// map h -> a h + x, so runs of steps compose to one map (A, B): per thread, per
-// CTA (shared memory) and per chunk. A chunk publishes its map, looks back over
-// the chunks before it (8 at a time, one per warp) until it meets one whose state
-// is known, and publishes its own state. A sequence border cuts the chain: what
-// follows it does not depend on the past. Borders are the same for all channels,
-// so every branch on them is uniform. The backward runs the same scheme from the
-// right and rebuilds h from the states that the forward kept per chunk.
+// One pass over the data, HBM-bound. An item is kChunk steps of 32 V channels
+// (rows of 128 bytes of the inputs); 8 warps x kSteps steps each work on it out
+// of shared memory, where a ninth warp's TMA copies bring the items of a
+// persistent CTA ahead of time. A step is the affine map h -> a h + x, so runs of
+// steps compose to one map (A, B): per thread, per warp prefix and per item. An
+// item publishes its map, looks back over the items before it in time (kBack at
+// a time) until it meets one whose state is known, and publishes its own state.
+// A sequence border cuts the chain: what follows it does not depend on the past.
+// Borders are the same for all channels, so every branch on them is uniform. The
+// backward runs the same scheme from the right, and rebuilds h from the states
+// that the forward kept per chunk.
 #include "common.cuh"
 #include "tma.cuh"
+#include "tmap.cuh"
 
 namespace mr {
 
 constexpr int kWarps = 8;
 constexpr int kSteps = 16;               // steps of a thread
-constexpr int kChunk = kWarps * kSteps;  // steps of a CTA
+constexpr int kChunk = kWarps * kSteps;  // steps of an item
+constexpr int kBack = 4;                 // items that one round of the look-back reads
 
 // A chunk's map or state for one channel, written and read as one 16-byte access
 // (single-copy atomic), so no flag or fence stands beside it.
@@ -66,426 +70,591 @@ __device__ __forceinline__ Rec rec_wait(const Rec* p) {
   return {0.f, 0.f, kState, 0};
 }
 
-// The borders inside a chunk, per token: the sequence that starts there (else -1)
-// and the sequence that ends there; tokens [lo, hi) of the chunk lie in sequences.
-struct Borders {
-  int start[kChunk], end[kChunk];
-  int lo, hi;
-  uint32_t starts, ends;  // bit w: a sequence starts (ends) in warp w's steps
+// The borders of a chunk, found ahead by packed_prep_kernel (a search in cu is a
+// chain of dependent loads): the first s with cu[s] >= t0, the tokens [lo, hi) of
+// the chunk that lie in sequences, and a bit per warp for the steps that hold a
+// sequence's start (its end).
+struct alignas(16) ChunkInfo {
+  int first, lo, hi;
+  uint32_t starts, ends;
+  int pad[3];
   // no border in warp w's steps, and all of them in a sequence: the short loops serve
   __device__ bool plain(int w) const {
     return !((starts | ends) >> w & 1) && w * kSteps >= lo && (w + 1) * kSteps <= hi;
   }
 };
 
-// All threads call it; the result is there after the next barrier.
-__device__ __forceinline__ void find_borders(Borders& b, const int* __restrict__ cu, int S, int64_t t0, int n) {
-  for (int i = threadIdx.x; i < kChunk; i += kWarps * 32) b.start[i] = b.end[i] = -1;
-  __syncthreads();
-  if (threadIdx.x >= 32) return;
-  int l = 0, r = S;  // the first s with cu[s] >= t0
+__device__ __forceinline__ ChunkInfo chunk_info(const int* __restrict__ cu, int S, int64_t t0, int n) {
+  int l = 0, r = S;
   while (l < r) {
     const int m = (l + r) >> 1;
     if (cu[m] < t0) l = m + 1; else r = m;
   }
-  uint32_t starts = 0, ends = 0;
-  for (int s = l + threadIdx.x; s <= S; s += 32) {
+  ChunkInfo c = {};
+  c.first = l;
+  for (int s = l; s <= S; ++s) {
     const int64_t at = cu[s] - t0;
     if (at > n) break;
-    if (at >= 0 && at < n && s < S && cu[s + 1] > cu[s]) b.start[at] = s, starts |= 1u << (at / kSteps);
-    if (at >= 1 && s > 0 && cu[s] > cu[s - 1]) b.end[at - 1] = s - 1, ends |= 1u << ((at - 1) / kSteps);
+    if (at >= 0 && at < n && s < S && cu[s + 1] > cu[s]) c.starts |= 1u << (at / kSteps);
+    if (at >= 1 && s > 0 && cu[s] > cu[s - 1]) c.ends |= 1u << ((at - 1) / kSteps);
   }
-  starts = __reduce_or_sync(0xffffffffu, starts);
-  ends = __reduce_or_sync(0xffffffffu, ends);
-  if (threadIdx.x == 0) {
-    b.lo = (int)min(max((int64_t)cu[0] - t0, (int64_t)0), (int64_t)n);
-    b.hi = (int)min(max((int64_t)cu[S] - t0, (int64_t)0), (int64_t)n);
-    b.starts = starts, b.ends = ends;
-  }
+  c.lo = (int)min(max((int64_t)cu[0] - t0, (int64_t)0), (int64_t)n);
+  c.hi = (int)min(max((int64_t)cu[S] - t0, (int64_t)0), (int64_t)n);
+  return c;
 }
 
-// V channels of one step; those at or behind D read as zero
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> ld_step(const T* p, bool ok) {
-  Vec<T, V> r;
-  if (ok) {
-    r = ld_vec<T, V>(p);
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) r.v[v] = from_f<T>(0.f);
-  }
-  return r;
+// Clears the ticket counter and the records, and describes the chunks.
+__global__ void __launch_bounds__(256) packed_prep_kernel(const int* __restrict__ cu, int S, int64_t L, int nchunk,
+                                                          uint4* ws, ChunkInfo* info, uint4* recs, int64_t nrec) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)gridDim.x * 256;
+  for (int64_t c = id; c < nchunk; c += all)
+    info[c] = chunk_info(cu, S, c * kChunk, (int)min((int64_t)kChunk, L - c * kChunk));
+  if (id == 0) *ws = make_uint4(0, 0, 0, 0);
+  for (int64_t i = id; i < nrec; i += all) recs[i] = make_uint4(0, 0, 0, 0);
 }
 
-struct Chain {
-  float A[kWarps][64], B[kWarps][64];  // the warps' maps
-  Rec back[kWarps][64];                // what the look-back read
-  float carry[64];                     // the state entering the chunk
+struct PackedArgs {
+  const int* cu;
+  int S, nchunk, ntile;
+  int64_t L, D;
+  const float *h0, *gf, *gy;
+  float *y, *ckpt, *fin, *gh0;
+  const void *a, *x;
+  void *ga, *gx;
+  uint32_t* counter;  // NULL when there is one chunk: item = blockIdx.x, no records
+  const ChunkInfo* info;
+  Rec* recs;
+  bool vec;  // rows of V elements may be accessed whole
 };
 
-// State entering chunk `rank` of the chain (0: the first to start). `cut`: the
-// chunk holds a border, so its outgoing state is B whatever enters; `need`:
-// whether anything in the chunk depends on what enters. Publishes this chunk's
-// own record. All threads call it, after the warps' maps are in sh.
-template <int V, typename F>
-__device__ __forceinline__ void look_back(Chain& sh, Rec* recs, int64_t stride, int64_t ch, bool live, int rank, int last,
-                                          bool cut, bool need, F total) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  float A[V], B[V];
-  if (w == 0) {
+template <typename T> constexpr int kV = 4 / sizeof(T);  // channels of a thread: 4 bytes of an input row
+template <typename T, bool BWD> constexpr int kStage = kChunk * 32 * kV<T> * (2 * (int)sizeof(T) + (BWD ? 4 : 0));
+
+template <typename T, int V, typename P>
+__device__ __forceinline__ Vec<T, V> get(const P* p, bool vec, int live) {
+  Vec<T, V> r;
+  if (vec && live == V) return ld_vec<T, V>(p);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      total(lane * V + v, A[v], B[v]);
-      if (live && rank < last) rec_store(recs + rank * stride + ch + v, A[v], B[v], cut || rank == 0 ? kState : kMap);
+  for (int v = 0; v < V; ++v) r.v[v] = v < live ? p[v] : from_f<T>(0.f);
+  return r;
+}
+template <typename T, int V> __device__ __forceinline__ void put(T* p, const float (&f)[V], bool vec, int live) {
+  if (vec && live == V) {
+    if constexpr (sizeof(T) == 4) st_stream_f32<V>(p, f);
+    else st_vec<T, V>(p, f);
+    return;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (v < live) p[v] = from_f<T>(f[v]);
+}
+
+// What a CTA keeps in shared memory beside the stages.
+template <int V> struct Work {
+  float A[kWarps][32 * V], B[kWarps][32 * V];    // the warps' maps along the chain
+  float fA[kWarps][32 * V], fB[kWarps][32 * V];  // backward: the warps' maps of the forward recurrence
+  float2 back[kBack][32 * V];                    // what the look-back read: A (or kKnown) and B
+  float carry[32 * V];                           // the state entering the item
+  int mark[kChunk];                              // per token at a border: its sequence, and which end of it
+  uint64_t full[2], empty[2];
+  ChunkInfo infos[2];
+  int items[2];
+  int open;
+};
+constexpr int kStart = 1 << 30, kEnd = INT32_MIN, kSeq = kStart - 1;  // of Work::mark; 0 in both bits: no border
+
+// stands for A in a record that holds a state (a product of gates is never this NaN: products give 0x7fffffff)
+__device__ __forceinline__ float known_mark() { return __uint_as_float(0xffffffffu); }
+
+__device__ __forceinline__ void sync_workers() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// The items of a CTA, in the order of the tickets. Tickets follow the order in
+// which CTAs ask, so whatever an item waits for has been taken by a running CTA,
+// which works through its items in order: the smallest one never waits.
+//
+// TMA form: warp kWarps takes tickets and fills the two (one) stages ahead. Plain
+// form (rows that are no multiple of 16 bytes): every thread brings its own
+// elements when the item begins.
+template <typename T, bool BWD, bool TMA, int STAGES> struct Feed {
+  static constexpr int V = kV<T>, CH = 32 * V;
+  unsigned char* stages;
+  Work<V>& sh;
+  const PackedArgs& P;
+  int n = 0;  // items so far
+
+  __device__ T* a(int st) const { return reinterpret_cast<T*>(stages + st * kStage<T, BWD>); }
+  __device__ T* x(int st) const { return a(st) + kChunk * CH; }
+  __device__ float* g(int st) const { return reinterpret_cast<float*>(x(st) + kChunk * CH); }
+  __device__ int64_t chunk_of(int item) const { return BWD ? P.nchunk - 1 - item / P.ntile : item / P.ntile; }
+
+  __device__ void produce(const CUtensorMap* ta, const CUtensorMap* tx, const CUtensorMap* tg) {
+    const int total = P.nchunk * P.ntile;
+    for (int i = 0;; ++i) {
+      const int st = i % STAGES;
+      const int item = P.counter ? (int)min(atomicAdd(P.counter, 1u), (uint32_t)INT32_MAX)
+                                 : (i == 0 ? (int)blockIdx.x : INT32_MAX);
+      if (i >= STAGES) mbar_wait(&sh.empty[st], (i / STAGES - 1) & 1);
+      if (item >= total) {
+        sh.items[st] = -1;
+        mbar_arrive(&sh.full[st]);
+        return;
+      }
+      const int64_t t0 = chunk_of(item) * kChunk;
+      const int c0 = item % P.ntile * CH;
+      sh.items[st] = item;
+      sh.infos[st] = P.info ? P.info[chunk_of(item)] : chunk_info(P.cu, P.S, t0, (int)min((int64_t)kChunk, P.L - t0));
+      mbar_arrive_expect_tx(&sh.full[st], kStage<T, BWD>);
+      tma_load_2d(a(st), ta, c0, (int)t0, &sh.full[st]);
+      tma_load_2d(x(st), tx, c0, (int)t0, &sh.full[st]);
+      if (BWD) tma_load_2d(g(st), tg, c0, (int)t0, &sh.full[st]);
     }
   }
-  float a[V], b[V];  // the composed map of the chunks looked at so far
-  bool known[V];     // a record may turn from map to state between two reads, so each channel stops by itself
+
+  // Next item into stage `st` (returned through st), or -1.
+  __device__ int next(int& st) {
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if constexpr (TMA) {
+      st = n % STAGES;
+      mbar_wait(&sh.full[st], (n / STAGES) & 1);
+      ++n;
+      return sh.items[st];
+    } else {
+      st = 0;
+      if (P.counter == nullptr) {
+        if (n++ > 0) return -1;
+        sh.items[0] = blockIdx.x;
+      } else {
+        sync_workers();  // everybody has read the last item's number
+        if (threadIdx.x == 0) sh.items[0] = (int)min(atomicAdd(P.counter, 1u), (uint32_t)INT32_MAX);
+      }
+      sync_workers();
+      const int item = sh.items[0];
+      if (item >= P.nchunk * P.ntile) return -1;
+      const int64_t t0 = chunk_of(item) * kChunk, ch = (int64_t)(item % P.ntile) * CH + lane * V;
+      const int live = (int)min((int64_t)V, max((int64_t)0, P.D - ch)), rows = (int)min((int64_t)kChunk, P.L - t0);
+      Vec<T, V> va[kSteps], vx[kSteps];
 #pragma unroll
-  for (int v = 0; v < V; ++v) a[v] = 1.f, b[v] = 0.f, known[v] = false;
-  if (need && rank > 0) {
-    for (int at = rank - 1;; at -= kWarps) {
-      const int mine = at - w;
+      for (int k = 0; k < kSteps; ++k) {
+        const int i = w * kSteps + k;
+        const int64_t at = (t0 + i) * P.D + ch;
+        va[k] = get<T, V>((const T*)P.a + at, P.vec, i < rows ? live : 0);
+        vx[k] = get<T, V>((const T*)P.x + at, P.vec, i < rows ? live : 0);
+      }
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const int i = (w * kSteps + k) * CH + lane * V;
+        *reinterpret_cast<Vec<T, V>*>(a(0) + i) = va[k];
+        *reinterpret_cast<Vec<T, V>*>(x(0) + i) = vx[k];
+      }
+      if constexpr (BWD) {
+        Vec<float, V> vg[kSteps];
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          const int i = w * kSteps + k;
+          vg[k] = get<float, V>(P.gy + (t0 + i) * P.D + ch, P.vec, i < rows ? live : 0);
+        }
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+          *reinterpret_cast<Vec<float, V>*>(g(0) + (w * kSteps + k) * CH + lane * V) = vg[k];
+      }
+      return item;
+    }
+  }
+  // The stage may be filled again.
+  __device__ void release(int st) {
+    if constexpr (TMA) {
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.empty[st]);
+    }
+  }
+};
+
+// Marks of a chunk that holds borders; all workers call it. A token belongs to
+// one sequence, so one entry serves its start and its end.
+template <int V> __device__ __forceinline__ void mark_borders(Work<V>& sh, const ChunkInfo& c, const PackedArgs& P, int64_t t0, int n) {
+  if (threadIdx.x < kChunk) sh.mark[threadIdx.x] = 0;
+  sync_workers();
+  for (int s = c.first + threadIdx.x; s <= P.S; s += kWarps * 32) {
+    const int64_t at = P.cu[s] - t0;
+    if (at > n) break;
+    if (at >= 0 && at < n && s < P.S && P.cu[s + 1] > P.cu[s]) atomicOr(&sh.mark[at], s | kStart);
+    if (at >= 1 && s > 0 && P.cu[s] > P.cu[s - 1]) atomicOr(&sh.mark[at - 1], (s - 1) | kEnd);
+  }
+  sync_workers();
+}
+
+// The sequence that starts (ends) at token i of the chunk, or -1. Marks are there when the chunk has borders
+// (clamped, so that a malformed cu stays in range).
+__device__ __forceinline__ int start_of(const int* mark, const ChunkInfo& c, int i, int S) {
+  return c.starts && (mark[i] & kStart) ? min(mark[i] & kSeq, S - 1) : -1;
+}
+__device__ __forceinline__ int end_of(const int* mark, const ChunkInfo& c, int i, int S) {
+  return c.ends && (mark[i] & kEnd) ? min(mark[i] & kSeq, S - 1) : -1;
+}
+
+// The chain. Along it (left to right in the forward, right to left in the
+// backward) item `rank` of a channel tile follows rank - 1. Composes the warps'
+// maps in sh.A, sh.B (bit w of `cut`: warp w's steps hold a border, so its
+// outgoing state is B whatever enters), publishes this item's record, and returns
+// in p, q the map from the state entering the item to the one entering this warp
+// and in carry the former. `need`: whether anything in the item depends on it.
+template <int V, bool BWD>
+__device__ __forceinline__ void chain(Work<V>& sh, const PackedArgs& P, int64_t ch, int live, int rank, uint32_t cut,
+                                      bool need, float (&carry)[V], float (&p)[V], float (&q)[V]) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = lane * V;
+  const bool wait = need && rank > 0, tell = P.counter != nullptr && rank < P.nchunk - 1;
+  Rec* recs = P.recs + ch;
+  // warps 1 .. kBack fetch the records of the items before this one while warp 0 publishes
+  auto fetch = [&](int at) {
+    const int mine = at - (w - 1);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const Rec r = mine >= 0 && v < live ? rec_wait(recs + mine * P.D + v) : Rec{0.f, 0.f, kState, 0};
+      sh.back[w - 1][c + v] = make_float2(r.tag == kState ? known_mark() : r.A, r.B);
+    }
+  };
+  auto through = [&](int i) {  // p, q <- the warps' maps up to and including warp i
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float A = sh.A[i][c + v], B = sh.B[i][c + v];
+      q[v] = cut >> i & 1 ? B : fmaf(A, q[v], B);
+      p[v] = cut >> i & 1 ? 0.f : p[v] * A;
+    }
+  };
+#pragma unroll
+  for (int v = 0; v < V; ++v) p[v] = 1.f, q[v] = 0.f;
+  if (w == 0) {
+    float tp[V], tq[V];
+    for (int i = 0; i < kWarps; ++i) {
+      if ((BWD ? kWarps - 1 - i : i) == 0 && BWD) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) tp[v] = p[v], tq[v] = q[v];  // what enters warp 0, the last on the chain
+      }
+      through(BWD ? kWarps - 1 - i : i);
+    }
+    if (tell)
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        sh.back[w][lane * V + v] = mine >= 0 && live ? rec_wait(recs + mine * stride + ch + v) : Rec{0.f, 0.f, kState, 0};
-      __syncthreads();
-      bool open = false;
+        if (v < live) rec_store(recs + rank * P.D + v, p[v], q[v], cut || !wait ? kState : kMap);
+    if (wait) {
+      float a[V], b[V];  // the composed map of the items looked at so far
+      bool known[V];     // a record may turn from map to state between two reads: each channel stops by itself
 #pragma unroll
-      for (int v = 0; w == 0 && v < V; ++v) {
-        for (int i = 0; i < kWarps && !known[v]; ++i) {
-          const Rec r = sh.back[i][lane * V + v];
-          b[v] = fmaf(a[v], r.B, b[v]);
-          a[v] *= r.A;
-          known[v] = r.tag == kState;
+      for (int v = 0; v < V; ++v) a[v] = 1.f, b[v] = 0.f, known[v] = false;
+      for (bool open = true; open;) {
+        sync_workers();
+        open = false;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+#pragma unroll
+          for (int i = 0; i < kBack; ++i) {
+            const float2 r = sh.back[i][c + v];
+            if (!known[v]) {
+              b[v] = fmaf(a[v], r.y, b[v]);
+              known[v] = __float_as_uint(r.x) == 0xffffffffu;
+              a[v] *= r.x;
+            }
+          }
+          open |= !known[v];
+          sh.carry[c + v] = b[v];
         }
-        open |= !known[v];
+        open = __any_sync(0xffffffffu, open);
+        if (lane == 0) sh.open = open;
+        if (!open && tell && !cut)
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (v < live) rec_store(recs + rank * P.D + v, 0.f, fmaf(p[v], b[v], q[v]), kState);
+        sync_workers();
       }
-      if (!__syncthreads_or(open)) break;
     }
-  }
-  if (w == 0) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      sh.carry[lane * V + v] = b[v];
-      if (live && rank < last && need && !cut && rank > 0)
-        rec_store(recs + rank * stride + ch + v, 0.f, fmaf(A[v], b[v], B[v]), kState);
-    }
+    for (int v = 0; v < V; ++v) p[v] = BWD ? tp[v] : 1.f, q[v] = BWD ? tq[v] : 0.f;
+  } else {
+    if (wait && w <= kBack) fetch(rank - 1);
+    if (BWD)
+      for (int i = kWarps - 1; i > w; --i) through(i);
+    else
+      for (int i = 0; i < w; ++i) through(i);
+    if (wait)
+      for (int at = rank - 1;;) {
+        sync_workers();
+        sync_workers();
+        if (!sh.open) break;
+        at -= kBack;
+        if (w <= kBack) fetch(at);
+      }
   }
-  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < V; ++v) carry[v] = wait ? sh.carry[c + v] : 0.f;
 }
 
-// (chunk rank, channel tile) of this CTA: tickets follow the order in which CTAs
-// start, so whatever a chunk waits for is already running.
-__device__ __forceinline__ int64_t take_ticket(uint32_t* counter) {
-  __shared__ uint32_t t;
-  if (counter == nullptr) return blockIdx.x;
-  if (threadIdx.x == 0) t = atomicAdd(counter, 1u);
-  __syncthreads();
-  return t;
-}
+// state entering the warp, from the one entering the item; a cut leaves p = 0 and q alone (0 x infinity would not)
+__device__ __forceinline__ float enter(float p, float q, float carry, bool cut) { return cut ? q : fmaf(p, carry, q); }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kWarps * 32, V == 1 ? 4 : 3)
-packed_fwd_kernel(const T* __restrict__ a, const T* __restrict__ x, const int* __restrict__ cu, int S, int64_t L,
-                  int64_t D, const float* __restrict__ h0, float* __restrict__ y, float* __restrict__ ckpt,
-                  float* __restrict__ fin, uint32_t* counter, Rec* recs, int nchunk, int ntile) {
-  __shared__ Chain sh;
-  __shared__ Borders bd;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t ticket = take_ticket(counter);
-  const int chunk = (int)(ticket / ntile);
-  const int64_t ch = (ticket % ntile) * (32 * V) + lane * V, t0 = (int64_t)chunk * kChunk;
-  const int n = (int)min((int64_t)kChunk, L - t0), k0 = w * kSteps;
-  const bool live = ch < D;
-  Vec<T, V> av[kSteps], xv[kSteps];
-#pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    const int64_t at = (t0 + k0 + k) * D + ch;
-    av[k] = ld_step<T, V>(a + at, live && k0 + k < n);
-    xv[k] = ld_step<T, V>(x + at, live && k0 + k < n);
+template <typename T, bool TMA>
+__global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), 3)
+packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ CUtensorMap ta,
+                  const __grid_constant__ CUtensorMap tx) {
+  constexpr int V = kV<T>, CH = 32 * V;
+  extern __shared__ __align__(128) unsigned char dyn[];
+  __shared__ Work<V> sh;
+  Feed<T, false, TMA, 2> feed{dyn, sh, P};
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, k0 = w * kSteps;
+  if constexpr (TMA) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < 2; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], kWarps);
+      fence_mbar_init();
+    }
+    __syncthreads();
+    if (w == kWarps) {
+      if (lane == 0) feed.produce(&ta, &tx, nullptr);
+      return;
+    }
   }
-  find_borders(bd, cu, S, t0, n);
-  __syncthreads();
-  const bool plain = bd.plain(w);
-  {
+  for (int st;;) {
+    const int item = feed.next(st);
+    if (item < 0) break;
+    const int chunk = item / P.ntile;
+    const int64_t ch = (int64_t)(item % P.ntile) * CH + lane * V, t0 = (int64_t)chunk * kChunk;
+    const int n = (int)min((int64_t)kChunk, P.L - t0), live = (int)min((int64_t)V, max((int64_t)0, P.D - ch));
+    const ChunkInfo info = TMA ? sh.infos[st] : P.info ? P.info[chunk] : chunk_info(P.cu, P.S, t0, n);
+    const bool plain = info.plain(w);
+    if (info.starts | info.ends) mark_borders(sh, info, P, t0, n);
+    const T *sa = feed.a(st) + k0 * CH + lane * V, *sx = feed.x(st) + k0 * CH + lane * V;
     float A[V], B[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
     if (plain) {
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k)
+      for (int k = 0; k < kSteps; ++k) {
+        const Vec<T, V> av = ld_vec<T, V>(sa + k * CH), xv = ld_vec<T, V>(sx + k * CH);
+#pragma unroll
+        for (int v = 0; v < V; ++v) B[v] = fmaf(to_f(av.v[v]), B[v], to_f(xv.v[v])), A[v] *= to_f(av.v[v]);
+      }
+    } else {
+      for (int k = 0; k < kSteps; ++k) {
+        const int i = k0 + k;
+        if (i < info.lo || i >= info.hi) continue;
+        const int s = start_of(sh.mark, info, i, P.S);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          B[v] = fmaf(to_f(av[k].v[v]), B[v], to_f(xv[k].v[v]));
-          A[v] *= to_f(av[k].v[v]);
+          if (s >= 0) B[v] = P.h0 && v < live ? P.h0[s * P.D + ch + v] : 0.f;
+          B[v] = fmaf(to_f(sa[k * CH + v]), B[v], to_f(sx[k * CH + v])), A[v] *= to_f(sa[k * CH + v]);
         }
-    } else {
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      const int i = k0 + k, s = bd.start[i];
-      if (i < bd.lo || i >= bd.hi) continue;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (s >= 0) B[v] = h0 && live ? h0[s * D + ch + v] : 0.f;
-        B[v] = fmaf(to_f(av[k].v[v]), B[v], to_f(xv[k].v[v]));
-        A[v] *= to_f(av[k].v[v]);
       }
-    }
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) sh.A[w][lane * V + v] = A[v], sh.B[w][lane * V + v] = B[v];
-  }
-  __syncthreads();
-  const uint32_t cut = bd.starts;
-  // the state after warps 0 .. e-1, given the one before them
-  auto through = [&](int c, int e, float& A, float& B) {
-    for (int i = 0; i < e; ++i) {
-      if (cut >> i & 1) {
-        A = 0.f;
-        B = sh.B[i][c];
-      } else {
-        B = fmaf(sh.A[i][c], B, sh.B[i][c]);
-        A *= sh.A[i][c];
-      }
-    }
-  };
-  const bool need = bd.lo == 0 && bd.hi > 0 && bd.start[0] < 0;
-  look_back<V>(sh, recs, D, ch, live, chunk, nchunk - 1, cut != 0, need, [&](int c, float& A, float& B) {
-    A = 1.f, B = 0.f;
-    through(c, kWarps, A, B);
-  });
-  float h[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    float A = 1.f;
-    h[v] = sh.carry[lane * V + v];
-    if (ckpt != nullptr && w == 0 && live && n > 0) ckpt[chunk * D + ch + v] = h[v];
-    through(lane * V + v, w, A, h[v]);
-  }
-  if (plain) {
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = fmaf(to_f(av[k].v[v]), h[v], to_f(xv[k].v[v]));
-      if (live) st_stream_f32<V>(y + (t0 + k0 + k) * D + ch, h);
-    }
-  } else {
-#pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    const int i = k0 + k;
-    if (i >= n) break;
-    const bool in = i >= bd.lo && i < bd.hi;
-    const int s = bd.start[i], e = bd.end[i];
-    float out[V];
+    sync_workers();
+    const bool need = info.lo == 0 && info.hi > 0 && start_of(sh.mark, info, 0, P.S) < 0;
+    float carry[V], p[V], q[V], h[V];
+    chain<V, false>(sh, P, ch, live, chunk, info.starts, need, carry, p, q);
+    const bool cut = info.starts & ((1u << w) - 1);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      if (in && s >= 0) h[v] = h0 && live ? h0[s * D + ch + v] : 0.f;
-      if (in) h[v] = fmaf(to_f(av[k].v[v]), h[v], to_f(xv[k].v[v]));
-      out[v] = in ? h[v] : 0.f;
-      if (fin != nullptr && in && e >= 0 && live) fin[e * D + ch + v] = h[v];
+      h[v] = enter(p[v], q[v], carry[v], cut);
+      if (P.ckpt != nullptr && w == 0 && v < live && n > 0) P.ckpt[chunk * P.D + ch + v] = h[v];
     }
-    if (live) st_stream_f32<V>(y + (t0 + i) * D + ch, out);
-  }
-  }
-  if (fin != nullptr && live)  // empty sequences, spread over the chunks
-    for (int s = (int)((int64_t)chunk * S / nchunk) + w; s < (int)((int64_t)(chunk + 1) * S / nchunk); s += kWarps)
-      if (cu[s + 1] <= cu[s])
-#pragma unroll
-        for (int v = 0; v < V; ++v) fin[s * D + ch + v] = h0 ? h0[s * D + ch + v] : 0.f;
-}
-
-template <typename T, int V>
-__global__ void __launch_bounds__(kWarps * 32, 2)
-packed_bwd_kernel(const float* __restrict__ gy, const float* __restrict__ gf, const float* __restrict__ ckpt,
-                  const T* __restrict__ a, const T* __restrict__ x, const int* __restrict__ cu, int S, int64_t L,
-                  int64_t D, const float* __restrict__ h0, T* __restrict__ ga, T* __restrict__ gx,
-                  float* __restrict__ gh0, uint32_t* counter, Rec* recs, int nchunk, int ntile) {
-  __shared__ Chain sh;
-  __shared__ float fA[kWarps][64], fB[kWarps][64];  // the warps' maps of the forward recurrence
-  __shared__ Borders bd;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t ticket = take_ticket(counter);
-  const int rank = (int)(ticket / ntile), chunk = nchunk - 1 - rank;
-  const int64_t ch = (ticket % ntile) * (32 * V) + lane * V, t0 = (int64_t)chunk * kChunk;
-  const int n = (int)min((int64_t)kChunk, L - t0), k0 = w * kSteps;
-  const bool live = ch < D;
-  Vec<T, V> av[kSteps], xv[kSteps];
-  Vec<float, V> gv[kSteps];
-#pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    const int64_t at = (t0 + k0 + k) * D + ch;
-    av[k] = ld_step<T, V>(a + at, live && k0 + k < n);
-    gv[k] = ld_step<float, V>(gy + at, live && k0 + k < n);
-    xv[k] = ld_step<T, V>(x + at, live && k0 + k < n);
-  }
-  find_borders(bd, cu, S, t0, n);
-  __syncthreads();
-  const bool plain = bd.plain(w);
-  {
-    float A[V], B[V], P[V], Q[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) A[v] = P[v] = 1.f, B[v] = Q[v] = 0.f;
+    float* y = P.y + (t0 + k0) * P.D + ch;
     if (plain) {
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k)
+      for (int k = 0; k < kSteps; ++k, y += P.D) {
+        const Vec<T, V> av = ld_vec<T, V>(sa + k * CH), xv = ld_vec<T, V>(sx + k * CH);
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = fmaf(to_f(av.v[v]), h[v], to_f(xv.v[v]));
+        put<float, V>(y, h, P.vec, live);
+      }
+    } else {
+      for (int k = 0; k < kSteps && k0 + k < n; ++k, y += P.D) {
+        const int i = k0 + k;
+        const bool in = i >= info.lo && i < info.hi;
+        const int s = in ? start_of(sh.mark, info, i, P.S) : -1, e = in ? end_of(sh.mark, info, i, P.S) : -1;
+        float out[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          B[v] = fmaf(to_f(av[k].v[v]), B[v], to_f(xv[k].v[v]));
-          A[v] *= to_f(av[k].v[v]);
+          if (s >= 0) h[v] = P.h0 && v < live ? P.h0[s * P.D + ch + v] : 0.f;
+          if (in) h[v] = fmaf(to_f(sa[k * CH + v]), h[v], to_f(sx[k * CH + v]));
+          out[v] = in ? h[v] : 0.f;
+          if (P.fin != nullptr && e >= 0 && v < live) P.fin[e * P.D + ch + v] = h[v];
+        }
+        put<float, V>(y, out, P.vec, live);
+      }
+    }
+    feed.release(st);
+    if (P.fin != nullptr)  // empty sequences, spread over the chunks
+      for (int s = (int)((int64_t)chunk * P.S / P.nchunk) + w; s < (int)((int64_t)(chunk + 1) * P.S / P.nchunk); s += kWarps)
+        if (P.cu[s + 1] <= P.cu[s])
+          for (int v = 0; v < live; ++v) P.fin[s * P.D + ch + v] = P.h0 ? P.h0[s * P.D + ch + v] : 0.f;
+    sync_workers();  // sh is free for the next item
+  }
+}
+
+template <typename T, bool TMA>
+__global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), 3)
+packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ CUtensorMap ta,
+                  const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tg) {
+  constexpr int V = kV<T>, CH = 32 * V;
+  extern __shared__ __align__(128) unsigned char dyn[];
+  __shared__ Work<V> sh;
+  Feed<T, true, TMA, 1> feed{dyn, sh, P};
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, k0 = w * kSteps;
+  if constexpr (TMA) {
+    if (threadIdx.x == 0) {
+      mbar_init(&sh.full[0], 1), mbar_init(&sh.empty[0], kWarps);
+      fence_mbar_init();
+    }
+    __syncthreads();
+    if (w == kWarps) {
+      if (lane == 0) feed.produce(&ta, &tx, &tg);
+      return;
+    }
+  }
+  for (int st;;) {
+    const int item = feed.next(st);
+    if (item < 0) break;
+    const int rank = item / P.ntile, chunk = P.nchunk - 1 - rank;
+    const int64_t ch = (int64_t)(item % P.ntile) * CH + lane * V, t0 = (int64_t)chunk * kChunk;
+    const int n = (int)min((int64_t)kChunk, P.L - t0), live = (int)min((int64_t)V, max((int64_t)0, P.D - ch));
+    const ChunkInfo info = TMA ? sh.infos[st] : P.info ? P.info[chunk] : chunk_info(P.cu, P.S, t0, n);
+    const bool plain = info.plain(w);
+    float h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = v < live && n > 0 ? P.ckpt[chunk * P.D + ch + v] : 0.f;
+    if (info.starts | info.ends) mark_borders(sh, info, P, t0, n);
+    const T *sa = feed.a(st) + k0 * CH + lane * V, *sx = feed.x(st) + k0 * CH + lane * V;
+    float* sg = feed.g(st) + k0 * CH + lane * V;
+    {
+      float A[V], B[V], C[V], Q[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) A[v] = C[v] = 1.f, B[v] = Q[v] = 0.f;
+      if (plain) {
+        // h forward, and r backward as sum of (product of the gates so far) x gy: Q = sum_k (a_0 .. a_k) gy_k
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          const Vec<T, V> av = ld_vec<T, V>(sa + k * CH), xv = ld_vec<T, V>(sx + k * CH);
+          const Vec<float, V> gv = ld_vec<float, V>(sg + k * CH);
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            B[v] = fmaf(to_f(av.v[v]), B[v], to_f(xv.v[v]));
+            A[v] *= to_f(av.v[v]);
+            Q[v] = fmaf(A[v], gv.v[v], Q[v]);
+          }
         }
 #pragma unroll
-      for (int k = kSteps - 1; k >= 0; --k)
-#pragma unroll
-        for (int v = 0; v < V; ++v) Q[v] = to_f(av[k].v[v]) * (gv[k].v[v] + Q[v]);
-#pragma unroll
-      for (int v = 0; v < V; ++v) P[v] = A[v];
-    } else {
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      const int i = k0 + k, s = bd.start[i];
-      if (i < bd.lo || i >= bd.hi) continue;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (s >= 0) B[v] = h0 && live ? h0[s * D + ch + v] : 0.f;
-        B[v] = fmaf(to_f(av[k].v[v]), B[v], to_f(xv[k].v[v]));
-        A[v] *= to_f(av[k].v[v]);
-      }
-    }
-#pragma unroll
-    for (int k = kSteps - 1; k >= 0; --k) {
-      const int i = k0 + k, e = bd.end[i];
-      if (i < bd.lo || i >= bd.hi) continue;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (e >= 0) Q[v] = gf && live ? gf[e * D + ch + v] : 0.f;
-        Q[v] = to_f(av[k].v[v]) * (gv[k].v[v] + Q[v]);
-        P[v] *= to_f(av[k].v[v]);
-      }
-    }
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      fA[w][lane * V + v] = A[v], fB[w][lane * V + v] = B[v];
-      sh.A[w][lane * V + v] = P[v], sh.B[w][lane * V + v] = Q[v];
-    }
-  }
-  __syncthreads();
-  const uint32_t cut = bd.starts, end = bd.ends;
-  // r left of warps 7 .. e, given the one right of them
-  auto through = [&](int c, int e, float& P, float& Q) {
-    for (int i = kWarps - 1; i >= e; --i) {
-      if (end >> i & 1) {
-        P = 0.f;
-        Q = sh.B[i][c];
+        for (int v = 0; v < V; ++v) C[v] = A[v];
       } else {
-        Q = fmaf(sh.A[i][c], Q, sh.B[i][c]);
-        P *= sh.A[i][c];
+        for (int k = 0; k < kSteps; ++k) {
+          const int i = k0 + k;
+          if (i < info.lo || i >= info.hi) continue;
+          const int s = start_of(sh.mark, info, i, P.S);
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            if (s >= 0) B[v] = P.h0 && v < live ? P.h0[s * P.D + ch + v] : 0.f;
+            B[v] = fmaf(to_f(sa[k * CH + v]), B[v], to_f(sx[k * CH + v])), A[v] *= to_f(sa[k * CH + v]);
+          }
+        }
+        for (int k = kSteps - 1; k >= 0; --k) {
+          const int i = k0 + k;
+          if (i < info.lo || i >= info.hi) continue;
+          const int e = end_of(sh.mark, info, i, P.S);
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            if (e >= 0) Q[v] = P.gf && v < live ? P.gf[e * P.D + ch + v] : 0.f;
+            Q[v] = to_f(sa[k * CH + v]) * (sg[k * CH + v] + Q[v]), C[v] *= to_f(sa[k * CH + v]);
+          }
+        }
       }
-    }
-  };
-  const bool need = bd.hi == n && bd.hi > bd.lo && bd.end[n - 1] < 0;
-  look_back<V>(sh, recs, D, ch, live, rank, nchunk - 1, end != 0, need, [&](int c, float& P, float& Q) {
-    P = 1.f, Q = 0.f;
-    through(c, 0, P, Q);
-  });
-  float r[V], h[V], before[kSteps][V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    float P = 1.f;
-    r[v] = sh.carry[lane * V + v];
-    through(lane * V + v, w + 1, P, r[v]);
-    h[v] = live && n > 0 ? ckpt[chunk * D + ch + v] : 0.f;
-    for (int i = 0; i < w; ++i)
-      h[v] = cut >> i & 1 ? fB[i][lane * V + v] : fmaf(fA[i][lane * V + v], h[v], fB[i][lane * V + v]);
-  }
-  if (plain) {
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k)
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        before[k][v] = h[v];
-        h[v] = fmaf(to_f(av[k].v[v]), h[v], to_f(xv[k].v[v]));
-      }
-#pragma unroll
-    for (int k = kSteps - 1; k >= 0; --k) {
-      float oa[V], ox[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        ox[v] = gv[k].v[v] + r[v];
-        oa[v] = ox[v] * before[k][v];
-        r[v] = to_f(av[k].v[v]) * ox[v];
-      }
-      if (live) {
-        st_vec<T, V>(ga + (t0 + k0 + k) * D + ch, oa);
-        st_vec<T, V>(gx + (t0 + k0 + k) * D + ch, ox);
+        sh.fA[w][lane * V + v] = A[v], sh.fB[w][lane * V + v] = B[v];
+        sh.A[w][lane * V + v] = C[v], sh.B[w][lane * V + v] = Q[v];
       }
     }
-  } else {
-#pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    const int i = k0 + k, s = bd.start[i];
+    sync_workers();
+    const bool need = info.hi == n && info.hi > info.lo && end_of(sh.mark, info, n - 1, P.S) < 0;
+    float carry[V], p[V], q[V], r[V];
+    chain<V, true>(sh, P, ch, live, rank, info.ends, need, carry, p, q);
+    const bool cut = info.ends >> (w + 1);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      if (s >= 0) h[v] = h0 && live ? h0[s * D + ch + v] : 0.f;
-      before[k][v] = h[v];
-      h[v] = fmaf(to_f(av[k].v[v]), h[v], to_f(xv[k].v[v]));
+      r[v] = enter(p[v], q[v], carry[v], cut);
+      for (int i = 0; i < w; ++i) {
+        const float A = sh.fA[i][lane * V + v], B = sh.fB[i][lane * V + v];
+        h[v] = info.starts >> i & 1 ? B : fmaf(A, h[v], B);
+      }
     }
-  }
+    T *ga = (T*)P.ga + (t0 + k0) * P.D + ch, *gx = (T*)P.gx + (t0 + k0) * P.D + ch;
+    if (plain) {
+      // right to left, adj over gy in shared memory; then left to right with h
 #pragma unroll
-  for (int k = kSteps - 1; k >= 0; --k) {
-    const int i = k0 + k;
-    if (i >= n) continue;
-    const bool in = i >= bd.lo && i < bd.hi;
-    const int s = bd.start[i], e = bd.end[i];
-    float oa[V], ox[V];
+      for (int k = kSteps - 1; k >= 0; --k) {
+        const Vec<T, V> av = ld_vec<T, V>(sa + k * CH);
+        Vec<float, V> gv = ld_vec<float, V>(sg + k * CH);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (in && e >= 0) r[v] = gf && live ? gf[e * D + ch + v] : 0.f;
-      const float adj = gv[k].v[v] + r[v];
-      oa[v] = in ? adj * before[k][v] : 0.f;
-      ox[v] = in ? adj : 0.f;
-      if (in) r[v] = to_f(av[k].v[v]) * adj;
-      if (gh0 != nullptr && in && s >= 0 && live) gh0[s * D + ch + v] = r[v];
+        for (int v = 0; v < V; ++v) {
+          gv.v[v] += r[v];
+          r[v] = to_f(av.v[v]) * gv.v[v];
+        }
+        *reinterpret_cast<Vec<float, V>*>(sg + k * CH) = gv;
+      }
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k, ga += P.D, gx += P.D) {
+        const Vec<T, V> av = ld_vec<T, V>(sa + k * CH), xv = ld_vec<T, V>(sx + k * CH);
+        const Vec<float, V> gv = ld_vec<float, V>(sg + k * CH);
+        float oa[V], ox[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          ox[v] = gv.v[v];
+          oa[v] = gv.v[v] * h[v];
+          h[v] = fmaf(to_f(av.v[v]), h[v], to_f(xv.v[v]));
+        }
+        put<T, V>(ga, oa, P.vec, live);
+        put<T, V>(gx, ox, P.vec, live);
+      }
+    } else {
+      for (int k = kSteps - 1; k >= 0; --k) {
+        const int i = k0 + k;
+        if (i < info.lo || i >= info.hi) continue;
+        const int s = start_of(sh.mark, info, i, P.S), e = end_of(sh.mark, info, i, P.S);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          if (e >= 0) r[v] = P.gf && v < live ? P.gf[e * P.D + ch + v] : 0.f;
+          const float adj = sg[k * CH + v] + r[v];
+          sg[k * CH + v] = adj;
+          r[v] = to_f(sa[k * CH + v]) * adj;
+          if (P.gh0 != nullptr && s >= 0 && v < live) P.gh0[s * P.D + ch + v] = r[v];
+        }
+      }
+      for (int k = 0; k < kSteps && k0 + k < n; ++k, ga += P.D, gx += P.D) {
+        const int i = k0 + k;
+        const bool in = i >= info.lo && i < info.hi;
+        const int s = in ? start_of(sh.mark, info, i, P.S) : -1;
+        float oa[V], ox[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          if (s >= 0) h[v] = P.h0 && v < live ? P.h0[s * P.D + ch + v] : 0.f;
+          ox[v] = in ? sg[k * CH + v] : 0.f;
+          oa[v] = in ? sg[k * CH + v] * h[v] : 0.f;
+          if (in) h[v] = fmaf(to_f(sa[k * CH + v]), h[v], to_f(sx[k * CH + v]));
+        }
+        put<T, V>(ga, oa, P.vec, live);
+        put<T, V>(gx, ox, P.vec, live);
+      }
     }
-    if (live) {
-      st_vec<T, V>(ga + (t0 + i) * D + ch, oa);
-      st_vec<T, V>(gx + (t0 + i) * D + ch, ox);
-    }
+    if constexpr (TMA) fence_proxy_async_smem();  // this thread's writes over gy before the next copy into it
+    feed.release(st);
+    if (P.gh0 != nullptr)
+      for (int s = (int)((int64_t)chunk * P.S / P.nchunk) + w; s < (int)((int64_t)(chunk + 1) * P.S / P.nchunk); s += kWarps)
+        if (P.cu[s + 1] <= P.cu[s])
+          for (int v = 0; v < live; ++v) P.gh0[s * P.D + ch + v] = P.gf ? P.gf[s * P.D + ch + v] : 0.f;
+    sync_workers();
   }
-  }
-  if (gh0 != nullptr && live)
-    for (int s = (int)((int64_t)chunk * S / nchunk) + w; s < (int)((int64_t)(chunk + 1) * S / nchunk); s += kWarps)
-      if (cu[s + 1] <= cu[s])
-#pragma unroll
-        for (int v = 0; v < V; ++v) gh0[s * D + ch + v] = gf ? gf[s * D + ch + v] : 0.f;
 }
 
 static int64_t chunks(int64_t T) { return (T + kChunk - 1) / kChunk; }
 static size_t ws_bytes_of(int64_t T, int64_t D) {
-  // a ticket counter, and a record per chunk and channel; one chunk needs neither
-  return chunks(T) > 1 ? 16 + (size_t)chunks(T) * D * sizeof(Rec) : 0;
-}
-
-static int prepare_ws(const char* what, int64_t T, int64_t D, int ntile, void* ws, size_t bytes, cudaStream_t st) {
-  const size_t need = ws_bytes_of(T, D);
-  if (need > 0 && (ws == nullptr || bytes < need || ((uintptr_t)ws & 15u)))
-    return set_error(MR_E_WORKSPACE, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", what, need, bytes);
-  if (chunks(T) * (int64_t)ntile > INT32_MAX) return set_error(MR_E_SHAPE, "%s: T * D too large", what);
-  if (need > 0) {
-    const cudaError_t e = cudaMemsetAsync(ws, 0, need, st);
-    if (e != cudaSuccess) return set_error(MR_E_LAUNCH, "%s: cudaMemsetAsync: %s", what, cudaGetErrorString(e));
-  }
-  return MR_OK;
-}
-
-// Two 2-byte channels per thread (128-byte rows per warp) where D and every
-// pointer allow it; float32 fills 128-byte rows with one.
-static bool pairs(int64_t D, std::initializer_list<const void*> half, std::initializer_list<const void*> full) {
-  bool ok = D % 2 == 0;
-  for (const void* p : half) ok = ok && ((uintptr_t)p & 3u) == 0;
-  for (const void* p : full) ok = ok && ((uintptr_t)p & 7u) == 0;
-  return ok;
+  // a ticket counter, the chunks' borders, and a record per chunk and channel; one chunk needs none
+  return chunks(T) > 1 ? 32 + (size_t)chunks(T) * (sizeof(ChunkInfo) + D * sizeof(Rec)) : 0;
 }
 
 static int packed_check(const char* what, int dtype, int64_t T, int64_t D, int64_t S) {
@@ -497,26 +666,54 @@ static int packed_check(const char* what, int dtype, int64_t T, int64_t D, int64
   return MR_OK;
 }
 
-template <typename T, int V>
-static int fwd_launch(const void* a, const void* x, const int* cu, int64_t S, int64_t L, int64_t D, const float* h0,
-                      float* y, float* ckpt, float* fin, void* ws, size_t wsb, cudaStream_t st) {
-  const int ntile = (int)((D + 32 * V - 1) / (32 * V)), nchunk = (int)(L > 0 ? chunks(L) : 1);
-  if (int rc = prepare_ws("mr_rglru_packed_fwd", L, D, ntile, ws, wsb, st)) return rc;
-  packed_fwd_kernel<T, V><<<(unsigned)(nchunk * ntile), kWarps * 32, 0, st>>>(
-      (const T*)a, (const T*)x, cu, (int)S, L, D, h0, y, ckpt, fin, nchunk > 1 ? (uint32_t*)ws : nullptr,
-      (Rec*)((char*)ws + 16), nchunk, ntile);
-  return check_launch("packed_fwd_kernel");
+static int prepare_ws(const char* what, PackedArgs& P, void* ws, size_t bytes, cudaStream_t st) {
+  const size_t need = ws_bytes_of(P.L, P.D);
+  if (need > 0 && (ws == nullptr || bytes < need || ((uintptr_t)ws & 15u)))
+    return set_error(MR_E_WORKSPACE, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", what, need, bytes);
+  if (chunks(P.L) * (int64_t)P.ntile > INT32_MAX / 2) return set_error(MR_E_SHAPE, "%s: T * D too large", what);
+  if (need == 0) return MR_OK;
+  P.counter = (uint32_t*)ws;
+  ChunkInfo* info = (ChunkInfo*)((char*)ws + 32);
+  P.info = info;
+  P.recs = (Rec*)(info + P.nchunk);
+  const int64_t nrec = P.nchunk * P.D, blocks = (nrec + 1023) / 1024;
+  packed_prep_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, st>>>(
+      P.cu, P.S, P.L, P.nchunk, (uint4*)ws, info, (uint4*)P.recs, nrec);
+  return check_launch("packed_prep_kernel");
 }
-template <typename T, int V>
-static int bwd_launch(const float* gy, const float* gf, const float* ckpt, const void* a, const void* x,
-                      const int* cu, int64_t S, int64_t L, int64_t D, const float* h0, void* ga, void* gx, float* gh0,
-                      void* ws, size_t wsb, cudaStream_t st) {
-  const int ntile = (int)((D + 32 * V - 1) / (32 * V)), nchunk = (int)(L > 0 ? chunks(L) : 1);
-  if (int rc = prepare_ws("mr_rglru_packed_bwd", L, D, ntile, ws, wsb, st)) return rc;
-  packed_bwd_kernel<T, V><<<(unsigned)(nchunk * ntile), kWarps * 32, 0, st>>>(
-      gy, gf, ckpt, (const T*)a, (const T*)x, cu, (int)S, L, D, h0, (T*)ga, (T*)gx, gh0,
-      nchunk > 1 ? (uint32_t*)ws : nullptr, (Rec*)((char*)ws + 16), nchunk, ntile);
-  return check_launch("packed_bwd_kernel");
+
+constexpr int kCtas = 148 * 3;  // three per SM
+
+template <typename T, bool BWD> static int launch(const char* what, PackedArgs P, void* ws, size_t wsb, cudaStream_t st) {
+  constexpr int V = kV<T>, e = sizeof(T);
+  P.ntile = (int)((P.D + 32 * V - 1) / (32 * V));
+  P.nchunk = (int)(P.L > 0 ? chunks(P.L) : 1);
+  if (int rc = prepare_ws(what, P, ws, wsb, st)) return rc;
+  auto at = [](const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; };
+  P.vec = P.D % V == 0 && (BWD ? at(P.ga, 4) && at(P.gx, 4) && at(P.gy, 4 * V) : at(P.y, 4 * V)) && at(P.a, 4) && at(P.x, 4);
+  // the copies take rows that are multiples of 16 bytes, 16-byte aligned
+  const bool tma = P.L > 0 && P.D * e % 16 == 0 && at(P.a, 16) && at(P.x, 16) && (!BWD || at(P.gy, 16));
+  const int64_t items = (int64_t)P.nchunk * P.ntile;
+  const unsigned grid = (unsigned)(P.counter && items > kCtas ? kCtas : items);
+  const int smem = kStage<T, BWD> * (BWD || !tma ? 1 : 2);
+  CUtensorMap ta, tx, tg;
+  if (tma) {
+    if (int rc = make_tmap_2d(&ta, P.a, TmapType<T>::v, e, P.D, P.L, P.D * e, 32 * V, kChunk)) return rc;
+    if (int rc = make_tmap_2d(&tx, P.x, TmapType<T>::v, e, P.D, P.L, P.D * e, 32 * V, kChunk)) return rc;
+    if (BWD)
+      if (int rc = make_tmap_2d(&tg, P.gy, TmapType<float>::v, 4, P.D, P.L, P.D * 4, 32 * V, kChunk)) return rc;
+  }
+  auto go = [&](auto kernel, int threads, auto... maps) {
+    const cudaError_t er = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (er != cudaSuccess) return set_error(MR_E_LAUNCH, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(er));
+    kernel<<<grid, threads, smem, st>>>(P, maps...);
+    return check_launch(what);
+  };
+  if constexpr (BWD) {
+    return tma ? go(packed_bwd_kernel<T, true>, kWarps * 32 + 32, ta, tx, tg) : go(packed_bwd_kernel<T, false>, kWarps * 32, ta, tx, tg);
+  } else {
+    return tma ? go(packed_fwd_kernel<T, true>, kWarps * 32 + 32, ta, tx) : go(packed_fwd_kernel<T, false>, kWarps * 32, ta, tx);
+  }
 }
 
 int packed_device_error(bool clear) { return read_device_error(clear); }
@@ -539,15 +736,15 @@ int mr_rglru_packed_fwd(const void* a, const void* x, const int32_t* cu_seqlens,
   if (T == 0 && S == 0) return MR_OK;
   if (cu_seqlens == nullptr || (T > 0 && (a == nullptr || x == nullptr || y == nullptr)))
     return set_error(MR_E_ALIGN, "%s: a pointer is NULL", what);
+  PackedArgs P{};
+  P.cu = cu_seqlens, P.S = (int)S, P.L = T, P.D = D, P.h0 = h0, P.y = y, P.ckpt = ckpt, P.fin = final_state;
+  P.a = a, P.x = x;
   const cudaStream_t st = (cudaStream_t)stream;
-  const bool two = pairs(D, {a, x}, {y});
-#define MR_CALL(T_, V_) fwd_launch<T_, V_>(a, x, cu_seqlens, S, T, D, h0, y, ckpt, final_state, ws, ws_bytes, st)
   switch (dtype) {
-    case MR_F32: return MR_CALL(float, 1);
-    case MR_BF16: return two ? MR_CALL(__nv_bfloat16, 2) : MR_CALL(__nv_bfloat16, 1);
-    default: return two ? MR_CALL(__half, 2) : MR_CALL(__half, 1);
+    case MR_F32: return launch<float, false>(what, P, ws, ws_bytes, st);
+    case MR_BF16: return launch<__nv_bfloat16, false>(what, P, ws, ws_bytes, st);
+    default: return launch<__half, false>(what, P, ws, ws_bytes, st);
   }
-#undef MR_CALL
 }
 
 int mr_rglru_packed_bwd(const float* grad_y, const float* grad_final, const float* ckpt, const void* a, const void* x,
@@ -559,17 +756,15 @@ int mr_rglru_packed_bwd(const float* grad_y, const float* grad_final, const floa
   if (cu_seqlens == nullptr || (T > 0 && (a == nullptr || x == nullptr || grad_y == nullptr || ckpt == nullptr ||
                                           grad_a == nullptr || grad_x == nullptr)))
     return set_error(MR_E_ALIGN, "%s: a pointer is NULL", what);
+  PackedArgs P{};
+  P.cu = cu_seqlens, P.S = (int)S, P.L = T, P.D = D, P.h0 = h0, P.gy = grad_y, P.gf = grad_final;
+  P.ckpt = const_cast<float*>(ckpt), P.gh0 = grad_h0, P.a = a, P.x = x, P.ga = grad_a, P.gx = grad_x;
   const cudaStream_t st = (cudaStream_t)stream;
-  const bool two = pairs(D, {a, x, grad_a, grad_x}, {grad_y});
-#define MR_CALL(T_, V_)                                                                                         \
-  bwd_launch<T_, V_>(grad_y, grad_final, ckpt, a, x, cu_seqlens, S, T, D, h0, grad_a, grad_x, grad_h0, ws, ws_bytes, \
-                     st)
   switch (dtype) {
-    case MR_F32: return MR_CALL(float, 1);
-    case MR_BF16: return two ? MR_CALL(__nv_bfloat16, 2) : MR_CALL(__nv_bfloat16, 1);
-    default: return two ? MR_CALL(__half, 2) : MR_CALL(__half, 1);
+    case MR_F32: return launch<float, true>(what, P, ws, ws_bytes, st);
+    case MR_BF16: return launch<__nv_bfloat16, true>(what, P, ws, ws_bytes, st);
+    default: return launch<__half, true>(what, P, ws, ws_bytes, st);
   }
-#undef MR_CALL
 }
 
 }  // extern "C"
