@@ -6,6 +6,7 @@ namespace mr {
 
 template <typename T> int attn_fwd_simt(const AttnArgs&, cudaStream_t);
 template <typename T> int attn_bwd_simt(const AttnArgs&, cudaStream_t);
+template <typename T> int attn_fwd_launch(const AttnArgs&, cudaStream_t);
 
 static int attn_check(const char* what, const AttnArgs& A, int64_t S, int64_t L, int dtype, int64_t T, int64_t Hq,
                       int64_t Hkv, int64_t Dh, int64_t window, int64_t sinks) {
@@ -71,8 +72,8 @@ int mr_window_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ts
   const cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
     case MR_F32: return attn_fwd_simt<float>(A, st);
-    case MR_BF16: return attn_fwd_simt<__nv_bfloat16>(A, st);
-    default: return attn_fwd_simt<__half>(A, st);
+    case MR_BF16: return attn_fwd_launch<__nv_bfloat16>(A, st);
+    default: return attn_fwd_launch<__half>(A, st);
   }
 }
 

@@ -1,0 +1,277 @@
+// Sliding-window attention with sinks, forward, on the tensor cores (tcgen05):
+// bf16 and fp16, Dh <= 128.
+//
+// A CTA takes 128 queries of one head and walks the keys they may see in tiles
+// of 128: S = Q K^T into TMEM, the online softmax by four warps (one thread per
+// query, so no reduction across threads), P back into TMEM over S as the A
+// operand of O += P V. The row's maximum is only moved when it grows by more
+// than 2^8 (the factor cancels in O / l), so O is rarely rescaled. A fifth warp's
+// first thread issues copies and products; a CTA's steps depend on each other,
+// and the second CTA of the SM fills the gaps (256 TMEM columns and at most 96 KB
+// of shared memory each).
+//
+// TMEM columns: S (P over it, two elements a column) at 0, O at 128.
+#include "window_attn.cuh"
+
+#include "tma.cuh"
+#include "tmap.cuh"
+#include "umma.cuh"
+
+namespace mr {
+
+constexpr int kTileBytes = 16384;  // [128 rows][64 2-byte elements], 128-byte swizzle
+constexpr int kFwdThreads = 160;
+constexpr float kRescale = 8.f;
+
+template <typename T> struct Fmt;
+template <> struct Fmt<__nv_bfloat16> {
+  static constexpr int id = 1;
+  static __device__ uint32_t pack(float a, float b) {
+    __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&r);
+  }
+};
+template <> struct Fmt<__half> {
+  static constexpr int id = 0;
+  static __device__ uint32_t pack(float a, float b) {
+    __half2 r = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&r);
+  }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// bits [a, b) of a 32-bit word, whatever the bounds
+__device__ __forceinline__ uint32_t bits(int a, int b) {
+  const uint32_t hi = b >= 32 ? 0xffffffffu : b <= 0 ? 0u : (1u << b) - 1;
+  const uint32_t lo = a >= 32 ? 0xffffffffu : a <= 0 ? 0u : (1u << a) - 1;
+  return hi & ~lo;
+}
+
+struct FwdShared {
+  uint64_t k_full, v_full, s_done, p_ready, o_done;
+  uint32_t tmem;
+  int lo_max;  // the largest first key of the tile's queries
+  uint32_t again[4];
+};
+
+template <typename T, int NB>  // NB = 64-wide blocks of a row
+__global__ void __launch_bounds__(kFwdThreads, 2)
+attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap tq,
+                const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
+  extern __shared__ unsigned char raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  unsigned char *sQ = sm, *sK = sQ + NB * kTileBytes, *sV = sK + NB * kTileBytes;
+  __shared__ FwdShared sh;
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int h = blockIdx.y, hk = h / (A.Hq / A.Hkv), q0 = blockIdx.x * 128, i = q0 + tid;
+  const KeyRange R = keys_of(A, q0, q0 + 128);
+  const int nsink = R.send > R.s0 ? 1 : 0;  // at most 64 sinks: one tile
+  const int ntile = R.kend > R.kmin ? nsink + (R.kend - R.kmin + 127) / 128 : 0;
+  T* y = (T*)A.y + ((int64_t)i * A.Hq + h) * A.Dh;
+  if (ntile == 0) {  // no sequence reaches this tile
+    if (tid < 128 && i < A.T) {
+      for (int d = 0; d < A.Dh; d += 8) *reinterpret_cast<int4*>(y + d) = make_int4(0, 0, 0, 0);
+      if (A.lse != nullptr) A.lse[(int64_t)h * A.T + i] = INFINITY;
+    }
+    return;
+  }
+  if (tid == 0) {
+    mbar_init(&sh.k_full, 1), mbar_init(&sh.v_full, 1), mbar_init(&sh.s_done, 1), mbar_init(&sh.o_done, 1);
+    mbar_init(&sh.p_ready, 128);
+    fence_mbar_init();
+    sh.lo_max = 0;
+  }
+  if (w == 4) {
+    umma::tmem_alloc(&sh.tmem, 256);
+    umma::tmem_relinquish();
+  }
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  const uint32_t tm = sh.tmem;
+  // the sink tile has few keys: products and softmax take whole 16 (32) column groups of it
+  const int sink_n = nsink ? (R.send - R.s0 + 15) & ~15 : 0;
+
+  if (w == 4) {
+    if (lane == 0) {
+      const uint32_t aq = smem_u32(sQ), ak = smem_u32(sK), av = smem_u32(sV);
+      auto load = [&](const CUtensorMap* m, unsigned char* dst, int head, int row, uint64_t* bar) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) tma_load_3d(dst + b * kTileBytes, m, b * 64, head, row, bar);
+      };
+      auto key0 = [&](int t) { return t < nsink ? R.s0 : R.kmin + (t - nsink) * 128; };
+      mbar_arrive_expect_tx(&sh.k_full, 2 * NB * kTileBytes);
+      load(&tq, sQ, h, q0, &sh.k_full);
+      load(&tk, sK, hk, key0(0), &sh.k_full);
+      mbar_arrive_expect_tx(&sh.v_full, NB * kTileBytes);
+      load(&tv, sV, hk, key0(0), &sh.v_full);
+      for (int t = 0; t < ntile; ++t) {
+        const int n = t < nsink ? sink_n : 128;
+        mbar_wait(&sh.k_full, t & 1);
+        const uint32_t ids = umma::idesc_f16(128, n, Fmt<T>::id, 0, 0);
+        for (int k = 0; k < A.Dh / 16; ++k) {
+          const uint32_t o = (k >> 2) * kTileBytes + (k & 3) * 32;
+          umma::mma_f16(tm, umma::sdesc_k(aq + o), umma::sdesc_k(ak + o), ids, k > 0);
+        }
+        umma::commit(&sh.s_done);
+        mbar_wait(&sh.s_done, t & 1);
+        if (t + 1 < ntile) {
+          mbar_arrive_expect_tx(&sh.k_full, NB * kTileBytes);
+          load(&tk, sK, hk, key0(t + 1), &sh.k_full);
+        }
+        mbar_wait(&sh.v_full, t & 1);
+        mbar_wait(&sh.p_ready, t & 1);
+        umma::fence_after_sync();
+        const uint32_t ido = umma::idesc_f16(128, A.Dh, Fmt<T>::id, 0, 1);
+        for (int k = 0; k < n / 16; ++k)
+          umma::mma_f16_ta(tm + 128, tm + k * 8, umma::sdesc_mn(av + k * 2048, kTileBytes), ido, t > 0 || k > 0);
+        umma::commit(&sh.o_done);
+        mbar_wait(&sh.o_done, t & 1);  // P is read (the next S overwrites it) and V too
+        if (t + 1 < ntile) {
+          mbar_arrive_expect_tx(&sh.v_full, NB * kTileBytes);
+          load(&tv, sV, hk, key0(t + 1), &sh.v_full);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    const RowMask rm = row_mask(A, i);
+    const int lo = rm.i < 0 ? 0 : rm.lo;
+    atomicMax(&sh.lo_max, __reduce_max_sync(0xffffffffu, lo));
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    const int lo_max = sh.lo_max, end = end_token(A);
+    const uint32_t trow = tm + ((uint32_t)(w * 32) << 16);
+    const float c = A.scale * kAttnLog2e;
+    float m = -INFINITY, l = 0.f;
+    for (int t = 0; t < ntile; ++t) {
+      const bool sink = t < nsink;
+      const int k0 = sink ? R.s0 : R.kmin + (t - nsink) * 128;
+      const int nch = sink ? (sink_n + 31) / 32 : 4;
+      // every query of the tile sees every key of a tile between the last window's start and the first query
+      const bool full = !sink && k0 >= lo_max && k0 + 127 <= q0;
+      mbar_wait(&sh.s_done, t & 1);
+      umma::fence_after_sync();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (b < nch) umma::tmem_ld32(trow + b * 32, s[b]);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        if (b >= nch) continue;
+        umma::tmem_wait_ld(s[b]);
+        if (!full) {
+          const int at = k0 + b * 32;
+          uint32_t see = bits(rm.start - at, min(min(rm.sink_end, rm.i + 1), sink ? R.send : INT32_MAX) - at);
+          if (!sink) see |= bits(rm.lo - at, rm.i + 1 - at);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) s[b][j] = see >> j & 1 ? s[b][j] : 0xff800000u;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(s[b][j]));
+      }
+      if (__any_sync(0xffffffffu, (mx - m) * c > kRescale || m == -INFINITY)) {
+        const float to = fmaxf(mx, m);
+        const float f = to == -INFINITY ? 1.f : ex2((m - to) * c);
+        m = to, l *= f;
+        if (t > 0)
+          for (int d = 0; d < A.Dh; d += 32) {
+            uint32_t o[32];
+            umma::tmem_ld32(trow + 128 + d, o);
+            umma::tmem_wait_ld(o);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+            umma::tmem_st32(trow + 128 + d, o);
+          }
+      }
+      const float mc = m == -INFINITY ? 0.f : m * c;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        if (b >= nch) continue;
+        uint32_t p[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float e0 = ex2(fmaf(__uint_as_float(s[b][2 * j]), c, -mc));
+          const float e1 = ex2(fmaf(__uint_as_float(s[b][2 * j + 1]), c, -mc));
+          sum[(2 * j) & 3] += e0, sum[(2 * j + 1) & 3] += e1;
+          p[j] = Fmt<T>::pack(e0, e1);
+        }
+        umma::tmem_st16(trow + b * 16, p);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      if (k0 + 128 > end) {  // rows behind the last sequence may hold anything: 0 x NaN would reach O
+        mbar_wait(&sh.v_full, t & 1);
+        if (k0 + tid >= end)
+#pragma unroll
+          for (int b = 0; b < NB * 8; ++b)
+            *reinterpret_cast<int4*>(sV + (b >> 3) * kTileBytes + tid * 128 + (b & 7) * 16) = make_int4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+      }
+      umma::tmem_wait_st();
+      umma::fence_before_sync();
+      mbar_arrive(&sh.p_ready);
+    }
+    mbar_wait(&sh.o_done, (ntile - 1) & 1);
+    umma::fence_after_sync();
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    float odd = 0.f;  // NaN as soon as one element is not finite
+    for (int d = 0; d < A.Dh; d += 32) {
+      uint32_t o[32];
+      umma::tmem_ld32(trow + 128 + d, o);
+      umma::tmem_wait_ld(o);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) odd = fmaf(__uint_as_float(o[j]), 0.f, odd);
+      if (i < A.T)
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+          uint32_t p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            p[e] = rm.i < 0 ? 0u : Fmt<T>::pack(__uint_as_float(o[j + 2 * e]) * inv, __uint_as_float(o[j + 2 * e + 1]) * inv);
+          *reinterpret_cast<uint4*>(y + d + j) = make_uint4(p[0], p[1], p[2], p[3]);
+        }
+    }
+    if (i < A.T && A.lse != nullptr) A.lse[(int64_t)h * A.T + i] = rm.i < 0 || l == 0.f ? INFINITY : m * c + log2f(l);
+    const uint32_t again = __ballot_sync(0xffffffffu, rm.i >= 0 && odd != 0.f);
+    __syncwarp();
+    for (int r = 0; r < 32 && again; ++r)
+      if (again >> r & 1) exact_fwd_row<T>(A, h, q0 + w * 32 + r);
+    umma::fence_before_sync();
+  }
+  __syncthreads();
+  if (w == 4) umma::tmem_dealloc(tm, 256);
+}
+
+static int head_map(CUtensorMap* m, const void* p, CUtensorMapDataType dt, const AttnArgs& A, int H, int64_t ts, int64_t hs) {
+  // [T, H, Dh] as (Dh, H, T); columns at and behind Dh and rows behind T read as zero
+  return make_tmap_3d(m, p, dt, 2, A.Dh, H, A.T, hs * 2, ts * 2, 64, 1, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <typename T, int NB> static int fwd_nb(const AttnArgs& A, cudaStream_t st) {
+  CUtensorMap tq, tk, tv;
+  constexpr auto dt = TmapType<T>::v;
+  if (int rc = head_map(&tq, A.q, dt, A, A.Hq, A.q_ts, A.q_hs)) return rc;
+  if (int rc = head_map(&tk, A.k, dt, A, A.Hkv, A.k_ts, A.k_hs)) return rc;
+  if (int rc = head_map(&tv, A.v, dt, A, A.Hkv, A.v_ts, A.v_hs)) return rc;
+  constexpr int smem = 3 * NB * kTileBytes + 1024;
+  const cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return set_error(MR_E_LAUNCH, "attn_fwd_kernel: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  attn_fwd_kernel<T, NB><<<dim3((A.T + 127) / 128, A.Hq), kFwdThreads, smem, st>>>(A, tq, tk, tv);
+  return check_launch("attn_fwd_kernel");
+}
+
+template <typename T> int attn_fwd_launch(const AttnArgs& A, cudaStream_t st) {
+  return A.Dh <= 64 ? fwd_nb<T, 1>(A, st) : fwd_nb<T, 2>(A, st);
+}
+template int attn_fwd_launch<__nv_bfloat16>(const AttnArgs&, cudaStream_t);
+template int attn_fwd_launch<__half>(const AttnArgs&, cudaStream_t);
+
+int attn_fwd_device_error(bool clear) { return read_device_error(clear); }
+
+}  // namespace mr
