@@ -60,6 +60,7 @@ int selftest_device_error(bool clear);
 int ssdc_device_error(bool clear);
 int packed_device_error(bool clear);
 int attn_fwd_device_error(bool clear);
+int attn_bwd_device_error(bool clear);
 bool ssd_chunk_supported(int dtype, int64_t L, int64_t Dh, int64_t N, int64_t seg, int64_t a_stride_n);
 bool ssd_chunk_bwd_supported(int dtype, int64_t L, int64_t Dh, int64_t N, int64_t seg, int64_t a_stride_n);
 int ssd_chunk_len();
@@ -164,7 +165,7 @@ uint64_t mr_launch_count(void) { return g_launches.load(std::memory_order_relaxe
 int mr_device_error_status(int clear) {
   const int words[] = {diag_device_error(clear != 0), selftest_device_error(clear != 0),
                        ssdc_device_error(clear != 0), packed_device_error(clear != 0),
-                       attn_fwd_device_error(clear != 0)};
+                       attn_fwd_device_error(clear != 0), attn_bwd_device_error(clear != 0)};
   int r = 0;
   for (int w : words) {
     if (w < 0) return -1;

@@ -7,6 +7,8 @@ namespace mr {
 template <typename T> int attn_fwd_simt(const AttnArgs&, cudaStream_t);
 template <typename T> int attn_bwd_simt(const AttnArgs&, cudaStream_t);
 template <typename T> int attn_fwd_launch(const AttnArgs&, cudaStream_t);
+template <typename T> int attn_bwd_launch(const AttnArgs&, void*, cudaStream_t);
+size_t attn_bwd_ws_bytes(int64_t T, int64_t Hq, int64_t Dh, int64_t sinks);
 
 static int attn_check(const char* what, const AttnArgs& A, int64_t S, int64_t L, int dtype, int64_t T, int64_t Hq,
                       int64_t Hkv, int64_t Dh, int64_t window, int64_t sinks) {
@@ -79,7 +81,7 @@ int mr_window_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ts
 
 size_t mr_window_attn_bwd_workspace_bytes(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t sinks) {
   if (T <= 0 || Hq <= 0 || Hkv <= 0 || Dh <= 0 || sinks < 0) return 0;
-  return (size_t)T * Hq * 4;
+  return dtype == MR_F32 ? (size_t)T * Hq * 4 : attn_bwd_ws_bytes(T, Hq, Dh, sinks);
 }
 
 int mr_window_attn_bwd(const void* grad_y, const void* y, const float* lse, const void* q, const void* k,
@@ -101,8 +103,8 @@ int mr_window_attn_bwd(const void* grad_y, const void* y, const float* lse, cons
   const cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
     case MR_F32: return attn_bwd_simt<float>(A, st);
-    case MR_BF16: return attn_bwd_simt<__nv_bfloat16>(A, st);
-    default: return attn_bwd_simt<__half>(A, st);
+    case MR_BF16: return attn_bwd_launch<__nv_bfloat16>(A, workspace, st);
+    default: return attn_bwd_launch<__half>(A, workspace, st);
   }
 }
 

@@ -1,0 +1,528 @@
+// Sliding-window attention with sinks, backward, on the tensor cores (tcgen05):
+// bf16 and fp16, Dh <= 128. No atomics: every sum has one order.
+//
+//   p_ij = exp(scale q_i.k_j - lse_i),  ds_ij = p_ij (gy_i.v_j - delta_i)
+//   grad_q = scale ds K,  grad_k = scale ds^T Q,  grad_v = p^T gy
+//
+// One kernel, twice: rows of a tile (128, resident in shared memory) against a
+// stream of 64-wide column tiles.
+//   KV = false: rows are queries, columns the keys they see; grad_q.
+//   KV = true:  rows are keys, columns the queries that see them, over every
+//               query head that shares the key head; grad_k, grad_v.
+// Per column tile S = R1 C1^T and dP = R2 C2^T land in TMEM, a warpgroup (a
+// thread per row) turns them into P and dS, written back over them as the A
+// operands of the sums dS C1 and P C2, which stay in TMEM. That is 7 products
+// where one pass with atomic sums would need 5.
+//
+// Dh <= 64: one warpgroup, 256 TMEM columns, two CTAs per SM fill each other's
+// gaps. Dh > 64: the sums take 256 columns, so one CTA with two warpgroups on
+// alternating column tiles.
+//
+// Sinks: a key that stays visible to the end of a long sequence would make its
+// row tile walk every later query. Instead a query tile whose window has left the
+// sinks (that is, whose band of keys starts behind them) adds their gradients on
+// the way: products over its 128 queries, with P and dS handed through shared
+// memory, written as float32 partials [query tile][head][k, v][sink][Dh]; a small
+// kernel sums them in order, and the row tile of the sink adds the sum.
+#include "window_tc.cuh"
+
+namespace mr {
+
+constexpr int kNC = 64;                  // columns of a tile
+constexpr int kColBytes = kNC * 128;     // one 64-wide block of a column tile
+constexpr int kStages = 3;               // column tiles in shared memory
+
+struct BwdArgs {
+  AttnArgs a;
+  float* part;           // sink partials, or NULL
+  const uint32_t* amax;  // fp16: the largest finite |gy| as float bits
+};
+
+// A query tile n (128 queries) is far from key j of its own sequence when 128 n >= j + window.
+__device__ __forceinline__ int first_far(const AttnArgs& A, int j) { return (int)(((int64_t)j + A.window + 127) >> 7); }
+
+__device__ __forceinline__ int64_t part_at(const AttnArgs& A, int n, int h, int kv, int r) {
+  return ((((int64_t)n * A.Hq + h) * 2 + kv) * A.sinks + r) * A.Dh;
+}
+
+// fp16 keeps dS near one: a power of two of the size of gy comes out of it and back in at the end
+template <typename T> __device__ __forceinline__ float ds_factor(const uint32_t*) { return 1.f; }
+template <> __device__ __forceinline__ float ds_factor<__half>(const uint32_t* amax) {
+  const uint32_t e = *amax >> 23;  // 0 for gy = 0
+  return e == 0 || e > 250 ? 1.f : __uint_as_float((254 - e) << 23);
+}
+
+struct BwdShared {
+  uint64_t r_full, c_full[kStages], s_done[2], dp_done[2], p_ready[2], acc_done, all_done, sink_done, sink_read;
+  uint32_t tmem;
+  int lo_max, lim_min;
+  int again[128];
+  float lse[2][kNC], delta[2][kNC];
+};
+
+template <typename T, int NB, bool KV>
+__global__ void __launch_bounds__(NB == 1 ? 160 : 288, NB == 1 ? 2 : 1)
+attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUtensorMap tr1,
+                const __grid_constant__ CUtensorMap tr2, const __grid_constant__ CUtensorMap tc1,
+                const __grid_constant__ CUtensorMap tc2) {
+  constexpr int NS = NB;  // warpgroups, and TMEM stages
+  constexpr int kStageBytes = 2 * NB * kColBytes;
+  constexpr uint32_t kAcc1 = NS * 128, kAcc2 = kAcc1 + NB * 64, kCols = NB == 1 ? 256 : 512;
+  extern __shared__ unsigned char raw[];
+  unsigned char* sC = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  unsigned char *sR1 = sC + kStages * kStageBytes, *sR2 = sR1 + NB * kTileBytes;
+  __shared__ BwdShared sh;
+  const AttnArgs& A = P.a;
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, G = A.Hq / A.Hkv;
+  const int hr = blockIdx.y, hk = KV ? hr : hr / G, r0 = blockIdx.x * 128;
+  const int first = first_token(A), end = end_token(A);
+
+  // the columns: keys (a sink tile, then the band) or queries, per query head
+  int c_beg = 0, c_end = 0, s0 = 0, send = 0;
+  if (KV) {
+    const int f = max(r0, first), e = min(r0 + 128, end);
+    if (f < e) {
+      const SeqRange s = seq_of(A, e - 1);
+      c_beg = f;
+      c_end = min(s.end, e - 1 + A.window);
+      const int last_sink = min(e - 1, s.start + A.sinks - 1);
+      if (last_sink >= max(f, s.start)) c_end = max(c_end, (int)min((int64_t)s.end, (int64_t)first_far(A, last_sink) * 128));
+      c_end = max(c_end, e);
+    }
+  } else {
+    const KeyRange R = keys_of(A, r0, r0 + 128);
+    c_beg = R.kmin, c_end = R.kend, s0 = R.s0, send = R.send;
+  }
+  const int nsink = send > s0 ? 1 : 0, per = (c_end - c_beg + kNC - 1) / kNC;
+  const int n = c_end > c_beg ? (KV ? G * per : nsink + per) : 0;
+  const int H = KV ? A.Hkv : A.Hq;
+  if (n == 0) {
+    if (tid < 128 && r0 + tid < A.T) {
+      const int64_t at = ((int64_t)(r0 + tid) * H + hr) * A.Dh;
+      for (int d = 0; d < A.Dh; d += 8) {
+        *reinterpret_cast<int4*>((T*)(KV ? A.gk : A.gq) + at + d) = make_int4(0, 0, 0, 0);
+        if (KV) *reinterpret_cast<int4*>((T*)A.gv + at + d) = make_int4(0, 0, 0, 0);
+      }
+    }
+    return;
+  }
+  auto col0 = [&](int t) { return KV ? c_beg + t % per * kNC : t < nsink ? s0 : c_beg + (t - nsink) * kNC; };
+
+  if (tid == 0) {
+    mbar_init(&sh.r_full, 1);
+    for (int i = 0; i < kStages; ++i) mbar_init(&sh.c_full[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&sh.s_done[i], 1), mbar_init(&sh.dp_done[i], 1), mbar_init(&sh.p_ready[i], 128);
+    mbar_init(&sh.acc_done, 1), mbar_init(&sh.all_done, 1), mbar_init(&sh.sink_done, 1), mbar_init(&sh.sink_read, 128);
+    fence_mbar_init();
+    sh.lo_max = 0, sh.lim_min = INT32_MAX;
+  }
+  if (tid < 128) sh.again[tid] = 0;
+  if (w == 4 * NS) {
+    umma::tmem_alloc(&sh.tmem, kCols);
+    umma::tmem_relinquish();
+  }
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  const uint32_t tm = sh.tmem;
+
+  if (w == 4 * NS) {
+    if (lane == 0) {
+      const uint32_t ar1 = smem_u32(sR1), ar2 = smem_u32(sR2), ac = smem_u32(sC);
+      auto load_c = [&](int t) {
+        const int st = t % kStages, hc = KV ? hr * G + t / per : hk;
+        unsigned char* dst = sC + st * kStageBytes;
+        mbar_arrive_expect_tx(&sh.c_full[st], kStageBytes);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          tma_load_3d(dst + b * kColBytes, &tc1, b * 64, hc, col0(t), &sh.c_full[st]);
+          tma_load_3d(dst + (NB + b) * kColBytes, &tc2, b * 64, hc, col0(t), &sh.c_full[st]);
+        }
+      };
+      const uint32_t id_s = umma::idesc_f16(128, kNC, Fmt<T>::id, 0, 0);
+      const uint32_t id_a = umma::idesc_f16(128, A.Dh, Fmt<T>::id, 0, 1);
+      auto issue_s = [&](int t) {
+        const int b = t % NS;
+        const uint32_t c1 = ac + t % kStages * kStageBytes, c2 = c1 + NB * kColBytes, d = tm + b * 128;
+        mbar_wait(&sh.c_full[t % kStages], (t / kStages) & 1);
+        umma::fence_after_sync();
+        for (int k = 0; k < A.Dh / 16; ++k) {
+          const uint32_t o = (k & 3) * 32;
+          umma::mma_f16(d, umma::sdesc_k(ar1 + (k >> 2) * kTileBytes + o), umma::sdesc_k(c1 + (k >> 2) * kColBytes + o), id_s, k > 0);
+        }
+        umma::commit(&sh.s_done[b]);
+        for (int k = 0; k < A.Dh / 16; ++k) {
+          const uint32_t o = (k & 3) * 32;
+          umma::mma_f16(d + 64, umma::sdesc_k(ar2 + (k >> 2) * kTileBytes + o), umma::sdesc_k(c2 + (k >> 2) * kColBytes + o), id_s, k > 0);
+        }
+        umma::commit(&sh.dp_done[b]);
+      };
+      auto issue_acc = [&](int t) {
+        const int b = t % NS;
+        const uint32_t c1 = ac + t % kStages * kStageBytes, c2 = c1 + NB * kColBytes, d = tm + b * 128;
+        mbar_wait(&sh.p_ready[b], (t / NS) & 1);
+        umma::fence_after_sync();
+        if (KV)
+          for (int k = 0; k < kNC / 16; ++k)
+            umma::mma_f16_ta(tm + kAcc2, d + k * 8, umma::sdesc_mn(c2 + k * 2048, kColBytes), id_a, t > 0 || k > 0);
+        for (int k = 0; k < kNC / 16; ++k)
+          umma::mma_f16_ta(tm + kAcc1, d + 64 + k * 8, umma::sdesc_mn(c1 + k * 2048, kColBytes), id_a, t > 0 || k > 0);
+        umma::commit(&sh.acc_done);
+      };
+      mbar_arrive_expect_tx(&sh.r_full, 2 * NB * kTileBytes);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        tma_load_3d(sR1 + b * kTileBytes, &tr1, b * 64, hr, r0, &sh.r_full);
+        tma_load_3d(sR2 + b * kTileBytes, &tr2, b * 64, hr, r0, &sh.r_full);
+      }
+      load_c(0);
+      if (nsink == 0)
+        for (int t = 1; t < min(n, kStages); ++t) load_c(t);
+      mbar_wait(&sh.r_full, 0);
+      issue_s(0);
+      if (nsink) {
+        // the sink tile by itself: its sums over the queries use the other stages' memory and columns
+        issue_acc(0);
+        mbar_wait(&sh.acc_done, 0);
+        const uint32_t id_t = umma::idesc_f16(128, A.Dh, Fmt<T>::id, 1, 1);  // rows at and behind 64 are not used
+        const uint32_t pt = ac + kStageBytes, dst = pt + kTileBytes;
+        for (int k = 0; k < 8; ++k)
+          umma::mma_f16(tm + kAcc2, umma::sdesc_mn(pt + k * 2048, kTileBytes), umma::sdesc_mn(ar2 + k * 2048, kTileBytes), id_t, k > 0);
+        for (int k = 0; k < 8; ++k)
+          umma::mma_f16(tm + (NS == 1 ? 0 : 128), umma::sdesc_mn(dst + k * 2048, kTileBytes),
+                        umma::sdesc_mn(ar1 + k * 2048, kTileBytes), id_t, k > 0);
+        umma::commit(&sh.sink_done);
+        mbar_wait(&sh.sink_read, 0);
+        umma::fence_after_sync();
+        for (int t = 1; t < min(n, kStages + 1); ++t) load_c(t);
+        if (n > 1) issue_s(1);
+      }
+      for (int t = nsink; t < n; ++t) {
+        if (NS == 2 && t + 1 < n) {
+          if (t > nsink) {
+            mbar_wait(&sh.acc_done, (t - 1) & 1);
+            if (t - 1 + kStages < n) load_c(t - 1 + kStages);
+          }
+          issue_s(t + 1);
+        }
+        issue_acc(t);
+        if (NS == 1 && t + 1 < n) {
+          mbar_wait(&sh.acc_done, t & 1);
+          if (t + kStages < n) load_c(t + kStages);
+          issue_s(t + 1);
+        }
+      }
+      umma::commit(&sh.all_done);
+    }
+    __syncwarp();
+  } else {
+    const int wg = w >> 2, row = tid & 127, r = r0 + row;
+    const uint32_t trow = tm + ((uint32_t)((w & 3) * 32) << 16);
+    const float c = A.scale * kAttnLog2e, f = ds_factor<T>(P.amax);
+    // what the row sees: columns [lo, hi) and (queries) sinks [s_lo, s_hi)
+    int lo = INT32_MAX, hi = 0, s_lo = INT32_MAX, s_hi = 0;
+    float lse_r = INFINITY, delta_r = 0.f;
+    bool alive = false;
+    if (KV) {
+      const SeqRange s = seq_of(A, r);
+      alive = s.end > r;
+      if (alive) {
+        lo = r;
+        hi = min(s.end, r + A.window);
+        if (r - s.start < A.sinks) hi = max(hi, (int)min((int64_t)s.end, (int64_t)first_far(A, r) * 128));
+        atomicMin(&sh.lim_min, hi);
+      }
+    } else {
+      const RowMask m = row_mask(A, r);
+      alive = m.i >= 0;
+      if (alive) {
+        lo = m.lo, hi = r + 1, s_lo = m.start, s_hi = min(m.sink_end, r + 1);
+        lse_r = A.lse[(int64_t)hr * A.T + r], delta_r = A.delta[(int64_t)hr * A.T + r];
+        atomicMax(&sh.lo_max, lo);
+      }
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(NS * 128) : "memory");
+    const int lo_max = sh.lo_max, lim_min = sh.lim_min;
+    if (!KV && nsink && r0 + 128 > end) {
+      // queries behind the last sequence may hold anything: they must not reach the sinks' sums as 0 x NaN
+      mbar_wait(&sh.r_full, 0);
+      if (r >= end && wg == 0)
+#pragma unroll
+        for (int b = 0; b < NB * 8; ++b) {
+          const int o = (b >> 3) * kTileBytes + row * 128 + (b & 7) * 16;
+          *reinterpret_cast<int4*>(sR1 + o) = make_int4(0, 0, 0, 0);
+          *reinterpret_cast<int4*>(sR2 + o) = make_int4(0, 0, 0, 0);
+        }
+      fence_proxy_async_smem();
+    }
+    for (int t = 0; t < n; ++t) {
+      const bool sink = !KV && t < nsink;
+      if (t % NS != wg) continue;
+      const int k0 = col0(t), b = t % NS, ph = (t / NS) & 1;
+      const bool full = KV ? k0 >= r0 + 127 && k0 + kNC <= lim_min : !sink && k0 >= lo_max && k0 + kNC - 1 <= r0;
+      if (KV) {
+        const int64_t hq = hr * G + t / per;
+        const int q = k0 + (row & 63);
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + wg) : "memory");  // the last tile's values have been read
+        if (row < 64) sh.lse[wg][row] = q < c_end ? A.lse[hq * A.T + q] : INFINITY;
+        else sh.delta[wg][row - 64] = q < c_end ? A.delta[hq * A.T + q] : 0.f;
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + wg) : "memory");
+      }
+      uint32_t s[2][32], p[32], ds[32], see[2] = {0xffffffffu, 0xffffffffu};
+      mbar_wait(&sh.s_done[b], ph);
+      umma::fence_after_sync();
+#pragma unroll
+      for (int x = 0; x < 2; ++x) umma::tmem_ld32(trow + b * 128 + x * 32, s[x]);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        umma::tmem_wait_ld(s[x]);
+        if (!full) {
+          const int at = k0 + x * 32;
+          see[x] = sink ? bits(s_lo - at, min(s_hi, send) - at) : bits(lo - at, hi - at) | bits(s_lo - at, s_hi - at);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          float l = lse_r;
+          if (KV) l = sh.lse[wg][x * 32 + j];
+          float e = ex2(fmaf(__uint_as_float(s[x][j]), c, -l));
+          if (!full) e = see[x] >> j & 1 ? e : 0.f;
+          s[x][j] = __float_as_uint(e);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) p[x * 16 + j] = Fmt<T>::pack(__uint_as_float(s[x][2 * j]), __uint_as_float(s[x][2 * j + 1]));
+      }
+      mbar_wait(&sh.dp_done[b], ph);
+      umma::fence_after_sync();
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint32_t dp[32];
+        umma::tmem_ld32(trow + b * 128 + 64 + x * 32, dp);
+        umma::tmem_wait_ld(dp);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const float e = __uint_as_float(s[x][j]);
+          float d = delta_r;
+          if (KV) d = sh.delta[wg][x * 32 + j];
+          float g = e * (__uint_as_float(dp[j]) - d);
+          if (sizeof(T) == 2 && Fmt<T>::id == 0) g *= f;
+          if (!full) g = see[x] >> j & 1 ? g : 0.f;  // not 0 x NaN of what the row does not see
+          dp[j] = __float_as_uint(g);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) ds[x * 16 + j] = Fmt<T>::pack(__uint_as_float(dp[2 * j]), __uint_as_float(dp[2 * j + 1]));
+      }
+      if (KV) umma::tmem_st32(trow + b * 128, p);
+      umma::tmem_st32(trow + b * 128 + 64, ds);
+      if (k0 + kNC > end) {  // columns behind the last sequence: as above
+        mbar_wait(&sh.c_full[t % kStages], (t / kStages) & 1);
+        for (int x = row; x < kNC * NB * 2; x += 128) {
+          const int cr = x % kNC;
+          if (k0 + cr >= end)
+#pragma unroll
+            for (int y = 0; y < 8; ++y)
+              *reinterpret_cast<int4*>(sC + t % kStages * kStageBytes + x / kNC * kColBytes + cr * 128 + y * 16) = make_int4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+      }
+      if (sink) {
+        unsigned char *sp = sC + kStageBytes, *sd = sp + kTileBytes;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          *reinterpret_cast<uint4*>(sp + umma::sw128_off(row, x * 8)) = make_uint4(p[x * 4], p[x * 4 + 1], p[x * 4 + 2], p[x * 4 + 3]);
+          *reinterpret_cast<uint4*>(sd + umma::sw128_off(row, x * 8)) = make_uint4(ds[x * 4], ds[x * 4 + 1], ds[x * 4 + 2], ds[x * 4 + 3]);
+        }
+        fence_proxy_async_smem();
+      }
+      umma::tmem_wait_st();
+      umma::fence_before_sync();
+      mbar_arrive(&sh.p_ready[b]);
+      if (sink) {
+        mbar_wait(&sh.sink_done, 0);
+        umma::fence_after_sync();
+        if (row < 64) {  // lanes 0 .. 63 hold the sinks
+          float* pk = P.part + part_at(A, blockIdx.x, hr, 0, row);
+          float* pv = P.part + part_at(A, blockIdx.x, hr, 1, row);
+          for (int d = 0; d < A.Dh; d += 32) {
+            uint32_t gk[32], gv[32];
+            umma::tmem_ld32(trow + (NS == 1 ? 0 : 128) + d, gk);
+            umma::tmem_ld32(trow + kAcc2 + d, gv);
+            umma::tmem_wait_ld(gk);
+            umma::tmem_wait_ld(gv);
+            if (row < send - s0)
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                *reinterpret_cast<float4*>(pk + d + j) = make_float4(
+                    __uint_as_float(gk[j]) / f, __uint_as_float(gk[j + 1]) / f, __uint_as_float(gk[j + 2]) / f, __uint_as_float(gk[j + 3]) / f);
+                *reinterpret_cast<uint4*>(pv + d + j) = make_uint4(gv[j], gv[j + 1], gv[j + 2], gv[j + 3]);
+              }
+          }
+        }
+        umma::fence_before_sync();
+        mbar_arrive(&sh.sink_read);
+      }
+    }
+    mbar_wait(&sh.all_done, 0);
+    umma::fence_after_sync();
+    const int64_t at = ((int64_t)r * H + hr) * A.Dh;
+    float odd = 0.f;  // NaN as soon as one element is not finite
+    // a sink's far queries
+    const float* far = nullptr;
+    if (KV && alive && P.part != nullptr) {
+      const SeqRange s = seq_of(A, r);
+      if (r - s.start < A.sinks && (int64_t)first_far(A, r) * 128 < s.end)
+        far = P.part + part_at(A, first_far(A, s.start), hk * G, 0, r - s.start);
+    }
+    // the warpgroups share the work: halves of grad_q, or grad_k and grad_v
+    for (int a = 0; a < (KV ? 2 : 1); ++a) {
+      if (KV && NS == 2 && a != wg) continue;
+      const float scale = a == 0 ? A.scale : 1.f, fa = a == 0 ? 1.f / f : 1.f;
+      T* g = (T*)(a == 1 ? A.gv : KV ? A.gk : A.gq) + at;
+      for (int d = 0; d < A.Dh; d += 32) {
+        if (!KV && NS == 2 && (d >> 6) != wg) continue;
+        uint32_t o[32];
+        umma::tmem_ld32(trow + (a == 0 ? kAcc1 : kAcc2) + d, o);
+        umma::tmem_wait_ld(o);
+        if (far != nullptr)
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            o[j] = __float_as_uint(fmaf(__uint_as_float(o[j]), fa, far[(int64_t)a * A.sinks * A.Dh + d + j]));
+        else if (Fmt<T>::id == 0)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * fa);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) odd = fmaf(__uint_as_float(o[j]), 0.f, odd);
+        if (r < A.T)
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[e] = alive ? Fmt<T>::pack(__uint_as_float(o[j + 2 * e]) * scale, __uint_as_float(o[j + 2 * e + 1]) * scale) : 0u;
+            *reinterpret_cast<uint4*>(g + d + j) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+      }
+    }
+    if (alive && odd != 0.f) sh.again[row] = 1;
+    asm volatile("bar.sync 1, %0;" ::"n"(NS * 128) : "memory");
+    for (int x = w; x < 128; x += 4 * NS)
+      if (sh.again[x]) {
+        if (KV) exact_gkv_row<T>(A, hr, r0 + x);
+        else exact_gq_row<T>(A, hr, r0 + x);
+      }
+    umma::fence_before_sync();
+  }
+  __syncthreads();
+  if (w == 4 * NS) umma::tmem_dealloc(tm, kCols);
+}
+
+// part[first far tile of a sequence][first head of a group] <- the sum over the
+// sequence's far tiles and the group's heads, in their order: 4 threads per
+// element take a quarter of the terms each. Grid: query tiles, key heads, sinks.
+__global__ void __launch_bounds__(1024) attn_sink_sum(const __grid_constant__ AttnArgs A, float* part) {
+  __shared__ float sums[4][256];
+  const int n = blockIdx.x, hk = blockIdx.y, r = blockIdx.z, G = A.Hq / A.Hkv;
+  const KeyRange R = keys_of(A, n * 128, n * 128 + 128);
+  if (R.send <= R.s0 || first_far(A, R.s0) != n) return;
+  const SeqRange s = seq_of(A, R.s0);
+  const int beg = max(n, first_far(A, s.start + r)), tiles = (s.end + 127) / 128 - beg;
+  if (tiles <= 0 || s.start + r >= s.end) return;
+  const int v = threadIdx.x & 255, quarter = threadIdx.x >> 8, terms = tiles * G;
+  const int kv = v / A.Dh, d = v % A.Dh;
+  float sum = 0.f;
+  if (kv < 2)
+#pragma unroll 8
+    for (int x = terms * quarter / 4; x < terms * (quarter + 1) / 4; ++x)
+      sum += part[part_at(A, beg + x / G, hk * G + x % G, kv, r) + d];
+  sums[quarter][v] = sum;
+  __syncthreads();
+  if (quarter == 0 && kv < 2)
+    part[part_at(A, n, hk * G, kv, r) + d] = (sums[0][v] + sums[1][v]) + (sums[2][v] + sums[3][v]);
+}
+
+// delta[h][t] = sum_d gy y, zero for rows outside every sequence; fp16: the
+// largest finite |gy| (the order of an integer maximum does not matter). 8 lanes
+// per row, 16 bytes each at a time.
+template <typename T> __global__ void __launch_bounds__(256) attn_delta_kernel(const __grid_constant__ AttnArgs A, uint32_t* amax) {
+  const int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+  const int sub = threadIdx.x & 7;
+  float s = 0.f;
+  uint32_t big = 0;
+  if (row < (int64_t)A.T * A.Hq) {
+    const int64_t t = row / A.Hq, h = row % A.Hq;
+    const bool in = A.lse[h * A.T + t] != INFINITY;
+    if (in)
+      for (int d = sub * 8; d < A.Dh; d += 64) {
+        const Vec<T, 8> g = ld_vec<T, 8>((const T*)A.gy + row * A.Dh + d), y = ld_vec<T, 8>((const T*)A.y + row * A.Dh + d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float x = to_f(g.v[j]);
+          s = fmaf(x, to_f(y.v[j]), s);
+          const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+          if (b < 0x7f800000u) big = max(big, b);
+        }
+      }
+  }
+#pragma unroll
+  for (int x = 4; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x, 8);
+  if (sub == 0 && row < (int64_t)A.T * A.Hq) A.delta[row % A.Hq * A.T + row / A.Hq] = s;
+  if (amax != nullptr) {
+    big = __reduce_max_sync(0xffffffffu, big);
+    if ((threadIdx.x & 31) == 0 && big != 0) atomicMax(amax, big);
+  }
+}
+
+static bool has_far(const AttnArgs& A) { return A.sinks > 0 && A.window < A.T; }
+
+size_t attn_bwd_ws_bytes(int64_t T, int64_t Hq, int64_t Dh, int64_t sinks) {
+  return 16 + (size_t)((T * Hq + 3) / 4 * 16) + (size_t)((T + 127) / 128 * Hq * 2 * sinks * Dh * 4);
+}
+
+template <typename T, int NB, bool KV>
+static int bwd_one(const BwdArgs& P, cudaStream_t st) {
+  const AttnArgs& A = P.a;
+  CUtensorMap r1, r2, c1, c2;
+  constexpr auto dt = TmapType<T>::v;
+  const int64_t gts = (int64_t)A.Hq * A.Dh;
+  if (int rc = head_map(KV ? &c1 : &r1, A.q, dt, A, A.Hq, A.q_ts, A.q_hs, KV ? kNC : 128)) return rc;
+  if (int rc = head_map(KV ? &c2 : &r2, A.gy, dt, A, A.Hq, gts, A.Dh, KV ? kNC : 128)) return rc;
+  if (int rc = head_map(KV ? &r1 : &c1, A.k, dt, A, A.Hkv, A.k_ts, A.k_hs, KV ? 128 : kNC)) return rc;
+  if (int rc = head_map(KV ? &r2 : &c2, A.v, dt, A, A.Hkv, A.v_ts, A.v_hs, KV ? 128 : kNC)) return rc;
+  constexpr int smem = kStages * 2 * NB * kColBytes + 2 * NB * kTileBytes + 1024;
+  auto kernel = attn_bwd_kernel<T, NB, KV>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return set_error(MR_E_LAUNCH, "attn_bwd_kernel: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  kernel<<<dim3((A.T + 127) / 128, KV ? A.Hkv : A.Hq), NB == 1 ? 160 : 288, smem, st>>>(P, r1, r2, c1, c2);
+  return check_launch(KV ? "attn_bwd_kernel (grad_k, grad_v)" : "attn_bwd_kernel (grad_q)");
+}
+
+template <typename T, int NB> static int bwd_nb(const BwdArgs& P, cudaStream_t st) {
+  if (int rc = bwd_one<T, NB, false>(P, st)) return rc;
+  if (P.part != nullptr) {
+    attn_sink_sum<<<dim3((P.a.T + 127) / 128, P.a.Hkv, P.a.sinks), 1024, 0, st>>>(P.a, P.part);
+    if (int rc = check_launch("attn_sink_sum")) return rc;
+  }
+  return bwd_one<T, NB, true>(P, st);
+}
+
+// ws: attn_bwd_ws_bytes, 16-byte aligned
+template <typename T> int attn_bwd_launch(const AttnArgs& A0, void* ws, cudaStream_t st) {
+  BwdArgs P{A0, nullptr, nullptr};
+  uint32_t* amax = (uint32_t*)ws;
+  P.a.delta = (float*)((char*)ws + 16);
+  if (has_far(A0)) P.part = P.a.delta + ((int64_t)A0.T * A0.Hq + 3) / 4 * 4;
+  const bool half = Fmt<T>::id == 0;
+  if (half) {
+    P.amax = amax;
+    const cudaError_t e = cudaMemsetAsync(amax, 0, 4, st);
+    if (e != cudaSuccess) return set_error(MR_E_LAUNCH, "cudaMemsetAsync: %s", cudaGetErrorString(e));
+  }
+  attn_delta_kernel<T><<<(unsigned)(((int64_t)A0.T * A0.Hq + 31) / 32), 256, 0, st>>>(P.a, half ? amax : nullptr);
+  if (int rc = check_launch("attn_delta_kernel")) return rc;
+  return A0.Dh <= 64 ? bwd_nb<T, 1>(P, st) : bwd_nb<T, 2>(P, st);
+}
+template int attn_bwd_launch<__nv_bfloat16>(const AttnArgs&, void*, cudaStream_t);
+template int attn_bwd_launch<__half>(const AttnArgs&, void*, cudaStream_t);
+
+int attn_bwd_device_error(bool clear) { return read_device_error(clear); }
+
+}  // namespace mr

@@ -334,8 +334,6 @@ template <typename T> int attn_bwd_simt(const AttnArgs& A, cudaStream_t st) {
   template int attn_fwd_simt<T>(const AttnArgs&, cudaStream_t);      \
   template int attn_bwd_simt<T>(const AttnArgs&, cudaStream_t);
 MR_INST(float)
-MR_INST(__nv_bfloat16)
-MR_INST(__half)
 #undef MR_INST
 
 }  // namespace mr

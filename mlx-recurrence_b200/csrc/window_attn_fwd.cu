@@ -11,46 +11,12 @@
 // of shared memory each).
 //
 // TMEM columns: S (P over it, two elements a column) at 0, O at 128.
-#include "window_attn.cuh"
-
-#include "tma.cuh"
-#include "tmap.cuh"
-#include "umma.cuh"
+#include "window_tc.cuh"
 
 namespace mr {
 
-constexpr int kTileBytes = 16384;  // [128 rows][64 2-byte elements], 128-byte swizzle
 constexpr int kFwdThreads = 160;
 constexpr float kRescale = 8.f;
-
-template <typename T> struct Fmt;
-template <> struct Fmt<__nv_bfloat16> {
-  static constexpr int id = 1;
-  static __device__ uint32_t pack(float a, float b) {
-    __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&r);
-  }
-};
-template <> struct Fmt<__half> {
-  static constexpr int id = 0;
-  static __device__ uint32_t pack(float a, float b) {
-    __half2 r = __floats2half2_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&r);
-  }
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-// bits [a, b) of a 32-bit word, whatever the bounds
-__device__ __forceinline__ uint32_t bits(int a, int b) {
-  const uint32_t hi = b >= 32 ? 0xffffffffu : b <= 0 ? 0u : (1u << b) - 1;
-  const uint32_t lo = a >= 32 ? 0xffffffffu : a <= 0 ? 0u : (1u << a) - 1;
-  return hi & ~lo;
-}
 
 struct FwdShared {
   uint64_t k_full, v_full, s_done, p_ready, o_done;
@@ -248,17 +214,12 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
   if (w == 4) umma::tmem_dealloc(tm, 256);
 }
 
-static int head_map(CUtensorMap* m, const void* p, CUtensorMapDataType dt, const AttnArgs& A, int H, int64_t ts, int64_t hs) {
-  // [T, H, Dh] as (Dh, H, T); columns at and behind Dh and rows behind T read as zero
-  return make_tmap_3d(m, p, dt, 2, A.Dh, H, A.T, hs * 2, ts * 2, 64, 1, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
 template <typename T, int NB> static int fwd_nb(const AttnArgs& A, cudaStream_t st) {
   CUtensorMap tq, tk, tv;
   constexpr auto dt = TmapType<T>::v;
-  if (int rc = head_map(&tq, A.q, dt, A, A.Hq, A.q_ts, A.q_hs)) return rc;
-  if (int rc = head_map(&tk, A.k, dt, A, A.Hkv, A.k_ts, A.k_hs)) return rc;
-  if (int rc = head_map(&tv, A.v, dt, A, A.Hkv, A.v_ts, A.v_hs)) return rc;
+  if (int rc = head_map(&tq, A.q, dt, A, A.Hq, A.q_ts, A.q_hs, 128)) return rc;
+  if (int rc = head_map(&tk, A.k, dt, A, A.Hkv, A.k_ts, A.k_hs, 128)) return rc;
+  if (int rc = head_map(&tv, A.v, dt, A, A.Hkv, A.v_ts, A.v_hs, 128)) return rc;
   constexpr int smem = 3 * NB * kTileBytes + 1024;
   const cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return set_error(MR_E_LAUNCH, "attn_fwd_kernel: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
