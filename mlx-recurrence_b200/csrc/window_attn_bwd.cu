@@ -57,7 +57,7 @@ struct BwdShared {
   uint32_t tmem;
   int lo_max, lim_min;
   int again[128];
-  float lse[2][kNC], delta[2][kNC];
+  alignas(16) float lse[2][kNC], delta[2][kNC];  // negated, of the column tile's queries
 };
 
 template <typename T, int NB, bool KV>
@@ -264,53 +264,67 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
         const int64_t hq = hr * G + t / per;
         const int q = k0 + (row & 63);
         asm volatile("bar.sync %0, 128;" ::"r"(2 + wg) : "memory");  // the last tile's values have been read
-        if (row < 64) sh.lse[wg][row] = q < c_end ? A.lse[hq * A.T + q] : INFINITY;
-        else sh.delta[wg][row - 64] = q < c_end ? A.delta[hq * A.T + q] : 0.f;
+        if (row < 64) sh.lse[wg][row] = q < c_end ? -A.lse[hq * A.T + q] : -INFINITY;
+        else sh.delta[wg][row - 64] = q < c_end ? -A.delta[hq * A.T + q] : 0.f;
         asm volatile("bar.sync %0, 128;" ::"r"(2 + wg) : "memory");
       }
-      uint32_t s[2][32], p[32], ds[32], see[2] = {0xffffffffu, 0xffffffffu};
+      uint32_t s[2][32], p[32], ds[32], see[2] = {0, 0};
       mbar_wait(&sh.s_done[b], ph);
       umma::fence_after_sync();
 #pragma unroll
       for (int x = 0; x < 2; ++x) umma::tmem_ld32(trow + b * 128 + x * 32, s[x]);
+      const uint64_t c2 = pair(c, c), l2 = pair(-lse_r, -lse_r), d2 = pair(-delta_r, -delta_r), f2 = pair(f, f);
+      // the masks' selects are kept out of the tiles that every row sees in full
+      auto to_p = [&](auto masked) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        umma::tmem_wait_ld(s[x]);
-        if (!full) {
-          const int at = k0 + x * 32;
-          see[x] = sink ? bits(s_lo - at, min(s_hi, send) - at) : bits(lo - at, hi - at) | bits(s_lo - at, s_hi - at);
+        for (int x = 0; x < 2; ++x) {
+          umma::tmem_wait_ld(s[x]);
+          if (masked) {
+            const int at = k0 + x * 32;
+            see[x] = sink ? bits(s_lo - at, min(s_hi, send) - at) : bits(lo - at, hi - at) | bits(s_lo - at, s_hi - at);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const uint64_t l = KV ? *reinterpret_cast<const uint64_t*>(&sh.lse[wg][x * 32 + 2 * j]) : l2;
+            float e0, e1;
+            unpair(fma2(pair(s[x][2 * j], s[x][2 * j + 1]), c2, l), e0, e1);
+            e0 = ex2(e0), e1 = ex2(e1);
+            if (masked) {
+              e0 = see[x] >> (2 * j) & 1 ? e0 : 0.f;
+              e1 = see[x] >> (2 * j + 1) & 1 ? e1 : 0.f;
+            }
+            s[x][2 * j] = __float_as_uint(e0), s[x][2 * j + 1] = __float_as_uint(e1);
+            p[x * 16 + j] = Fmt<T>::pack(e0, e1);
+          }
         }
+      };
+      auto to_ds = [&](auto masked) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          float l = lse_r;
-          if (KV) l = sh.lse[wg][x * 32 + j];
-          float e = ex2(fmaf(__uint_as_float(s[x][j]), c, -l));
-          if (!full) e = see[x] >> j & 1 ? e : 0.f;
-          s[x][j] = __float_as_uint(e);
+        for (int x = 0; x < 2; ++x) {
+          uint32_t dp[32];
+          umma::tmem_ld32(trow + b * 128 + 64 + x * 32, dp);
+          umma::tmem_wait_ld(dp);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const uint64_t d = KV ? *reinterpret_cast<const uint64_t*>(&sh.delta[wg][x * 32 + 2 * j]) : d2;
+            uint64_t g = mul2(pair(s[x][2 * j], s[x][2 * j + 1]), add2(pair(dp[2 * j], dp[2 * j + 1]), d));
+            if (Fmt<T>::id == 0) g = mul2(g, f2);
+            float g0, g1;
+            unpair(g, g0, g1);
+            if (masked) {  // not 0 x NaN of what the row does not see
+              g0 = see[x] >> (2 * j) & 1 ? g0 : 0.f;
+              g1 = see[x] >> (2 * j + 1) & 1 ? g1 : 0.f;
+            }
+            ds[x * 16 + j] = Fmt<T>::pack(g0, g1);
+          }
         }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) p[x * 16 + j] = Fmt<T>::pack(__uint_as_float(s[x][2 * j]), __uint_as_float(s[x][2 * j + 1]));
-      }
+      };
+      if (full) to_p(std::false_type{});
+      else to_p(std::true_type{});
       mbar_wait(&sh.dp_done[b], ph);
       umma::fence_after_sync();
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        uint32_t dp[32];
-        umma::tmem_ld32(trow + b * 128 + 64 + x * 32, dp);
-        umma::tmem_wait_ld(dp);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float e = __uint_as_float(s[x][j]);
-          float d = delta_r;
-          if (KV) d = sh.delta[wg][x * 32 + j];
-          float g = e * (__uint_as_float(dp[j]) - d);
-          if (sizeof(T) == 2 && Fmt<T>::id == 0) g *= f;
-          if (!full) g = see[x] >> j & 1 ? g : 0.f;  // not 0 x NaN of what the row does not see
-          dp[j] = __float_as_uint(g);
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) ds[x * 16 + j] = Fmt<T>::pack(__uint_as_float(dp[2 * j]), __uint_as_float(dp[2 * j + 1]));
-      }
+      if (full) to_ds(std::false_type{});
+      else to_ds(std::true_type{});
       if (KV) umma::tmem_st32(trow + b * 128, p);
       umma::tmem_st32(trow + b * 128 + 64, ds);
       if (k0 + kNC > end) {  // columns behind the last sequence: as above

@@ -9,8 +9,6 @@
 // first thread issues copies and products; a CTA's steps depend on each other,
 // and the second CTA of the SM fills the gaps (256 TMEM columns and at most 96 KB
 // of shared memory each).
-//
-// TMEM columns: S (P over it, two elements a column) at 0, O at 128.
 #include "window_tc.cuh"
 
 namespace mr {
@@ -29,6 +27,9 @@ template <typename T, int NB>  // NB = 64-wide blocks of a row
 __global__ void __launch_bounds__(kFwdThreads, 2)
 attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap tq,
                 const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
+  // TMEM columns: S at 0; P over it (its first half, as S is used up) or, where O leaves room, in columns of its own
+  constexpr bool kOwnP = NB == 1;
+  constexpr uint32_t kP = kOwnP ? 128 : 0, kO = kOwnP ? 192 : 128;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   unsigned char *sQ = sm, *sK = sQ + NB * kTileBytes, *sV = sK + NB * kTileBytes;
@@ -76,31 +77,44 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
       load(&tk, sK, hk, key0(0), &sh.k_full);
       mbar_arrive_expect_tx(&sh.v_full, NB * kTileBytes);
       load(&tv, sV, hk, key0(0), &sh.v_full);
-      for (int t = 0; t < ntile; ++t) {
-        const int n = t < nsink ? sink_n : 128;
+      const uint32_t ido = umma::idesc_f16(128, A.Dh, Fmt<T>::id, 0, 1);
+      auto cols = [&](int t) { return t < nsink ? sink_n : 128; };
+      auto issue_s = [&](int t) {
         mbar_wait(&sh.k_full, t & 1);
-        const uint32_t ids = umma::idesc_f16(128, n, Fmt<T>::id, 0, 0);
+        umma::fence_after_sync();
+        const uint32_t ids = umma::idesc_f16(128, cols(t), Fmt<T>::id, 0, 0);
         for (int k = 0; k < A.Dh / 16; ++k) {
           const uint32_t o = (k >> 2) * kTileBytes + (k & 3) * 32;
           umma::mma_f16(tm, umma::sdesc_k(aq + o), umma::sdesc_k(ak + o), ids, k > 0);
         }
         umma::commit(&sh.s_done);
+      };
+      auto load_v = [&](int t) {
+        mbar_arrive_expect_tx(&sh.v_full, NB * kTileBytes);
+        load(&tv, sV, hk, key0(t), &sh.v_full);
+      };
+      issue_s(0);
+      for (int t = 0; t < ntile; ++t) {
         mbar_wait(&sh.s_done, t & 1);
         if (t + 1 < ntile) {
           mbar_arrive_expect_tx(&sh.k_full, NB * kTileBytes);
           load(&tk, sK, hk, key0(t + 1), &sh.k_full);
         }
-        mbar_wait(&sh.v_full, t & 1);
+        if (kOwnP && t > 0) {
+          mbar_wait(&sh.o_done, (t - 1) & 1);
+          load_v(t);
+        }
         mbar_wait(&sh.p_ready, t & 1);
+        if (kOwnP && t + 1 < ntile) issue_s(t + 1);  // S has been read; P lies elsewhere
+        mbar_wait(&sh.v_full, t & 1);
         umma::fence_after_sync();
-        const uint32_t ido = umma::idesc_f16(128, A.Dh, Fmt<T>::id, 0, 1);
-        for (int k = 0; k < n / 16; ++k)
-          umma::mma_f16_ta(tm + 128, tm + k * 8, umma::sdesc_mn(av + k * 2048, kTileBytes), ido, t > 0 || k > 0);
+        for (int k = 0; k < cols(t) / 16; ++k)
+          umma::mma_f16_ta(tm + kO, tm + kP + k * 8, umma::sdesc_mn(av + k * 2048, kTileBytes), ido, t > 0 || k > 0);
         umma::commit(&sh.o_done);
-        mbar_wait(&sh.o_done, t & 1);  // P is read (the next S overwrites it) and V too
-        if (t + 1 < ntile) {
-          mbar_arrive_expect_tx(&sh.v_full, NB * kTileBytes);
-          load(&tv, sV, hk, key0(t + 1), &sh.v_full);
+        if (!kOwnP && t + 1 < ntile) {
+          mbar_wait(&sh.o_done, t & 1);  // P is read: the next S overwrites it
+          load_v(t + 1);
+          issue_s(t + 1);
         }
       }
     }
@@ -122,24 +136,36 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
       const bool full = !sink && k0 >= lo_max && k0 + 127 <= q0;
       mbar_wait(&sh.s_done, t & 1);
       umma::fence_after_sync();
-      uint32_t s[4][32];
+      // what the query sees of the tile, a word per 32 keys (uniformly all ones in most tiles)
+      uint32_t see[4];
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        if (b < nch) umma::tmem_ld32(trow + b * 32, s[b]);
-      float mx = -INFINITY;
+      for (int b = 0; b < 4; ++b) {
+        const int at = k0 + b * 32;
+        see[b] = bits(rm.start - at, min(min(rm.sink_end, rm.i + 1), sink ? R.send : INT32_MAX) - at);
+        if (!sink) see[b] |= bits(rm.lo - at, rm.i + 1 - at);
+      }
+      // first over S for the maximum, then again for the exponentials: S stays in TMEM, not in 128 registers
+      auto masked = [&](uint32_t (&s)[32], int b) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) s[j] = see[b] >> j & 1 ? s[j] : 0xff800000u;
+      };
+      uint32_t s[2][32];
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      umma::tmem_ld32(trow, s[0]);
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         if (b >= nch) continue;
-        umma::tmem_wait_ld(s[b]);
-        if (!full) {
-          const int at = k0 + b * 32;
-          uint32_t see = bits(rm.start - at, min(min(rm.sink_end, rm.i + 1), sink ? R.send : INT32_MAX) - at);
-          if (!sink) see |= bits(rm.lo - at, rm.i + 1 - at);
+        umma::tmem_wait_ld(s[b & 1]);
+        if (b + 1 < nch) umma::tmem_ld32(trow + (b + 1) * 32, s[(b + 1) & 1]);
+        if (!full) masked(s[b & 1], b);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) s[b][j] = see >> j & 1 ? s[b][j] : 0xff800000u;
-        }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(s[b][j]));
+        for (int j = 0; j < 32; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(s[b & 1][j]));
+      }
+      umma::tmem_ld32(trow, s[0]);
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      if (t > 0) {  // P and O are free
+        mbar_wait(&sh.o_done, (t - 1) & 1);
+        umma::fence_after_sync();
       }
       if (__any_sync(0xffffffffu, (mx - m) * c > kRescale || m == -INFINITY)) {
         const float to = fmaxf(mx, m);
@@ -147,30 +173,36 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
         m = to, l *= f;
         if (t > 0)
           for (int d = 0; d < A.Dh; d += 32) {
-            uint32_t o[32];
-            umma::tmem_ld32(trow + 128 + d, o);
-            umma::tmem_wait_ld(o);
+            umma::tmem_ld32(trow + kO + d, s[1]);
+            umma::tmem_wait_ld(s[1]);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-            umma::tmem_st32(trow + 128 + d, o);
+            for (int j = 0; j < 32; ++j) s[1][j] = __float_as_uint(__uint_as_float(s[1][j]) * f);
+            umma::tmem_st32(trow + kO + d, s[1]);
           }
       }
       const float mc = m == -INFINITY ? 0.f : m * c;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t c2 = pair(c, c), mc2 = pair(-mc, -mc);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         if (b >= nch) continue;
+        umma::tmem_wait_ld(s[b & 1]);
+        if (b + 1 < nch) umma::tmem_ld32(trow + (b + 1) * 32, s[(b + 1) & 1]);
+        if (!full) masked(s[b & 1], b);
         uint32_t p[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const float e0 = ex2(fmaf(__uint_as_float(s[b][2 * j]), c, -mc));
-          const float e1 = ex2(fmaf(__uint_as_float(s[b][2 * j + 1]), c, -mc));
-          sum[(2 * j) & 3] += e0, sum[(2 * j + 1) & 3] += e1;
-          p[j] = Fmt<T>::pack(e0, e1);
+          float x0, x1;
+          unpair(fma2(pair(s[b & 1][2 * j], s[b & 1][2 * j + 1]), c2, mc2), x0, x1);
+          x0 = ex2(x0), x1 = ex2(x1);
+          sum[j & 1] = add2(sum[j & 1], pair(x0, x1));
+          p[j] = Fmt<T>::pack(x0, x1);
         }
-        umma::tmem_st16(trow + b * 16, p);
+        umma::tmem_st16(trow + kP + b * 16, p);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      float l0, l1;
+      unpair(add2(sum[0], sum[1]), l0, l1);
+      l += l0 + l1;
       if (k0 + 128 > end) {  // rows behind the last sequence may hold anything: 0 x NaN would reach O
         mbar_wait(&sh.v_full, t & 1);
         if (k0 + tid >= end)
@@ -189,7 +221,7 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
     float odd = 0.f;  // NaN as soon as one element is not finite
     for (int d = 0; d < A.Dh; d += 32) {
       uint32_t o[32];
-      umma::tmem_ld32(trow + 128 + d, o);
+      umma::tmem_ld32(trow + kO + d, o);
       umma::tmem_wait_ld(o);
 #pragma unroll
       for (int j = 0; j < 32; ++j) odd = fmaf(__uint_as_float(o[j]), 0.f, odd);
