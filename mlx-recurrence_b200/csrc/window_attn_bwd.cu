@@ -129,6 +129,11 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
   if (w == 4 * NS) {
     if (lane == 0) {
       const uint32_t ar1 = smem_u32(sR1), ar2 = smem_u32(sR2), ac = smem_u32(sC);
+      // one thread issues every product: descriptors are made once and stepped by additions
+      const uint64_t dr1 = umma::sdesc_k(ar1), dr2 = umma::sdesc_k(ar2), dck = umma::sdesc_k(ac), dcm = umma::sdesc_mn(ac, kColBytes);
+      const int ks = A.Dh / 16;
+      auto row_step = [](int k) { return (k >> 2) * (kTileBytes / 16) + (k & 3) * 2; };
+      auto col_step = [](int k) { return (k >> 2) * (kColBytes / 16) + (k & 3) * 2; };
       auto load_c = [&](int t) {
         const int st = t % kStages, hc = KV ? hr * G + t / per : hk;
         unsigned char* dst = sC + st * kStageBytes;
@@ -143,30 +148,30 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
       const uint32_t id_a = umma::idesc_f16(128, A.Dh, Fmt<T>::id, 0, 1);
       auto issue_s = [&](int t) {
         const int b = t % NS;
-        const uint32_t c1 = ac + t % kStages * kStageBytes, c2 = c1 + NB * kColBytes, d = tm + b * 128;
+        const uint32_t d = tm + b * 128;
+        const uint64_t c1 = dck + t % kStages * (kStageBytes / 16), c2 = c1 + NB * kColBytes / 16;
         mbar_wait(&sh.c_full[t % kStages], (t / kStages) & 1);
         umma::fence_after_sync();
-        for (int k = 0; k < A.Dh / 16; ++k) {
-          const uint32_t o = (k & 3) * 32;
-          umma::mma_f16(d, umma::sdesc_k(ar1 + (k >> 2) * kTileBytes + o), umma::sdesc_k(c1 + (k >> 2) * kColBytes + o), id_s, k > 0);
-        }
+#pragma unroll
+        for (int k = 0; k < NB * 4; ++k)
+          if (k < ks) umma::mma_f16(d, dr1 + row_step(k), c1 + col_step(k), id_s, k > 0);
         umma::commit(&sh.s_done[b]);
-        for (int k = 0; k < A.Dh / 16; ++k) {
-          const uint32_t o = (k & 3) * 32;
-          umma::mma_f16(d + 64, umma::sdesc_k(ar2 + (k >> 2) * kTileBytes + o), umma::sdesc_k(c2 + (k >> 2) * kColBytes + o), id_s, k > 0);
-        }
+#pragma unroll
+        for (int k = 0; k < NB * 4; ++k)
+          if (k < ks) umma::mma_f16(d + 64, dr2 + row_step(k), c2 + col_step(k), id_s, k > 0);
         umma::commit(&sh.dp_done[b]);
       };
       auto issue_acc = [&](int t) {
         const int b = t % NS;
-        const uint32_t c1 = ac + t % kStages * kStageBytes, c2 = c1 + NB * kColBytes, d = tm + b * 128;
+        const uint32_t d = tm + b * 128;
+        const uint64_t c1 = dcm + t % kStages * (kStageBytes / 16), c2 = c1 + NB * kColBytes / 16;
         mbar_wait(&sh.p_ready[b], (t / NS) & 1);
         umma::fence_after_sync();
         if (KV)
-          for (int k = 0; k < kNC / 16; ++k)
-            umma::mma_f16_ta(tm + kAcc2, d + k * 8, umma::sdesc_mn(c2 + k * 2048, kColBytes), id_a, t > 0 || k > 0);
-        for (int k = 0; k < kNC / 16; ++k)
-          umma::mma_f16_ta(tm + kAcc1, d + 64 + k * 8, umma::sdesc_mn(c1 + k * 2048, kColBytes), id_a, t > 0 || k > 0);
+#pragma unroll
+          for (int k = 0; k < kNC / 16; ++k) umma::mma_f16_ta(tm + kAcc2, d + k * 8, c2 + k * 128, id_a, t > 0 || k > 0);
+#pragma unroll
+        for (int k = 0; k < kNC / 16; ++k) umma::mma_f16_ta(tm + kAcc1, d + 64 + k * 8, c1 + k * 128, id_a, t > 0 || k > 0);
         umma::commit(&sh.acc_done);
       };
       mbar_arrive_expect_tx(&sh.r_full, 2 * NB * kTileBytes);

@@ -66,7 +66,9 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
 
   if (w == 4) {
     if (lane == 0) {
-      const uint32_t aq = smem_u32(sQ), ak = smem_u32(sK), av = smem_u32(sV);
+      // one thread issues every product: descriptors are made once and stepped by additions
+      const uint64_t dq = umma::sdesc_k(smem_u32(sQ)), dk = umma::sdesc_k(smem_u32(sK)), dv = umma::sdesc_mn(smem_u32(sV), kTileBytes);
+      const int ks = A.Dh / 16;
       auto load = [&](const CUtensorMap* m, unsigned char* dst, int head, int row, uint64_t* bar) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) tma_load_3d(dst + b * kTileBytes, m, b * 64, head, row, bar);
@@ -83,9 +85,11 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
         mbar_wait(&sh.k_full, t & 1);
         umma::fence_after_sync();
         const uint32_t ids = umma::idesc_f16(128, cols(t), Fmt<T>::id, 0, 0);
-        for (int k = 0; k < A.Dh / 16; ++k) {
-          const uint32_t o = (k >> 2) * kTileBytes + (k & 3) * 32;
-          umma::mma_f16(tm, umma::sdesc_k(aq + o), umma::sdesc_k(ak + o), ids, k > 0);
+#pragma unroll
+        for (int k = 0; k < NB * 4; ++k) {
+          constexpr int kBlock = kTileBytes / 16;
+          const int o = (k >> 2) * kBlock + (k & 3) * 2;
+          if (k < ks) umma::mma_f16(tm, dq + o, dk + o, ids, k > 0);
         }
         umma::commit(&sh.s_done);
       };
@@ -108,8 +112,10 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
         if (kOwnP && t + 1 < ntile) issue_s(t + 1);  // S has been read; P lies elsewhere
         mbar_wait(&sh.v_full, t & 1);
         umma::fence_after_sync();
-        for (int k = 0; k < cols(t) / 16; ++k)
-          umma::mma_f16_ta(tm + kO, tm + kP + k * 8, umma::sdesc_mn(av + k * 2048, kTileBytes), ido, t > 0 || k > 0);
+        const int kp = cols(t) / 16;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < kp) umma::mma_f16_ta(tm + kO, tm + kP + k * 8, dv + k * 128, ido, t > 0 || k > 0);
         umma::commit(&sh.o_done);
         if (!kOwnP && t + 1 < ntile) {
           mbar_wait(&sh.o_done, t & 1);  // P is read: the next S overwrites it
