@@ -66,6 +66,14 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 
+// One lane of a converged warp (the same one every time). The warp runs the issuing code as a whole, so that addresses
+// and descriptors live in uniform registers, which tcgen05.mma takes; only the instruction itself is the lane's.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // ---- MMA (one thread issues) ------------------------------------------------
 // D[tmem] (+)= A[smem] * B[smem]^T (per the descriptors' majorness).
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,

@@ -127,9 +127,10 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
   const uint32_t tm = sh.tmem;
 
   if (w == 4 * NS) {
-    if (lane == 0) {
+    {
+      const bool lead = umma::elect_one();
       const uint32_t ar1 = smem_u32(sR1), ar2 = smem_u32(sR2), ac = smem_u32(sC);
-      // one thread issues every product: descriptors are made once and stepped by additions
+      // descriptors are made once and stepped by additions
       const uint64_t dr1 = umma::sdesc_k(ar1), dr2 = umma::sdesc_k(ar2), dck = umma::sdesc_k(ac), dcm = umma::sdesc_mn(ac, kColBytes);
       const int ks = A.Dh / 16;
       auto row_step = [](int k) { return (k >> 2) * (kTileBytes / 16) + (k & 3) * 2; };
@@ -137,7 +138,8 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
       auto load_c = [&](int t) {
         const int st = t % kStages, hc = KV ? hr * G + t / per : hk;
         unsigned char* dst = sC + st * kStageBytes;
-        mbar_arrive_expect_tx(&sh.c_full[st], kStageBytes);
+        if (lead) mbar_arrive_expect_tx(&sh.c_full[st], kStageBytes);
+        if (lead)
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           tma_load_3d(dst + b * kColBytes, &tc1, b * 64, hc, col0(t), &sh.c_full[st]);
@@ -154,12 +156,12 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
         umma::fence_after_sync();
 #pragma unroll
         for (int k = 0; k < NB * 4; ++k)
-          if (k < ks) umma::mma_f16(d, dr1 + row_step(k), c1 + col_step(k), id_s, k > 0);
-        umma::commit(&sh.s_done[b]);
+          if (k < ks && lead) umma::mma_f16(d, dr1 + row_step(k), c1 + col_step(k), id_s, k > 0);
+        if (lead) umma::commit(&sh.s_done[b]);
 #pragma unroll
         for (int k = 0; k < NB * 4; ++k)
-          if (k < ks) umma::mma_f16(d + 64, dr2 + row_step(k), c2 + col_step(k), id_s, k > 0);
-        umma::commit(&sh.dp_done[b]);
+          if (k < ks && lead) umma::mma_f16(d + 64, dr2 + row_step(k), c2 + col_step(k), id_s, k > 0);
+        if (lead) umma::commit(&sh.dp_done[b]);
       };
       auto issue_acc = [&](int t) {
         const int b = t % NS;
@@ -169,12 +171,15 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
         umma::fence_after_sync();
         if (KV)
 #pragma unroll
-          for (int k = 0; k < kNC / 16; ++k) umma::mma_f16_ta(tm + kAcc2, d + k * 8, c2 + k * 128, id_a, t > 0 || k > 0);
+          for (int k = 0; k < kNC / 16; ++k)
+            if (lead) umma::mma_f16_ta(tm + kAcc2, d + k * 8, c2 + k * 128, id_a, t > 0 || k > 0);
 #pragma unroll
-        for (int k = 0; k < kNC / 16; ++k) umma::mma_f16_ta(tm + kAcc1, d + 64 + k * 8, c1 + k * 128, id_a, t > 0 || k > 0);
-        umma::commit(&sh.acc_done);
+        for (int k = 0; k < kNC / 16; ++k)
+            if (lead) umma::mma_f16_ta(tm + kAcc1, d + 64 + k * 8, c1 + k * 128, id_a, t > 0 || k > 0);
+        if (lead) umma::commit(&sh.acc_done);
       };
-      mbar_arrive_expect_tx(&sh.r_full, 2 * NB * kTileBytes);
+      if (lead) mbar_arrive_expect_tx(&sh.r_full, 2 * NB * kTileBytes);
+      if (lead)
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         tma_load_3d(sR1 + b * kTileBytes, &tr1, b * 64, hr, r0, &sh.r_full);
@@ -192,11 +197,11 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
         const uint32_t id_t = umma::idesc_f16(128, A.Dh, Fmt<T>::id, 1, 1);  // rows at and behind 64 are not used
         const uint32_t pt = ac + kStageBytes, dst = pt + kTileBytes;
         for (int k = 0; k < 8; ++k)
-          umma::mma_f16(tm + kAcc2, umma::sdesc_mn(pt + k * 2048, kTileBytes), umma::sdesc_mn(ar2 + k * 2048, kTileBytes), id_t, k > 0);
+          if (lead) umma::mma_f16(tm + kAcc2, umma::sdesc_mn(pt + k * 2048, kTileBytes), umma::sdesc_mn(ar2 + k * 2048, kTileBytes), id_t, k > 0);
         for (int k = 0; k < 8; ++k)
-          umma::mma_f16(tm + (NS == 1 ? 0 : 128), umma::sdesc_mn(dst + k * 2048, kTileBytes),
+          if (lead) umma::mma_f16(tm + (NS == 1 ? 0 : 128), umma::sdesc_mn(dst + k * 2048, kTileBytes),
                         umma::sdesc_mn(ar1 + k * 2048, kTileBytes), id_t, k > 0);
-        umma::commit(&sh.sink_done);
+        if (lead) umma::commit(&sh.sink_done);
         mbar_wait(&sh.sink_read, 0);
         umma::fence_after_sync();
         for (int t = 1; t < min(n, kStages + 1); ++t) load_c(t);
@@ -217,7 +222,7 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
           issue_s(t + 1);
         }
       }
-      umma::commit(&sh.all_done);
+      if (lead) umma::commit(&sh.all_done);
     }
     __syncwarp();
   } else {

@@ -65,19 +65,21 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
   const int sink_n = nsink ? (R.send - R.s0 + 15) & ~15 : 0;
 
   if (w == 4) {
-    if (lane == 0) {
-      // one thread issues every product: descriptors are made once and stepped by additions
+    {
+      const bool lead = umma::elect_one();
+      // descriptors are made once and stepped by additions
       const uint64_t dq = umma::sdesc_k(smem_u32(sQ)), dk = umma::sdesc_k(smem_u32(sK)), dv = umma::sdesc_mn(smem_u32(sV), kTileBytes);
       const int ks = A.Dh / 16;
       auto load = [&](const CUtensorMap* m, unsigned char* dst, int head, int row, uint64_t* bar) {
+        if (lead)
 #pragma unroll
         for (int b = 0; b < NB; ++b) tma_load_3d(dst + b * kTileBytes, m, b * 64, head, row, bar);
       };
       auto key0 = [&](int t) { return t < nsink ? R.s0 : R.kmin + (t - nsink) * 128; };
-      mbar_arrive_expect_tx(&sh.k_full, 2 * NB * kTileBytes);
+      if (lead) mbar_arrive_expect_tx(&sh.k_full, 2 * NB * kTileBytes);
       load(&tq, sQ, h, q0, &sh.k_full);
       load(&tk, sK, hk, key0(0), &sh.k_full);
-      mbar_arrive_expect_tx(&sh.v_full, NB * kTileBytes);
+      if (lead) mbar_arrive_expect_tx(&sh.v_full, NB * kTileBytes);
       load(&tv, sV, hk, key0(0), &sh.v_full);
       const uint32_t ido = umma::idesc_f16(128, A.Dh, Fmt<T>::id, 0, 1);
       auto cols = [&](int t) { return t < nsink ? sink_n : 128; };
@@ -89,19 +91,19 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
         for (int k = 0; k < NB * 4; ++k) {
           constexpr int kBlock = kTileBytes / 16;
           const int o = (k >> 2) * kBlock + (k & 3) * 2;
-          if (k < ks) umma::mma_f16(tm, dq + o, dk + o, ids, k > 0);
+          if (k < ks && lead) umma::mma_f16(tm, dq + o, dk + o, ids, k > 0);
         }
-        umma::commit(&sh.s_done);
+        if (lead) umma::commit(&sh.s_done);
       };
       auto load_v = [&](int t) {
-        mbar_arrive_expect_tx(&sh.v_full, NB * kTileBytes);
+        if (lead) mbar_arrive_expect_tx(&sh.v_full, NB * kTileBytes);
         load(&tv, sV, hk, key0(t), &sh.v_full);
       };
       issue_s(0);
       for (int t = 0; t < ntile; ++t) {
         mbar_wait(&sh.s_done, t & 1);
         if (t + 1 < ntile) {
-          mbar_arrive_expect_tx(&sh.k_full, NB * kTileBytes);
+          if (lead) mbar_arrive_expect_tx(&sh.k_full, NB * kTileBytes);
           load(&tk, sK, hk, key0(t + 1), &sh.k_full);
         }
         if (kOwnP && t > 0) {
@@ -115,8 +117,8 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
         const int kp = cols(t) / 16;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (k < kp) umma::mma_f16_ta(tm + kO, tm + kP + k * 8, dv + k * 128, ido, t > 0 || k > 0);
-        umma::commit(&sh.o_done);
+          if (k < kp && lead) umma::mma_f16_ta(tm + kO, tm + kP + k * 8, dv + k * 128, ido, t > 0 || k > 0);
+        if (lead) umma::commit(&sh.o_done);
         if (!kOwnP && t + 1 < ntile) {
           mbar_wait(&sh.o_done, t & 1);  // P is read: the next S overwrites it
           load_v(t + 1);
