@@ -11,12 +11,15 @@
 //               query head that shares the key head; grad_k, grad_v.
 // Per column tile S = R1 C1^T and dP = R2 C2^T land in TMEM, a warpgroup (a
 // thread per row) turns them into P and dS, written back over them as the A
-// operands of the sums dS C1 and P C2, which stay in TMEM. That is 7 products
+// operands of the sums P C2 and dS C1, which stay in TMEM. That is 7 products
 // where one pass with atomic sums would need 5.
 //
-// Dh <= 64: one warpgroup, 256 TMEM columns, two CTAs per SM fill each other's
-// gaps. Dh > 64: the sums take 256 columns, so one CTA with two warpgroups on
-// alternating column tiles.
+// Two column tiles are in flight per SM, a warpgroup each: in two CTAs of 256 TMEM
+// columns (Dh <= 64), or in one, whose sums take 256 of its 512 columns. What
+// bounds it: a tile is a chain (S, exponentials, dS, sums), so the issuing warp
+// starts the next S of a stage before the last sum of the old tile: P C2 runs
+// under the dS arithmetic, the next S follows as soon as P (KV = false: S) has
+// been read, the next dP after dS C1.
 //
 // Sinks: a key that stays visible to the end of a long sequence would make its
 // row tile walk every later query. Instead a query tile whose window has left the
@@ -30,7 +33,9 @@ namespace mr {
 
 constexpr int kNC = 64;                  // columns of a tile
 constexpr int kColBytes = kNC * 128;     // one 64-wide block of a column tile
-constexpr int kStages = 3;               // column tiles in shared memory
+template <int NB> constexpr int kNS = NB;      // column tiles in flight: TMEM stages and warpgroups
+constexpr int kStages = 4;                     // column tiles in shared memory
+template <int NB> constexpr int kBwdThreads = kNS<NB> * 128 + 32;
 
 struct BwdArgs {
   AttnArgs a;
@@ -53,7 +58,7 @@ template <> __device__ __forceinline__ float ds_factor<__half>(const uint32_t* a
 }
 
 struct BwdShared {
-  uint64_t r_full, c_full[kStages], s_done[2], dp_done[2], p_ready[2], acc_done, all_done, sink_done, sink_read;
+  uint64_t r_full, c_full[kStages], s_done[2], dp_done[2], p_ready[2], ds_ready[2], acc2_done, acc1_done, all_done, sink_done, sink_read;
   uint32_t tmem;
   int lo_max, lim_min;
   int again[128];
@@ -61,19 +66,19 @@ struct BwdShared {
 };
 
 template <typename T, int NB, bool KV>
-__global__ void __launch_bounds__(NB == 1 ? 160 : 288, NB == 1 ? 2 : 1)
+__global__ void __launch_bounds__(kBwdThreads<NB>, NB == 1 ? 2 : 1)
 attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUtensorMap tr1,
                 const __grid_constant__ CUtensorMap tr2, const __grid_constant__ CUtensorMap tc1,
                 const __grid_constant__ CUtensorMap tc2) {
-  constexpr int NS = NB;  // warpgroups, and TMEM stages
+  constexpr int NS = kNS<NB>, NC = kStages;
   constexpr int kStageBytes = 2 * NB * kColBytes;
-  constexpr uint32_t kAcc1 = NS * 128, kAcc2 = kAcc1 + NB * 64, kCols = NB == 1 ? 256 : 512;
+  constexpr uint32_t kAcc1 = NS * 128, kAcc2 = kAcc1 + NB * 64, kCols = NB == 1 ? 256 : 512, kSinkK = NB == 1 ? 0 : 128;
   extern __shared__ unsigned char raw[];
   unsigned char* sC = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  unsigned char *sR1 = sC + kStages * kStageBytes, *sR2 = sR1 + NB * kTileBytes;
+  unsigned char *sR1 = sC + NC * kStageBytes, *sR2 = sR1 + NB * kTileBytes;
   __shared__ BwdShared sh;
   const AttnArgs& A = P.a;
-  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, G = A.Hq / A.Hkv;
+  const int tid = threadIdx.x, w = tid >> 5, G = A.Hq / A.Hkv;
   const int hr = blockIdx.y, hk = KV ? hr : hr / G, r0 = blockIdx.x * 128;
   const int first = first_token(A), end = end_token(A);
 
@@ -110,9 +115,13 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
 
   if (tid == 0) {
     mbar_init(&sh.r_full, 1);
-    for (int i = 0; i < kStages; ++i) mbar_init(&sh.c_full[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&sh.s_done[i], 1), mbar_init(&sh.dp_done[i], 1), mbar_init(&sh.p_ready[i], 128);
-    mbar_init(&sh.acc_done, 1), mbar_init(&sh.all_done, 1), mbar_init(&sh.sink_done, 1), mbar_init(&sh.sink_read, 128);
+    for (int i = 0; i < NC; ++i) mbar_init(&sh.c_full[i], 1);
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&sh.s_done[i], 1), mbar_init(&sh.dp_done[i], 1);
+      mbar_init(&sh.p_ready[i], 128), mbar_init(&sh.ds_ready[i], 128);
+    }
+    mbar_init(&sh.acc1_done, 1), mbar_init(&sh.acc2_done, 1), mbar_init(&sh.all_done, 1);
+    mbar_init(&sh.sink_done, 1), mbar_init(&sh.sink_read, 128);
     fence_mbar_init();
     sh.lo_max = 0, sh.lim_min = INT32_MAX;
   }
@@ -136,91 +145,102 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
       auto row_step = [](int k) { return (k >> 2) * (kTileBytes / 16) + (k & 3) * 2; };
       auto col_step = [](int k) { return (k >> 2) * (kColBytes / 16) + (k & 3) * 2; };
       auto load_c = [&](int t) {
-        const int st = t % kStages, hc = KV ? hr * G + t / per : hk;
+        const int st = t % NC, hc = KV ? hr * G + t / per : hk;
         unsigned char* dst = sC + st * kStageBytes;
-        if (lead) mbar_arrive_expect_tx(&sh.c_full[st], kStageBytes);
-        if (lead)
+        if (lead) {
+          mbar_arrive_expect_tx(&sh.c_full[st], kStageBytes);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          tma_load_3d(dst + b * kColBytes, &tc1, b * 64, hc, col0(t), &sh.c_full[st]);
-          tma_load_3d(dst + (NB + b) * kColBytes, &tc2, b * 64, hc, col0(t), &sh.c_full[st]);
+          for (int b = 0; b < NB; ++b) {
+            tma_load_3d(dst + b * kColBytes, &tc1, b * 64, hc, col0(t), &sh.c_full[st]);
+            tma_load_3d(dst + (NB + b) * kColBytes, &tc2, b * 64, hc, col0(t), &sh.c_full[st]);
+          }
         }
       };
       const uint32_t id_s = umma::idesc_f16(128, kNC, Fmt<T>::id, 0, 0);
       const uint32_t id_a = umma::idesc_f16(128, A.Dh, Fmt<T>::id, 0, 1);
       auto issue_s = [&](int t) {
-        const int b = t % NS;
-        const uint32_t d = tm + b * 128;
-        const uint64_t c1 = dck + t % kStages * (kStageBytes / 16), c2 = c1 + NB * kColBytes / 16;
-        mbar_wait(&sh.c_full[t % kStages], (t / kStages) & 1);
+        const uint32_t d = tm + t % NS * 128;
+        const uint64_t c1 = dck + t % NC * (kStageBytes / 16);
+        mbar_wait(&sh.c_full[t % NC], (t / NC) & 1);
         umma::fence_after_sync();
 #pragma unroll
         for (int k = 0; k < NB * 4; ++k)
           if (k < ks && lead) umma::mma_f16(d, dr1 + row_step(k), c1 + col_step(k), id_s, k > 0);
-        if (lead) umma::commit(&sh.s_done[b]);
+        if (lead) umma::commit(&sh.s_done[t % NS]);
+      };
+      auto issue_dp = [&](int t) {
+        const uint32_t d = tm + t % NS * 128 + 64;
+        const uint64_t c2 = dck + t % NC * (kStageBytes / 16) + NB * kColBytes / 16;
 #pragma unroll
         for (int k = 0; k < NB * 4; ++k)
-          if (k < ks && lead) umma::mma_f16(d + 64, dr2 + row_step(k), c2 + col_step(k), id_s, k > 0);
-        if (lead) umma::commit(&sh.dp_done[b]);
+          if (k < ks && lead) umma::mma_f16(d, dr2 + row_step(k), c2 + col_step(k), id_s, k > 0);
+        if (lead) umma::commit(&sh.dp_done[t % NS]);
       };
-      auto issue_acc = [&](int t) {
-        const int b = t % NS;
-        const uint32_t d = tm + b * 128;
-        const uint64_t c1 = dcm + t % kStages * (kStageBytes / 16), c2 = c1 + NB * kColBytes / 16;
-        mbar_wait(&sh.p_ready[b], (t / NS) & 1);
+      auto issue_acc = [&](int t, uint32_t acc, int which, uint64_t* bar) {  // which = 0: dS C1, 1: P C2
+        const uint32_t d = tm + t % NS * 128 + (which ? 0 : 64);
+        const uint64_t cm = dcm + t % NC * (kStageBytes / 16) + which * (NB * kColBytes / 16);
         umma::fence_after_sync();
-        if (KV)
-#pragma unroll
-          for (int k = 0; k < kNC / 16; ++k)
-            if (lead) umma::mma_f16_ta(tm + kAcc2, d + k * 8, c2 + k * 128, id_a, t > 0 || k > 0);
 #pragma unroll
         for (int k = 0; k < kNC / 16; ++k)
-            if (lead) umma::mma_f16_ta(tm + kAcc1, d + 64 + k * 8, c1 + k * 128, id_a, t > 0 || k > 0);
-        if (lead) umma::commit(&sh.acc_done);
+          if (lead) umma::mma_f16_ta(tm + acc, d + k * 8, cm + k * 128, id_a, t > 0 || k > 0);
+        if (lead) umma::commit(bar);
       };
-      if (lead) mbar_arrive_expect_tx(&sh.r_full, 2 * NB * kTileBytes);
-      if (lead)
+      if (lead) {
+        mbar_arrive_expect_tx(&sh.r_full, 2 * NB * kTileBytes);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        tma_load_3d(sR1 + b * kTileBytes, &tr1, b * 64, hr, r0, &sh.r_full);
-        tma_load_3d(sR2 + b * kTileBytes, &tr2, b * 64, hr, r0, &sh.r_full);
+        for (int b = 0; b < NB; ++b) {
+          tma_load_3d(sR1 + b * kTileBytes, &tr1, b * 64, hr, r0, &sh.r_full);
+          tma_load_3d(sR2 + b * kTileBytes, &tr2, b * 64, hr, r0, &sh.r_full);
+        }
       }
       load_c(0);
       if (nsink == 0)
-        for (int t = 1; t < min(n, kStages); ++t) load_c(t);
+        for (int t = 1; t < min(n, NC); ++t) load_c(t);
       mbar_wait(&sh.r_full, 0);
-      issue_s(0);
       if (nsink) {
         // the sink tile by itself: its sums over the queries use the other stages' memory and columns
-        issue_acc(0);
-        mbar_wait(&sh.acc_done, 0);
+        issue_s(0);
+        issue_dp(0);
+        mbar_wait(&sh.p_ready[0], 0);
+        mbar_wait(&sh.ds_ready[0], 0);
+        issue_acc(0, kAcc1, 0, &sh.acc1_done);
         const uint32_t id_t = umma::idesc_f16(128, A.Dh, Fmt<T>::id, 1, 1);  // rows at and behind 64 are not used
-        const uint32_t pt = ac + kStageBytes, dst = pt + kTileBytes;
+        const uint64_t pt = umma::sdesc_mn(ac + kStageBytes, kTileBytes), dst = pt + kTileBytes / 16;
+        const uint64_t r1m = umma::sdesc_mn(ar1, kTileBytes), r2m = umma::sdesc_mn(ar2, kTileBytes);
+#pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (lead) umma::mma_f16(tm + kAcc2, umma::sdesc_mn(pt + k * 2048, kTileBytes), umma::sdesc_mn(ar2 + k * 2048, kTileBytes), id_t, k > 0);
+          if (lead) umma::mma_f16(tm + kAcc2, pt + k * 128, r2m + k * 128, id_t, k > 0);
+#pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (lead) umma::mma_f16(tm + (NS == 1 ? 0 : 128), umma::sdesc_mn(dst + k * 2048, kTileBytes),
-                        umma::sdesc_mn(ar1 + k * 2048, kTileBytes), id_t, k > 0);
+          if (lead) umma::mma_f16(tm + kSinkK, dst + k * 128, r1m + k * 128, id_t, k > 0);
         if (lead) umma::commit(&sh.sink_done);
+        mbar_wait(&sh.acc1_done, 0);
         mbar_wait(&sh.sink_read, 0);
         umma::fence_after_sync();
-        for (int t = 1; t < min(n, kStages + 1); ++t) load_c(t);
-        if (n > 1) issue_s(1);
+        for (int t = 1; t < min(n, NC + 1); ++t) load_c(t);
       }
+      for (int t = nsink; t < min(n, nsink + NS); ++t) {
+        issue_s(t);
+        issue_dp(t);
+      }
+      auto next_dp = [&](int t) {  // the dP that takes the place of tile t's dS
+        mbar_wait(&sh.acc1_done, t & 1);
+        umma::fence_after_sync();
+        if (t + NC < n) load_c(t + NC);
+        if (t + NS < n) issue_dp(t + NS);
+      };
       for (int t = nsink; t < n; ++t) {
-        if (NS == 2 && t + 1 < n) {
-          if (t > nsink) {
-            mbar_wait(&sh.acc_done, (t - 1) & 1);
-            if (t - 1 + kStages < n) load_c(t - 1 + kStages);
-          }
-          issue_s(t + 1);
+        if (NS == 1 && t > nsink) next_dp(t - 1);
+        mbar_wait(&sh.p_ready[t % NS], (t / NS) & 1);
+        if (KV) issue_acc(t, kAcc2, 1, &sh.acc2_done);
+        else if (t + NS < n) issue_s(t + NS);
+        if (NS > 1 && t > nsink) next_dp(t - 1);
+        mbar_wait(&sh.ds_ready[t % NS], (t / NS) & 1);
+        if (KV && t + NS < n) {
+          mbar_wait(&sh.acc2_done, t & 1);
+          issue_s(t + NS);
         }
-        issue_acc(t);
-        if (NS == 1 && t + 1 < n) {
-          mbar_wait(&sh.acc_done, t & 1);
-          if (t + kStages < n) load_c(t + kStages);
-          issue_s(t + 1);
-        }
+        issue_acc(t, kAcc1, 0, &sh.acc1_done);
       }
       if (lead) umma::commit(&sh.all_done);
     }
@@ -279,20 +299,17 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
         asm volatile("bar.sync %0, 128;" ::"r"(2 + wg) : "memory");
       }
       uint32_t s[2][32], p[32], ds[32], see[2] = {0, 0};
-      mbar_wait(&sh.s_done[b], ph);
-      umma::fence_after_sync();
-#pragma unroll
-      for (int x = 0; x < 2; ++x) umma::tmem_ld32(trow + b * 128 + x * 32, s[x]);
       const uint64_t c2 = pair(c, c), l2 = pair(-lse_r, -lse_r), d2 = pair(-delta_r, -delta_r), f2 = pair(f, f);
+      if (!full)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int at = k0 + x * 32;
+          see[x] = sink ? bits(s_lo - at, min(s_hi, send) - at) : bits(lo - at, hi - at) | bits(s_lo - at, s_hi - at);
+        }
       // the masks' selects are kept out of the tiles that every row sees in full
       auto to_p = [&](auto masked) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          umma::tmem_wait_ld(s[x]);
-          if (masked) {
-            const int at = k0 + x * 32;
-            see[x] = sink ? bits(s_lo - at, min(s_hi, send) - at) : bits(lo - at, hi - at) | bits(s_lo - at, s_hi - at);
-          }
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const uint64_t l = KV ? *reinterpret_cast<const uint64_t*>(&sh.lse[wg][x * 32 + 2 * j]) : l2;
@@ -304,9 +321,8 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
               e1 = see[x] >> (2 * j + 1) & 1 ? e1 : 0.f;
             }
             s[x][2 * j] = __float_as_uint(e0), s[x][2 * j + 1] = __float_as_uint(e1);
-            p[x * 16 + j] = Fmt<T>::pack(e0, e1);
+            if (KV || sink) p[x * 16 + j] = Fmt<T>::pack(e0, e1);
           }
-        }
       };
       auto to_ds = [&](auto masked) {
 #pragma unroll
@@ -329,25 +345,40 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
           }
         }
       };
+      mbar_wait(&sh.s_done[b], ph);
+      umma::fence_after_sync();
+#pragma unroll
+      for (int x = 0; x < 2; ++x) umma::tmem_ld32(trow + b * 128 + x * 32, s[x]);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) umma::tmem_wait_ld(s[x]);
+      if (!KV) {  // S has been read
+        umma::fence_before_sync();
+        mbar_arrive(&sh.p_ready[b]);
+      }
       if (full) to_p(std::false_type{});
       else to_p(std::true_type{});
-      mbar_wait(&sh.dp_done[b], ph);
-      umma::fence_after_sync();
-      if (full) to_ds(std::false_type{});
-      else to_ds(std::true_type{});
-      if (KV) umma::tmem_st32(trow + b * 128, p);
-      umma::tmem_st32(trow + b * 128 + 64, ds);
       if (k0 + kNC > end) {  // columns behind the last sequence: as above
-        mbar_wait(&sh.c_full[t % kStages], (t / kStages) & 1);
+        mbar_wait(&sh.c_full[t % NC], (t / NC) & 1);
         for (int x = row; x < kNC * NB * 2; x += 128) {
           const int cr = x % kNC;
           if (k0 + cr >= end)
 #pragma unroll
             for (int y = 0; y < 8; ++y)
-              *reinterpret_cast<int4*>(sC + t % kStages * kStageBytes + x / kNC * kColBytes + cr * 128 + y * 16) = make_int4(0, 0, 0, 0);
+              *reinterpret_cast<int4*>(sC + t % NC * kStageBytes + x / kNC * kColBytes + cr * 128 + y * 16) = make_int4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
       }
+      if (KV) {
+        umma::tmem_st32(trow + b * 128, p);
+        umma::tmem_wait_st();
+        umma::fence_before_sync();
+        mbar_arrive(&sh.p_ready[b]);
+      }
+      mbar_wait(&sh.dp_done[b], ph);
+      umma::fence_after_sync();
+      if (full) to_ds(std::false_type{});
+      else to_ds(std::true_type{});
+      umma::tmem_st32(trow + b * 128 + 64, ds);
       if (sink) {
         unsigned char *sp = sC + kStageBytes, *sd = sp + kTileBytes;
 #pragma unroll
@@ -359,7 +390,7 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
       }
       umma::tmem_wait_st();
       umma::fence_before_sync();
-      mbar_arrive(&sh.p_ready[b]);
+      mbar_arrive(&sh.ds_ready[b]);
       if (sink) {
         mbar_wait(&sh.sink_done, 0);
         umma::fence_after_sync();
@@ -368,7 +399,7 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
           float* pv = P.part + part_at(A, blockIdx.x, hr, 1, row);
           for (int d = 0; d < A.Dh; d += 32) {
             uint32_t gk[32], gv[32];
-            umma::tmem_ld32(trow + (NS == 1 ? 0 : 128) + d, gk);
+            umma::tmem_ld32(trow + kSinkK + d, gk);
             umma::tmem_ld32(trow + kAcc2 + d, gv);
             umma::tmem_wait_ld(gk);
             umma::tmem_wait_ld(gv);
@@ -396,13 +427,12 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
       if (r - s.start < A.sinks && (int64_t)first_far(A, r) * 128 < s.end)
         far = P.part + part_at(A, first_far(A, s.start), hk * G, 0, r - s.start);
     }
-    // the warpgroups share the work: halves of grad_q, or grad_k and grad_v
+    // the warpgroups share the blocks of 32 columns
     for (int a = 0; a < (KV ? 2 : 1); ++a) {
-      if (KV && NS == 2 && a != wg) continue;
       const float scale = a == 0 ? A.scale : 1.f, fa = a == 0 ? 1.f / f : 1.f;
       T* g = (T*)(a == 1 ? A.gv : KV ? A.gk : A.gq) + at;
       for (int d = 0; d < A.Dh; d += 32) {
-        if (!KV && NS == 2 && (d >> 6) != wg) continue;
+        if ((a * A.Dh + d) / 32 % NS != wg) continue;
         uint32_t o[32];
         umma::tmem_ld32(trow + (a == 0 ? kAcc1 : kAcc2) + d, o);
         umma::tmem_wait_ld(o);
@@ -515,7 +545,7 @@ static int bwd_one(const BwdArgs& P, cudaStream_t st) {
   auto kernel = attn_bwd_kernel<T, NB, KV>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return set_error(MR_E_LAUNCH, "attn_bwd_kernel: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  kernel<<<dim3((A.T + 127) / 128, KV ? A.Hkv : A.Hq), NB == 1 ? 160 : 288, smem, st>>>(P, r1, r2, c1, c2);
+  kernel<<<dim3((A.T + 127) / 128, KV ? A.Hkv : A.Hq), kBwdThreads<NB>, smem, st>>>(P, r1, r2, c1, c2);
   return check_launch(KV ? "attn_bwd_kernel (grad_k, grad_v)" : "attn_bwd_kernel (grad_q)");
 }
 
