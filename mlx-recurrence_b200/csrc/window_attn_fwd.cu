@@ -3,21 +3,21 @@
 //
 // A CTA takes 128 queries of one head and walks the keys they may see in tiles
 // of 128: S = Q K^T into TMEM, the online softmax by four warps (one thread per
-// query, so no reduction across threads), P back into TMEM over S as the A
-// operand of O += P V. The row's maximum is only moved when it grows by more
-// than 2^8 (the factor cancels in O / l), so O is rarely rescaled. A fifth warp's
-// first thread issues copies and products; a CTA's steps depend on each other,
-// and the second CTA of the SM fills the gaps (256 TMEM columns and at most 96 KB
-// of shared memory each).
+// query, so no reduction across threads), P back into TMEM as the A operand of
+// O += P V. The row's maximum is only moved when it grows by more
+// than 2^8 (the factor cancels in O / l), so O is rarely rescaled. Where TMEM has
+// room for P beside S (Dh <= 64) the next S runs under this tile's exponentials.
+// Two CTAs per SM (256 TMEM columns and at most 96 KB of shared memory each) fill
+// each other's gaps.
 #include "window_tc.cuh"
 
 namespace mr {
 
-constexpr int kFwdThreads = 160;
+constexpr int kFwdThreads = 256;  // a warpgroup for the softmax, one (a single busy warp) that issues
 constexpr float kRescale = 8.f;
 
 struct FwdShared {
-  uint64_t k_full, v_full, s_done, p_ready, o_done;
+  uint64_t k_full, v_full, s_done, s_read, p_ready, o_done;
   uint32_t tmem;
   int lo_max;  // the largest first key of the tile's queries
   uint32_t again[4];
@@ -34,7 +34,7 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   unsigned char *sQ = sm, *sK = sQ + NB * kTileBytes, *sV = sK + NB * kTileBytes;
   __shared__ FwdShared sh;
-  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, w = tid >> 5;
   const int h = blockIdx.y, hk = h / (A.Hq / A.Hkv), q0 = blockIdx.x * 128, i = q0 + tid;
   const KeyRange R = keys_of(A, q0, q0 + 128);
   const int nsink = R.send > R.s0 ? 1 : 0;  // at most 64 sinks: one tile
@@ -49,7 +49,7 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
   }
   if (tid == 0) {
     mbar_init(&sh.k_full, 1), mbar_init(&sh.v_full, 1), mbar_init(&sh.s_done, 1), mbar_init(&sh.o_done, 1);
-    mbar_init(&sh.p_ready, 128);
+    mbar_init(&sh.s_read, 128), mbar_init(&sh.p_ready, 128);
     fence_mbar_init();
     sh.lo_max = 0;
   }
@@ -64,70 +64,83 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
   // the sink tile has few keys: products and softmax take whole 16 (32) column groups of it
   const int sink_n = nsink ? (R.send - R.s0 + 15) & ~15 : 0;
 
-  if (w == 4) {
-    {
-      const bool lead = umma::elect_one();
-      // descriptors are made once and stepped by additions
-      const uint64_t dq = umma::sdesc_k(smem_u32(sQ)), dk = umma::sdesc_k(smem_u32(sK)), dv = umma::sdesc_mn(smem_u32(sV), kTileBytes);
-      const int ks = A.Dh / 16;
-      auto load = [&](const CUtensorMap* m, unsigned char* dst, int head, int row, uint64_t* bar) {
-        if (lead)
+  if (w >= 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (w == 4) {
+  // Descriptors are made once and stepped by additions.
+  const bool lead = umma::elect_one();
+  const uint64_t dq = umma::sdesc_k(smem_u32(sQ)), dk = umma::sdesc_k(smem_u32(sK)), dv = umma::sdesc_mn(smem_u32(sV), kTileBytes);
+  const int ks = A.Dh / 16;
+  const uint32_t ido = umma::idesc_f16(128, A.Dh, Fmt<T>::id, 0, 1);
+  auto load = [&](const CUtensorMap* m, unsigned char* dst, int head, int r, uint64_t* bar) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) tma_load_3d(dst + b * kTileBytes, m, b * 64, head, row, bar);
-      };
-      auto key0 = [&](int t) { return t < nsink ? R.s0 : R.kmin + (t - nsink) * 128; };
-      if (lead) mbar_arrive_expect_tx(&sh.k_full, 2 * NB * kTileBytes);
+    for (int b = 0; b < NB; ++b) tma_load_3d(dst + b * kTileBytes, m, b * 64, head, r, bar);
+  };
+  auto key0 = [&](int t) { return t < nsink ? R.s0 : R.kmin + (t - nsink) * 128; };
+  auto cols = [&](int t) { return t < nsink ? sink_n : 128; };
+  auto load_k = [&](int t) {
+    if (lead) {
+      mbar_arrive_expect_tx(&sh.k_full, NB * kTileBytes);
+      load(&tk, sK, hk, key0(t), &sh.k_full);
+    }
+  };
+  auto load_v = [&](int t) {
+    if (lead) {
+      mbar_arrive_expect_tx(&sh.v_full, NB * kTileBytes);
+      load(&tv, sV, hk, key0(t), &sh.v_full);
+    }
+  };
+  auto issue_s = [&](int t) {
+    mbar_wait(&sh.k_full, t & 1);
+    umma::fence_after_sync();
+    const uint32_t ids = umma::idesc_f16(128, cols(t), Fmt<T>::id, 0, 0);
+#pragma unroll
+    for (int k = 0; k < NB * 4; ++k) {
+      const int o = (k >> 2) * (kTileBytes / 16) + (k & 3) * 2;
+      if (k < ks && lead) umma::mma_f16(tm, dq + o, dk + o, ids, k > 0);
+    }
+    if (lead) umma::commit(&sh.s_done);
+  };
+  auto issue_o = [&](int t) {
+    mbar_wait(&sh.v_full, t & 1);
+    umma::fence_after_sync();
+    const int kp = cols(t) / 16;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < kp && lead) umma::mma_f16_ta(tm + kO, tm + kP + k * 8, dv + k * 128, ido, t > 0 || k > 0);
+    if (lead) umma::commit(&sh.o_done);
+  };
+    if (lead) {
+      mbar_arrive_expect_tx(&sh.k_full, 2 * NB * kTileBytes);
       load(&tq, sQ, h, q0, &sh.k_full);
       load(&tk, sK, hk, key0(0), &sh.k_full);
-      if (lead) mbar_arrive_expect_tx(&sh.v_full, NB * kTileBytes);
-      load(&tv, sV, hk, key0(0), &sh.v_full);
-      const uint32_t ido = umma::idesc_f16(128, A.Dh, Fmt<T>::id, 0, 1);
-      auto cols = [&](int t) { return t < nsink ? sink_n : 128; };
-      auto issue_s = [&](int t) {
-        mbar_wait(&sh.k_full, t & 1);
-        umma::fence_after_sync();
-        const uint32_t ids = umma::idesc_f16(128, cols(t), Fmt<T>::id, 0, 0);
-#pragma unroll
-        for (int k = 0; k < NB * 4; ++k) {
-          constexpr int kBlock = kTileBytes / 16;
-          const int o = (k >> 2) * kBlock + (k & 3) * 2;
-          if (k < ks && lead) umma::mma_f16(tm, dq + o, dk + o, ids, k > 0);
-        }
-        if (lead) umma::commit(&sh.s_done);
-      };
-      auto load_v = [&](int t) {
-        if (lead) mbar_arrive_expect_tx(&sh.v_full, NB * kTileBytes);
-        load(&tv, sV, hk, key0(t), &sh.v_full);
-      };
-      issue_s(0);
-      for (int t = 0; t < ntile; ++t) {
-        mbar_wait(&sh.s_done, t & 1);
+    }
+    load_v(0);
+    issue_s(0);
+    for (int t = 0; t < ntile; ++t) {
+      mbar_wait(&sh.s_done, t & 1);
+      if (t + 1 < ntile) load_k(t + 1);
+      if (kOwnP) {
         if (t + 1 < ntile) {
-          if (lead) mbar_arrive_expect_tx(&sh.k_full, NB * kTileBytes);
-          load(&tk, sK, hk, key0(t + 1), &sh.k_full);
+          mbar_wait(&sh.s_read, t & 1);
+          issue_s(t + 1);
         }
-        if (kOwnP && t > 0) {
+        if (t > 0) {
           mbar_wait(&sh.o_done, (t - 1) & 1);
           load_v(t);
         }
-        mbar_wait(&sh.p_ready, t & 1);
-        if (kOwnP && t + 1 < ntile) issue_s(t + 1);  // S has been read; P lies elsewhere
-        mbar_wait(&sh.v_full, t & 1);
-        umma::fence_after_sync();
-        const int kp = cols(t) / 16;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (k < kp && lead) umma::mma_f16_ta(tm + kO, tm + kP + k * 8, dv + k * 128, ido, t > 0 || k > 0);
-        if (lead) umma::commit(&sh.o_done);
-        if (!kOwnP && t + 1 < ntile) {
-          mbar_wait(&sh.o_done, t & 1);  // P is read: the next S overwrites it
-          load_v(t + 1);
-          issue_s(t + 1);
-        }
+      }
+      mbar_wait(&sh.p_ready, t & 1);
+      issue_o(t);
+      if (!kOwnP && t + 1 < ntile) {
+        mbar_wait(&sh.o_done, t & 1);  // P is read: the next S overwrites it
+        load_v(t + 1);
+        issue_s(t + 1);
       }
     }
-    __syncwarp();
+    }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const RowMask rm = row_mask(A, i);
     const int lo = rm.i < 0 ? 0 : rm.lo;
     atomicMax(&sh.lo_max, __reduce_max_sync(0xffffffffu, lo));
@@ -152,24 +165,24 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
         see[b] = bits(rm.start - at, min(min(rm.sink_end, rm.i + 1), sink ? R.send : INT32_MAX) - at);
         if (!sink) see[b] |= bits(rm.lo - at, rm.i + 1 - at);
       }
-      // first over S for the maximum, then again for the exponentials: S stays in TMEM, not in 128 registers
-      auto masked = [&](uint32_t (&s)[32], int b) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = see[b] >> j & 1 ? s[j] : 0xff800000u;
-      };
-      uint32_t s[2][32];
+      uint32_t s[4][32];
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       umma::tmem_ld32(trow, s[0]);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
+      for (int b = 0; b < 4; ++b) {  // a block's maximum while the next block comes
         if (b >= nch) continue;
-        umma::tmem_wait_ld(s[b & 1]);
-        if (b + 1 < nch) umma::tmem_ld32(trow + (b + 1) * 32, s[(b + 1) & 1]);
-        if (!full) masked(s[b & 1], b);
+        umma::tmem_wait_ld(s[b]);
+        if (b + 1 < nch) umma::tmem_ld32(trow + (b + 1) * 32, s[b + 1 < 4 ? b + 1 : 3]);
+        if (!full)
 #pragma unroll
-        for (int j = 0; j < 32; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(s[b & 1][j]));
+          for (int j = 0; j < 32; ++j) s[b][j] = see[b] >> j & 1 ? s[b][j] : 0xff800000u;
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) mx4[j >> 1 & 3] = max3(mx4[j >> 1 & 3], __uint_as_float(s[b][j]), __uint_as_float(s[b][j + 1]));
       }
-      umma::tmem_ld32(trow, s[0]);
+      if (kOwnP) {  // the next S may start under this tile's exponentials
+        umma::fence_before_sync();
+        mbar_arrive(&sh.s_read);
+      }
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       if (t > 0) {  // P and O are free
         mbar_wait(&sh.o_done, (t - 1) & 1);
@@ -181,11 +194,12 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
         m = to, l *= f;
         if (t > 0)
           for (int d = 0; d < A.Dh; d += 32) {
-            umma::tmem_ld32(trow + kO + d, s[1]);
-            umma::tmem_wait_ld(s[1]);
+            uint32_t o[32];
+            umma::tmem_ld32(trow + kO + d, o);
+            umma::tmem_wait_ld(o);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) s[1][j] = __float_as_uint(__uint_as_float(s[1][j]) * f);
-            umma::tmem_st32(trow + kO + d, s[1]);
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+            umma::tmem_st32(trow + kO + d, o);
           }
       }
       const float mc = m == -INFINITY ? 0.f : m * c;
@@ -194,14 +208,11 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         if (b >= nch) continue;
-        umma::tmem_wait_ld(s[b & 1]);
-        if (b + 1 < nch) umma::tmem_ld32(trow + (b + 1) * 32, s[(b + 1) & 1]);
-        if (!full) masked(s[b & 1], b);
         uint32_t p[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           float x0, x1;
-          unpair(fma2(pair(s[b & 1][2 * j], s[b & 1][2 * j + 1]), c2, mc2), x0, x1);
+          unpair(fma2(pair(s[b][2 * j], s[b][2 * j + 1]), c2, mc2), x0, x1);
           x0 = ex2(x0), x1 = ex2(x1);
           sum[j & 1] = add2(sum[j & 1], pair(x0, x1));
           p[j] = Fmt<T>::pack(x0, x1);

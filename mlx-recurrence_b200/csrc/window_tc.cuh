@@ -33,6 +33,12 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // two float32 operations in one instruction
 __device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
   uint64_t r;
