@@ -5,9 +5,13 @@
 // Slot of token t: t (t < sinks), else sinks + (t - sinks) % window. The
 // visible tokens at position p are then exactly the slots below
 // min(p + 1, sinks + window), the newest one among them.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
 namespace mr {
+
+namespace cg = cooperative_groups;
 
 struct StepArgs {
   const void *q, *k, *v;  // [B, Hq, Dh], [B, Hkv, Dh] dense
@@ -84,6 +88,260 @@ __global__ void __launch_bounds__(32 * kStepWarps2) window_step_kernel(const __g
   }
 }
 
+// ---- bf16 and fp16 ------------------------------------------------------------
+// HBM-bound: each visible slot of both caches is read once, for all query heads
+// of the group (up to 16 at a time as the rows of m16n8k16 products, so the
+// arithmetic stays far below the loads whatever the group). A cluster of up to 8
+// CTAs splits a (batch row, key head)'s slots in tiles of 64, brought into shared
+// memory by asynchronous copies kRing tiles ahead; a warp takes 16 slots of a tile
+// with its own online softmax. Warps, then CTAs (over distributed shared memory)
+// join their maxima, sums and outputs in a fixed order; one launch, no workspace.
+
+constexpr int kTile = 64, kRing = 3;
+
+template <typename T> struct Mma;
+template <> struct Mma<__nv_bfloat16> {
+  static __device__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ uint32_t pack(float a, float b) {
+    __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&r);
+  }
+};
+template <> struct Mma<__half> {
+  static __device__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ uint32_t pack(float a, float b) {
+    __half2 r = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&r);
+  }
+};
+
+template <bool TRANS> __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 16 bytes, or zeros where `bytes` is 0
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// 16-byte chunk c of slot row r of a tile: rotated so that the 8 rows of a matrix lie in different banks
+template <int DH> __device__ __forceinline__ int chunk_at(int r, int c) {
+  return r * (DH / 8) + (DH % 64 == 0 ? c ^ (r & 7) : c ^ (r >> 1 & 3));
+}
+
+template <typename T, int DH> constexpr int kStepSmem = kRing * 2 * kTile * DH * 2;
+
+template <typename T, int DH>
+__global__ void __launch_bounds__(128) window_step_mma(const __grid_constant__ StepArgs A, int splits, int head_tiles) {
+  constexpr int NC = DH / 8, KS = DH / 16, kTileB = kTile * DH * 2;
+  extern __shared__ __align__(128) unsigned char sm[];
+  __shared__ float wm[4][16], wl[4][16], cm[16], cl[16];
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int rank = blockIdx.x % splits, unit = blockIdx.x / splits;
+  const int b = blockIdx.y, hk = unit / head_tiles, h0 = unit % head_tiles * 16, G = A.Hq / A.Hkv;
+  const int rows = min(16, G - h0);
+  const int64_t qat = ((int64_t)b * A.Hq + hk * G + h0) * DH;
+  T* y = (T*)A.y + qat;
+  const int64_t p = step_pos(A, b);
+  if (p < 0) {  // the whole cluster
+    if (rank == 0)
+      for (int e = tid; e < rows * DH; e += 128) y[e] = from_f<T>(0.f);
+    return;
+  }
+  const int n = (int)(p < A.slots - 1 ? p + 1 : A.slots), cur = slot_of(p, A.slots, A.sinks);
+  const int tiles = (n + kTile - 1) / kTile, t0 = tiles * rank / splits, t1 = tiles * (rank + 1) / splits;
+  const int64_t in = ((int64_t)b * A.Hkv + hk) * DH, at = ((int64_t)b * A.slots * A.Hkv + hk) * DH;
+  const int64_t step = (int64_t)A.Hkv * DH;
+  const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(sm));
+
+  auto load = [&](int t) {
+    if (t < t1) {
+      const uint32_t dst = base + (t % kRing) * 2 * kTileB;
+      for (int e = tid; e < kTile * NC; e += 128) {
+        const int r = e / NC, c = e % NC, slot = t * kTile + r;
+        const bool now = slot == cur;  // the new token comes from the call, not from the cache
+        const int bytes = slot < n ? 16 : 0;
+        const int64_t off = now ? in + c * 8 : at + min(slot, n - 1) * step + c * 8;
+        copy16(dst + chunk_at<DH>(r, c) * 16, (now ? (const T*)A.k : (const T*)A.ck) + off, bytes);
+        copy16(dst + kTileB + chunk_at<DH>(r, c) * 16, (now ? (const T*)A.v : (const T*)A.cv) + off, bytes);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int i = 0; i < kRing - 1; ++i) load(t0 + i);
+  if (cur / kTile >= t0 && cur / kTile < t1 && h0 == 0 && tid < 2 * NC) {
+    const int c = tid % NC;
+    const T* src = (tid < NC ? (const T*)A.k : (const T*)A.v) + in + c * 8;
+    T* dst = (tid < NC ? (T*)A.ck : (T*)A.cv) + at + cur * step + c * 8;
+    *reinterpret_cast<int4*>(dst) = *reinterpret_cast<const int4*>(src);
+  }
+  // Q as the A operand: rows lane / 4 and + 8
+  uint32_t q[KS][4];
+#pragma unroll
+  for (int k = 0; k < KS; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = (lane >> 2) + (i & 1) * 8, d = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
+      q[k][i] = r < rows ? *reinterpret_cast<const uint32_t*>((const T*)A.q + qat + r * DH + d) : 0u;
+    }
+  const float c = A.scale * 1.4426950408889634f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[NC][4];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+
+  for (int t = t0; t < t1; ++t) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+    __syncthreads();
+    load(t + kRing - 1);
+    const uint32_t sk = base + (t % kRing) * 2 * kTileB, sv = sk + kTileB;
+    const int s0 = w * 16;  // this warp's slots of the tile
+    if (t * kTile + s0 >= n) continue;
+    float s[2][4] = {};
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      uint32_t f[4];
+      ldmatrix4<false>(f, sk + chunk_at<DH>(s0 + (lane >> 4) * 8 + (lane & 7), k * 2 + (lane >> 3 & 1)) * 16);
+      Mma<T>::run(s[0], q[k], f[0], f[1]);
+      Mma<T>::run(s[1], q[k], f[2], f[3]);
+    }
+    uint32_t pa[4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {  // rows lane / 4 and + 8
+      float mx = m[r];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int slot = t * kTile + s0 + (i >> 1) * 8 + (lane & 3) * 2 + (i & 1);
+        float& v = s[i >> 1][r * 2 + (i & 1)];
+        v = slot < n ? v * c : -INFINITY;
+        mx = fmaxf(mx, v);
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float to = mx == -INFINITY ? 0.f : mx, keep = exp2f(m[r] - to);
+      m[r] = mx;
+      l[r] *= keep;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float& v = s[i >> 1][r * 2 + (i & 1)];
+        v = exp2f(v - to);
+        l[r] += v;
+      }
+      pa[r] = Mma<T>::pack(s[0][r * 2], s[0][r * 2 + 1]);
+      pa[r + 2] = Mma<T>::pack(s[1][r * 2], s[1][r * 2 + 1]);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) o[i][r * 2] *= keep, o[i][r * 2 + 1] *= keep;
+    }
+#pragma unroll
+    for (int i = 0; i < NC; i += 2) {
+      uint32_t f[4];
+      ldmatrix4<true>(f, sv + chunk_at<DH>(s0 + (lane >> 3 & 1) * 8 + (lane & 7), i + (lane >> 4)) * 16);
+      Mma<T>::run(o[i], pa, f[0], f[1]);
+      Mma<T>::run(o[i + 1], pa, f[2], f[3]);
+    }
+  }
+  // join the warps: the ring's memory is free
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    if ((lane & 3) == 0) wm[w][(lane >> 2) + r * 8] = m[r], wl[w][(lane >> 2) + r * 8] = l[r];
+  }
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(sm);  // [warp][16][DH], then the sum in warp 0's place
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      *reinterpret_cast<float2*>(so + (w * 16 + (lane >> 2) + r * 8) * DH + i * 8 + (lane & 3) * 2) =
+          make_float2(o[i][r * 2], o[i][r * 2 + 1]);
+  __syncthreads();
+  for (int e = tid; e < rows * DH; e += 128) {
+    const int r = e / DH;
+    float mx = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
+    const float to = mx == -INFINITY ? 0.f : mx;
+    float os = 0.f, ls = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = exp2f(wm[i][r] - to);
+      os = fmaf(so[i * 16 * DH + e], f, os);
+      ls = fmaf(wl[i][r], f, ls);
+    }
+    if (splits == 1) {
+      y[e] = from_f<T>(os / ls);
+    } else {
+      so[e] = os;  // this element's own slot of warp 0
+      if (e % DH == 0) cm[r] = mx, cl[r] = ls;
+    }
+  }
+  if (splits == 1) return;
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  const int all = rows * DH;
+  for (int e = all * rank / splits + tid; e < all * (rank + 1) / splits; e += 128) {
+    const int r = e / DH;
+    float mx = -INFINITY;
+    for (int i = 0; i < splits; ++i) mx = fmaxf(mx, *cluster.map_shared_rank(&cm[r], i));
+    const float to = mx == -INFINITY ? 0.f : mx;
+    float os = 0.f, ls = 0.f;
+    for (int i = 0; i < splits; ++i) {
+      const float f = exp2f(*cluster.map_shared_rank(&cm[r], i) - to);
+      os = fmaf(*cluster.map_shared_rank(&so[e], i), f, os);
+      ls = fmaf(*cluster.map_shared_rank(&cl[r], i), f, ls);
+    }
+    y[e] = from_f<T>(os / ls);
+  }
+  cluster.sync();  // nobody leaves while its memory is read
+}
+
+template <typename T, int DH> static int step_mma_dh(const StepArgs& A, cudaStream_t st) {
+  const int G = A.Hq / A.Hkv, head_tiles = (G + 15) / 16, tiles = (A.slots + kTile - 1) / kTile;
+  const int64_t units = (int64_t)A.B * A.Hkv * head_tiles;
+  // CTAs for four on every SM, each with two tiles at least
+  int splits = 1;
+  while (splits < 8 && units * splits < 148 * 4 && splits * 4 <= tiles) splits *= 2;
+  auto kernel = window_step_mma<T, DH>;
+  constexpr int smem = kStepSmem<T, DH>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return set_error(MR_E_LAUNCH, "window_step_mma: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(A.Hkv * head_tiles * splits), (unsigned)A.B);
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, A, splits, head_tiles);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(MR_E_LAUNCH, "window_step_mma: %s", cudaGetErrorString(e));
+  }
+  return check_launch("window_step_mma");
+}
+template <typename T> static int step_mma(const StepArgs& A, cudaStream_t st) {
+  switch (A.Dh) {
+    case 32: return step_mma_dh<T, 32>(A, st);
+    case 64: return step_mma_dh<T, 64>(A, st);
+    case 96: return step_mma_dh<T, 96>(A, st);
+    default: return step_mma_dh<T, 128>(A, st);
+  }
+}
+
 // cache[s][slot] <- the token that the slot holds after sequence s, or zeros
 template <typename V>
 __global__ void __launch_bounds__(256) window_cache_kernel(const V* __restrict__ k, const V* __restrict__ v,
@@ -150,8 +408,8 @@ int mr_window_step(const void* q, const void* k, const void* v, void* cache_k, v
                    (int)sinks, scale, y};
   switch (dtype) {
     case MR_F32: return window_step_launch<float>(A, (cudaStream_t)stream);
-    case MR_BF16: return window_step_launch<__nv_bfloat16>(A, (cudaStream_t)stream);
-    default: return window_step_launch<__half>(A, (cudaStream_t)stream);
+    case MR_BF16: return step_mma<__nv_bfloat16>(A, (cudaStream_t)stream);
+    default: return step_mma<__half>(A, (cudaStream_t)stream);
   }
 }
 
