@@ -55,7 +55,8 @@ def common_dtype(*tensors):
     """
     dt = tensors[0].dtype
     for t in tensors[1:]:
-        dt = torch.promote_types(dt, t.dtype)
+        if t.dtype != dt:
+            dt = torch.promote_types(dt, t.dtype)
     if dt not in _lib.DTYPE_CODE:
         dt = torch.float32
     return dt

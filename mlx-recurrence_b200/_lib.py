@@ -164,13 +164,24 @@ def stream_of(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def addr(t):
+    """The address of a tensor's data, or None: what a void* argument takes without a ctypes object of its own."""
+    return None if t is None else t.data_ptr()
+
+
+# the stream's handle without a torch.cuda.Stream object around it, where this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def call_on(dev, name, *args):
     """:func:`call` on ``dev``, with its current stream as the last argument."""
-    if torch.cuda.current_device() == dev.index:
-        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
-    else:
+    if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
-            call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+            return call_on(dev, name, *args)
+    call(name, *args, _raw_stream(dev.index) if _raw_stream else torch.cuda.current_stream(dev).cuda_stream)
+
+
+_usable = set()  # devices that have passed require_cuda's check
 
 
 def require_cuda(*tensors):
@@ -182,7 +193,9 @@ def require_cuda(*tensors):
                                "there is no CPU path")
         if t.device != dev:
             raise RuntimeError("all scan inputs must be on the same CUDA device")
-    major, _ = torch.cuda.get_device_capability(dev)
-    if major != 10:
-        raise RuntimeError(f"libmlrec is built for sm_100a; device {dev} is sm_{major}x")
+    if dev not in _usable:
+        major, _ = torch.cuda.get_device_capability(dev)
+        if major != 10:
+            raise RuntimeError(f"libmlrec is built for sm_100a; device {dev} is sm_{major}x")
+        _usable.add(dev)
     return dev

@@ -19,6 +19,7 @@
 // backward runs the same scheme from the right, and rebuilds h from the states
 // that the forward kept per chunk.
 #include "common.cuh"
+#include "launch.cuh"
 #include "tma.cuh"
 #include "tmap.cuh"
 
@@ -703,17 +704,21 @@ template <typename T, bool BWD> static int launch(const char* what, PackedArgs P
     if (BWD)
       if (int rc = make_tmap_2d(&tg, P.gy, TmapType<float>::v, 4, P.D, P.L, P.D * 4, 32 * V, kChunk)) return rc;
   }
-  auto go = [&](auto kernel, int threads, auto... maps) {
-    const cudaError_t er = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (er != cudaSuccess) return set_error(MR_E_LAUNCH, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(er));
-    kernel<<<grid, threads, smem, st>>>(P, maps...);
-    return check_launch(what);
-  };
+  // (one instantiation each: the shared memory is the same for every call of it)
+#define MR_GO(KERNEL, THREADS, ...)                                \
+  do {                                                             \
+    if (int rc = allow_smem<KERNEL>(smem, what)) return rc;        \
+    KERNEL<<<grid, THREADS, smem, st>>>(P, __VA_ARGS__);           \
+    return check_launch(what);                                     \
+  } while (0)
   if constexpr (BWD) {
-    return tma ? go(packed_bwd_kernel<T, true>, kWarps * 32 + 32, ta, tx, tg) : go(packed_bwd_kernel<T, false>, kWarps * 32, ta, tx, tg);
+    if (tma) MR_GO((packed_bwd_kernel<T, true>), kWarps * 32 + 32, ta, tx, tg);
+    MR_GO((packed_bwd_kernel<T, false>), kWarps * 32, ta, tx, tg);
   } else {
-    return tma ? go(packed_fwd_kernel<T, true>, kWarps * 32 + 32, ta, tx) : go(packed_fwd_kernel<T, false>, kWarps * 32, ta, tx);
+    if (tma) MR_GO((packed_fwd_kernel<T, true>), kWarps * 32 + 32, ta, tx);
+    MR_GO((packed_fwd_kernel<T, false>), kWarps * 32, ta, tx);
   }
+#undef MR_GO
 }
 
 int packed_device_error(bool clear) { return read_device_error(clear); }

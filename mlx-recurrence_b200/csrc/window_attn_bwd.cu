@@ -542,10 +542,8 @@ static int bwd_one(const BwdArgs& P, cudaStream_t st) {
   if (int rc = head_map(KV ? &r1 : &c1, A.k, dt, A, A.Hkv, A.k_ts, A.k_hs, KV ? 128 : kNC)) return rc;
   if (int rc = head_map(KV ? &r2 : &c2, A.v, dt, A, A.Hkv, A.v_ts, A.v_hs, KV ? 128 : kNC)) return rc;
   constexpr int smem = kStages * 2 * NB * kColBytes + 2 * NB * kTileBytes + 1024;
-  auto kernel = attn_bwd_kernel<T, NB, KV>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return set_error(MR_E_LAUNCH, "attn_bwd_kernel: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  kernel<<<dim3((A.T + 127) / 128, KV ? A.Hkv : A.Hq), kBwdThreads<NB>, smem, st>>>(P, r1, r2, c1, c2);
+  if (int rc = allow_smem<attn_bwd_kernel<T, NB, KV>>(smem, "attn_bwd_kernel")) return rc;
+  attn_bwd_kernel<T, NB, KV><<<dim3((A.T + 127) / 128, KV ? A.Hkv : A.Hq), kBwdThreads<NB>, smem, st>>>(P, r1, r2, c1, c2);
   return check_launch(KV ? "attn_bwd_kernel (grad_k, grad_v)" : "attn_bwd_kernel (grad_q)");
 }
 

@@ -272,8 +272,7 @@ template <typename T, int NB> static int fwd_nb(const AttnArgs& A, cudaStream_t 
   if (int rc = head_map(&tk, A.k, dt, A, A.Hkv, A.k_ts, A.k_hs, 128)) return rc;
   if (int rc = head_map(&tv, A.v, dt, A, A.Hkv, A.v_ts, A.v_hs, 128)) return rc;
   constexpr int smem = 3 * NB * kTileBytes + 1024;
-  const cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return set_error(MR_E_LAUNCH, "attn_fwd_kernel: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  if (int rc = allow_smem<attn_fwd_kernel<T, NB>>(smem, "attn_fwd_kernel")) return rc;
   attn_fwd_kernel<T, NB><<<dim3((A.T + 127) / 128, A.Hq), kFwdThreads, smem, st>>>(A, tq, tk, tv);
   return check_launch("attn_fwd_kernel");
 }

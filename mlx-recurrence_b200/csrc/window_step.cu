@@ -8,6 +8,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "launch.cuh"
 
 namespace mr {
 
@@ -314,8 +315,7 @@ template <typename T, int DH> static int step_mma_dh(const StepArgs& A, cudaStre
   while (splits < 8 && units * splits < 148 * 4 && splits * 4 <= tiles) splits *= 2;
   auto kernel = window_step_mma<T, DH>;
   constexpr int smem = kStepSmem<T, DH>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return set_error(MR_E_LAUNCH, "window_step_mma: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  if (int rc = allow_smem<window_step_mma<T, DH>>(smem, "window_step_mma")) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(A.Hkv * head_tiles * splits), (unsigned)A.B);
   cfg.blockDim = dim3(128);
@@ -326,7 +326,7 @@ template <typename T, int DH> static int step_mma_dh(const StepArgs& A, cudaStre
   attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, A, splits, head_tiles);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, A, splits, head_tiles);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return set_error(MR_E_LAUNCH, "window_step_mma: %s", cudaGetErrorString(e));

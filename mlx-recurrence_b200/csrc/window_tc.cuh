@@ -4,6 +4,7 @@
 
 #include "window_attn.cuh"
 
+#include "launch.cuh"
 #include "tma.cuh"
 #include "tmap.cuh"
 #include "umma.cuh"

@@ -200,30 +200,34 @@ def rglru_scan_gated_with_state(x, r, i, lam, c=8.0, seg=DEFAULT_SEG, h0=None):
     return _RGLRUGatedScan.apply(x, r, i, lam, c, seg, h0, True)
 
 
+def _packed_forward(a, x, cu_seqlens, h0, want_final, want_ckpt):
+    if a.dim() != 2 or x.shape != a.shape or a.shape[1] == 0:
+        raise ValueError(f"a and x must both be [T, D] with D > 0, got {tuple(a.shape)} and {tuple(x.shape)}")
+    T, D = a.shape
+    dev = _lib.require_cuda(a, x)
+    dt = common_dtype(a, x)
+    cu = prep_cu(cu_seqlens, dev)
+    S = cu.numel() - 1
+    a_, x_ = prep(a, dt), prep(x, dt)
+    h0_ = prep_h0(h0, (S, D), dev)
+    lib = _lib.load()
+    f32 = dict(dtype=torch.float32, device=dev)
+    y = torch.empty((T, D), **f32)
+    final = torch.empty((S, D), **f32) if want_final else None
+    ckpt = torch.empty((-(-T // lib.mr_rglru_packed_chunk()), D), **f32) if want_ckpt else None
+    nws = lib.mr_rglru_packed_workspace_bytes(T, D)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    _lib.call_on(dev, "mr_rglru_packed_fwd", a_.data_ptr(), x_.data_ptr(), cu.data_ptr(), S, _lib.DTYPE_CODE[dt], T, D,
+                 _lib.addr(h0_), y.data_ptr(), _lib.addr(ckpt), _lib.addr(final), _lib.addr(ws), nws)
+    return y, final, (a_, x_, cu, ckpt, h0_)
+
+
 class _RGLRUPacked(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, x, cu_seqlens, h0, want_final):
         ctx.set_materialize_grads(False)
-        if a.dim() != 2 or x.shape != a.shape or a.shape[1] == 0:
-            raise ValueError(f"a and x must both be [T, D] with D > 0, got {tuple(a.shape)} and {tuple(x.shape)}")
-        T, D = a.shape
-        dev = _lib.require_cuda(a, x)
-        dt = common_dtype(a, x)
-        cu = prep_cu(cu_seqlens, dev)
-        S = cu.numel() - 1
-        a_, x_ = prep(a, dt), prep(x, dt)
-        h0_ = prep_h0(h0, (S, D), dev)
-        lib = _lib.load()
-        y = torch.empty((T, D), dtype=torch.float32, device=dev)
-        final = torch.empty((S, D), dtype=torch.float32, device=dev) if want_final else None
-        ckpt = None
-        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or ctx.needs_input_grad[3]:
-            ckpt = torch.empty((-(-T // lib.mr_rglru_packed_chunk()), D), dtype=torch.float32, device=dev)
-        nws = lib.mr_rglru_packed_workspace_bytes(T, D)
-        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-        _lib.call_on(dev, "mr_rglru_packed_fwd", a_.data_ptr(), x_.data_ptr(), cu.data_ptr(), S, _lib.DTYPE_CODE[dt],
-                     T, D, _lib.ptr(h0_), y.data_ptr(), _lib.ptr(ckpt), _lib.ptr(final), _lib.ptr(ws), nws)
-        ctx.save_for_backward(a_, x_, cu, ckpt, h0_)
+        y, final, saved = _packed_forward(a, x, cu_seqlens, h0, want_final, True)
+        ctx.save_for_backward(*saved)
         return y, final
 
     @staticmethod
@@ -238,10 +242,16 @@ class _RGLRUPacked(torch.autograd.Function):
         gh0 = torch.empty_like(h0_) if (h0_ is not None and ctx.needs_input_grad[3]) else None
         nws = _lib.load().mr_rglru_packed_workspace_bytes(T, D)
         ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-        _lib.call_on(dev, "mr_rglru_packed_bwd", gy.data_ptr(), _lib.ptr(gf), ckpt.data_ptr(), a_.data_ptr(),
-                     x_.data_ptr(), cu.data_ptr(), cu.numel() - 1, _lib.DTYPE_CODE[dt], T, D, _lib.ptr(h0_),
-                     ga.data_ptr(), gx.data_ptr(), _lib.ptr(gh0), _lib.ptr(ws), nws)
+        _lib.call_on(dev, "mr_rglru_packed_bwd", gy.data_ptr(), _lib.addr(gf), ckpt.data_ptr(), a_.data_ptr(),
+                     x_.data_ptr(), cu.data_ptr(), cu.numel() - 1, _lib.DTYPE_CODE[dt], T, D, _lib.addr(h0_),
+                     ga.data_ptr(), gx.data_ptr(), _lib.addr(gh0), _lib.addr(ws), nws)
         return ga, gx, None, gh0, None
+
+
+def _packed(a, x, cu_seqlens, h0, want_final):
+    if torch.is_grad_enabled() and (a.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
+        return _RGLRUPacked.apply(a, x, cu_seqlens, h0, want_final)
+    return _packed_forward(a, x, cu_seqlens, h0, want_final, False)[:2]
 
 
 def rglru_scan_packed(a, x, cu_seqlens, h0=None):
@@ -265,14 +275,14 @@ def rglru_scan_packed(a, x, cu_seqlens, h0=None):
         y:   [T, D] float32. State and accumulation are float32; gradients
              come in the inputs' dtype.
     """
-    return _RGLRUPacked.apply(a, x, cu_seqlens, h0, False)[0]
+    return _packed(a, x, cu_seqlens, h0, False)[0]
 
 
 def rglru_scan_packed_with_state(a, x, cu_seqlens, h0=None):
     """:func:`rglru_scan_packed` that also returns the final states [S, D] (an
     empty sequence's is its h0). Passed back as ``h0`` they continue the scan;
     passed to :func:`rglru_step` they start decoding."""
-    return _RGLRUPacked.apply(a, x, cu_seqlens, h0, True)
+    return _packed(a, x, cu_seqlens, h0, True)
 
 
 def rglru_scan_packed_reference(a, x, cu_seqlens, h0=None):

@@ -73,33 +73,39 @@ def _rows(t, dt, packed_dims):
 
 
 def _dense16(t, dt):
-    t = prep(t, dt)
+    t = prep(t.detach() if t.requires_grad else t, dt)
     return t.clone() if t.data_ptr() % 16 else t
+
+
+def _attend(q, k, v, cu, window, sinks, scale, want_lse):
+    packed = q.dim() == 3
+    dev = _lib.require_cuda(q, k, v)
+    dt = common_dtype(q, k, v)
+    if packed:
+        cu = prep_cu(cu, dev)
+        S, L = cu.numel() - 1, 0
+    else:
+        S, L = q.shape[:2]
+    q_, qt, qh = _rows(q, dt, packed)
+    k_, kt, kh = _rows(k, dt, packed)
+    v_, vt, vh = _rows(v, dt, packed)
+    T, Hq, Dh = q_.shape
+    y = torch.empty((T, Hq, Dh), dtype=dt, device=dev)
+    lse = torch.empty((Hq, T), dtype=torch.float32, device=dev) if want_lse else None
+    args = (qt, qh, kt, kh, vt, vh, _lib.addr(cu), S, L, _lib.DTYPE_CODE[dt], T, Hq, k_.shape[1], Dh, window, sinks,
+            scale)
+    _lib.call_on(dev, "mr_window_attn_fwd", q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), *args, y.data_ptr(),
+                 _lib.addr(lse))
+    return y if packed else y.view(q.shape), args, (q_, k_, v_, cu, y, lse)
 
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, window, sinks, scale):
-        packed = q.dim() == 3
-        dev = _lib.require_cuda(q, k, v)
-        dt = common_dtype(q, k, v)
-        shape = q.shape
-        if packed:
-            cu = prep_cu(cu, dev)
-            S, L = cu.numel() - 1, 0
-        else:
-            S, L = shape[:2]
-        (q_, *qs), (k_, *ks), (v_, *vs) = (_rows(t, dt, packed) for t in (q, k, v))
-        T, Hq, Dh = q_.shape
-        Hkv = k_.shape[1]
-        y = torch.empty((T, Hq, Dh), dtype=dt, device=dev)
-        lse = torch.empty((Hq, T), dtype=torch.float32, device=dev) if any(ctx.needs_input_grad[:3]) else None
-        ctx.args = (*qs, *ks, *vs, _lib.ptr(cu), S, L, _lib.DTYPE_CODE[dt], T, Hq, Hkv, Dh, window, sinks, scale)
-        _lib.call_on(dev, "mr_window_attn_fwd", q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), *ctx.args, y.data_ptr(),
-                     _lib.ptr(lse))
-        ctx.save_for_backward(q_, k_, v_, cu, y, lse)
-        ctx.shapes = (shape, k.shape)
-        return y.view(shape)
+        y, ctx.args, saved = _attend(q, k, v, cu, window, sinks, scale, True)
+        ctx.save_for_backward(*saved)
+        ctx.shapes = (q.shape, k.shape)
+        return y
 
     @staticmethod
     @once_differentiable
@@ -117,7 +123,15 @@ class _WindowAttention(torch.autograd.Function):
                      k_.data_ptr(), v_.data_ptr(), *ctx.args, gq.data_ptr(), gk.data_ptr(), gv.data_ptr(),
                      ws.data_ptr(), ws.numel())
         sq, sk = ctx.shapes
-        return gq.view(sq), gk.view(sk), gv.view(sk), None, None, None, None
+        if len(sq) == 4:
+            gq, gk, gv = gq.view(sq), gk.view(sk), gv.view(sk)
+        return gq, gk, gv, None, None, None, None
+
+
+def _dispatch(q, k, v, cu, window, sinks, scale):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _WindowAttention.apply(q, k, v, cu, window, sinks, scale)
+    return _attend(q, k, v, cu, window, sinks, scale, False)[0]
 
 
 def window_attention(q, k, v, window, sinks=0, scale=None):
@@ -139,7 +153,7 @@ def window_attention(q, k, v, window, sinks=0, scale=None):
         projection are read in place.
     """
     scale = _check(q, k, v, window, sinks, scale, 4, "[B, L, H, Dh]")
-    return _WindowAttention.apply(q, k, v, None, window, sinks, scale)
+    return _dispatch(q, k, v, None, window, sinks, scale)
 
 
 def window_attention_packed(q, k, v, cu_seqlens, window, sinks=0, scale=None):
@@ -147,7 +161,7 @@ def window_attention_packed(q, k, v, cu_seqlens, window, sinks=0, scale=None):
     [T, Hkv, Dh], and ``cu_seqlens`` as in :func:`rglru_scan_packed` (rows
     behind the last border come out as zeros, gradients too)."""
     scale = _check(q, k, v, window, sinks, scale, 3, "[T, H, Dh]")
-    return _WindowAttention.apply(q, k, v, cu_seqlens, window, sinks, scale)
+    return _dispatch(q, k, v, cu_seqlens, window, sinks, scale)
 
 
 def _caches(k, v, cu, window, sinks):
@@ -160,7 +174,7 @@ def _caches(k, v, cu, window, sinks):
     slots = sinks + window
     ck, cv = (torch.empty((S, slots, Hkv, Dh), dtype=dt, device=dev) for _ in range(2))
     cu_ = prep_cu(cu, dev) if packed else None
-    _lib.call_on(dev, "mr_window_cache", k_.data_ptr(), v_.data_ptr(), *ks, *vs, _lib.ptr(cu_), S, L,
+    _lib.call_on(dev, "mr_window_cache", k_.data_ptr(), v_.data_ptr(), *ks, *vs, _lib.addr(cu_), S, L,
                  _lib.DTYPE_CODE[dt], T, Hkv, Dh, slots, sinks, ck.data_ptr(), cv.data_ptr())
     return ck, cv
 
@@ -212,14 +226,13 @@ def window_attention_step(q, k, v, cache_k, cache_v, pos, sinks=0, scale=None):
             or (B and (cache_k.data_ptr() % 16 or cache_v.data_ptr() % 16))):
         raise ValueError(f"caches must be contiguous, 16-byte aligned {dt} tensors (updated in place), got "
                          f"{cache_k.dtype} and {cache_v.dtype}")
-    n = cache_k.numel() * cache_k.element_size()
-    if abs(cache_k.data_ptr() - cache_v.data_ptr()) < n:
+    if abs(cache_k.data_ptr() - cache_v.data_ptr()) < cache_k.numel() * cache_k.element_size():
         raise ValueError("cache_k and cache_v must not overlap")
     if not isinstance(pos, torch.Tensor) or tuple(pos.shape) != (B,) or pos.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"pos must be an int64 or int32 tensor of shape [{B}]")
     if pos.device != dev:
         raise ValueError(f"pos must be on {dev}, got {pos.device}")
-    q_, k_, v_ = (_dense16(t.detach(), dt) for t in (q, k, v))
+    q_, k_, v_ = _dense16(q, dt), _dense16(k, dt), _dense16(v, dt)
     pos = pos.contiguous()
     y = torch.empty((B, Hq, Dh), dtype=dt, device=dev)
     _lib.call_on(dev, "mr_window_step", q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), cache_k.data_ptr(),
