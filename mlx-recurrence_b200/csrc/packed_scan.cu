@@ -284,13 +284,25 @@ template <int V> __device__ __forceinline__ void mark_borders(Work<V>& sh, const
   sync_workers();
 }
 
-// The sequence that starts (ends) at token i of the chunk, or -1. Marks are there when the chunk has borders
-// (clamped, so that a malformed cu stays in range).
-__device__ __forceinline__ int start_of(const int* mark, const ChunkInfo& c, int i, int S) {
-  return c.starts && (mark[i] & kStart) ? min(mark[i] & kSeq, S - 1) : -1;
+// A warp's steps as bit masks: in a sequence, at a start, at an end; the same in every lane, so the unrolled loops branch
+// on them without divergence.
+struct StepMasks {
+  uint32_t in, start, end;
+};
+__device__ __forceinline__ StepMasks step_masks(const int* mark, const ChunkInfo& c, int w) {
+  const int lane = threadIdx.x & 31, k0 = w * kSteps;
+  const int m = lane < kSteps && (c.starts | c.ends) ? mark[k0 + lane] : 0;
+  const int lo = max(c.lo - k0, 0), hi = min(c.hi - k0, kSteps);
+  const uint32_t in = hi > lo ? ((1u << hi) - 1) & ~((1u << lo) - 1) : 0;
+  return {in, __ballot_sync(0xffffffffu, m & kStart) & in, __ballot_sync(0xffffffffu, m & kEnd) & in};
 }
-__device__ __forceinline__ int end_of(const int* mark, const ChunkInfo& c, int i, int S) {
-  return c.ends && (mark[i] & kEnd) ? min(mark[i] & kSeq, S - 1) : -1;
+
+// The sequence of a marked token (clamped, so that a malformed cu stays in range).
+__device__ __forceinline__ int seq_at(const int* mark, int i, int S) { return min(mark[i] & kSeq, S - 1); }
+// v <- the V channels of row s of a [S, D] state, or zeros without one
+template <int V> __device__ __forceinline__ void begin(const float* state, int s, int64_t D, int64_t ch, int live, float (&v)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = state && i < live ? state[s * D + ch + i] : 0.f;
 }
 
 // The chain. Along it (left to right in the forward, right to left in the
@@ -419,8 +431,9 @@ packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
     const int64_t ch = (int64_t)(item % P.ntile) * CH + lane * V, t0 = (int64_t)chunk * kChunk;
     const int n = (int)min((int64_t)kChunk, P.L - t0), live = (int)min((int64_t)V, max((int64_t)0, P.D - ch));
     const ChunkInfo info = TMA ? sh.infos[st] : P.info ? P.info[chunk] : chunk_info(P.cu, P.S, t0, n);
-    const bool plain = info.plain(w);
     if (info.starts | info.ends) mark_borders(sh, info, P, t0, n);
+    const bool plain = info.plain(w);
+    const StepMasks mask = step_masks(sh.mark, info, w);
     const T *sa = feed.a(st) + k0 * CH + lane * V, *sx = feed.x(st) + k0 * CH + lane * V;
     float A[V], B[V];
 #pragma unroll
@@ -433,21 +446,19 @@ packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
         for (int v = 0; v < V; ++v) B[v] = fmaf(to_f(av.v[v]), B[v], to_f(xv.v[v])), A[v] *= to_f(av.v[v]);
       }
     } else {
-      for (int k = 0; k < kSteps; ++k) {
-        const int i = k0 + k;
-        if (i < info.lo || i >= info.hi) continue;
-        const int s = start_of(sh.mark, info, i, P.S);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          if (s >= 0) B[v] = P.h0 && v < live ? P.h0[s * P.D + ch + v] : 0.f;
+      for (int k = 0; k < kSteps; ++k) {
+        if (!(mask.in >> k & 1)) continue;
+        if (mask.start >> k & 1) begin(P.h0, seq_at(sh.mark, k0 + k, P.S), P.D, ch, live, B);
+#pragma unroll
+        for (int v = 0; v < V; ++v)
           B[v] = fmaf(to_f(sa[k * CH + v]), B[v], to_f(sx[k * CH + v])), A[v] *= to_f(sa[k * CH + v]);
-        }
       }
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) sh.A[w][lane * V + v] = A[v], sh.B[w][lane * V + v] = B[v];
     sync_workers();
-    const bool need = info.lo == 0 && info.hi > 0 && start_of(sh.mark, info, 0, P.S) < 0;
+    const bool need = info.lo == 0 && info.hi > 0 && !(info.starts && (sh.mark[0] & kStart));
     float carry[V], p[V], q[V], h[V];
     chain<V, false>(sh, P, ch, live, chunk, info.starts, need, carry, p, q);
     const bool cut = info.starts & ((1u << w) - 1);
@@ -466,17 +477,22 @@ packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
         put<float, V>(y, h, P.vec, live);
       }
     } else {
-      for (int k = 0; k < kSteps && k0 + k < n; ++k, y += P.D) {
-        const int i = k0 + k;
-        const bool in = i >= info.lo && i < info.hi;
-        const int s = in ? start_of(sh.mark, info, i, P.S) : -1, e = in ? end_of(sh.mark, info, i, P.S) : -1;
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k, y += P.D) {
+        if (k0 + k >= n) continue;
+        const bool in = mask.in >> k & 1;
         float out[V];
+        if (mask.start >> k & 1) begin(P.h0, seq_at(sh.mark, k0 + k, P.S), P.D, ch, live, h);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          if (s >= 0) h[v] = P.h0 && v < live ? P.h0[s * P.D + ch + v] : 0.f;
           if (in) h[v] = fmaf(to_f(sa[k * CH + v]), h[v], to_f(sx[k * CH + v]));
           out[v] = in ? h[v] : 0.f;
-          if (P.fin != nullptr && e >= 0 && v < live) P.fin[e * P.D + ch + v] = h[v];
+        }
+        if (P.fin != nullptr && (mask.end >> k & 1)) {
+          const int64_t at = (int64_t)seq_at(sh.mark, k0 + k, P.S) * P.D + ch;
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (v < live) P.fin[at + v] = h[v];
         }
         put<float, V>(y, out, P.vec, live);
       }
@@ -517,11 +533,12 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
     const int64_t ch = (int64_t)(item % P.ntile) * CH + lane * V, t0 = (int64_t)chunk * kChunk;
     const int n = (int)min((int64_t)kChunk, P.L - t0), live = (int)min((int64_t)V, max((int64_t)0, P.D - ch));
     const ChunkInfo info = TMA ? sh.infos[st] : P.info ? P.info[chunk] : chunk_info(P.cu, P.S, t0, n);
-    const bool plain = info.plain(w);
     float h[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = v < live && n > 0 ? P.ckpt[chunk * P.D + ch + v] : 0.f;
     if (info.starts | info.ends) mark_borders(sh, info, P, t0, n);
+    const bool plain = info.plain(w);
+    const StepMasks mask = step_masks(sh.mark, info, w);
     const T *sa = feed.a(st) + k0 * CH + lane * V, *sx = feed.x(st) + k0 * CH + lane * V;
     float* sg = feed.g(st) + k0 * CH + lane * V;
     {
@@ -544,25 +561,21 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
 #pragma unroll
         for (int v = 0; v < V; ++v) C[v] = A[v];
       } else {
+#pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-          const int i = k0 + k;
-          if (i < info.lo || i >= info.hi) continue;
-          const int s = start_of(sh.mark, info, i, P.S);
+          if (!(mask.in >> k & 1)) continue;
+          if (mask.start >> k & 1) begin(P.h0, seq_at(sh.mark, k0 + k, P.S), P.D, ch, live, B);
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            if (s >= 0) B[v] = P.h0 && v < live ? P.h0[s * P.D + ch + v] : 0.f;
+          for (int v = 0; v < V; ++v)
             B[v] = fmaf(to_f(sa[k * CH + v]), B[v], to_f(sx[k * CH + v])), A[v] *= to_f(sa[k * CH + v]);
-          }
         }
-        for (int k = kSteps - 1; k >= 0; --k) {
-          const int i = k0 + k;
-          if (i < info.lo || i >= info.hi) continue;
-          const int e = end_of(sh.mark, info, i, P.S);
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            if (e >= 0) Q[v] = P.gf && v < live ? P.gf[e * P.D + ch + v] : 0.f;
+        for (int k = kSteps - 1; k >= 0; --k) {
+          if (!(mask.in >> k & 1)) continue;
+          if (mask.end >> k & 1) begin(P.gf, seq_at(sh.mark, k0 + k, P.S), P.D, ch, live, Q);
+#pragma unroll
+          for (int v = 0; v < V; ++v)
             Q[v] = to_f(sa[k * CH + v]) * (sg[k * CH + v] + Q[v]), C[v] *= to_f(sa[k * CH + v]);
-          }
         }
       }
 #pragma unroll
@@ -572,7 +585,7 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
       }
     }
     sync_workers();
-    const bool need = info.hi == n && info.hi > info.lo && end_of(sh.mark, info, n - 1, P.S) < 0;
+    const bool need = info.hi == n && info.hi > info.lo && !(info.ends && (sh.mark[n - 1] & kEnd));
     float carry[V], p[V], q[V], r[V];
     chain<V, true>(sh, P, ch, live, rank, info.ends, need, carry, p, q);
     const bool cut = info.ends >> (w + 1);
@@ -613,27 +626,31 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
         put<T, V>(gx, ox, P.vec, live);
       }
     } else {
+#pragma unroll
       for (int k = kSteps - 1; k >= 0; --k) {
-        const int i = k0 + k;
-        if (i < info.lo || i >= info.hi) continue;
-        const int s = start_of(sh.mark, info, i, P.S), e = end_of(sh.mark, info, i, P.S);
+        if (!(mask.in >> k & 1)) continue;
+        if (mask.end >> k & 1) begin(P.gf, seq_at(sh.mark, k0 + k, P.S), P.D, ch, live, r);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          if (e >= 0) r[v] = P.gf && v < live ? P.gf[e * P.D + ch + v] : 0.f;
           const float adj = sg[k * CH + v] + r[v];
           sg[k * CH + v] = adj;
           r[v] = to_f(sa[k * CH + v]) * adj;
-          if (P.gh0 != nullptr && s >= 0 && v < live) P.gh0[s * P.D + ch + v] = r[v];
+        }
+        if (P.gh0 != nullptr && (mask.start >> k & 1)) {
+          const int64_t at = (int64_t)seq_at(sh.mark, k0 + k, P.S) * P.D + ch;
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (v < live) P.gh0[at + v] = r[v];
         }
       }
-      for (int k = 0; k < kSteps && k0 + k < n; ++k, ga += P.D, gx += P.D) {
-        const int i = k0 + k;
-        const bool in = i >= info.lo && i < info.hi;
-        const int s = in ? start_of(sh.mark, info, i, P.S) : -1;
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k, ga += P.D, gx += P.D) {
+        if (k0 + k >= n) continue;
+        const bool in = mask.in >> k & 1;
         float oa[V], ox[V];
+        if (mask.start >> k & 1) begin(P.h0, seq_at(sh.mark, k0 + k, P.S), P.D, ch, live, h);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          if (s >= 0) h[v] = P.h0 && v < live ? P.h0[s * P.D + ch + v] : 0.f;
           ox[v] = in ? sg[k * CH + v] : 0.f;
           oa[v] = in ? sg[k * CH + v] * h[v] : 0.f;
           if (in) h[v] = fmaf(to_f(sa[k * CH + v]), h[v], to_f(sx[k * CH + v]));
