@@ -192,9 +192,10 @@ template <typename T, bool BWD, bool TMA, int STAGES> struct Feed {
     const int total = P.nchunk * P.ntile;
     for (int i = 0;; ++i) {
       const int st = i % STAGES;
+      // (only with room for it: an item taken early and left waiting holds up those behind it)
+      if (i >= STAGES) mbar_wait(&sh.empty[st], (i / STAGES - 1) & 1);
       const int item = P.counter ? (int)min(atomicAdd(P.counter, 1u), (uint32_t)INT32_MAX)
                                  : (i == 0 ? (int)blockIdx.x : INT32_MAX);
-      if (i >= STAGES) mbar_wait(&sh.empty[st], (i / STAGES - 1) & 1);
       if (item >= total) {
         sh.items[st] = -1;
         mbar_arrive(&sh.full[st]);
