@@ -9,8 +9,8 @@
 //
 // One pass over the data, HBM-bound. An item is kChunk steps of 32 V channels
 // (rows of 128 bytes of the inputs); 8 warps x kSteps steps each work on it out
-// of shared memory, where a ninth warp's TMA copies bring the items of a
-// persistent CTA ahead of time. A step is the affine map h -> a h + x, so runs of
+// of shared memory, where a ninth warp's TMA copies bring it; the other CTAs of
+// the SM (four forward, three backward) cover the copies and the waits. A step is the affine map h -> a h + x, so runs of
 // steps compose to one map (A, B): per thread, per warp prefix and per item. An
 // item publishes its map, looks back over the items before it in time (kBack at
 // a time) until it meets one whose state is known, and publishes its own state.
@@ -28,7 +28,7 @@ namespace mr {
 constexpr int kWarps = 8;
 constexpr int kSteps = 16;               // steps of a thread
 constexpr int kChunk = kWarps * kSteps;  // steps of an item
-constexpr int kBack = 4;                 // items that one round of the look-back reads
+constexpr int kBack = 2;                 // items that one round of the look-back reads
 
 // A chunk's map or state for one channel, written and read as one 16-byte access
 // (single-copy atomic), so no flag or fence stands beside it.
@@ -128,6 +128,9 @@ struct PackedArgs {
   bool vec;  // rows of V elements may be accessed whole
 };
 
+// CTAs per SM: by registers (forward), by shared memory (backward)
+template <bool BWD> constexpr int kCtas = BWD ? 3 : 4;
+
 template <typename T> constexpr int kV = 4 / sizeof(T);  // channels of a thread: 4 bytes of an input row
 template <typename T, bool BWD> constexpr int kStage = kChunk * 32 * kV<T> * (2 * (int)sizeof(T) + (BWD ? 4 : 0));
 
@@ -157,9 +160,9 @@ template <int V> struct Work {
   float2 back[kBack][32 * V];                    // what the look-back read: A (or kKnown) and B
   float carry[32 * V];                           // the state entering the item
   int mark[kChunk];                              // per token at a border: its sequence, and which end of it
-  uint64_t full[2], empty[2];
-  ChunkInfo infos[2];
-  int items[2];
+  uint64_t full, empty;
+  ChunkInfo info;
+  int item;
   int open;
 };
 constexpr int kStart = 1 << 30, kEnd = INT32_MIN, kSeq = kStart - 1;  // of Work::mark; 0 in both bits: no border
@@ -173,64 +176,60 @@ __device__ __forceinline__ void sync_workers() { asm volatile("bar.sync 1, 256;"
 // which CTAs ask, so whatever an item waits for has been taken by a running CTA,
 // which works through its items in order: the smallest one never waits.
 //
-// TMA form: warp kWarps takes tickets and fills the two (one) stages ahead. Plain
-// form (rows that are no multiple of 16 bytes): every thread brings its own
+// TMA form: warp kWarps takes a ticket and brings its data as soon as the last
+// item has been read. Plain form (rows that are no multiple of 16 bytes): every thread brings its own
 // elements when the item begins.
-template <typename T, bool BWD, bool TMA, int STAGES> struct Feed {
+template <typename T, bool BWD, bool TMA> struct Feed {
   static constexpr int V = kV<T>, CH = 32 * V;
-  unsigned char* stages;
+  unsigned char* stage;
   Work<V>& sh;
   const PackedArgs& P;
   int n = 0;  // items so far
 
-  __device__ T* a(int st) const { return reinterpret_cast<T*>(stages + st * kStage<T, BWD>); }
-  __device__ T* x(int st) const { return a(st) + kChunk * CH; }
-  __device__ float* g(int st) const { return reinterpret_cast<float*>(x(st) + kChunk * CH); }
+  __device__ T* a() const { return reinterpret_cast<T*>(stage); }
+  __device__ T* x() const { return a() + kChunk * CH; }
+  __device__ float* g() const { return reinterpret_cast<float*>(x() + kChunk * CH); }
   __device__ int64_t chunk_of(int item) const { return BWD ? P.nchunk - 1 - item / P.ntile : item / P.ntile; }
 
   __device__ void produce(const CUtensorMap* ta, const CUtensorMap* tx, const CUtensorMap* tg) {
     const int total = P.nchunk * P.ntile;
     for (int i = 0;; ++i) {
-      const int st = i % STAGES;
       // (only with room for it: an item taken early and left waiting holds up those behind it)
-      if (i >= STAGES) mbar_wait(&sh.empty[st], (i / STAGES - 1) & 1);
+      if (i > 0) mbar_wait(&sh.empty, (i - 1) & 1);
       const int item = P.counter ? (int)min(atomicAdd(P.counter, 1u), (uint32_t)INT32_MAX)
                                  : (i == 0 ? (int)blockIdx.x : INT32_MAX);
       if (item >= total) {
-        sh.items[st] = -1;
-        mbar_arrive(&sh.full[st]);
+        sh.item = -1;
+        mbar_arrive(&sh.full);
         return;
       }
       const int64_t t0 = chunk_of(item) * kChunk;
       const int c0 = item % P.ntile * CH;
-      sh.items[st] = item;
-      sh.infos[st] = P.info ? P.info[chunk_of(item)] : chunk_info(P.cu, P.S, t0, (int)min((int64_t)kChunk, P.L - t0));
-      mbar_arrive_expect_tx(&sh.full[st], kStage<T, BWD>);
-      tma_load_2d(a(st), ta, c0, (int)t0, &sh.full[st]);
-      tma_load_2d(x(st), tx, c0, (int)t0, &sh.full[st]);
-      if (BWD) tma_load_2d(g(st), tg, c0, (int)t0, &sh.full[st]);
+      sh.item = item;
+      sh.info = P.info ? P.info[chunk_of(item)] : chunk_info(P.cu, P.S, t0, (int)min((int64_t)kChunk, P.L - t0));
+      mbar_arrive_expect_tx(&sh.full, kStage<T, BWD>);
+      tma_load_2d(a(), ta, c0, (int)t0, &sh.full);
+      tma_load_2d(x(), tx, c0, (int)t0, &sh.full);
+      if (BWD) tma_load_2d(g(), tg, c0, (int)t0, &sh.full);
     }
   }
 
-  // Next item into stage `st` (returned through st), or -1.
-  __device__ int next(int& st) {
+  // The next item, once its data is there, or -1.
+  __device__ int next() {
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if constexpr (TMA) {
-      st = n % STAGES;
-      mbar_wait(&sh.full[st], (n / STAGES) & 1);
-      ++n;
-      return sh.items[st];
+      mbar_wait(&sh.full, n++ & 1);
+      return sh.item;
     } else {
-      st = 0;
       if (P.counter == nullptr) {
         if (n++ > 0) return -1;
-        sh.items[0] = blockIdx.x;
+        sh.item = blockIdx.x;
       } else {
         sync_workers();  // everybody has read the last item's number
-        if (threadIdx.x == 0) sh.items[0] = (int)min(atomicAdd(P.counter, 1u), (uint32_t)INT32_MAX);
+        if (threadIdx.x == 0) sh.item = (int)min(atomicAdd(P.counter, 1u), (uint32_t)INT32_MAX);
       }
       sync_workers();
-      const int item = sh.items[0];
+      const int item = sh.item;
       if (item >= P.nchunk * P.ntile) return -1;
       const int64_t t0 = chunk_of(item) * kChunk, ch = (int64_t)(item % P.ntile) * CH + lane * V;
       const int live = (int)min((int64_t)V, max((int64_t)0, P.D - ch)), rows = (int)min((int64_t)kChunk, P.L - t0);
@@ -245,8 +244,8 @@ template <typename T, bool BWD, bool TMA, int STAGES> struct Feed {
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
         const int i = (w * kSteps + k) * CH + lane * V;
-        *reinterpret_cast<Vec<T, V>*>(a(0) + i) = va[k];
-        *reinterpret_cast<Vec<T, V>*>(x(0) + i) = vx[k];
+        *reinterpret_cast<Vec<T, V>*>(a() + i) = va[k];
+        *reinterpret_cast<Vec<T, V>*>(x() + i) = vx[k];
       }
       if constexpr (BWD) {
         Vec<float, V> vg[kSteps];
@@ -257,16 +256,16 @@ template <typename T, bool BWD, bool TMA, int STAGES> struct Feed {
         }
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
-          *reinterpret_cast<Vec<float, V>*>(g(0) + (w * kSteps + k) * CH + lane * V) = vg[k];
+          *reinterpret_cast<Vec<float, V>*>(g() + (w * kSteps + k) * CH + lane * V) = vg[k];
       }
       return item;
     }
   }
   // The stage may be filled again.
-  __device__ void release(int st) {
+  __device__ void release() {
     if constexpr (TMA) {
       __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.empty[st]);
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.empty);
     }
   }
 };
@@ -406,17 +405,17 @@ __device__ __forceinline__ void chain(Work<V>& sh, const PackedArgs& P, int64_t 
 __device__ __forceinline__ float enter(float p, float q, float carry, bool cut) { return cut ? q : fmaf(p, carry, q); }
 
 template <typename T, bool TMA>
-__global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), 3)
+__global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kCtas<false>)
 packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ CUtensorMap ta,
                   const __grid_constant__ CUtensorMap tx) {
   constexpr int V = kV<T>, CH = 32 * V;
   extern __shared__ __align__(128) unsigned char dyn[];
   __shared__ Work<V> sh;
-  Feed<T, false, TMA, 2> feed{dyn, sh, P};
+  Feed<T, false, TMA> feed{dyn, sh, P};
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, k0 = w * kSteps;
   if constexpr (TMA) {
     if (threadIdx.x == 0) {
-      for (int i = 0; i < 2; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], kWarps);
+      mbar_init(&sh.full, 1), mbar_init(&sh.empty, kWarps);
       fence_mbar_init();
     }
     __syncthreads();
@@ -425,17 +424,15 @@ packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
       return;
     }
   }
-  for (int st;;) {
-    const int item = feed.next(st);
-    if (item < 0) break;
+  for (int item; (item = feed.next()) >= 0;) {
     const int chunk = item / P.ntile;
     const int64_t ch = (int64_t)(item % P.ntile) * CH + lane * V, t0 = (int64_t)chunk * kChunk;
     const int n = (int)min((int64_t)kChunk, P.L - t0), live = (int)min((int64_t)V, max((int64_t)0, P.D - ch));
-    const ChunkInfo info = TMA ? sh.infos[st] : P.info ? P.info[chunk] : chunk_info(P.cu, P.S, t0, n);
+    const ChunkInfo info = TMA ? sh.info : P.info ? P.info[chunk] : chunk_info(P.cu, P.S, t0, n);
     if (info.starts | info.ends) mark_borders(sh, info, P, t0, n);
     const bool plain = info.plain(w);
     const StepMasks mask = step_masks(sh.mark, info, w);
-    const T *sa = feed.a(st) + k0 * CH + lane * V, *sx = feed.x(st) + k0 * CH + lane * V;
+    const T *sa = feed.a() + k0 * CH + lane * V, *sx = feed.x() + k0 * CH + lane * V;
     float A[V], B[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
@@ -498,7 +495,7 @@ packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
         put<float, V>(y, out, P.vec, live);
       }
     }
-    feed.release(st);
+    feed.release();
     if (P.fin != nullptr)  // empty sequences, spread over the chunks
       for (int s = (int)((int64_t)chunk * P.S / P.nchunk) + w; s < (int)((int64_t)(chunk + 1) * P.S / P.nchunk); s += kWarps)
         if (P.cu[s + 1] <= P.cu[s])
@@ -508,17 +505,17 @@ packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
 }
 
 template <typename T, bool TMA>
-__global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), 3)
+__global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kCtas<true>)
 packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ CUtensorMap ta,
                   const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tg) {
   constexpr int V = kV<T>, CH = 32 * V;
   extern __shared__ __align__(128) unsigned char dyn[];
   __shared__ Work<V> sh;
-  Feed<T, true, TMA, 1> feed{dyn, sh, P};
+  Feed<T, true, TMA> feed{dyn, sh, P};
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, k0 = w * kSteps;
   if constexpr (TMA) {
     if (threadIdx.x == 0) {
-      mbar_init(&sh.full[0], 1), mbar_init(&sh.empty[0], kWarps);
+      mbar_init(&sh.full, 1), mbar_init(&sh.empty, kWarps);
       fence_mbar_init();
     }
     __syncthreads();
@@ -527,21 +524,19 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
       return;
     }
   }
-  for (int st;;) {
-    const int item = feed.next(st);
-    if (item < 0) break;
+  for (int item; (item = feed.next()) >= 0;) {
     const int rank = item / P.ntile, chunk = P.nchunk - 1 - rank;
     const int64_t ch = (int64_t)(item % P.ntile) * CH + lane * V, t0 = (int64_t)chunk * kChunk;
     const int n = (int)min((int64_t)kChunk, P.L - t0), live = (int)min((int64_t)V, max((int64_t)0, P.D - ch));
-    const ChunkInfo info = TMA ? sh.infos[st] : P.info ? P.info[chunk] : chunk_info(P.cu, P.S, t0, n);
+    const ChunkInfo info = TMA ? sh.info : P.info ? P.info[chunk] : chunk_info(P.cu, P.S, t0, n);
     float h[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = v < live && n > 0 ? P.ckpt[chunk * P.D + ch + v] : 0.f;
     if (info.starts | info.ends) mark_borders(sh, info, P, t0, n);
     const bool plain = info.plain(w);
     const StepMasks mask = step_masks(sh.mark, info, w);
-    const T *sa = feed.a(st) + k0 * CH + lane * V, *sx = feed.x(st) + k0 * CH + lane * V;
-    float* sg = feed.g(st) + k0 * CH + lane * V;
+    const T *sa = feed.a() + k0 * CH + lane * V, *sx = feed.x() + k0 * CH + lane * V;
+    float* sg = feed.g() + k0 * CH + lane * V;
     {
       float A[V], B[V], C[V], Q[V];
 #pragma unroll
@@ -661,7 +656,7 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
       }
     }
     if constexpr (TMA) fence_proxy_async_smem();  // this thread's writes over gy before the next copy into it
-    feed.release(st);
+    feed.release();
     if (P.gh0 != nullptr)
       for (int s = (int)((int64_t)chunk * P.S / P.nchunk) + w; s < (int)((int64_t)(chunk + 1) * P.S / P.nchunk); s += kWarps)
         if (P.cu[s + 1] <= P.cu[s])
@@ -701,8 +696,6 @@ static int prepare_ws(const char* what, PackedArgs& P, void* ws, size_t bytes, c
   return check_launch("packed_prep_kernel");
 }
 
-constexpr int kCtas = 148 * 3;  // three per SM
-
 template <typename T, bool BWD> static int launch(const char* what, PackedArgs P, void* ws, size_t wsb, cudaStream_t st) {
   constexpr int V = kV<T>, e = sizeof(T);
   P.ntile = (int)((P.D + 32 * V - 1) / (32 * V));
@@ -713,8 +706,8 @@ template <typename T, bool BWD> static int launch(const char* what, PackedArgs P
   // the copies take rows that are multiples of 16 bytes, 16-byte aligned
   const bool tma = P.L > 0 && P.D * e % 16 == 0 && at(P.a, 16) && at(P.x, 16) && (!BWD || at(P.gy, 16));
   const int64_t items = (int64_t)P.nchunk * P.ntile;
-  const unsigned grid = (unsigned)(P.counter && items > kCtas ? kCtas : items);
-  const int smem = kStage<T, BWD> * (BWD || !tma ? 1 : 2);
+  const unsigned grid = (unsigned)(P.counter && items > 148 * kCtas<BWD> ? 148 * kCtas<BWD> : items);
+  constexpr int smem = kStage<T, BWD>;
   CUtensorMap ta, tx, tg;
   if (tma) {
     if (int rc = make_tmap_2d(&ta, P.a, TmapType<T>::v, e, P.D, P.L, P.D * e, 32 * V, kChunk)) return rc;
