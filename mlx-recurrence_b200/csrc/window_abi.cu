@@ -4,8 +4,9 @@
 
 namespace mr {
 
-template <typename T> int attn_fwd_simt(const AttnArgs&, cudaStream_t);
-template <typename T> int attn_bwd_simt(const AttnArgs&, cudaStream_t);
+int attn_fwd_f32_launch(const AttnArgs&, cudaStream_t);
+int attn_bwd_f32_launch(const AttnArgs&, void* ws, cudaStream_t);
+size_t attn_bwd_f32_ws_bytes(int64_t T, int64_t Hq, int64_t Dh, int64_t sinks);
 template <typename T> int attn_fwd_launch(const AttnArgs&, cudaStream_t);
 template <typename T> int attn_bwd_launch(const AttnArgs&, void*, cudaStream_t);
 size_t attn_bwd_ws_bytes(int64_t T, int64_t Hq, int64_t Dh, int64_t sinks);
@@ -73,7 +74,7 @@ int mr_window_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ts
   A.y = y, A.lse = lse;
   const cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
-    case MR_F32: return attn_fwd_simt<float>(A, st);
+    case MR_F32: return attn_fwd_f32_launch(A, st);
     case MR_BF16: return attn_fwd_launch<__nv_bfloat16>(A, st);
     default: return attn_fwd_launch<__half>(A, st);
   }
@@ -81,7 +82,7 @@ int mr_window_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ts
 
 size_t mr_window_attn_bwd_workspace_bytes(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t sinks) {
   if (T <= 0 || Hq <= 0 || Hkv <= 0 || Dh <= 0 || sinks < 0) return 0;
-  return dtype == MR_F32 ? (size_t)T * Hq * 4 : attn_bwd_ws_bytes(T, Hq, Dh, sinks);
+  return dtype == MR_F32 ? attn_bwd_f32_ws_bytes(T, Hq, Dh, sinks) : attn_bwd_ws_bytes(T, Hq, Dh, sinks);
 }
 
 int mr_window_attn_bwd(const void* grad_y, const void* y, const float* lse, const void* q, const void* k,
@@ -99,10 +100,10 @@ int mr_window_attn_bwd(const void* grad_y, const void* y, const float* lse, cons
   if (lse == nullptr || workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace & 15u))
     return set_error(MR_E_WORKSPACE, "%s: needs lse and %zu bytes of workspace, got %zu", what, need, workspace_bytes);
   A.y = const_cast<void*>(y), A.lse = const_cast<float*>(lse), A.gy = grad_y;
-  A.gq = grad_q, A.gk = grad_k, A.gv = grad_v, A.delta = (float*)workspace;
+  A.gq = grad_q, A.gk = grad_k, A.gv = grad_v;
   const cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
-    case MR_F32: return attn_bwd_simt<float>(A, st);
+    case MR_F32: return attn_bwd_f32_launch(A, workspace, st);
     case MR_BF16: return attn_bwd_launch<__nv_bfloat16>(A, workspace, st);
     default: return attn_bwd_launch<__half>(A, workspace, st);
   }

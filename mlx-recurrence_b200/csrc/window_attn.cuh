@@ -26,6 +26,7 @@ struct AttnArgs {
   const void* gy;                   // [T, Hq, Dh] dense
   float* delta;                     // [Hq, T]: sum_d gy y
   void *gq, *gk, *gv;               // [T, Hq, Dh], [T, Hkv, Dh] dense
+  float* part;                      // sink partials (below), or NULL
 };
 
 struct SeqRange {
@@ -86,16 +87,82 @@ __device__ __forceinline__ int key_limit(const AttnArgs& A, int j) {
   return j - s.start < A.sinks ? s.end : min(s.end, j + A.window);
 }
 
-// Queries [qbeg, qend) that may see the keys [k0, k1).
+// ---- the sinks' far queries ----------------------------------------------------
+// A key that stays visible to the end of a long sequence would make the pass over
+// its row tile walk every later query. Instead a query tile (2^SH queries) whose
+// window has left the sinks (its band of keys starts behind them) adds their
+// gradients on the way, as float32 partials [query tile][head][k, v][sink][Dh];
+// attn_sink_sum adds them up in their order, and the sink's row tile takes the sum.
+
+// Query tiles from this one on are far from key j of their own sequence: 2^SH n >= j + window.
+template <int SH> __device__ __forceinline__ int first_far(const AttnArgs& A, int j) {
+  return (int)(((int64_t)j + A.window + (1 << SH) - 1) >> SH);
+}
+__device__ __forceinline__ int64_t part_at(const AttnArgs& A, int n, int h, int kv, int r) {
+  return ((((int64_t)n * A.Hq + h) * 2 + kv) * A.sinks + r) * A.Dh;
+}
+// The first query that the pass over key tiles leaves to the partials, for a sink j of a sequence that ends at `end`.
+template <int SH> __device__ __forceinline__ int near_end(const AttnArgs& A, int j, int end) {
+  return (int)min((int64_t)end, (int64_t)first_far<SH>(A, j) << SH);
+}
+// key_limit without the far queries.
+template <int SH> __device__ __forceinline__ int near_limit(const AttnArgs& A, int j) {
+  const SeqRange s = seq_of(A, j);
+  if (s.end <= j) return 0;
+  const int hi = min(s.end, j + A.window);
+  return j - s.start < A.sinks ? max(hi, near_end<SH>(A, j, s.end)) : hi;
+}
+// Queries [qbeg, qend) that may see the keys [k0, k1), without the far ones.
 struct QueryRange {
   int qbeg, qend;
 };
-__device__ __forceinline__ QueryRange queries_of(const AttnArgs& A, int k0, int k1) {
+template <int SH> __device__ __forceinline__ QueryRange near_queries(const AttnArgs& A, int k0, int k1) {
   const int f = max(k0, first_token(A)), e = min(k1, end_token(A));
   if (f >= e) return {0, 0};
   const SeqRange s = seq_of(A, e - 1);
-  const bool sink = max(f, s.start) - s.start < A.sinks;
-  return {f, max(sink ? s.end : min(s.end, e - 1 + A.window), e)};
+  int end = max(e, min(s.end, e - 1 + A.window));
+  const int last_sink = min(e - 1, s.start + A.sinks - 1);
+  if (last_sink >= max(f, s.start)) end = max(end, near_end<SH>(A, last_sink, s.end));
+  return {f, end};
+}
+// The summed partials (k, then v `A.sinks * A.Dh` further on) of key j for key head hk, or NULL.
+template <int SH> __device__ __forceinline__ const float* far_sum(const AttnArgs& A, int j, int hk) {
+  if (A.part == nullptr) return nullptr;
+  const SeqRange s = seq_of(A, j);
+  if (s.end <= j || j - s.start >= A.sinks || (int64_t)first_far<SH>(A, j) << SH >= s.end) return nullptr;
+  return A.part + part_at(A, first_far<SH>(A, s.start), hk * (A.Hq / A.Hkv), 0, j - s.start);
+}
+template <int SH> size_t part_bytes(int64_t T, int64_t Hq, int64_t Dh, int64_t sinks) {
+  return (size_t)((T + (1 << SH) - 1) / (1 << SH) * Hq * 2 * sinks * Dh * 4);
+}
+static inline bool has_far(const AttnArgs& A) { return A.sinks > 0 && A.window < A.T; }
+
+// part[first far tile of a sequence][first head of a group] <- the sum over the
+// sequence's far tiles and the group's heads, in their order: 4 threads per
+// element take a quarter of the terms each. Grid: query tiles, key heads, sinks.
+template <int SH> __global__ void __launch_bounds__(1024) attn_sink_sum(const __grid_constant__ AttnArgs A) {
+  __shared__ float sums[4][256];
+  const int n = blockIdx.x, hk = blockIdx.y, r = blockIdx.z, G = A.Hq / A.Hkv;
+  const KeyRange R = keys_of(A, n << SH, (n + 1) << SH);
+  if (R.send <= R.s0 || first_far<SH>(A, R.s0) != n) return;
+  const SeqRange s = seq_of(A, R.s0);
+  const int beg = max(n, first_far<SH>(A, s.start + r)), tiles = ((s.end + (1 << SH) - 1) >> SH) - beg;
+  if (tiles <= 0 || s.start + r >= s.end) return;
+  const int v = threadIdx.x & 255, quarter = threadIdx.x >> 8, terms = tiles * G;
+  const int kv = v / A.Dh, d = v % A.Dh;
+  float sum = 0.f;
+  if (kv < 2)
+#pragma unroll 8
+    for (int x = terms * quarter / 4; x < terms * (quarter + 1) / 4; ++x)
+      sum += A.part[part_at(A, beg + x / G, hk * G + x % G, kv, r) + d];
+  sums[quarter][v] = sum;
+  __syncthreads();
+  if (quarter == 0 && kv < 2)
+    A.part[part_at(A, n, hk * G, kv, r) + d] = (sums[0][v] + sums[1][v]) + (sums[2][v] + sums[3][v]);
+}
+template <int SH> int attn_sink_sum_launch(const AttnArgs& A, cudaStream_t st) {
+  attn_sink_sum<SH><<<dim3((A.T + (1 << SH) - 1) >> SH, A.Hkv, A.sinks), 1024, 0, st>>>(A);
+  return check_launch("attn_sink_sum");
 }
 
 // ---- exact rows --------------------------------------------------------------

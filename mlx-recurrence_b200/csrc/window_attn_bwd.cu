@@ -21,12 +21,9 @@
 // under the dS arithmetic, the next S follows as soon as P (KV = false: S) has
 // been read, the next dP after dS C1.
 //
-// Sinks: a key that stays visible to the end of a long sequence would make its
-// row tile walk every later query. Instead a query tile whose window has left the
-// sinks (that is, whose band of keys starts behind them) adds their gradients on
-// the way: products over its 128 queries, with P and dS handed through shared
-// memory, written as float32 partials [query tile][head][k, v][sink][Dh]; a small
-// kernel sums them in order, and the row tile of the sink adds the sum.
+// The sinks' far queries (window_attn.cuh): a query tile that meets a sink tile adds
+// the sinks' gradients by products over its 128 queries, with P and dS handed
+// through shared memory.
 #include "window_tc.cuh"
 
 namespace mr {
@@ -39,16 +36,8 @@ template <int NB> constexpr int kBwdThreads = kNS<NB> * 128 + 32;
 
 struct BwdArgs {
   AttnArgs a;
-  float* part;           // sink partials, or NULL
   const uint32_t* amax;  // fp16: the largest finite |gy| as float bits
 };
-
-// A query tile n (128 queries) is far from key j of its own sequence when 128 n >= j + window.
-__device__ __forceinline__ int first_far(const AttnArgs& A, int j) { return (int)(((int64_t)j + A.window + 127) >> 7); }
-
-__device__ __forceinline__ int64_t part_at(const AttnArgs& A, int n, int h, int kv, int r) {
-  return ((((int64_t)n * A.Hq + h) * 2 + kv) * A.sinks + r) * A.Dh;
-}
 
 // fp16 keeps dS near one: a power of two of the size of gy comes out of it and back in at the end
 template <typename T> __device__ __forceinline__ float ds_factor(const uint32_t*) { return 1.f; }
@@ -80,20 +69,13 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
   const AttnArgs& A = P.a;
   const int tid = threadIdx.x, w = tid >> 5, G = A.Hq / A.Hkv;
   const int hr = blockIdx.y, hk = KV ? hr : hr / G, r0 = blockIdx.x * 128;
-  const int first = first_token(A), end = end_token(A);
+  const int end = end_token(A);
 
   // the columns: keys (a sink tile, then the band) or queries, per query head
   int c_beg = 0, c_end = 0, s0 = 0, send = 0;
   if (KV) {
-    const int f = max(r0, first), e = min(r0 + 128, end);
-    if (f < e) {
-      const SeqRange s = seq_of(A, e - 1);
-      c_beg = f;
-      c_end = min(s.end, e - 1 + A.window);
-      const int last_sink = min(e - 1, s.start + A.sinks - 1);
-      if (last_sink >= max(f, s.start)) c_end = max(c_end, (int)min((int64_t)s.end, (int64_t)first_far(A, last_sink) * 128));
-      c_end = max(c_end, e);
-    }
+    const QueryRange Q = near_queries<7>(A, r0, r0 + 128);
+    c_beg = Q.qbeg, c_end = Q.qend;
   } else {
     const KeyRange R = keys_of(A, r0, r0 + 128);
     c_beg = R.kmin, c_end = R.kend, s0 = R.s0, send = R.send;
@@ -254,12 +236,10 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
     float lse_r = INFINITY, delta_r = 0.f;
     bool alive = false;
     if (KV) {
-      const SeqRange s = seq_of(A, r);
-      alive = s.end > r;
+      hi = near_limit<7>(A, r);
+      alive = hi > 0;
       if (alive) {
         lo = r;
-        hi = min(s.end, r + A.window);
-        if (r - s.start < A.sinks) hi = max(hi, (int)min((int64_t)s.end, (int64_t)first_far(A, r) * 128));
         atomicMin(&sh.lim_min, hi);
       }
     } else {
@@ -395,8 +375,8 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
         mbar_wait(&sh.sink_done, 0);
         umma::fence_after_sync();
         if (row < 64) {  // lanes 0 .. 63 hold the sinks
-          float* pk = P.part + part_at(A, blockIdx.x, hr, 0, row);
-          float* pv = P.part + part_at(A, blockIdx.x, hr, 1, row);
+          float* pk = A.part + part_at(A, blockIdx.x, hr, 0, row);
+          float* pv = A.part + part_at(A, blockIdx.x, hr, 1, row);
           for (int d = 0; d < A.Dh; d += 32) {
             uint32_t gk[32], gv[32];
             umma::tmem_ld32(trow + kSinkK + d, gk);
@@ -421,12 +401,7 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
     const int64_t at = ((int64_t)r * H + hr) * A.Dh;
     float odd = 0.f;  // NaN as soon as one element is not finite
     // a sink's far queries
-    const float* far = nullptr;
-    if (KV && alive && P.part != nullptr) {
-      const SeqRange s = seq_of(A, r);
-      if (r - s.start < A.sinks && (int64_t)first_far(A, r) * 128 < s.end)
-        far = P.part + part_at(A, first_far(A, s.start), hk * G, 0, r - s.start);
-    }
+    const float* far = KV ? far_sum<7>(A, r, hk) : nullptr;
     // the warpgroups share the blocks of 32 columns
     for (int a = 0; a < (KV ? 2 : 1); ++a) {
       const float scale = a == 0 ? A.scale : 1.f, fa = a == 0 ? 1.f / f : 1.f;
@@ -469,30 +444,6 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
   if (w == 4 * NS) umma::tmem_dealloc(tm, kCols);
 }
 
-// part[first far tile of a sequence][first head of a group] <- the sum over the
-// sequence's far tiles and the group's heads, in their order: 4 threads per
-// element take a quarter of the terms each. Grid: query tiles, key heads, sinks.
-__global__ void __launch_bounds__(1024) attn_sink_sum(const __grid_constant__ AttnArgs A, float* part) {
-  __shared__ float sums[4][256];
-  const int n = blockIdx.x, hk = blockIdx.y, r = blockIdx.z, G = A.Hq / A.Hkv;
-  const KeyRange R = keys_of(A, n * 128, n * 128 + 128);
-  if (R.send <= R.s0 || first_far(A, R.s0) != n) return;
-  const SeqRange s = seq_of(A, R.s0);
-  const int beg = max(n, first_far(A, s.start + r)), tiles = (s.end + 127) / 128 - beg;
-  if (tiles <= 0 || s.start + r >= s.end) return;
-  const int v = threadIdx.x & 255, quarter = threadIdx.x >> 8, terms = tiles * G;
-  const int kv = v / A.Dh, d = v % A.Dh;
-  float sum = 0.f;
-  if (kv < 2)
-#pragma unroll 8
-    for (int x = terms * quarter / 4; x < terms * (quarter + 1) / 4; ++x)
-      sum += part[part_at(A, beg + x / G, hk * G + x % G, kv, r) + d];
-  sums[quarter][v] = sum;
-  __syncthreads();
-  if (quarter == 0 && kv < 2)
-    part[part_at(A, n, hk * G, kv, r) + d] = (sums[0][v] + sums[1][v]) + (sums[2][v] + sums[3][v]);
-}
-
 // delta[h][t] = sum_d gy y, zero for rows outside every sequence; fp16: the
 // largest finite |gy| (the order of an integer maximum does not matter). 8 lanes
 // per row, 16 bytes each at a time.
@@ -525,10 +476,8 @@ template <typename T> __global__ void __launch_bounds__(256) attn_delta_kernel(c
   }
 }
 
-static bool has_far(const AttnArgs& A) { return A.sinks > 0 && A.window < A.T; }
-
 size_t attn_bwd_ws_bytes(int64_t T, int64_t Hq, int64_t Dh, int64_t sinks) {
-  return 16 + (size_t)((T * Hq + 3) / 4 * 16) + (size_t)((T + 127) / 128 * Hq * 2 * sinks * Dh * 4);
+  return 16 + (size_t)((T * Hq + 3) / 4 * 16) + part_bytes<7>(T, Hq, Dh, sinks);
 }
 
 template <typename T, int NB, bool KV>
@@ -549,19 +498,17 @@ static int bwd_one(const BwdArgs& P, cudaStream_t st) {
 
 template <typename T, int NB> static int bwd_nb(const BwdArgs& P, cudaStream_t st) {
   if (int rc = bwd_one<T, NB, false>(P, st)) return rc;
-  if (P.part != nullptr) {
-    attn_sink_sum<<<dim3((P.a.T + 127) / 128, P.a.Hkv, P.a.sinks), 1024, 0, st>>>(P.a, P.part);
-    if (int rc = check_launch("attn_sink_sum")) return rc;
-  }
+  if (P.a.part != nullptr)
+    if (int rc = attn_sink_sum_launch<7>(P.a, st)) return rc;
   return bwd_one<T, NB, true>(P, st);
 }
 
 // ws: attn_bwd_ws_bytes, 16-byte aligned
 template <typename T> int attn_bwd_launch(const AttnArgs& A0, void* ws, cudaStream_t st) {
-  BwdArgs P{A0, nullptr, nullptr};
+  BwdArgs P{A0, nullptr};
   uint32_t* amax = (uint32_t*)ws;
   P.a.delta = (float*)((char*)ws + 16);
-  if (has_far(A0)) P.part = P.a.delta + ((int64_t)A0.T * A0.Hq + 3) / 4 * 4;
+  if (has_far(A0)) P.a.part = P.a.delta + ((int64_t)A0.T * A0.Hq + 3) / 4 * 4;
   const bool half = Fmt<T>::id == 0;
   if (half) {
     P.amax = amax;

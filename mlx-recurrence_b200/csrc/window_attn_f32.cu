@@ -18,14 +18,27 @@ constexpr int kBT = 64;        // tile edge
 constexpr int kPitch = kBT + 4;
 constexpr int kThreads = 128;
 
-// rows r0 .. r0+63 of one head as [d][kPitch] float32, zeros outside [lo, hi)
-template <typename T, int DH>
-__device__ __forceinline__ void load_t(float* dst, const T* src, int64_t ts, int r0, int lo, int hi) {
-  for (int e = threadIdx.x; e < kBT * DH; e += kThreads) {
-    const int r = e / DH, d = e % DH, t = r0 + r;
-    dst[d * kPitch + r] = (t >= lo && t < hi) ? to_f(src[t * ts + d]) : 0.f;
+// rows r0 .. r0+63 of one head, on their way to [d][kPitch] in shared memory; zeros outside [lo, hi). In two steps, so
+// that the next tile's loads run under this tile's arithmetic. Lanes take consecutive rows: conflict-free stores.
+template <int DH> struct Tile {
+  static constexpr int N = kBT * DH / 4 / kThreads;
+  float4 v[N];
+  __device__ __forceinline__ void fetch(const float* src, int64_t ts, int r0, int lo, int hi) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = threadIdx.x + i * kThreads, t = r0 + (e & 63);
+      v[i] = t >= lo && t < hi ? *reinterpret_cast<const float4*>(src + t * ts + (e >> 6) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
   }
-}
+  __device__ __forceinline__ void stash(float* dst) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = threadIdx.x + i * kThreads;
+      float* p = dst + (e >> 6) * 4 * kPitch + (e & 63);
+      p[0] = v[i].x, p[kPitch] = v[i].y, p[2 * kPitch] = v[i].z, p[3 * kPitch] = v[i].w;
+    }
+  }
+};
 
 // acc[8][4] = sum_d R[d][8 rows of ty] C[d][4 columns of tx]
 template <int DH>
@@ -74,7 +87,7 @@ __device__ __forceinline__ void put_block(float* P, const float (&v)[8][4], int 
   }
 }
 
-template <typename T, int DH>
+template <int DH>
 __global__ void __launch_bounds__(kThreads) attn_fwd_f32(const __grid_constant__ AttnArgs A) {
   extern __shared__ float sm[];
   float *sQ = sm, *sK = sQ + DH * kPitch, *sV = sK + DH * kPitch, *sP = sV + DH * kPitch;
@@ -82,13 +95,15 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_f32(const __grid_constant__
   __shared__ int again[kBT];
   const int q0 = blockIdx.x * kBT, h = blockIdx.y, hk = h / (A.Hq / A.Hkv);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const T* q = (const T*)A.q + h * A.q_hs;
-  const T* k = (const T*)A.k + hk * A.k_hs;
-  const T* v = (const T*)A.v + hk * A.v_hs;
+  const float* q = (const float*)A.q + h * A.q_hs;
+  const float* k = (const float*)A.k + hk * A.k_hs;
+  const float* v = (const float*)A.v + hk * A.v_hs;
   const KeyRange R = keys_of(A, q0, q0 + kBT);
   const int first = first_token(A), last = end_token(A);
   if (threadIdx.x < kBT) rows[threadIdx.x] = row_mask(A, q0 + threadIdx.x), again[threadIdx.x] = 0;
-  load_t<T, DH>(sQ, q, A.q_ts, q0, first, last);
+  Tile<DH> tq;
+  tq.fetch(q, A.q_ts, q0, first, last);
+  tq.stash(sQ);
   const float c = A.scale * kAttnLog2e;
   float m[8], l[8], o[8][DH / 16];
 #pragma unroll
@@ -99,13 +114,21 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_f32(const __grid_constant__
   }
   const int nsink = R.send > R.s0 ? (R.send - R.s0 + kBT - 1) / kBT : 0;
   const int nband = R.kend > R.kmin ? (R.kend - R.kmin + kBT - 1) / kBT : 0;
+  auto beg = [&](int it) { return it < nsink ? R.s0 + it * kBT : R.kmin + (it - nsink) * kBT; };
+  auto lim = [&](int it) { return min(beg(it) + kBT, it < nsink ? R.send : R.kend); };
+  Tile<DH> tk, tv;
+  auto fetch = [&](int it) {
+    tk.fetch(k, A.k_ts, beg(it), first, lim(it));
+    tv.fetch(v, A.v_ts, beg(it), first, lim(it));
+  };
+  if (nsink + nband > 0) fetch(0);
   for (int it = 0; it < nsink + nband; ++it) {
-    const int k0 = it < nsink ? R.s0 + it * kBT : R.kmin + (it - nsink) * kBT;
-    const int k1 = min(k0 + kBT, it < nsink ? R.send : R.kend);
+    const int k0 = beg(it), k1 = lim(it);
     __syncthreads();
-    load_t<T, DH>(sK, k, A.k_ts, k0, first, k1);
-    load_t<T, DH>(sV, v, A.v_ts, k0, first, k1);
+    tk.stash(sK);
+    tv.stash(sV);
     __syncthreads();
+    if (it + 1 < nsink + nband) fetch(it + 1);
     float s[8][4];
     tile_dot<DH>(s, sQ, sK, ty, tx);
 #pragma unroll
@@ -143,11 +166,11 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_f32(const __grid_constant__
     const int t = q0 + ty * 8 + i;
     if (t >= A.T) continue;
     const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
-    T* y = (T*)A.y + ((int64_t)t * A.Hq + h) * A.Dh;
+    float* y = (float*)A.y + ((int64_t)t * A.Hq + h) * A.Dh;
     float odd = 0.f;  // NaN as soon as one element is not finite
 #pragma unroll
     for (int n = 0; n < DH / 16; ++n) {
-      y[tx + 16 * n] = from_f<T>(o[i][n] * inv);
+      y[tx + 16 * n] = (o[i][n] * inv);
       odd = fmaf(o[i][n], 0.f, odd);
     }
     if (A.lse != nullptr && tx == 0) A.lse[(int64_t)h * A.T + t] = l[i] == 0.f ? INFINITY : m[i] + log2f(l[i]);
@@ -155,19 +178,18 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_f32(const __grid_constant__
   }
   __syncthreads();
   for (int r = threadIdx.x >> 5; r < kBT; r += kThreads / 32)
-    if (again[r]) exact_fwd_row<T>(A, h, q0 + r);
+    if (again[r]) exact_fwd_row<float>(A, h, q0 + r);
 }
 
 // delta[h][t] = sum_d gy y: one warp per row
-template <typename T>
-__global__ void __launch_bounds__(256) attn_delta(const __grid_constant__ AttnArgs A) {
+__global__ void __launch_bounds__(256) attn_delta_f32(const __grid_constant__ AttnArgs A) {
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= (int64_t)A.T * A.Hq) return;
-  const T* g = (const T*)A.gy + row * A.Dh;
-  const T* y = (const T*)A.y + row * A.Dh;
+  const float* g = (const float*)A.gy + row * A.Dh;
+  const float* y = (const float*)A.y + row * A.Dh;
   float s = 0.f;
-  for (int d = lane; d < A.Dh; d += 32) s = fmaf(to_f(g[d]), to_f(y[d]), s);
+  for (int d = lane; d < A.Dh; d += 32) s = fmaf((g[d]), (y[d]), s);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
   if (lane == 0) A.delta[(row % A.Hq) * A.T + row / A.Hq] = s;
@@ -175,7 +197,7 @@ __global__ void __launch_bounds__(256) attn_delta(const __grid_constant__ AttnAr
 
 // KV = false: rows are queries, columns keys, out1 = grad_q.
 // KV = true: rows are keys, columns queries, out1 = grad_k, out2 = grad_v.
-template <typename T, int DH, bool KV>
+template <int DH, bool KV>
 __global__ void __launch_bounds__(kThreads) attn_bwd_f32(const __grid_constant__ AttnArgs A) {
   extern __shared__ float sm[];
   float *sR1 = sm, *sR2 = sR1 + DH * kPitch, *sC1 = sR2 + DH * kPitch, *sC2 = sC1 + DH * kPitch, *sP = sC2 + DH * kPitch;
@@ -186,8 +208,8 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_f32(const __grid_constant__
   const int hk = KV ? blockIdx.y : blockIdx.y / G;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int first = first_token(A), last = end_token(A);
-  const T* k = (const T*)A.k + hk * A.k_hs;
-  const T* v = (const T*)A.v + hk * A.v_hs;
+  const float* k = (const float*)A.k + hk * A.k_hs;
+  const float* v = (const float*)A.v + hk * A.v_hs;
   const int64_t gts = (int64_t)A.Hq * A.Dh;
   const float c = A.scale * kAttnLog2e;
   float o1[8][DH / 16], o2[KV ? 8 : 1][DH / 16];
@@ -197,7 +219,7 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_f32(const __grid_constant__
     for (int n = 0; n < DH / 16; ++n) o1[i][n] = o2[KV ? i : 0][n] = 0.f;
 
   const KeyRange R = keys_of(A, r0, r0 + kBT);
-  const QueryRange Q = queries_of(A, r0, r0 + kBT);
+  const QueryRange Q = near_queries<6>(A, r0, r0 + kBT);
   const int nsink = !KV && R.send > R.s0 ? (R.send - R.s0 + kBT - 1) / kBT : 0;
   const int nband = KV ? (Q.qend > Q.qbeg ? (Q.qend - Q.qbeg + kBT - 1) / kBT : 0)
                        : (R.kend > R.kmin ? (R.kend - R.kmin + kBT - 1) / kBT : 0);
@@ -205,39 +227,53 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_f32(const __grid_constant__
     const int t = r0 + threadIdx.x;
     again[threadIdx.x] = 0;
     if (KV) {
-      limit[threadIdx.x] = key_limit(A, t);
+      limit[threadIdx.x] = near_limit<6>(A, t);
     } else {
       rows[threadIdx.x] = row_mask(A, t);
       lse[threadIdx.x] = t < A.T ? A.lse[(int64_t)blockIdx.y * A.T + t] : INFINITY;
       delta[threadIdx.x] = t < A.T ? A.delta[(int64_t)blockIdx.y * A.T + t] : 0.f;
     }
   }
+  Tile<DH> t1, t2;
   if (KV) {
-    load_t<T, DH>(sR1, k, A.k_ts, r0, first, last);
-    load_t<T, DH>(sR2, v, A.v_ts, r0, first, last);
+    t1.fetch(k, A.k_ts, r0, first, last);
+    t2.fetch(v, A.v_ts, r0, first, last);
   } else {
-    load_t<T, DH>(sR1, (const T*)A.q + blockIdx.y * A.q_hs, A.q_ts, r0, first, last);
-    load_t<T, DH>(sR2, (const T*)A.gy + (int64_t)blockIdx.y * A.Dh, gts, r0, first, last);
+    t1.fetch((const float*)A.q + blockIdx.y * A.q_hs, A.q_ts, r0, first, last);
+    t2.fetch((const float*)A.gy + (int64_t)blockIdx.y * A.Dh, gts, r0, first, last);
   }
-  for (int it = 0; it < (KV ? G : 1) * (nsink + nband); ++it) {
-    const int h = KV ? hk * G + it / nband : blockIdx.y;
+  t1.stash(sR1);
+  t2.stash(sR2);
+  const int n_it = (KV ? G : 1) * (nsink + nband);
+  auto head = [&](int it) { return KV ? hk * G + it / nband : (int)blockIdx.y; };
+  auto beg = [&](int it) {
     const int n = KV ? it % nband : it;
-    const int c0 = KV ? Q.qbeg + n * kBT : n < nsink ? R.s0 + n * kBT : R.kmin + (n - nsink) * kBT;
-    const int c1 = min(c0 + kBT, KV ? Q.qend : n < nsink ? R.send : R.kend);
-    __syncthreads();
+    return KV ? Q.qbeg + n * kBT : n < nsink ? R.s0 + n * kBT : R.kmin + (n - nsink) * kBT;
+  };
+  auto lim = [&](int it) { return min(beg(it) + kBT, KV ? Q.qend : it < nsink ? R.send : R.kend); };
+  float lse_n = INFINITY, delta_n = 0.f;
+  auto fetch = [&](int it) {
+    const int h = head(it), c0 = beg(it), c1 = lim(it);
     if (KV) {
-      load_t<T, DH>(sC1, (const T*)A.q + h * A.q_hs, A.q_ts, c0, first, c1);
-      load_t<T, DH>(sC2, (const T*)A.gy + (int64_t)h * A.Dh, gts, c0, first, c1);
-      if (threadIdx.x < kBT) {
-        const int t = c0 + threadIdx.x;
-        lse[threadIdx.x] = t < c1 ? A.lse[(int64_t)h * A.T + t] : INFINITY;
-        delta[threadIdx.x] = t < c1 ? A.delta[(int64_t)h * A.T + t] : 0.f;
-      }
+      t1.fetch((const float*)A.q + h * A.q_hs, A.q_ts, c0, first, c1);
+      t2.fetch((const float*)A.gy + (int64_t)h * A.Dh, gts, c0, first, c1);
+      const int t = c0 + (threadIdx.x & 63);
+      lse_n = t < c1 ? A.lse[(int64_t)h * A.T + t] : INFINITY;
+      delta_n = t < c1 ? A.delta[(int64_t)h * A.T + t] : 0.f;
     } else {
-      load_t<T, DH>(sC1, k, A.k_ts, c0, first, c1);
-      load_t<T, DH>(sC2, v, A.v_ts, c0, first, c1);
+      t1.fetch(k, A.k_ts, c0, first, c1);
+      t2.fetch(v, A.v_ts, c0, first, c1);
     }
+  };
+  if (n_it > 0) fetch(0);
+  for (int it = 0; it < n_it; ++it) {
+    const int c0 = beg(it), c1 = lim(it);
     __syncthreads();
+    t1.stash(sC1);
+    t2.stash(sC2);
+    if (KV && threadIdx.x < kBT) lse[threadIdx.x] = lse_n, delta[threadIdx.x] = delta_n;
+    __syncthreads();
+    if (it + 1 < n_it) fetch(it + 1);
     float s[8][4], dp[8][4];
     tile_dot<DH>(s, sR1, sC1, ty, tx);
     tile_dot<DH>(dp, sR2, sC2, ty, tx);
@@ -261,6 +297,28 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_f32(const __grid_constant__
     put_block(sP, dp, ty, tx);
     __syncthreads();
     tile_acc<DH>(o1, sP, sC1, ty, tx);
+    if (!KV && it < nsink) {  // the sinks' gradients from these queries: P and dS once more, as [query][key]
+      float og[8][DH / 16];
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float(&b)[4] = kv ? s[i] : dp[i];
+          *reinterpret_cast<float4*>(sP + (ty * 8 + i) * kPitch + tx * 4) = make_float4(b[0], b[1], b[2], b[3]);
+#pragma unroll
+          for (int n = 0; n < DH / 16; ++n) og[i][n] = 0.f;
+        }
+        __syncthreads();
+        tile_acc<DH>(og, sP, kv ? sR2 : sR1, ty, tx);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (ty * 8 + i < c1 - c0)
+#pragma unroll
+            for (int n = 0; n < DH / 16; ++n)
+              A.part[part_at(A, blockIdx.x, blockIdx.y, kv, ty * 8 + i) + tx + 16 * n] = og[i][n];
+      }
+    }
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -268,12 +326,19 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_f32(const __grid_constant__
     if (t >= A.T) continue;
     const int H = KV ? A.Hkv : A.Hq;
     const int64_t at = ((int64_t)t * H + blockIdx.y) * A.Dh;
-    T* g1 = (T*)(KV ? A.gk : A.gq) + at;
+    float* g1 = (float*)(KV ? A.gk : A.gq) + at;
     float odd = 0.f;  // NaN as soon as one element is not finite
+    if (KV)
+      if (const float* far = far_sum<6>(A, t, hk))
+#pragma unroll
+        for (int n = 0; n < DH / 16; ++n) {
+          o1[i][n] += far[tx + 16 * n];
+          o2[KV ? i : 0][n] += far[A.sinks * A.Dh + tx + 16 * n];
+        }
 #pragma unroll
     for (int n = 0; n < DH / 16; ++n) {
-      g1[tx + 16 * n] = from_f<T>(o1[i][n] * A.scale);
-      if (KV) ((T*)A.gv + at)[tx + 16 * n] = from_f<T>(o2[KV ? i : 0][n]);
+      g1[tx + 16 * n] = (o1[i][n] * A.scale);
+      if (KV) ((float*)A.gv + at)[tx + 16 * n] = (o2[KV ? i : 0][n]);
       odd = fmaf(o1[i][n], 0.f, fmaf(o2[KV ? i : 0][n], 0.f, odd));
     }
     if (odd != 0.f) again[ty * 8 + i] = 1;
@@ -281,8 +346,8 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_f32(const __grid_constant__
   __syncthreads();
   for (int r = threadIdx.x >> 5; r < kBT; r += kThreads / 32)
     if (again[r]) {
-      if (KV) exact_gkv_row<T>(A, blockIdx.y, r0 + r);
-      else exact_gq_row<T>(A, blockIdx.y, r0 + r);
+      if (KV) exact_gkv_row<float>(A, blockIdx.y, r0 + r);
+      else exact_gq_row<float>(A, blockIdx.y, r0 + r);
     }
 }
 
@@ -296,44 +361,44 @@ static int launch(K kernel, dim3 grid, size_t smem, const AttnArgs& A, cudaStrea
   return check_launch(what);
 }
 
-template <typename T, int DH> static int fwd_dh(const AttnArgs& A, cudaStream_t st) {
-  return launch(attn_fwd_f32<T, DH>, dim3((A.T + kBT - 1) / kBT, A.Hq), (3 * DH + kBT) * kPitch * 4, A, st, "attn_fwd_f32");
+template <int DH> static int fwd_dh(const AttnArgs& A, cudaStream_t st) {
+  return launch(attn_fwd_f32<DH>, dim3((A.T + kBT - 1) / kBT, A.Hq), (3 * DH + kBT) * kPitch * 4, A, st, "attn_fwd_f32");
 }
-template <typename T, int DH> static int bwd_dh(const AttnArgs& A, cudaStream_t st) {
+template <int DH> static int bwd_dh(const AttnArgs& A, cudaStream_t st) {
   const size_t sm = (4 * DH + kBT) * kPitch * 4;
   const unsigned n = (A.T + kBT - 1) / kBT;
-  if (int rc = launch(attn_bwd_f32<T, DH, false>, dim3(n, A.Hq), sm, A, st, "attn_bwd_f32 (grad_q)")) return rc;
-  return launch(attn_bwd_f32<T, DH, true>, dim3(n, A.Hkv), sm, A, st, "attn_bwd_f32 (grad_k, grad_v)");
+  if (int rc = launch(attn_bwd_f32<DH, false>, dim3(n, A.Hq), sm, A, st, "attn_bwd_f32 (grad_q)")) return rc;
+  if (A.part != nullptr)
+    if (int rc = attn_sink_sum_launch<6>(A, st)) return rc;
+  return launch(attn_bwd_f32<DH, true>, dim3(n, A.Hkv), sm, A, st, "attn_bwd_f32 (grad_k, grad_v)");
 }
 
-template <typename T> int attn_delta_launch(const AttnArgs& A, cudaStream_t st) {
-  attn_delta<T><<<(unsigned)(((int64_t)A.T * A.Hq + 7) / 8), 256, 0, st>>>(A);
-  return check_launch("attn_delta");
-}
-
-template <typename T> int attn_fwd_simt(const AttnArgs& A, cudaStream_t st) {
+int attn_fwd_f32_launch(const AttnArgs& A, cudaStream_t st) {
   switch (A.Dh) {
-    case 32: return fwd_dh<T, 32>(A, st);
-    case 64: return fwd_dh<T, 64>(A, st);
-    case 96: return fwd_dh<T, 96>(A, st);
-    default: return fwd_dh<T, 128>(A, st);
-  }
-}
-template <typename T> int attn_bwd_simt(const AttnArgs& A, cudaStream_t st) {
-  if (int rc = attn_delta_launch<T>(A, st)) return rc;
-  switch (A.Dh) {
-    case 32: return bwd_dh<T, 32>(A, st);
-    case 64: return bwd_dh<T, 64>(A, st);
-    case 96: return bwd_dh<T, 96>(A, st);
-    default: return bwd_dh<T, 128>(A, st);
+    case 32: return fwd_dh<32>(A, st);
+    case 64: return fwd_dh<64>(A, st);
+    case 96: return fwd_dh<96>(A, st);
+    default: return fwd_dh<128>(A, st);
   }
 }
 
-#define MR_INST(T)                                                   \
-  template int attn_delta_launch<T>(const AttnArgs&, cudaStream_t);  \
-  template int attn_fwd_simt<T>(const AttnArgs&, cudaStream_t);      \
-  template int attn_bwd_simt<T>(const AttnArgs&, cudaStream_t);
-MR_INST(float)
-#undef MR_INST
+size_t attn_bwd_f32_ws_bytes(int64_t T, int64_t Hq, int64_t Dh, int64_t sinks) {
+  return (size_t)((T * Hq + 3) / 4 * 16) + part_bytes<6>(T, Hq, Dh, sinks);
+}
+
+// ws: attn_bwd_f32_ws_bytes, 16-byte aligned
+int attn_bwd_f32_launch(const AttnArgs& A0, void* ws, cudaStream_t st) {
+  AttnArgs A = A0;
+  A.delta = (float*)ws;
+  if (has_far(A)) A.part = A.delta + ((int64_t)A.T * A.Hq + 3) / 4 * 4;
+  attn_delta_f32<<<(unsigned)(((int64_t)A.T * A.Hq + 7) / 8), 256, 0, st>>>(A);
+  if (int rc = check_launch("attn_delta_f32")) return rc;
+  switch (A.Dh) {
+    case 32: return bwd_dh<32>(A, st);
+    case 64: return bwd_dh<64>(A, st);
+    case 96: return bwd_dh<96>(A, st);
+    default: return bwd_dh<128>(A, st);
+  }
+}
 
 }  // namespace mr
