@@ -7,7 +7,7 @@
 //   ds_ij = p_ij (gy_i.v_j - delta_i),  delta_i = gy_i.y_i
 //   grad_q_i = scale sum_j ds_ij k_j,  grad_k_j = scale sum_i ds_ij q_i,  grad_v_j = sum_i p_ij gy_i
 //
-// Tiles are 64 x 64; 128 threads own 8 x 4 results of a tile and 8 rows x Dh/16
+// Tiles are 64 x 64; 256 threads own 4 x 4 results of a tile and 4 rows x Dh/16
 // columns of the products that follow. Operands lie transposed ([d][64 + 4]) in
 // shared memory, so a thread's rows and columns come as 16-byte reads.
 #include "window_attn.cuh"
@@ -16,7 +16,8 @@ namespace mr {
 
 constexpr int kBT = 64;        // tile edge
 constexpr int kPitch = kBT + 4;
-constexpr int kThreads = 128;
+constexpr int kThreads = 256;
+constexpr int kR = 4;  // rows of a thread
 
 // rows r0 .. r0+63 of one head, on their way to [d][kPitch] in shared memory; zeros outside [lo, hi). In two steps, so
 // that the next tile's loads run under this tile's arithmetic. Lanes take consecutive rows: conflict-free stores.
@@ -40,55 +41,71 @@ template <int DH> struct Tile {
   }
 };
 
-// acc[8][4] = sum_d R[d][8 rows of ty] C[d][4 columns of tx]
+// acc = sum_d R[d][kR rows of ty] C[d][4 columns of tx], two rows to an instruction
 template <int DH>
-__device__ __forceinline__ void tile_dot(float (&acc)[8][4], const float* R, const float* C, int ty, int tx) {
+__device__ __forceinline__ void tile_dot(float (&acc)[kR][4], const float* R, const float* C, int ty, int tx) {
+  uint64_t a[kR / 2][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < kR / 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) a[i][j] = 0;
 #pragma unroll 4
   for (int d = 0; d < DH; ++d) {
-    float r[8], c[4];
-    *reinterpret_cast<float4*>(r) = *reinterpret_cast<const float4*>(R + d * kPitch + ty * 8);
-    *reinterpret_cast<float4*>(r + 4) = *reinterpret_cast<const float4*>(R + d * kPitch + ty * 8 + 4);
-    *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(C + d * kPitch + tx * 4);
+    const ulonglong2 rr = *reinterpret_cast<const ulonglong2*>(R + d * kPitch + ty * kR);
+    const float4 c = *reinterpret_cast<const float4*>(C + d * kPitch + tx * 4);
+    const uint64_t cc[4] = {pair(c.x, c.x), pair(c.y, c.y), pair(c.z, c.z), pair(c.w, c.w)};
+    const uint64_t r[kR / 2] = {rr.x, rr.y};
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < kR / 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(r[i], c[j], acc[i][j]);
+      for (int j = 0; j < 4; ++j) a[i][j] = fma2(r[i], cc[j], a[i][j]);
   }
+#pragma unroll
+  for (int i = 0; i < kR / 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) unpair(a[i][j], acc[2 * i][j], acc[2 * i + 1][j]);
 }
 
-// out[8][DH/16] += sum_n P[n][8 rows of ty] C[tx + 16 m][n]
+// out[row pairs][DH/16] += sum_n P[n][kR rows of ty] C[tx + 16 m][n], four n at a time: their columns come as one
+// 16-byte read
 template <int DH>
-__device__ __forceinline__ void tile_acc(float (&out)[8][DH / 16], const float* P, const float* C, int ty, int tx) {
-#pragma unroll 2
-  for (int n = 0; n < kBT; ++n) {
-    float r[8];
-    *reinterpret_cast<float4*>(r) = *reinterpret_cast<const float4*>(P + n * kPitch + ty * 8);
-    *reinterpret_cast<float4*>(r + 4) = *reinterpret_cast<const float4*>(P + n * kPitch + ty * 8 + 4);
+__device__ __forceinline__ void tile_acc(uint64_t (&out)[kR / 2][DH / 16], const float* P, const float* C, int ty, int tx) {
+#pragma unroll 1
+  for (int n = 0; n < kBT; n += 4) {
+    float c[DH / 16][4];
 #pragma unroll
-    for (int m = 0; m < DH / 16; ++m) {
-      const float c = C[(tx + 16 * m) * kPitch + n];
+    for (int m = 0; m < DH / 16; ++m)
+      *reinterpret_cast<float4*>(c[m]) = *reinterpret_cast<const float4*>(C + (tx + 16 * m) * kPitch + n);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out[i][m] = fmaf(r[i], c, out[i][m]);
+    for (int x = 0; x < 4; ++x) {
+      const ulonglong2 r = *reinterpret_cast<const ulonglong2*>(P + (n + x) * kPitch + ty * kR);
+#pragma unroll
+      for (int m = 0; m < DH / 16; ++m) {
+        const uint64_t cc = pair(c[m][x], c[m][x]);
+        out[0][m] = fma2(r.x, cc, out[0][m]);
+        out[1][m] = fma2(r.y, cc, out[1][m]);
+      }
     }
   }
 }
+template <int N> __device__ __forceinline__ void rows_of(float (&v)[kR][N], const uint64_t (&a)[kR / 2][N]) {
+#pragma unroll
+  for (int i = 0; i < kR / 2; ++i)
+#pragma unroll
+    for (int n = 0; n < N; ++n) unpair(a[i][n], v[2 * i][n], v[2 * i + 1][n]);
+}
 
-// P[column][row] <- a thread's 8 x 4 block
-__device__ __forceinline__ void put_block(float* P, const float (&v)[8][4], int ty, int tx) {
+// P[column][row] <- a thread's kR x 4 block
+__device__ __forceinline__ void put_block(float* P, const float (&v)[kR][4], int ty, int tx) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    float* p = P + (tx * 4 + j) * kPitch + ty * 8;
+    float* p = P + (tx * 4 + j) * kPitch + ty * kR;
     *reinterpret_cast<float4*>(p) = make_float4(v[0][j], v[1][j], v[2][j], v[3][j]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4][j], v[5][j], v[6][j], v[7][j]);
   }
 }
 
 template <int DH>
-__global__ void __launch_bounds__(kThreads) attn_fwd_f32(const __grid_constant__ AttnArgs A) {
+__global__ void __launch_bounds__(kThreads, DH <= 64 ? 2 : 1) attn_fwd_f32(const __grid_constant__ AttnArgs A) {
   extern __shared__ float sm[];
   float *sQ = sm, *sK = sQ + DH * kPitch, *sV = sK + DH * kPitch, *sP = sV + DH * kPitch;
   __shared__ RowMask rows[kBT];
@@ -105,12 +122,13 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_f32(const __grid_constant__
   tq.fetch(q, A.q_ts, q0, first, last);
   tq.stash(sQ);
   const float c = A.scale * kAttnLog2e;
-  float m[8], l[8], o[8][DH / 16];
+  float m[kR], l[kR], keep[kR], o[kR][DH / 16];
+  uint64_t o2[kR / 2][DH / 16];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < kR; ++i) {
     m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
-    for (int n = 0; n < DH / 16; ++n) o[i][n] = 0.f;
+    for (int n = 0; n < DH / 16; ++n) o2[i / 2][n] = 0;
   }
   const int nsink = R.send > R.s0 ? (R.send - R.s0 + kBT - 1) / kBT : 0;
   const int nband = R.kend > R.kmin ? (R.kend - R.kmin + kBT - 1) / kBT : 0;
@@ -129,11 +147,11 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_f32(const __grid_constant__
     tv.stash(sV);
     __syncthreads();
     if (it + 1 < nsink + nband) fetch(it + 1);
-    float s[8][4];
+    float s[kR][4];
     tile_dot<DH>(s, sQ, sK, ty, tx);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const RowMask w = rows[ty * 8 + i];
+    for (int i = 0; i < kR; ++i) {
+      const RowMask w = rows[ty * kR + i];
       float mx = m[i];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -144,26 +162,29 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_f32(const __grid_constant__
 #pragma unroll
       for (int x = 8; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x, 16));
       const float base = mx == -INFINITY ? 0.f : mx;  // nothing visible so far: every term is exp2(-inf)
-      const float keep = exp2f(m[i] - base);
+      keep[i] = exp2f(m[i] - base);
       m[i] = mx;
-      l[i] *= keep;
-#pragma unroll
-      for (int n = 0; n < DH / 16; ++n) o[i][n] *= keep;
+      l[i] *= keep[i];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         s[i][j] = exp2f(s[i][j] - base);
         l[i] += s[i][j];
       }
     }
+#pragma unroll
+    for (int i = 0; i < kR / 2; ++i)
+#pragma unroll
+      for (int n = 0; n < DH / 16; ++n) o2[i][n] = mul2(o2[i][n], pair(keep[2 * i], keep[2 * i + 1]));
     put_block(sP, s, ty, tx);
     __syncthreads();
-    tile_acc<DH>(o, sP, sV, ty, tx);
+    tile_acc<DH>(o2, sP, sV, ty, tx);
   }
+  rows_of(o, o2);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < kR; ++i) {
 #pragma unroll
     for (int x = 8; x > 0; x >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x, 16);
-    const int t = q0 + ty * 8 + i;
+    const int t = q0 + ty * kR + i;
     if (t >= A.T) continue;
     const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
     float* y = (float*)A.y + ((int64_t)t * A.Hq + h) * A.Dh;
@@ -174,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_f32(const __grid_constant__
       odd = fmaf(o[i][n], 0.f, odd);
     }
     if (A.lse != nullptr && tx == 0) A.lse[(int64_t)h * A.T + t] = l[i] == 0.f ? INFINITY : m[i] + log2f(l[i]);
-    if (odd != 0.f) again[ty * 8 + i] = 1;
+    if (odd != 0.f) again[ty * kR + i] = 1;
   }
   __syncthreads();
   for (int r = threadIdx.x >> 5; r < kBT; r += kThreads / 32)
@@ -198,7 +219,7 @@ __global__ void __launch_bounds__(256) attn_delta_f32(const __grid_constant__ At
 // KV = false: rows are queries, columns keys, out1 = grad_q.
 // KV = true: rows are keys, columns queries, out1 = grad_k, out2 = grad_v.
 template <int DH, bool KV>
-__global__ void __launch_bounds__(kThreads) attn_bwd_f32(const __grid_constant__ AttnArgs A) {
+__global__ void __launch_bounds__(kThreads, DH <= 64 ? 2 : 1) attn_bwd_f32(const __grid_constant__ AttnArgs A) {
   extern __shared__ float sm[];
   float *sR1 = sm, *sR2 = sR1 + DH * kPitch, *sC1 = sR2 + DH * kPitch, *sC2 = sC1 + DH * kPitch, *sP = sC2 + DH * kPitch;
   __shared__ RowMask rows[kBT];
@@ -212,11 +233,11 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_f32(const __grid_constant__
   const float* v = (const float*)A.v + hk * A.v_hs;
   const int64_t gts = (int64_t)A.Hq * A.Dh;
   const float c = A.scale * kAttnLog2e;
-  float o1[8][DH / 16], o2[KV ? 8 : 1][DH / 16];
+  uint64_t a1[kR / 2][DH / 16], a2[kR / 2][DH / 16];  // (a2: KV only)
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < kR / 2; ++i)
 #pragma unroll
-    for (int n = 0; n < DH / 16; ++n) o1[i][n] = o2[KV ? i : 0][n] = 0.f;
+    for (int n = 0; n < DH / 16; ++n) a1[i][n] = a2[i][n] = 0;
 
   const KeyRange R = keys_of(A, r0, r0 + kBT);
   const QueryRange Q = near_queries<6>(A, r0, r0 + kBT);
@@ -274,14 +295,14 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_f32(const __grid_constant__
     if (KV && threadIdx.x < kBT) lse[threadIdx.x] = lse_n, delta[threadIdx.x] = delta_n;
     __syncthreads();
     if (it + 1 < n_it) fetch(it + 1);
-    float s[8][4], dp[8][4];
+    float s[kR][4], dp[kR][4];
     tile_dot<DH>(s, sR1, sC1, ty, tx);
     tile_dot<DH>(dp, sR2, sC2, ty, tx);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < kR; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int r = ty * 8 + i, col = tx * 4 + j;
+        const int r = ty * kR + i, col = tx * 4 + j;
         const bool see = c0 + col < c1 && (KV ? (c0 + col >= r0 + r && c0 + col < limit[r]) : rows[r].sees(c0 + col));
         const int qi = KV ? col : r;
         const float p = see ? exp2f(s[i][j] * c - lse[qi]) : 0.f;
@@ -291,38 +312,43 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_f32(const __grid_constant__
     if (KV) {
       put_block(sP, s, ty, tx);
       __syncthreads();
-      tile_acc<DH>(reinterpret_cast<float(&)[8][DH / 16]>(o2), sP, sC2, ty, tx);
+      tile_acc<DH>(a2, sP, sC2, ty, tx);
       __syncthreads();
     }
     put_block(sP, dp, ty, tx);
     __syncthreads();
-    tile_acc<DH>(o1, sP, sC1, ty, tx);
+    tile_acc<DH>(a1, sP, sC1, ty, tx);
     if (!KV && it < nsink) {  // the sinks' gradients from these queries: P and dS once more, as [query][key]
-      float og[8][DH / 16];
+      float og[kR][DH / 16];
+      uint64_t ag[kR / 2][DH / 16];
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kR; ++i) {
           const float(&b)[4] = kv ? s[i] : dp[i];
-          *reinterpret_cast<float4*>(sP + (ty * 8 + i) * kPitch + tx * 4) = make_float4(b[0], b[1], b[2], b[3]);
+          *reinterpret_cast<float4*>(sP + (ty * kR + i) * kPitch + tx * 4) = make_float4(b[0], b[1], b[2], b[3]);
 #pragma unroll
-          for (int n = 0; n < DH / 16; ++n) og[i][n] = 0.f;
+          for (int n = 0; n < DH / 16; ++n) ag[i / 2][n] = 0;
         }
         __syncthreads();
-        tile_acc<DH>(og, sP, kv ? sR2 : sR1, ty, tx);
+        tile_acc<DH>(ag, sP, kv ? sR2 : sR1, ty, tx);
+        rows_of(og, ag);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (ty * 8 + i < c1 - c0)
+        for (int i = 0; i < kR; ++i)
+          if (ty * kR + i < c1 - c0)
 #pragma unroll
             for (int n = 0; n < DH / 16; ++n)
-              A.part[part_at(A, blockIdx.x, blockIdx.y, kv, ty * 8 + i) + tx + 16 * n] = og[i][n];
+              A.part[part_at(A, blockIdx.x, blockIdx.y, kv, ty * kR + i) + tx + 16 * n] = og[i][n];
       }
     }
   }
+  float o1[kR][DH / 16], o2[kR][DH / 16];
+  rows_of(o1, a1);
+  rows_of(o2, a2);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int t = r0 + ty * 8 + i;
+  for (int i = 0; i < kR; ++i) {
+    const int t = r0 + ty * kR + i;
     if (t >= A.T) continue;
     const int H = KV ? A.Hkv : A.Hq;
     const int64_t at = ((int64_t)t * H + blockIdx.y) * A.Dh;
@@ -333,15 +359,15 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_f32(const __grid_constant__
 #pragma unroll
         for (int n = 0; n < DH / 16; ++n) {
           o1[i][n] += far[tx + 16 * n];
-          o2[KV ? i : 0][n] += far[A.sinks * A.Dh + tx + 16 * n];
+          o2[i][n] += far[A.sinks * A.Dh + tx + 16 * n];
         }
 #pragma unroll
     for (int n = 0; n < DH / 16; ++n) {
       g1[tx + 16 * n] = (o1[i][n] * A.scale);
-      if (KV) ((float*)A.gv + at)[tx + 16 * n] = (o2[KV ? i : 0][n]);
-      odd = fmaf(o1[i][n], 0.f, fmaf(o2[KV ? i : 0][n], 0.f, odd));
+      if (KV) ((float*)A.gv + at)[tx + 16 * n] = (o2[i][n]);
+      odd = fmaf(o1[i][n], 0.f, fmaf(o2[i][n], 0.f, odd));
     }
-    if (odd != 0.f) again[ty * 8 + i] = 1;
+    if (odd != 0.f) again[ty * kR + i] = 1;
   }
   __syncthreads();
   for (int r = threadIdx.x >> 5; r < kBT; r += kThreads / 32)
