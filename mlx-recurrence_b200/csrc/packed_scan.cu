@@ -675,8 +675,8 @@ static int packed_check(const char* what, int dtype, int64_t T, int64_t D, int64
   if (dtype != MR_F32 && dtype != MR_BF16 && dtype != MR_F16)
     return set_error(MR_E_DTYPE, "%s: unsupported dtype code %d (0=f32, 1=bf16, 2=f16)", what, dtype);
   if (T < 0 || D <= 0 || S < 0) return set_error(MR_E_SHAPE, "%s: T and S must not be negative, D positive", what);
-  if (T > (int64_t)INT32_MAX / 2 || S > (int64_t)INT32_MAX / 2)
-    return set_error(MR_E_SHAPE, "%s: T=%lld or S=%lld too large", what, (long long)T, (long long)S);
+  if (T > (int64_t)INT32_MAX / 2 || S > (int64_t)INT32_MAX / 2 || D > (int64_t)INT32_MAX / 2)
+    return set_error(MR_E_SHAPE, "%s: T=%lld, S=%lld or D=%lld too large", what, (long long)T, (long long)S, (long long)D);
   return MR_OK;
 }
 

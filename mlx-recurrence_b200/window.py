@@ -15,6 +15,7 @@ dtype (float32 inputs: float32). Kernels: ``csrc/window_*.cu``.
 from __future__ import annotations
 
 import math
+import operator
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -36,6 +37,7 @@ def _check(q, k, v, window, sinks, scale, dims, layout):
                          f"{tuple(k.shape)}, {tuple(v.shape)}")
     if Dh not in HEAD_DIMS:
         raise ValueError(f"Dh={Dh} must be one of {HEAD_DIMS}")
+    window, sinks = operator.index(window), operator.index(sinks)
     if window < 1:
         raise ValueError(f"window must be positive, got {window}")
     if not 0 <= sinks <= MAX_SINKS:
@@ -43,7 +45,7 @@ def _check(q, k, v, window, sinks, scale, dims, layout):
     scale = Dh ** -0.5 if scale is None else float(scale)
     if not (0.0 < scale < 3e38):
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    return scale
+    return window, sinks, scale
 
 
 def _rows(t, dt, packed_dims):
@@ -152,7 +154,7 @@ def window_attention(q, k, v, window, sinks=0, scale=None):
         its row, even if it holds infinities or NaN. Slices of a fused
         projection are read in place.
     """
-    scale = _check(q, k, v, window, sinks, scale, 4, "[B, L, H, Dh]")
+    window, sinks, scale = _check(q, k, v, window, sinks, scale, 4, "[B, L, H, Dh]")
     return _dispatch(q, k, v, None, window, sinks, scale)
 
 
@@ -160,7 +162,7 @@ def window_attention_packed(q, k, v, cu_seqlens, window, sinks=0, scale=None):
     """:func:`window_attention` over a packed batch: q [T, Hq, Dh], k, v
     [T, Hkv, Dh], and ``cu_seqlens`` as in :func:`rglru_scan_packed` (rows
     behind the last border come out as zeros, gradients too)."""
-    scale = _check(q, k, v, window, sinks, scale, 3, "[T, H, Dh]")
+    window, sinks, scale = _check(q, k, v, window, sinks, scale, 3, "[T, H, Dh]")
     return _dispatch(q, k, v, cu_seqlens, window, sinks, scale)
 
 
@@ -185,14 +187,14 @@ def window_attention_with_state(q, k, v, window, sinks=0, scale=None):
     dtype. Token t lies in slot t (t < sinks) or sinks + (t - sinks) % window;
     unused slots are zero. The caches are state, not differentiable."""
     y = window_attention(q, k, v, window, sinks, scale)
-    return (y, *_caches(k, v, None, window, sinks))
+    return (y, *_caches(k, v, None, operator.index(window), operator.index(sinks)))
 
 
 def window_attention_packed_with_state(q, k, v, cu_seqlens, window, sinks=0, scale=None):
     """:func:`window_attention_packed` that also returns every sequence's caches
     [S, sinks + window, Hkv, Dh] (see :func:`window_attention_with_state`)."""
     y = window_attention_packed(q, k, v, cu_seqlens, window, sinks, scale)
-    return (y, *_caches(k, v, cu_seqlens, window, sinks))
+    return (y, *_caches(k, v, cu_seqlens, operator.index(window), operator.index(sinks)))
 
 
 def window_attention_step(q, k, v, cache_k, cache_v, pos, sinks=0, scale=None):
@@ -214,7 +216,7 @@ def window_attention_step(q, k, v, cache_k, cache_v, pos, sinks=0, scale=None):
     """
     dims = "[B, H, Dh]"
     B, Hq, Dh = q.shape if q.dim() == 3 else (0, 0, 0)
-    scale = _check(q, k, v, 1, sinks, scale, 3, dims)
+    _, sinks, scale = _check(q, k, v, 1, sinks, scale, 3, dims)
     Hkv = k.shape[1]
     dev = _lib.require_cuda(q, k, v, cache_k, cache_v)
     dt = common_dtype(q, k, v)

@@ -228,3 +228,20 @@ def test_decode_continues_a_packed_prefill(mr, cuda_dev):
     want = an * state + xn
     y = mr.rglru_step(an, xn, state)
     assert torch.allclose(y, want, rtol=2 ** -22, atol=2 ** -22) and torch.equal(y, state)
+
+
+def test_offsets_past_32_bits(mr, cuda_dev):
+    """More than 2^31 elements. With gates of zero y = x, grad_x = grad_y and grad_a = grad_y h_{t-1}, exactly (but
+    for the rounding of grad_a)."""
+    T, D = 1 << 20, 2112
+    a = torch.zeros(T, D, dtype=torch.bfloat16, device=cuda_dev)
+    x = torch.arange(T, device=cuda_dev).remainder(251).to(torch.bfloat16)[:, None].expand(T, D).contiguous()
+    gy = torch.full((T, D), 2.0, device=cuda_dev)
+    cu = torch.tensor([0, T // 3, T], device=cuda_dev)
+    y = mr.rglru_scan_packed(a.requires_grad_(), x.requires_grad_(), cu)
+    ga, gx = torch.autograd.grad(y, (a, x), gy)
+    for rows in (slice(0, 3), slice(T // 3 - 2, T // 3 + 3), slice(T - 3, T)):
+        assert torch.equal(y[rows], x[rows].float()) and (gx[rows] == 2).all()
+    assert torch.equal(ga[T - 3:], (2 * x[T - 4:T - 1])) and torch.equal(ga[T // 3 + 1], 2 * x[T // 3])
+    assert (ga[T // 3] == 0).all() and (ga[0] == 0).all()
+    assert bool((gx == 2).all())

@@ -380,3 +380,47 @@ def test_hybrid_layer_trains_and_decodes(mr, cuda_dev):
         yt = mr.window_attention_step(ht.view(-1, H, Dh), k[rows], v[rows], ck, cv, pos, sinks=sinks)
         assert (yt.double() - W.y[rows]).abs().max() <= 1e-4 * W.y.abs().max()
         pos += 1
+
+
+def test_offsets_past_32_bits(mr, cuda_dev):
+    """More than 2^31 elements in q, k, v. A window of one token returns v, and passes grad_y to v alone."""
+    T, H, Dh = 1 << 20, 17, 128
+    r = dict(device=cuda_dev, dtype=torch.bfloat16)
+    v = torch.arange(T, device=cuda_dev).remainder(253).to(torch.bfloat16)[:, None, None].expand(T, H, Dh).contiguous()
+    q, k, gy = torch.ones(T, H, Dh, **r), torch.ones(T, H, Dh, **r), torch.full((T, H, Dh), 3.0, **r)
+    for t in (q, k, v):
+        t.requires_grad_()
+    y = mr.window_attention(q[None], k[None], v[None], 1)[0]
+    gq, gk, gv = torch.autograd.grad(y, (q, k, v), gy)
+    assert torch.equal(y, v) and bool((gv == 3).all())
+    # dS = p (gy.v - delta) with delta from the same v: a rounding of sums of 128 terms of up to 3 * 252
+    assert gq.abs().max() <= 128 * 756 * 256 * O.U32 and gk.abs().max() <= 128 * 756 * 256 * O.U32
+
+
+def test_step_offsets_past_32_bits(mr, cuda_dev):
+    B, Hkv, Dh, window, dt = 3, 8, 128, 1 << 20, torch.bfloat16
+    ck, cv = (torch.empty(B, window, Hkv, Dh, dtype=dt, device=cuda_dev) for _ in range(2))
+    assert ck[:2].numel() >= 1 << 31
+    g = torch.Generator(device=cuda_dev).manual_seed(18)
+    q, k, v = (torch.randn(B, Hkv, Dh, device=cuda_dev, generator=g).to(dt) for _ in range(3))
+    n = 100
+    ck[2, :n], cv[2, :n] = (torch.randn(n, Hkv, Dh, device=cuda_dev, generator=g).to(dt) for _ in range(2))
+    y = mr.window_attention_step(q, k, v, ck, cv, torch.tensor([-1, 0, n], device=cuda_dev))
+    assert (y[0] == 0).all() and torch.equal(y[1], v[1]) and torch.equal(ck[2, n], k[2]) and torch.equal(cv[2, n], v[2])
+    qq = torch.zeros(n + 1, Hkv, Dh, dtype=dt, device=cuda_dev)
+    qq[-1] = q[2]
+    W = O.Attention(qq, ck[2, :n + 1], cv[2, :n + 1], torch.tensor([0, n + 1]), n + 1, 0)
+    O.check("y", y[2], W.y[-1], W.tol_y[-1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_many_query_heads_per_key_head(mr, cuda_dev, dtype):
+    """40 query heads on one key head: the step takes them 16 at a time, the gradient sums them all."""
+    window, sinks, dt = 20, 1, DT[dtype]
+    ins = _inputs(cuda_dev, [70, 33], 40, 1, 32, dt, seed=19)
+    _check(mr, ins, window, sinks)
+    q, k, v, _, cu = ins
+    W = O.Attention(q, k, v, cu, window, sinks)
+    _, ck, cv = mr.window_attention_packed_with_state(q[:69], k[:69], v[:69], cu[:1].new_tensor([0, 69]), window, sinks=sinks)
+    y = mr.window_attention_step(q[69:70], k[69:70], v[69:70], ck, cv, cu.new_tensor([69]), sinks=sinks)
+    O.check("step", y, W.y[69:70], W.tol_y[69:70])

@@ -36,6 +36,9 @@ def test_window_attention_refuses_bad_arguments(mr):
         args = dict(q=q, k=k, v=k, window=4) | change
         with pytest.raises(ValueError, match=match):
             mr.window_attention(**args)
+    for bad in (dict(window=4.0), dict(sinks=1.5)):
+        with pytest.raises(TypeError):
+            mr.window_attention(**(dict(q=q, k=k, v=k, window=4) | bad))
     with pytest.raises(RuntimeError, match="CUDA"):
         mr.window_attention(q, k, k, 4)
     with pytest.raises(ValueError, match="must be"):
@@ -71,6 +74,10 @@ def test_c_abi_status_codes(mr):
     assert lib.mr_rglru_packed_fwd(p, p, p, 1, 7, 8, 4, n, p, n, n, n, 0, n) == m.MR_E_DTYPE
     assert lib.mr_rglru_packed_fwd(p, p, p, 1, 1, 8, 0, n, p, n, n, n, 0, n) == m.MR_E_SHAPE
     assert lib.mr_rglru_packed_fwd(p, p, p, 1, 1, 1 << 31, 4, n, p, n, n, n, 0, n) == m.MR_E_SHAPE
+    assert lib.mr_rglru_packed_fwd(p, p, p, 1, 1, 8, 1 << 31, n, p, n, n, n, 0, n) == m.MR_E_SHAPE
+    assert lib.mr_rglru_packed_fwd(p, p, p, 1, 1, 300, 4, n, p, n, n, n, 0, n) == m.MR_E_WORKSPACE
+    assert lib.mr_rglru_packed_fwd(n, p, p, 1, 1, 8, 4, n, p, n, n, n, 0, n) == m.MR_E_ALIGN
+    assert lib.mr_rglru_packed_workspace_bytes(128, 64) == 0 < lib.mr_rglru_packed_workspace_bytes(129, 64)
     assert lib.mr_rglru_packed_bwd(p, n, p, p, p, p, -1, 1, 8, 4, n, p, p, n, n, 0, n) == m.MR_E_SHAPE
 
     def fwd(q=p, ts=64, cu=p, S=1, L=0, dtype=1, T=8, Hq=2, Hkv=1, Dh=64, window=4, sinks=0, scale=0.1, y=p):
