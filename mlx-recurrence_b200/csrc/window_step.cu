@@ -31,17 +31,22 @@ __device__ __forceinline__ int slot_of(int64_t p, int slots, int sinks) {
   return p < sinks ? (int)p : sinks + (int)((p - sinks) % (slots - sinks));
 }
 
-constexpr int kStepWarps2 = 8;
+// ---- float32 -------------------------------------------------------------------
+// One CTA per (batch row, query head): a warp takes kAhead slots at a time (their
+// loads and dot products are independent), lanes over Dh, one online softmax per
+// warp, joined in the warps' order. Key heads that several query heads share are
+// read once each from L2.
+constexpr int kStepWarps2 = 16, kAhead = 8;
 
-template <typename T, int NV>  // NV = Dh / 32
-__global__ void __launch_bounds__(32 * kStepWarps2) window_step_kernel(const __grid_constant__ StepArgs A) {
+template <int NV>  // NV = Dh / 32
+__global__ void __launch_bounds__(32 * kStepWarps2) window_step_f32(const __grid_constant__ StepArgs A) {
   __shared__ float sm[kStepWarps2], sl[kStepWarps2], so[kStepWarps2][NV * 32];
   const int b = blockIdx.y, h = blockIdx.x, G = A.Hq / A.Hkv, hk = h / G;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  T* y = (T*)A.y + ((int64_t)b * A.Hq + h) * A.Dh;
+  float* y = (float*)A.y + ((int64_t)b * A.Hq + h) * A.Dh;
   const int64_t p = step_pos(A, b);
   if (p < 0) {
-    for (int d = threadIdx.x; d < A.Dh; d += blockDim.x) y[d] = from_f<T>(0.f);
+    for (int d = threadIdx.x; d < A.Dh; d += blockDim.x) y[d] = 0.f;
     return;
   }
   const int n = (int)(p < A.slots - 1 ? p + 1 : A.slots), cur = slot_of(p, A.slots, A.sinks);
@@ -50,31 +55,51 @@ __global__ void __launch_bounds__(32 * kStepWarps2) window_step_kernel(const __g
   float q[NV], o[NV], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    q[i] = to_f(((const T*)A.q)[((int64_t)b * A.Hq + h) * A.Dh + lane + 32 * i]) * (A.scale * 1.4426950408889634f);
+    q[i] = ((const float*)A.q)[((int64_t)b * A.Hq + h) * A.Dh + lane + 32 * i] * (A.scale * 1.4426950408889634f);
     o[i] = 0.f;
   }
-  for (int s = w; s < n; s += kStepWarps2) {
-    const T* kp = s == cur ? (const T*)A.k + in : (const T*)A.ck + at + s * step;
-    const T* vp = s == cur ? (const T*)A.v + in : (const T*)A.cv + at + s * step;
-    float dot = 0.f;
+  for (int s = w * kAhead; s < n; s += kStepWarps2 * kAhead) {
+    float dot[kAhead], v[kAhead][NV], mx = m;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) dot = fmaf(q[i], to_f(kp[lane + 32 * i]), dot);
+    for (int x = 0; x < kAhead; ++x) {  // (slots behind the last: that one again, with weight zero)
+      const int slot = min(s + x, n - 1);
+      const float* kp = slot == cur ? (const float*)A.k + in : (const float*)A.ck + at + slot * step;
+      const float* vp = slot == cur ? (const float*)A.v + in : (const float*)A.cv + at + slot * step;
+      dot[x] = 0.f;
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, x);
-    const float mx = fmaxf(m, dot), base = mx == -INFINITY ? 0.f : mx, keep = exp2f(m - base), e = exp2f(dot - base);
+      for (int i = 0; i < NV; ++i) {
+        dot[x] = fmaf(q[i], kp[lane + 32 * i], dot[x]);
+        v[x][i] = vp[lane + 32 * i];
+      }
+    }
+#pragma unroll
+    for (int e = 16; e > 0; e >>= 1)
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) dot[x] += __shfl_xor_sync(0xffffffffu, dot[x], e);
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) mx = fmaxf(mx, dot[x]);
+    const float base = mx == -INFINITY ? 0.f : mx, keep = exp2f(m - base);
     m = mx;
-    l = l * keep + e;
+    l *= keep;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) o[i] = o[i] * keep + e * to_f(vp[lane + 32 * i]);
+    for (int i = 0; i < NV; ++i) o[i] *= keep;
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x)
+      if (s + x < n) {
+        const float e = exp2f(dot[x] - base);
+        l += e;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) o[i] = fmaf(e, v[x][i], o[i]);
+      }
   }
   if (lane == 0) sm[w] = m, sl[w] = l;
 #pragma unroll
   for (int i = 0; i < NV; ++i) so[w][lane + 32 * i] = o[i];
   __syncthreads();
-  if (h % G == 0)
+  if (h % G == 0)  // after every warp has read the caches (no CTA reads the slot itself)
     for (int d = threadIdx.x; d < A.Dh; d += blockDim.x) {
-      ((T*)A.ck)[at + cur * step + d] = ((const T*)A.k)[in + d];
-      ((T*)A.cv)[at + cur * step + d] = ((const T*)A.v)[in + d];
+      ((float*)A.ck)[at + cur * step + d] = ((const float*)A.k)[in + d];
+      ((float*)A.cv)[at + cur * step + d] = ((const float*)A.v)[in + d];
     }
   for (int d = threadIdx.x; d < A.Dh; d += blockDim.x) {
     float mx = -INFINITY, ls = 0.f, os = 0.f;
@@ -85,7 +110,7 @@ __global__ void __launch_bounds__(32 * kStepWarps2) window_step_kernel(const __g
       ls += sl[i] * e;
       os += so[i][d] * e;
     }
-    y[d] = from_f<T>(os / ls);
+    y[d] = os / ls;
   }
 }
 
@@ -367,15 +392,15 @@ __global__ void __launch_bounds__(256) window_cache_kernel(const V* __restrict__
   }
 }
 
-template <typename T> int window_step_launch(const StepArgs& A, cudaStream_t st) {
+static int step_f32(const StepArgs& A, cudaStream_t st) {
   const dim3 g(A.Hq, A.B);
   switch (A.Dh) {
-    case 32: window_step_kernel<T, 1><<<g, 32 * kStepWarps2, 0, st>>>(A); break;
-    case 64: window_step_kernel<T, 2><<<g, 32 * kStepWarps2, 0, st>>>(A); break;
-    case 96: window_step_kernel<T, 3><<<g, 32 * kStepWarps2, 0, st>>>(A); break;
-    default: window_step_kernel<T, 4><<<g, 32 * kStepWarps2, 0, st>>>(A); break;
+    case 32: window_step_f32<1><<<g, 32 * kStepWarps2, 0, st>>>(A); break;
+    case 64: window_step_f32<2><<<g, 32 * kStepWarps2, 0, st>>>(A); break;
+    case 96: window_step_f32<3><<<g, 32 * kStepWarps2, 0, st>>>(A); break;
+    default: window_step_f32<4><<<g, 32 * kStepWarps2, 0, st>>>(A); break;
   }
-  return check_launch("window_step_kernel");
+  return check_launch("window_step_f32");
 }
 
 }  // namespace mr
@@ -407,7 +432,7 @@ int mr_window_step(const void* q, const void* k, const void* v, void* cache_k, v
   const StepArgs A{q, k, v, cache_k, cache_v, pos, pos_is_int64, (int)batch, (int)Hq, (int)Hkv, (int)Dh, (int)slots,
                    (int)sinks, scale, y};
   switch (dtype) {
-    case MR_F32: return window_step_launch<float>(A, (cudaStream_t)stream);
+    case MR_F32: return step_f32(A, (cudaStream_t)stream);
     case MR_BF16: return step_mma<__nv_bfloat16>(A, (cudaStream_t)stream);
     default: return step_mma<__half>(A, (cudaStream_t)stream);
   }
