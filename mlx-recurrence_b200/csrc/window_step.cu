@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(32 * kStepWarps2) window_step_f32(const __grid
 // with its own online softmax. Warps, then CTAs (over distributed shared memory)
 // join their maxima, sums and outputs in a fixed order; one launch, no workspace.
 
-constexpr int kTile = 64, kRing = 3;
+constexpr int kTile = 64, kRing = 2;
 
 template <typename T> struct Mma;
 template <> struct Mma<__nv_bfloat16> {
@@ -335,9 +335,10 @@ __global__ void __launch_bounds__(128) window_step_mma(const __grid_constant__ S
 template <typename T, int DH> static int step_mma_dh(const StepArgs& A, cudaStream_t st) {
   const int G = A.Hq / A.Hkv, head_tiles = (G + 15) / 16, tiles = (A.slots + kTile - 1) / kTile;
   const int64_t units = (int64_t)A.B * A.Hkv * head_tiles;
-  // CTAs for four on every SM, each with two tiles at least
+  // CTAs for two on every SM (three fit: one wave), each with two tiles at least. At B=96, Hkv=4, Dh=128, 2052 slots:
+  // 66 us unsplit, 76 in two, 85 in four (later waves leave SMs idle); at B=8: 12 us in eight
   int splits = 1;
-  while (splits < 8 && units * splits < 148 * 4 && splits * 4 <= tiles) splits *= 2;
+  while (splits < 8 && units * splits < 148 * 2 && splits * 4 <= tiles) splits *= 2;
   auto kernel = window_step_mma<T, DH>;
   constexpr int smem = kStepSmem<T, DH>;
   if (int rc = allow_smem<window_step_mma<T, DH>>(smem, "window_step_mma")) return rc;
