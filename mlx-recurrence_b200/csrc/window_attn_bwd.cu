@@ -21,6 +21,16 @@
 // under the dS arithmetic, the next S follows as soon as P (KV = false: S) has
 // been read, the next dP after dS C1.
 //
+// P and dS are rounded to the inputs' type, which the products take (fp16: dS at a
+// power-of-two scale of max |gy|, so that neither large nor small loss scales leave
+// its range); lse, delta and the sums are float32.
+//
+// bf16, 16384 tokens, 32 heads of 64, window 1024: 851 us (379 TFLOP/s of the 5
+// products); 16 heads of 128 on 4, window 2048, 4 sinks: 762 us (486). Measured and
+// not kept: both products of S and dP before any sum of the old tile (918 and 826
+// us), three warpgroups in one CTA for Dh <= 64 (1,034 us), two threads per row (827
+// and 790 us).
+//
 // The sinks' far queries (window_attn.cuh): a query tile that meets a sink tile adds
 // the sinks' gradients by products over its 128 queries, with P and dS handed
 // through shared memory.

@@ -4,11 +4,21 @@
 // A CTA takes 128 queries of one head and walks the keys they may see in tiles
 // of 128: S = Q K^T into TMEM, the online softmax by four warps (one thread per
 // query, so no reduction across threads), P back into TMEM as the A operand of
-// O += P V. The row's maximum is only moved when it grows by more
-// than 2^8 (the factor cancels in O / l), so O is rarely rescaled. Where TMEM has
-// room for P beside S (Dh <= 64) the next S runs under this tile's exponentials.
-// Two CTAs per SM (256 TMEM columns and at most 96 KB of shared memory each) fill
-// each other's gaps.
+// O += P V. The row's maximum is only moved when it grows by more than 2^8 (the
+// factor cancels in O / l), so O is rarely rescaled. P is rounded to the inputs'
+// type, which the product takes; l sums it unrounded. Where TMEM has room for P
+// beside S (Dh <= 64) the next S runs under this tile's exponentials. Two CTAs per
+// SM (256 TMEM columns and at most 96 KB of shared memory each) fill each other's
+// gaps; the issuing warpgroup gives its registers to the softmax's, which holds a
+// row of S.
+//
+// bf16, 16384 tokens, 32 heads of 64, window 1024: 297 us (433 TFLOP/s); 16 heads of
+// 128 on 4, window 2048, 4 sinks: 265 us (559). Bound by the chain of a tile (load S,
+// maximum, exponentials: about 3,000 cycles on two warps per scheduler), not by one
+// pipe: a tile's exponentials alone would take 1,024 cycles, its products 500 or
+// 1,000. Measured and not kept: two threads per query (304 us), a quarter of the
+// exponentials by a polynomial on the FMA pipe (299 us), the issuing done by a
+// softmax warp (352 us).
 #include "window_tc.cuh"
 
 namespace mr {
@@ -27,7 +37,7 @@ template <typename T, int NB>  // NB = 64-wide blocks of a row
 __global__ void __launch_bounds__(kFwdThreads, 2)
 attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap tq,
                 const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
-  // TMEM columns: S at 0; P over it (its first half, as S is used up) or, where O leaves room, in columns of its own
+  // TMEM columns: S at 0; P over its first half or, where O leaves room, in columns of its own
   constexpr bool kOwnP = NB == 1;
   constexpr uint32_t kP = kOwnP ? 128 : 0, kO = kOwnP ? 192 : 128;
   extern __shared__ unsigned char raw[];
@@ -67,77 +77,77 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
   if (w >= 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (w == 4) {
-  // Descriptors are made once and stepped by additions.
-  const bool lead = umma::elect_one();
-  const uint64_t dq = umma::sdesc_k(smem_u32(sQ)), dk = umma::sdesc_k(smem_u32(sK)), dv = umma::sdesc_mn(smem_u32(sV), kTileBytes);
-  const int ks = A.Dh / 16;
-  const uint32_t ido = umma::idesc_f16(128, A.Dh, Fmt<T>::id, 0, 1);
-  auto load = [&](const CUtensorMap* m, unsigned char* dst, int head, int r, uint64_t* bar) {
+      // Descriptors are made once and stepped by additions.
+      const bool lead = umma::elect_one();
+      const uint64_t dq = umma::sdesc_k(smem_u32(sQ)), dk = umma::sdesc_k(smem_u32(sK)), dv = umma::sdesc_mn(smem_u32(sV), kTileBytes);
+      const int ks = A.Dh / 16;
+      const uint32_t ido = umma::idesc_f16(128, A.Dh, Fmt<T>::id, 0, 1);
+      auto load = [&](const CUtensorMap* m, unsigned char* dst, int head, int r, uint64_t* bar) {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) tma_load_3d(dst + b * kTileBytes, m, b * 64, head, r, bar);
-  };
-  auto key0 = [&](int t) { return t < nsink ? R.s0 : R.kmin + (t - nsink) * 128; };
-  auto cols = [&](int t) { return t < nsink ? sink_n : 128; };
-  auto load_k = [&](int t) {
-    if (lead) {
-      mbar_arrive_expect_tx(&sh.k_full, NB * kTileBytes);
-      load(&tk, sK, hk, key0(t), &sh.k_full);
-    }
-  };
-  auto load_v = [&](int t) {
-    if (lead) {
-      mbar_arrive_expect_tx(&sh.v_full, NB * kTileBytes);
-      load(&tv, sV, hk, key0(t), &sh.v_full);
-    }
-  };
-  auto issue_s = [&](int t) {
-    mbar_wait(&sh.k_full, t & 1);
-    umma::fence_after_sync();
-    const uint32_t ids = umma::idesc_f16(128, cols(t), Fmt<T>::id, 0, 0);
+        for (int b = 0; b < NB; ++b) tma_load_3d(dst + b * kTileBytes, m, b * 64, head, r, bar);
+      };
+      auto key0 = [&](int t) { return t < nsink ? R.s0 : R.kmin + (t - nsink) * 128; };
+      auto cols = [&](int t) { return t < nsink ? sink_n : 128; };
+      auto load_k = [&](int t) {
+        if (lead) {
+          mbar_arrive_expect_tx(&sh.k_full, NB * kTileBytes);
+          load(&tk, sK, hk, key0(t), &sh.k_full);
+        }
+      };
+      auto load_v = [&](int t) {
+        if (lead) {
+          mbar_arrive_expect_tx(&sh.v_full, NB * kTileBytes);
+          load(&tv, sV, hk, key0(t), &sh.v_full);
+        }
+      };
+      auto issue_s = [&](int t) {
+        mbar_wait(&sh.k_full, t & 1);
+        umma::fence_after_sync();
+        const uint32_t ids = umma::idesc_f16(128, cols(t), Fmt<T>::id, 0, 0);
 #pragma unroll
-    for (int k = 0; k < NB * 4; ++k) {
-      const int o = (k >> 2) * (kTileBytes / 16) + (k & 3) * 2;
-      if (k < ks && lead) umma::mma_f16(tm, dq + o, dk + o, ids, k > 0);
-    }
-    if (lead) umma::commit(&sh.s_done);
-  };
-  auto issue_o = [&](int t) {
-    mbar_wait(&sh.v_full, t & 1);
-    umma::fence_after_sync();
-    const int kp = cols(t) / 16;
+        for (int k = 0; k < NB * 4; ++k) {
+          const int o = (k >> 2) * (kTileBytes / 16) + (k & 3) * 2;
+          if (k < ks && lead) umma::mma_f16(tm, dq + o, dk + o, ids, k > 0);
+        }
+        if (lead) umma::commit(&sh.s_done);
+      };
+      auto issue_o = [&](int t) {
+        mbar_wait(&sh.v_full, t & 1);
+        umma::fence_after_sync();
+        const int kp = cols(t) / 16;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < kp && lead) umma::mma_f16_ta(tm + kO, tm + kP + k * 8, dv + k * 128, ido, t > 0 || k > 0);
-    if (lead) umma::commit(&sh.o_done);
-  };
-    if (lead) {
-      mbar_arrive_expect_tx(&sh.k_full, 2 * NB * kTileBytes);
-      load(&tq, sQ, h, q0, &sh.k_full);
-      load(&tk, sK, hk, key0(0), &sh.k_full);
-    }
-    load_v(0);
-    issue_s(0);
-    for (int t = 0; t < ntile; ++t) {
-      mbar_wait(&sh.s_done, t & 1);
-      if (t + 1 < ntile) load_k(t + 1);
-      if (kOwnP) {
-        if (t + 1 < ntile) {
-          mbar_wait(&sh.s_read, t & 1);
+        for (int k = 0; k < 8; ++k)
+          if (k < kp && lead) umma::mma_f16_ta(tm + kO, tm + kP + k * 8, dv + k * 128, ido, t > 0 || k > 0);
+        if (lead) umma::commit(&sh.o_done);
+      };
+      if (lead) {
+        mbar_arrive_expect_tx(&sh.k_full, 2 * NB * kTileBytes);
+        load(&tq, sQ, h, q0, &sh.k_full);
+        load(&tk, sK, hk, key0(0), &sh.k_full);
+      }
+      load_v(0);
+      issue_s(0);
+      for (int t = 0; t < ntile; ++t) {
+        mbar_wait(&sh.s_done, t & 1);
+        if (t + 1 < ntile) load_k(t + 1);
+        if (kOwnP) {
+          if (t + 1 < ntile) {
+            mbar_wait(&sh.s_read, t & 1);
+            issue_s(t + 1);
+          }
+          if (t > 0) {
+            mbar_wait(&sh.o_done, (t - 1) & 1);
+            load_v(t);
+          }
+        }
+        mbar_wait(&sh.p_ready, t & 1);
+        issue_o(t);
+        if (!kOwnP && t + 1 < ntile) {
+          mbar_wait(&sh.o_done, t & 1);  // P is read: the next S overwrites it
+          load_v(t + 1);
           issue_s(t + 1);
         }
-        if (t > 0) {
-          mbar_wait(&sh.o_done, (t - 1) & 1);
-          load_v(t);
-        }
       }
-      mbar_wait(&sh.p_ready, t & 1);
-      issue_o(t);
-      if (!kOwnP && t + 1 < ntile) {
-        mbar_wait(&sh.o_done, t & 1);  // P is read: the next S overwrites it
-        load_v(t + 1);
-        issue_s(t + 1);
-      }
-    }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
