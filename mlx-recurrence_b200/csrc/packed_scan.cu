@@ -9,27 +9,27 @@
 //
 // One pass over the data, HBM-bound. An item is kChunk steps of 32 V channels
 // (rows of 128 bytes of the inputs); 8 warps x kSteps steps each work on it out
-// of shared memory, where a ninth warp's TMA copies bring it; the other CTAs of
-// the SM (four forward, three backward) cover the copies and the waits. A step is
-// the affine map h -> a h + x, so runs of steps compose to one map (A, B): per
-// thread, per warp prefix and per item. An item publishes its map, looks back over
-// the items before it in time (kBack at a time) until it meets one whose state is
-// known, and publishes its own state. A sequence border cuts the chain: what
-// follows it does not depend on the past. Borders are the same for all channels,
-// so every branch on them is uniform. The backward runs the same scheme from the
-// right, and rebuilds h from the states that the forward kept per chunk.
+// of shared memory, where TMA copies bring it; the other CTAs of the SM (five
+// forward, three backward) cover the copies and the waits. A step is the affine
+// map h -> a h + x, so runs of steps compose to one map (A, B): per thread, per
+// warp prefix and per item. An item publishes its map, looks back over the items
+// before it in time until it meets one whose state is known, and publishes its
+// own state. A sequence border cuts the chain: what follows it does not depend on
+// the past. Borders are the same for all channels, so every branch on them is
+// uniform. The backward runs the same scheme from the right, and rebuilds h from
+// the states that the forward kept per chunk.
 //
 // Composed maps need products of gates that stay in float32's range: |a| <= 1
 // always does, larger gates as long as their products along a sequence do.
 //
-// bf16, T=32768, D=2560, 24 sequences: forward 154 us (4.4 TB/s of the 8 bytes an
-// element needs), backward 253 us (4.0 TB/s of 12 bytes). What is left is the wait
+// bf16, T=32768, D=2560, 24 sequences: forward 137 us (4.9 TB/s of the 8 bytes an
+// element needs), backward 224 us (4.5 TB/s of 12 bytes). What is left is the wait
 // for the items before (clock stamps: a fold takes 900 cycles, the rest of the work
-// 1,500, the wait 2,000 to 30,000). So nothing delays an item that others wait for:
-// tickets are taken only with room for the data (taking them ahead: 182 and 304 us),
-// steps at borders run unrolled behind bit masks (a plain loop there: 227 us), and a
-// round of the look-back reads 2 items (4: the same; 7: 173 and 299 us, 209 us for
-// T=131072, D=512, where it reads records that are not there yet).
+// 1,500, the wait some 6,000), so nothing delays an item that others wait for.
+// Measured at that size, forward and backward: tickets taken a stage ahead of the
+// data 182 and 304 us; a plain loop for the steps at borders 227 us; rounds of 4 (8)
+// records of the look-back in place of 1: 160 and 268 us (199 and 343), since they
+// read maps that are not there yet where a state is about to come.
 #include "common.cuh"
 #include "launch.cuh"
 #include "tma.cuh"
@@ -40,7 +40,6 @@ namespace mr {
 constexpr int kWarps = 8;
 constexpr int kSteps = 16;               // steps of a thread
 constexpr int kChunk = kWarps * kSteps;  // steps of an item
-constexpr int kBack = 2;                 // items that one round of the look-back reads
 
 // A chunk's map or state for one channel, written and read as one 16-byte access
 // (single-copy atomic), so no flag or fence stands beside it.
@@ -140,8 +139,8 @@ struct PackedArgs {
   bool vec;  // rows of V elements may be accessed whole
 };
 
-// CTAs per SM: by registers (forward), by shared memory (backward)
-template <bool BWD> constexpr int kCtas = BWD ? 3 : 4;
+// CTAs per SM, by shared memory
+template <bool BWD> constexpr int kCtas = BWD ? 3 : 5;
 
 template <typename T> constexpr int kV = 4 / sizeof(T);  // channels of a thread: 4 bytes of an input row
 template <typename T, bool BWD> constexpr int kStage = kChunk * 32 * kV<T> * (2 * (int)sizeof(T) + (BWD ? 4 : 0));
@@ -169,33 +168,28 @@ template <typename T, int V> __device__ __forceinline__ void put(T* p, const flo
 template <int V> struct Work {
   float A[kWarps][32 * V], B[kWarps][32 * V];    // the warps' maps along the chain
   float fA[kWarps][32 * V], fB[kWarps][32 * V];  // backward: the warps' maps of the forward recurrence
-  float2 back[kBack][32 * V];                    // what the look-back read: A (or kKnown) and B
   float carry[32 * V];                           // the state entering the item
   int mark[kChunk];                              // per token at a border: its sequence, and which end of it
-  uint64_t full, empty;
+  uint64_t full;
   ChunkInfo info;
   int item;
-  int open;
 };
 constexpr int kStart = 1 << 30, kEnd = INT32_MIN, kSeq = kStart - 1;  // of Work::mark; 0 in both bits: no border
-
-// stands for A in a record that holds a state (a product of gates is never this NaN: products give 0x7fffffff)
-__device__ __forceinline__ float known_mark() { return __uint_as_float(0xffffffffu); }
-
-__device__ __forceinline__ void sync_workers() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // The items of a CTA, in the order of the tickets. Tickets follow the order in
 // which CTAs ask, so whatever an item waits for has been taken by a running CTA,
 // which works through its items in order: the smallest one never waits.
 //
-// TMA form: warp kWarps takes a ticket and brings its data as soon as the last
-// item has been read. Plain form (rows that are no multiple of 16 bytes): every thread brings its own
-// elements when the item begins.
+// TMA form: thread 0 takes a ticket and issues the copies once the last item has
+// been read (not before: an item taken early and left waiting holds up those
+// behind it). Plain form (rows that are no multiple of 16 bytes): every thread brings its own
+// elements.
 template <typename T, bool BWD, bool TMA> struct Feed {
   static constexpr int V = kV<T>, CH = 32 * V;
   unsigned char* stage;
   Work<V>& sh;
   const PackedArgs& P;
+  const CUtensorMap *ta, *tx, *tg;
   int n = 0;  // items so far
 
   __device__ T* a() const { return reinterpret_cast<T*>(stage); }
@@ -203,33 +197,27 @@ template <typename T, bool BWD, bool TMA> struct Feed {
   __device__ float* g() const { return reinterpret_cast<float*>(x() + kChunk * CH); }
   __device__ int64_t chunk_of(int item) const { return BWD ? P.nchunk - 1 - item / P.ntile : item / P.ntile; }
 
-  __device__ void produce(const CUtensorMap* ta, const CUtensorMap* tx, const CUtensorMap* tg) {
-    const int total = P.nchunk * P.ntile;
-    for (int i = 0;; ++i) {
-      // (only with room for it: an item taken early and left waiting holds up those behind it)
-      if (i > 0) mbar_wait(&sh.empty, (i - 1) & 1);
-      const int item = P.counter ? (int)min(atomicAdd(P.counter, 1u), (uint32_t)INT32_MAX)
-                                 : (i == 0 ? (int)blockIdx.x : INT32_MAX);
-      if (item >= total) {
-        sh.item = -1;
-        mbar_arrive(&sh.full);
-        return;
-      }
-      const int64_t t0 = chunk_of(item) * kChunk;
-      const int c0 = item % P.ntile * CH;
-      sh.item = item;
-      sh.info = P.info ? P.info[chunk_of(item)] : chunk_info(P.cu, P.S, t0, (int)min((int64_t)kChunk, P.L - t0));
-      mbar_arrive_expect_tx(&sh.full, kStage<T, BWD>);
-      tma_load_2d(a(), ta, c0, (int)t0, &sh.full);
-      tma_load_2d(x(), tx, c0, (int)t0, &sh.full);
-      if (BWD) tma_load_2d(g(), tg, c0, (int)t0, &sh.full);
-    }
-  }
-
   // The next item, once its data is there, or -1.
   __device__ int next() {
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if constexpr (TMA) {
+      if (threadIdx.x == 0) {
+        const int next = P.counter ? (int)min(atomicAdd(P.counter, 1u), (uint32_t)INT32_MAX)
+                                   : (n == 0 ? (int)blockIdx.x : INT32_MAX);
+        const bool more = next < P.nchunk * P.ntile;
+        sh.item = more ? next : -1;
+        if (more) {
+          const int64_t chunk = chunk_of(next), t0 = chunk * kChunk;
+          const int c0 = next % P.ntile * CH;
+          sh.info = P.info ? P.info[chunk] : chunk_info(P.cu, P.S, t0, (int)min((int64_t)kChunk, P.L - t0));
+          mbar_arrive_expect_tx(&sh.full, kStage<T, BWD>);
+          tma_load_2d(a(), ta, c0, (int)t0, &sh.full);
+          tma_load_2d(x(), tx, c0, (int)t0, &sh.full);
+          if (BWD) tma_load_2d(g(), tg, c0, (int)t0, &sh.full);
+        } else {
+          mbar_arrive(&sh.full);
+        }
+      }
       mbar_wait(&sh.full, n++ & 1);
       return sh.item;
     } else {
@@ -237,10 +225,10 @@ template <typename T, bool BWD, bool TMA> struct Feed {
         if (n++ > 0) return -1;
         sh.item = blockIdx.x;
       } else {
-        sync_workers();  // everybody has read the last item's number
+        __syncthreads();  // everybody has read the last item's number
         if (threadIdx.x == 0) sh.item = (int)min(atomicAdd(P.counter, 1u), (uint32_t)INT32_MAX);
       }
-      sync_workers();
+      __syncthreads();
       const int item = sh.item;
       if (item >= P.nchunk * P.ntile) return -1;
       const int64_t t0 = chunk_of(item) * kChunk, ch = (int64_t)(item % P.ntile) * CH + lane * V;
@@ -273,27 +261,20 @@ template <typename T, bool BWD, bool TMA> struct Feed {
       return item;
     }
   }
-  // The stage may be filled again.
-  __device__ void release() {
-    if constexpr (TMA) {
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.empty);
-    }
-  }
 };
 
-// Marks of a chunk that holds borders; all workers call it. A token belongs to
+// Marks of a chunk that holds borders; all threads call it. A token belongs to
 // one sequence, so one entry serves its start and its end.
 template <int V> __device__ __forceinline__ void mark_borders(Work<V>& sh, const ChunkInfo& c, const PackedArgs& P, int64_t t0, int n) {
   if (threadIdx.x < kChunk) sh.mark[threadIdx.x] = 0;
-  sync_workers();
+  __syncthreads();
   for (int s = c.first + threadIdx.x; s <= P.S; s += kWarps * 32) {
     const int64_t at = P.cu[s] - t0;
     if (at > n) break;
     if (at >= 0 && at < n && s < P.S && P.cu[s + 1] > P.cu[s]) atomicOr(&sh.mark[at], s | kStart);
     if (at >= 1 && s > 0 && P.cu[s] > P.cu[s - 1]) atomicOr(&sh.mark[at - 1], (s - 1) | kEnd);
   }
-  sync_workers();
+  __syncthreads();
 }
 
 // A warp's steps as bit masks: in a sequence, at a start, at an end; the same in every lane, so the unrolled loops branch
@@ -329,15 +310,6 @@ __device__ __forceinline__ void chain(Work<V>& sh, const PackedArgs& P, int64_t 
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = lane * V;
   const bool wait = need && rank > 0, tell = P.counter != nullptr && rank < P.nchunk - 1;
   Rec* recs = P.recs + ch;
-  // warps 1 .. kBack fetch the records of the items before this one while warp 0 publishes
-  auto fetch = [&](int at) {
-    const int mine = at - (w - 1);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const Rec r = mine >= 0 && v < live ? rec_wait(recs + mine * P.D + v) : Rec{0.f, 0.f, kState, 0};
-      sh.back[w - 1][c + v] = make_float2(r.tag == kState ? known_mark() : r.A, r.B);
-    }
-  };
   auto through = [&](int i) {  // p, q <- the warps' maps up to and including warp i
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -350,8 +322,9 @@ __device__ __forceinline__ void chain(Work<V>& sh, const PackedArgs& P, int64_t 
   for (int v = 0; v < V; ++v) p[v] = 1.f, q[v] = 0.f;
   if (w == 0) {
     float tp[V], tq[V];
+#pragma unroll
     for (int i = 0; i < kWarps; ++i) {
-      if ((BWD ? kWarps - 1 - i : i) == 0 && BWD) {
+      if (BWD && i == kWarps - 1) {
 #pragma unroll
         for (int v = 0; v < V; ++v) tp[v] = p[v], tq[v] = q[v];  // what enters warp 0, the last on the chain
       }
@@ -365,50 +338,39 @@ __device__ __forceinline__ void chain(Work<V>& sh, const PackedArgs& P, int64_t 
       float a[V], b[V];  // the composed map of the items looked at so far
       bool known[V];     // a record may turn from map to state between two reads: each channel stops by itself
 #pragma unroll
-      for (int v = 0; v < V; ++v) a[v] = 1.f, b[v] = 0.f, known[v] = false;
-      for (bool open = true; open;) {
-        sync_workers();
+      for (int v = 0; v < V; ++v) a[v] = 1.f, b[v] = 0.f, known[v] = v >= live;
+      bool open = true;
+      for (int at = rank - 1; open; --at) {
+        Rec r[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) r[v] = at >= 0 && !known[v] ? rec_load(recs + at * P.D + v) : Rec{0.f, 0.f, kState, 0};
         open = false;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-#pragma unroll
-          for (int i = 0; i < kBack; ++i) {
-            const float2 r = sh.back[i][c + v];
-            if (!known[v]) {
-              b[v] = fmaf(a[v], r.y, b[v]);
-              known[v] = __float_as_uint(r.x) == 0xffffffffu;
-              a[v] *= r.x;
-            }
+          if (!known[v]) {
+            if (r[v].tag == 0) r[v] = rec_wait(recs + at * P.D + v);
+            b[v] = fmaf(a[v], r[v].B, b[v]);
+            a[v] *= r[v].A;
+            known[v] = r[v].tag == kState;
           }
           open |= !known[v];
-          sh.carry[c + v] = b[v];
         }
-        open = __any_sync(0xffffffffu, open);
-        if (lane == 0) sh.open = open;
-        if (!open && tell && !cut)
+      }
 #pragma unroll
-          for (int v = 0; v < V; ++v)
-            if (v < live) rec_store(recs + rank * P.D + v, 0.f, fmaf(p[v], b[v], q[v]), kState);
-        sync_workers();
+      for (int v = 0; v < V; ++v) {
+        sh.carry[c + v] = b[v];
+        if (tell && !cut && v < live) rec_store(recs + rank * P.D + v, 0.f, fmaf(p[v], b[v], q[v]), kState);
       }
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) p[v] = BWD ? tp[v] : 1.f, q[v] = BWD ? tq[v] : 0.f;
   } else {
-    if (wait && w <= kBack) fetch(rank - 1);
     if (BWD)
       for (int i = kWarps - 1; i > w; --i) through(i);
     else
       for (int i = 0; i < w; ++i) through(i);
-    if (wait)
-      for (int at = rank - 1;;) {
-        sync_workers();
-        sync_workers();
-        if (!sh.open) break;
-        at -= kBack;
-        if (w <= kBack) fetch(at);
-      }
   }
+  if (wait) __syncthreads();
 #pragma unroll
   for (int v = 0; v < V; ++v) carry[v] = wait ? sh.carry[c + v] : 0.f;
 }
@@ -417,24 +379,20 @@ __device__ __forceinline__ void chain(Work<V>& sh, const PackedArgs& P, int64_t 
 __device__ __forceinline__ float enter(float p, float q, float carry, bool cut) { return cut ? q : fmaf(p, carry, q); }
 
 template <typename T, bool TMA>
-__global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kCtas<false>)
+__global__ void __launch_bounds__(kWarps * 32, kCtas<false>)
 packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ CUtensorMap ta,
                   const __grid_constant__ CUtensorMap tx) {
   constexpr int V = kV<T>, CH = 32 * V;
   extern __shared__ __align__(128) unsigned char dyn[];
   __shared__ Work<V> sh;
-  Feed<T, false, TMA> feed{dyn, sh, P};
+  Feed<T, false, TMA> feed{dyn, sh, P, &ta, &tx, nullptr};
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, k0 = w * kSteps;
   if constexpr (TMA) {
     if (threadIdx.x == 0) {
-      mbar_init(&sh.full, 1), mbar_init(&sh.empty, kWarps);
+      mbar_init(&sh.full, 1);
       fence_mbar_init();
     }
     __syncthreads();
-    if (w == kWarps) {
-      if (lane == 0) feed.produce(&ta, &tx, nullptr);
-      return;
-    }
   }
   for (int item; (item = feed.next()) >= 0;) {
     const int chunk = item / P.ntile;
@@ -467,7 +425,7 @@ packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) sh.A[w][lane * V + v] = A[v], sh.B[w][lane * V + v] = B[v];
-    sync_workers();
+    __syncthreads();
     const bool need = info.lo == 0 && info.hi > 0 && !(info.starts && (sh.mark[0] & kStart));
     float carry[V], p[V], q[V], h[V];
     chain<V, false>(sh, P, ch, live, chunk, info.starts, need, carry, p, q);
@@ -507,34 +465,29 @@ packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
         put<float, V>(y, out, P.vec, live);
       }
     }
-    feed.release();
     if (P.fin != nullptr)  // empty sequences, spread over the chunks
       for (int s = (int)((int64_t)chunk * P.S / P.nchunk) + w; s < (int)((int64_t)(chunk + 1) * P.S / P.nchunk); s += kWarps)
         if (P.cu[s + 1] <= P.cu[s])
           for (int v = 0; v < live; ++v) P.fin[s * P.D + ch + v] = P.h0 ? P.h0[s * P.D + ch + v] : 0.f;
-    sync_workers();  // sh is free for the next item
+    __syncthreads();  // sh is free for the next item
   }
 }
 
 template <typename T, bool TMA>
-__global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kCtas<true>)
+__global__ void __launch_bounds__(kWarps * 32, kCtas<true>)
 packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ CUtensorMap ta,
                   const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tg) {
   constexpr int V = kV<T>, CH = 32 * V;
   extern __shared__ __align__(128) unsigned char dyn[];
   __shared__ Work<V> sh;
-  Feed<T, true, TMA> feed{dyn, sh, P};
+  Feed<T, true, TMA> feed{dyn, sh, P, &ta, &tx, &tg};
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, k0 = w * kSteps;
   if constexpr (TMA) {
     if (threadIdx.x == 0) {
-      mbar_init(&sh.full, 1), mbar_init(&sh.empty, kWarps);
+      mbar_init(&sh.full, 1);
       fence_mbar_init();
     }
     __syncthreads();
-    if (w == kWarps) {
-      if (lane == 0) feed.produce(&ta, &tx, &tg);
-      return;
-    }
   }
   for (int item; (item = feed.next()) >= 0;) {
     const int rank = item / P.ntile, chunk = P.nchunk - 1 - rank;
@@ -592,7 +545,7 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
         sh.A[w][lane * V + v] = C[v], sh.B[w][lane * V + v] = Q[v];
       }
     }
-    sync_workers();
+    __syncthreads();
     const bool need = info.hi == n && info.hi > info.lo && !(info.ends && (sh.mark[n - 1] & kEnd));
     float carry[V], p[V], q[V], r[V];
     chain<V, true>(sh, P, ch, live, rank, info.ends, need, carry, p, q);
@@ -668,12 +621,11 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
       }
     }
     if constexpr (TMA) fence_proxy_async_smem();  // this thread's writes over gy before the next copy into it
-    feed.release();
     if (P.gh0 != nullptr)
       for (int s = (int)((int64_t)chunk * P.S / P.nchunk) + w; s < (int)((int64_t)(chunk + 1) * P.S / P.nchunk); s += kWarps)
         if (P.cu[s + 1] <= P.cu[s])
           for (int v = 0; v < live; ++v) P.gh0[s * P.D + ch + v] = P.gf ? P.gf[s * P.D + ch + v] : 0.f;
-    sync_workers();
+    __syncthreads();
   }
 }
 
@@ -735,10 +687,10 @@ template <typename T, bool BWD> static int launch(const char* what, PackedArgs P
     return check_launch(what);                                     \
   } while (0)
   if constexpr (BWD) {
-    if (tma) MR_GO((packed_bwd_kernel<T, true>), kWarps * 32 + 32, ta, tx, tg);
+    if (tma) MR_GO((packed_bwd_kernel<T, true>), kWarps * 32, ta, tx, tg);
     MR_GO((packed_bwd_kernel<T, false>), kWarps * 32, ta, tx, tg);
   } else {
-    if (tma) MR_GO((packed_fwd_kernel<T, true>), kWarps * 32 + 32, ta, tx);
+    if (tma) MR_GO((packed_fwd_kernel<T, true>), kWarps * 32, ta, tx);
     MR_GO((packed_fwd_kernel<T, false>), kWarps * 32, ta, tx);
   }
 #undef MR_GO
