@@ -1,4 +1,5 @@
-// Dynamic shared memory beyond 48 KB, asked for once per kernel and device.
+// Launch preliminaries: dynamic shared memory beyond 48 KB, asked for once per
+// kernel and device, and the register count of kernels that redistribute theirs.
 #pragma once
 
 #include <atomic>
@@ -20,6 +21,25 @@ template <auto Kernel> int allow_smem(int bytes, const char* what) {
     cudaGetLastError();
     return set_error(MR_E_LAUNCH, "%s: shared memory: %s", what, cudaGetErrorString(e));
   }
+  return MR_OK;
+}
+
+// A kernel whose warpgroups pass registers on (setmaxnreg) needs the launch's own
+// count to be `regs` a thread: with fewer, the increase would wait for ever.
+template <auto Kernel> int expect_regs(int regs, const char* what) {
+  static std::atomic<int> seen{0};
+  int n = seen.load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaFuncAttributes a;
+    const cudaError_t e = cudaFuncGetAttributes(&a, Kernel);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return set_error(MR_E_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
+    }
+    n = a.numRegs;
+    seen.store(n, std::memory_order_relaxed);
+  }
+  if (n != regs) return set_error(MR_E_LAUNCH, "%s: built with %d registers a thread, not %d", what, n, regs);
   return MR_OK;
 }
 

@@ -25,6 +25,8 @@ namespace mr {
 
 constexpr int kFwdThreads = 256;  // a warpgroup for the softmax, one (a single busy warp) that issues
 constexpr float kRescale = 8.f;
+// Registers a thread: at launch, and after the issuing warpgroup has passed its own on (128 threads each).
+constexpr int kFwdRegs = 128, kIssueRegs = 40, kSoftmaxRegs = 2 * kFwdRegs - kIssueRegs;
 
 struct FwdShared {
   uint64_t k_full, v_full, s_done, s_read, p_ready, o_done;
@@ -75,7 +77,7 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
   const int sink_n = nsink ? (R.send - R.s0 + 15) & ~15 : 0;
 
   if (w >= 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
     if (w == 4) {
       // Descriptors are made once and stepped by additions.
       const bool lead = umma::elect_one();
@@ -150,7 +152,7 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const RowMask rm = row_mask(A, i);
     const int lo = rm.i < 0 ? 0 : rm.lo;
     atomicMax(&sh.lo_max, __reduce_max_sync(0xffffffffu, lo));
@@ -283,6 +285,7 @@ template <typename T, int NB> static int fwd_nb(const AttnArgs& A, cudaStream_t 
   if (int rc = head_map(&tv, A.v, dt, A, A.Hkv, A.v_ts, A.v_hs, 128)) return rc;
   constexpr int smem = 3 * NB * kTileBytes + 1024;
   if (int rc = allow_smem<attn_fwd_kernel<T, NB>>(smem, "attn_fwd_kernel")) return rc;
+  if (int rc = expect_regs<attn_fwd_kernel<T, NB>>(kFwdRegs, "attn_fwd_kernel")) return rc;
   attn_fwd_kernel<T, NB><<<dim3((A.T + 127) / 128, A.Hq), kFwdThreads, smem, st>>>(A, tq, tk, tv);
   return check_launch("attn_fwd_kernel");
 }

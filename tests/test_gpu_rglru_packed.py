@@ -89,6 +89,20 @@ def test_padding_rows_come_out_as_zeros(mr, cuda_dev, dtype):
         want = got
 
 
+def test_padded_front(mr, cuda_dev):
+    """Borders that do not start at 0: the rows before them belong to no sequence either."""
+    a, x, gy, _, _, _ = _inputs(cuda_dev, [140, 200], 32, torch.float32, seed=13)
+    a[:140], x[:140], gy[:140] = float("nan"), float("inf"), float("nan")
+    cu = torch.tensor([140, 150, 340], device=cuda_dev)
+    la, lx = (t.clone().requires_grad_() for t in (a, x))
+    y = mr.rglru_scan_packed(la, lx, cu)
+    got = [y.detach(), *torch.autograd.grad(y, (la, lx), gy)]
+    want = mr.rglru_scan_packed(a[140:], x[140:], cu - 140)
+    assert all((t[:140] == 0).all() for t in got)
+    tol, *_ = O.scan_bounds(a[140:], x[140:], cu - 140, gy[140:])
+    assert ((got[0][140:] - want).double().abs() <= 2 * tol).all() and all(torch.isfinite(t).all() for t in got)
+
+
 def test_nan_stays_in_its_sequence(mr, cuda_dev):
     lens = [130, 60, 140]
     a, x, gy, h0, gf, cu = _inputs(cuda_dev, lens, 64, torch.bfloat16, seed=5)

@@ -220,6 +220,31 @@ def test_graph_replay_and_side_stream(mr, cuda_dev):
     assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want))
 
 
+def test_two_streams_at_once(mr, cuda_dev):
+    """Forward and backward of different head sizes (TMEM and shared memory shares) at the same time."""
+    ins = [_inputs(cuda_dev, [900, 700], 8, 4, Dh, torch.bfloat16, seed=20 + Dh) for Dh in (64, 128)]
+    want = [_step(mr, *i, 200, 4) for i in ins]
+    streams = [torch.cuda.Stream(cuda_dev) for _ in ins]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for n, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[n].append(_step(mr, *ins[n], 200, 4))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for n in range(2) for g in got[n] for a, b in zip(g, want[n]))
+
+
+def test_padded_front(mr, cuda_dev):
+    """Borders that do not start at 0: the rows before them belong to no sequence either."""
+    q, k, v, gy, _ = _inputs(cuda_dev, [50, 160, 90], 2, 1, 64, torch.bfloat16, seed=23)
+    for t in (q, k, v, gy):
+        t[:50] = float("nan")
+    cu = torch.tensor([50, 210, 300], device=cuda_dev)
+    got = _check(mr, (q, k, v, gy, cu), 40, 2)
+    assert all((t[:50] == 0).all() for t in got)
+
+
 def test_empty_batches(mr, cuda_dev):
     z = torch.zeros(0, 2, 64, device=cuda_dev, dtype=torch.bfloat16, requires_grad=True)
     cu = torch.tensor([0, 0, 0], device=cuda_dev)
