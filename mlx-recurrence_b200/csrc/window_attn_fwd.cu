@@ -32,7 +32,6 @@ struct FwdShared {
   uint64_t k_full, v_full, s_done, s_read, p_ready, o_done;
   uint32_t tmem;
   int lo_max;  // the largest first key of the tile's queries
-  uint32_t again[4];
 };
 
 template <typename T, int NB>  // NB = 64-wide blocks of a row
@@ -169,13 +168,15 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
       const bool full = !sink && k0 >= lo_max && k0 + 127 <= q0;
       mbar_wait(&sh.s_done, t & 1);
       umma::fence_after_sync();
-      // what the query sees of the tile, a word per 32 keys (uniformly all ones in most tiles)
-      uint32_t see[4];
+      // what the query sees of the tile, a word per 32 keys
+      uint32_t see[4] = {};
+      if (!full) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int at = k0 + b * 32;
-        see[b] = bits(rm.start - at, min(min(rm.sink_end, rm.i + 1), sink ? R.send : INT32_MAX) - at);
-        if (!sink) see[b] |= bits(rm.lo - at, rm.i + 1 - at);
+        for (int b = 0; b < 4; ++b) {
+          const int at = k0 + b * 32;
+          see[b] = bits(rm.start - at, min(min(rm.sink_end, rm.i + 1), sink ? R.send : INT32_MAX) - at);
+          if (!sink) see[b] |= bits(rm.lo - at, rm.i + 1 - at);
+        }
       }
       uint32_t s[4][32];
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
