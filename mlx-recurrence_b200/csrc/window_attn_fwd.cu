@@ -179,24 +179,29 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
         }
       }
       uint32_t s[4][32];
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      umma::tmem_ld32(trow, s[0]);
+      // the blocks' bounds and the masks' selects are kept out of the tiles that every query sees in full
+      auto maximum = [&](auto whole) {
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        umma::tmem_ld32(trow, s[0]);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {  // a block's maximum while the next block comes
-        if (b >= nch) continue;
-        umma::tmem_wait_ld(s[b]);
-        if (b + 1 < nch) umma::tmem_ld32(trow + (b + 1) * 32, s[b + 1 < 4 ? b + 1 : 3]);
-        if (!full)
+        for (int b = 0; b < 4; ++b) {  // a block's maximum while the next block comes
+          if (!whole && b >= nch) continue;
+          umma::tmem_wait_ld(s[b]);
+          if (b + 1 < 4 && (whole || b + 1 < nch)) umma::tmem_ld32(trow + (b + 1) * 32, s[b + 1 < 4 ? b + 1 : 3]);
+          if (!whole)
 #pragma unroll
-          for (int j = 0; j < 32; ++j) s[b][j] = see[b] >> j & 1 ? s[b][j] : 0xff800000u;
+            for (int j = 0; j < 32; ++j) s[b][j] = see[b] >> j & 1 ? s[b][j] : 0xff800000u;
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) mx4[j >> 1 & 3] = max3(mx4[j >> 1 & 3], __uint_as_float(s[b][j]), __uint_as_float(s[b][j + 1]));
-      }
+          for (int j = 0; j < 32; j += 2)
+            mx4[j >> 1 & 3] = max3(mx4[j >> 1 & 3], __uint_as_float(s[b][j]), __uint_as_float(s[b][j + 1]));
+        }
+        return fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      };
+      const float mx = full ? maximum(std::true_type{}) : maximum(std::false_type{});
       if (kOwnP) {  // the next S may start under this tile's exponentials
         umma::fence_before_sync();
         mbar_arrive(&sh.s_read);
       }
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       if (t > 0) {  // P and O are free
         mbar_wait(&sh.o_done, (t - 1) & 1);
         umma::fence_after_sync();
@@ -218,20 +223,24 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
       const float mc = m == -INFINITY ? 0.f : m * c;
       const uint64_t c2 = pair(c, c), mc2 = pair(-mc, -mc);
       uint64_t sum[2] = {0, 0};
+      auto exponentials = [&](auto whole) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        if (b >= nch) continue;
-        uint32_t p[16];
+        for (int b = 0; b < 4; ++b) {
+          if (!whole && b >= nch) continue;
+          uint32_t p[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          float x0, x1;
-          unpair(fma2(pair(s[b][2 * j], s[b][2 * j + 1]), c2, mc2), x0, x1);
-          x0 = ex2(x0), x1 = ex2(x1);
-          sum[j & 1] = add2(sum[j & 1], pair(x0, x1));
-          p[j] = Fmt<T>::pack(x0, x1);
+          for (int j = 0; j < 16; ++j) {
+            float x0, x1;
+            unpair(fma2(pair(s[b][2 * j], s[b][2 * j + 1]), c2, mc2), x0, x1);
+            x0 = ex2(x0), x1 = ex2(x1);
+            sum[j & 1] = add2(sum[j & 1], pair(x0, x1));
+            p[j] = Fmt<T>::pack(x0, x1);
+          }
+          umma::tmem_st16(trow + kP + b * 16, p);
         }
-        umma::tmem_st16(trow + kP + b * 16, p);
-      }
+      };
+      if (full) exponentials(std::true_type{});
+      else exponentials(std::false_type{});
       float l0, l1;
       unpair(add2(sum[0], sum[1]), l0, l1);
       l += l0 + l1;
