@@ -298,11 +298,13 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
         }
       // the masks' selects are kept out of the tiles that every row sees in full
       auto to_p = [&](auto masked) {
+        ulonglong2 l4 = {};
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const uint64_t l = KV ? *reinterpret_cast<const uint64_t*>(&sh.lse[wg][x * 32 + 2 * j]) : l2;
+            if (KV && j % 2 == 0) l4 = *reinterpret_cast<const ulonglong2*>(&sh.lse[wg][x * 32 + 2 * j]);
+            const uint64_t l = KV ? (j % 2 ? l4.y : l4.x) : l2;
             float e0, e1;
             unpair(fma2(pair(s[x][2 * j], s[x][2 * j + 1]), c2, l), e0, e1);
             e0 = ex2(e0), e1 = ex2(e1);
@@ -311,10 +313,11 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
               e1 = see[x] >> (2 * j + 1) & 1 ? e1 : 0.f;
             }
             s[x][2 * j] = __float_as_uint(e0), s[x][2 * j + 1] = __float_as_uint(e1);
-            if (KV || sink) p[x * 16 + j] = Fmt<T>::pack(e0, e1);
+            if (KV || (masked && sink)) p[x * 16 + j] = Fmt<T>::pack(e0, e1);
           }
       };
       auto to_ds = [&](auto masked) {
+        ulonglong2 d4 = {};
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           uint32_t dp[32];
@@ -322,7 +325,8 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
           umma::tmem_wait_ld(dp);
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const uint64_t d = KV ? *reinterpret_cast<const uint64_t*>(&sh.delta[wg][x * 32 + 2 * j]) : d2;
+            if (KV && j % 2 == 0) d4 = *reinterpret_cast<const ulonglong2*>(&sh.delta[wg][x * 32 + 2 * j]);
+            const uint64_t d = KV ? (j % 2 ? d4.y : d4.x) : d2;
             uint64_t g = mul2(pair(s[x][2 * j], s[x][2 * j + 1]), add2(pair(dp[2 * j], dp[2 * j + 1]), d));
             if (Fmt<T>::id == 0) g = mul2(g, f2);
             float g0, g1;
