@@ -275,18 +275,26 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
         }
       fence_proxy_async_smem();
     }
-    for (int t = 0; t < n; ++t) {
+    // KV: lse (rows below 64) or delta of a column tile's query, a tile ahead of its use
+    auto stat = [&](int head, int c) {
+      const int q = c_beg + c * kNC + (row & 63);
+      const float* v = (row < 64 ? A.lse : A.delta) + (int64_t)(hr * G + head) * A.T;
+      return q < c_end ? -v[q] : row < 64 ? -INFINITY : 0.f;
+    };
+    int head = 0, c_at = wg;  // KV: query head of the group, and tile of its columns
+    while (KV && c_at >= per) c_at -= per, ++head;
+    float next_stat = KV && wg < n ? stat(head, c_at) : 0.f;
+    for (int t = wg; t < n; t += NS) {
       const bool sink = !KV && t < nsink;
-      if (t % NS != wg) continue;
-      const int k0 = col0(t), b = t % NS, ph = (t / NS) & 1;
+      const int k0 = KV ? c_beg + c_at * kNC : col0(t), b = t % NS, ph = (t / NS) & 1;
       const bool full = KV ? k0 >= r0 + 127 && k0 + kNC <= lim_min : !sink && k0 >= lo_max && k0 + kNC - 1 <= r0;
       if (KV) {
-        const int64_t hq = hr * G + t / per;
-        const int q = k0 + (row & 63);
         asm volatile("bar.sync %0, 128;" ::"r"(2 + wg) : "memory");  // the last tile's values have been read
-        if (row < 64) sh.lse[wg][row] = q < c_end ? -A.lse[hq * A.T + q] : -INFINITY;
-        else sh.delta[wg][row - 64] = q < c_end ? -A.delta[hq * A.T + q] : 0.f;
+        (row < 64 ? sh.lse[wg] : sh.delta[wg])[row & 63] = next_stat;
         asm volatile("bar.sync %0, 128;" ::"r"(2 + wg) : "memory");
+        c_at += NS;
+        while (c_at >= per) c_at -= per, ++head;
+        if (t + NS < n) next_stat = stat(head, c_at);
       }
       uint32_t s[2][32], p[32], ds[32], see[2] = {0, 0};
       const uint64_t c2 = pair(c, c), l2 = pair(-lse_r, -lse_r), d2 = pair(-delta_r, -delta_r), f2 = pair(f, f);
