@@ -387,16 +387,17 @@ MR_API int mr_rglru_packed_bwd(const float* grad_y, const float* grad_final, con
  * key/value head), Dh 32, 64, 96 or 128, sinks 0..64. *_ts, *_hs: token and
  * head strides in elements (multiples of 16 bytes; the last axis is dense).
  * cu_seqlens NULL: S sequences of L tokens (T = S L). y and the gradients are
- * dense and in `dtype`; lse [Hq,T] f32 (NULL when no backward follows) holds
- * what the backward needs. */
+ * dense and in `dtype`; lse [Hq,T] f32 and (not for f32) y_low, like y, hold
+ * what the backward needs: the rows' sums and what rounding y dropped. Both NULL
+ * when no backward follows. */
 MR_API int mr_window_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ts, int64_t q_hs, int64_t k_ts,
                               int64_t k_hs, int64_t v_ts, int64_t v_hs, const int32_t* cu_seqlens, int64_t S,
                               int64_t L, int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t window,
-                              int64_t sinks, float scale, void* y, float* lse, void* stream);
+                              int64_t sinks, float scale, void* y, void* y_low, float* lse, void* stream);
 MR_API size_t mr_window_attn_bwd_workspace_bytes(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t Dh,
                                                  int64_t sinks);
-MR_API int mr_window_attn_bwd(const void* grad_y, const void* y, const float* lse, const void* q, const void* k,
-                              const void* v, int64_t q_ts, int64_t q_hs, int64_t k_ts, int64_t k_hs, int64_t v_ts,
+MR_API int mr_window_attn_bwd(const void* grad_y, const void* y, const void* y_low, const float* lse, const void* q,
+                              const void* k, const void* v, int64_t q_ts, int64_t q_hs, int64_t k_ts, int64_t k_hs, int64_t v_ts,
                               int64_t v_hs, const int32_t* cu_seqlens, int64_t S, int64_t L, int dtype, int64_t T,
                               int64_t Hq, int64_t Hkv, int64_t Dh, int64_t window, int64_t sinks, float scale,
                               void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes,

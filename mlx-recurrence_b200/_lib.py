@@ -102,9 +102,9 @@ SIGNATURES = {
     "mr_rglru_packed_fwd": (_int, [_p, _p, _p, _i64, _int, _i64, _i64, _p, _p, _p, _p, _p, _sz, _p]),
     "mr_rglru_packed_bwd": (_int, [_p, _p, _p, _p, _p, _p, _i64, _int, _i64, _i64, _p, _p, _p, _p, _p, _sz, _p]),
     "mr_window_attn_fwd": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64,
-                                  _i64, _i64, _i64, _i64, ctypes.c_float, _p, _p, _p]),
+                                  _i64, _i64, _i64, _i64, ctypes.c_float, _p, _p, _p, _p]),
     "mr_window_attn_bwd_workspace_bytes": (_sz, [_int, _i64, _i64, _i64, _i64, _i64]),
-    "mr_window_attn_bwd": (_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _int,
+    "mr_window_attn_bwd": (_int, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _int,
                                   _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _p, _p, _p, _p, _sz, _p]),
     "mr_window_cache": (_int, [_p, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _int, _i64, _i64, _i64, _i64, _i64, _p,
                                _p, _p]),

@@ -64,14 +64,16 @@ extern "C" {
 int mr_window_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ts, int64_t q_hs, int64_t k_ts,
                        int64_t k_hs, int64_t v_ts, int64_t v_hs, const int32_t* cu_seqlens, int64_t S, int64_t L,
                        int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t window, int64_t sinks,
-                       float scale, void* y, float* lse, void* stream) {
+                       float scale, void* y, void* y_low, float* lse, void* stream) {
   const char* what = "mr_window_attn_fwd";
   AttnArgs A = attn_args(q, k, v, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, cu_seqlens, S, L, T, Hq, Hkv, Dh, window, sinks,
                          scale);
   if (int rc = attn_check(what, A, S, L, dtype, T, Hq, Hkv, Dh, window, sinks)) return rc;
   if (T == 0) return MR_OK;
   if (int rc = ptrs(what, {q, k, v, y})) return rc;
-  A.y = y, A.lse = lse;
+  if (dtype != MR_F32 && lse != nullptr)
+    if (int rc = ptrs(what, {y_low})) return rc;
+  A.y = y, A.y_low = dtype == MR_F32 ? nullptr : y_low, A.lse = lse;
   const cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
     case MR_F32: return attn_fwd_f32_launch(A, st);
@@ -85,8 +87,8 @@ size_t mr_window_attn_bwd_workspace_bytes(int dtype, int64_t T, int64_t Hq, int6
   return dtype == MR_F32 ? attn_bwd_f32_ws_bytes(T, Hq, Dh, sinks) : attn_bwd_ws_bytes(T, Hq, Dh, sinks);
 }
 
-int mr_window_attn_bwd(const void* grad_y, const void* y, const float* lse, const void* q, const void* k,
-                       const void* v, int64_t q_ts, int64_t q_hs, int64_t k_ts, int64_t k_hs, int64_t v_ts,
+int mr_window_attn_bwd(const void* grad_y, const void* y, const void* y_low, const float* lse, const void* q,
+                       const void* k, const void* v, int64_t q_ts, int64_t q_hs, int64_t k_ts, int64_t k_hs, int64_t v_ts,
                        int64_t v_hs, const int32_t* cu_seqlens, int64_t S, int64_t L, int dtype, int64_t T,
                        int64_t Hq, int64_t Hkv, int64_t Dh, int64_t window, int64_t sinks, float scale, void* grad_q,
                        void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, void* stream) {
@@ -96,10 +98,12 @@ int mr_window_attn_bwd(const void* grad_y, const void* y, const float* lse, cons
   if (int rc = attn_check(what, A, S, L, dtype, T, Hq, Hkv, Dh, window, sinks)) return rc;
   if (T == 0) return MR_OK;
   if (int rc = ptrs(what, {grad_y, y, q, k, v, grad_q, grad_k, grad_v})) return rc;
+  if (dtype != MR_F32)
+    if (int rc = ptrs(what, {y_low})) return rc;
   const size_t need = mr_window_attn_bwd_workspace_bytes(dtype, T, Hq, Hkv, Dh, sinks);
   if (lse == nullptr || workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace & 15u))
     return set_error(MR_E_WORKSPACE, "%s: needs lse and %zu bytes of workspace, got %zu", what, need, workspace_bytes);
-  A.y = const_cast<void*>(y), A.lse = const_cast<float*>(lse), A.gy = grad_y;
+  A.y = const_cast<void*>(y), A.y_low = const_cast<void*>(y_low), A.lse = const_cast<float*>(lse), A.gy = grad_y;
   A.gq = grad_q, A.gk = grad_k, A.gv = grad_v;
   const cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {

@@ -49,6 +49,7 @@ struct AttnArgs {
   int window, sinks;                // window <= T
   float scale;                      // > 0
   void* y;                          // [T, Hq, Dh] dense
+  void* y_low;                      // [T, Hq, Dh]: what rounding y to its type drops, rounded too; NULL when not wanted
   float* lse;                       // [Hq, T]: log2 of the row's sum of exponentials; NULL when not wanted
   // backward
   const void* gy;                   // [T, Hq, Dh] dense
@@ -256,7 +257,13 @@ template <typename T> __device__ __noinline__ void exact_fwd_row(const AttnArgs&
     ++j;
     if (j >= w.sink_end && j < w.lo) j = w.lo;
   }
-  row_store((T*)A.y + ((int64_t)i * A.Hq + h) * A.Dh, o, 1.f / l, A.Dh, lane);
+  const int64_t at = ((int64_t)i * A.Hq + h) * A.Dh;
+  row_store((T*)A.y + at, o, 1.f / l, A.Dh, lane);
+  if (A.y_low != nullptr) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) o.v[n] = o.v[n] / l - to_f(from_f<T>(o.v[n] / l));
+    row_store((T*)A.y_low + at, o, 1.f, A.Dh, lane);
+  }
   if (A.lse != nullptr && lane == 0) A.lse[(int64_t)h * A.T + i] = m + log2f(l);
 }
 

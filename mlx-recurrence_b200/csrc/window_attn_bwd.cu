@@ -25,11 +25,11 @@
 // power-of-two scale of max |gy|, so that neither large nor small loss scales leave
 // its range); lse, delta and the sums are float32.
 //
-// bf16, 16384 tokens, 32 heads of 64, window 1024: 851 us (379 TFLOP/s of the 5
-// products); 16 heads of 128 on 4, window 2048, 4 sinks: 762 us (486). Measured and
-// not kept: both products of S and dP before any sum of the old tile (918 and 826
-// us), three warpgroups in one CTA for Dh <= 64 (1,034 us), two threads per row (827
-// and 790 us).
+// bf16, 16384 tokens, 32 heads of 64, window 1024: 824 us (391 TFLOP/s of the 5
+// products); 16 heads of 128 on 4, window 2048, 4 sinks: 772 us (480). Measured and
+// not kept (where this form took 851 and 762 us): both products of S and dP before
+// any sum of the old tile (918 and 826 us), three warpgroups in one CTA for Dh <= 64
+// (1,034 us), two threads per row (827 and 790 us).
 //
 // The sinks' far queries (window_attn.cuh): a query tile that meets a sink tile adds
 // the sinks' gradients by products over its 128 queries, with P and dS handed
@@ -466,7 +466,8 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
   if (w == 4 * NS) umma::tmem_dealloc(tm, kCols);
 }
 
-// delta[h][t] = sum_d gy y, zero for rows outside every sequence; fp16: the
+// delta[h][t] = sum_d gy y with y and what its rounding dropped (from the rounded y alone the gradients' error is 1.55
+// times the output rounding's, so 1.4), zero for rows outside every sequence; fp16: the
 // largest finite |gy| (the order of an integer maximum does not matter). 8 lanes
 // per row, 16 bytes each at a time.
 template <typename T> __global__ void __launch_bounds__(256) attn_delta_kernel(const __grid_constant__ AttnArgs A, uint32_t* amax) {
@@ -480,10 +481,11 @@ template <typename T> __global__ void __launch_bounds__(256) attn_delta_kernel(c
     if (in)
       for (int d = sub * 8; d < A.Dh; d += 64) {
         const Vec<T, 8> g = ld_vec<T, 8>((const T*)A.gy + row * A.Dh + d), y = ld_vec<T, 8>((const T*)A.y + row * A.Dh + d);
+        const Vec<T, 8> r = ld_vec<T, 8>((const T*)A.y_low + row * A.Dh + d);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float x = to_f(g.v[j]);
-          s = fmaf(x, to_f(y.v[j]), s);
+          s = fmaf(x, to_f(y.v[j]) + to_f(r.v[j]), s);
           const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
           if (b < 0x7f800000u) big = max(big, b);
         }

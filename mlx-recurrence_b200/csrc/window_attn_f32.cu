@@ -11,7 +11,7 @@
 // columns of the products that follow. Operands lie transposed ([d][64 + 4]) in
 // shared memory, so a thread's rows and columns come as 16-byte reads. Bound by
 // the latency between a tile's barriers (few warps per SM): T=3001, 8 heads of 32,
-// window 300: forward 76 us, backward 269 us; T=4000, 8 heads of 128 on 4, window
+// window 300: forward 75 us, backward 269 us; T=4000, 8 heads of 128 on 4, window
 // 1000: 547 us (19 TFLOP/s) and 1.92 ms. (128 threads with 8 x 4 results: 831 us, 3.14
 // ms.)
 #include "window_attn.cuh"

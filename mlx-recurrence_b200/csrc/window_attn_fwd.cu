@@ -12,13 +12,17 @@
 // gaps; the issuing warpgroup gives its registers to the softmax's, which holds a
 // row of S.
 //
-// bf16, 16384 tokens, 32 heads of 64, window 1024: 297 us (433 TFLOP/s); 16 heads of
-// 128 on 4, window 2048, 4 sinks: 265 us (559). Bound by the chain of a tile (load S,
-// maximum, exponentials: about 3,000 cycles on two warps per scheduler), not by one
-// pipe: a tile's exponentials alone would take 1,024 cycles, its products 500 or
-// 1,000. Measured and not kept: two threads per query (304 us), a quarter of the
-// exponentials by a polynomial on the FMA pipe (299 us), the issuing done by a
-// softmax warp (352 us).
+// For a backward pass it also writes what the rounding of y drops (y_low), so that
+// delta = gy.y is of float32 quality.
+//
+// bf16, 16384 tokens, 32 heads of 64, window 1024: 259 us (497 TFLOP/s), 273 with
+// y_low; 16 heads of 128 on 4, window 2048, 4 sinks: 248 us (597), 272 with y_low.
+// Bound by the chain of a tile (load S, maximum, exponentials, on two warps per
+// scheduler), not by one pipe: a tile's exponentials alone would take 1,024 cycles,
+// its products 500 or 1,000, a tile takes about 1,800. Measured and not kept (at 297
+// us, before whole tiles had loops without bounds): two threads per query 304 us, a
+// quarter of the exponentials by a polynomial on the FMA pipe 299 us, the issuing
+// done by a softmax warp 352 us.
 #include "window_tc.cuh"
 
 namespace mr {
@@ -51,9 +55,13 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
   const int nsink = R.send > R.s0 ? 1 : 0;  // at most 64 sinks: one tile
   const int ntile = R.kend > R.kmin ? nsink + (R.kend - R.kmin + 127) / 128 : 0;
   T* y = (T*)A.y + ((int64_t)i * A.Hq + h) * A.Dh;
+  T* low = A.y_low ? (T*)A.y_low + ((int64_t)i * A.Hq + h) * A.Dh : nullptr;
   if (ntile == 0) {  // no sequence reaches this tile
     if (tid < 128 && i < A.T) {
-      for (int d = 0; d < A.Dh; d += 8) *reinterpret_cast<int4*>(y + d) = make_int4(0, 0, 0, 0);
+      for (int d = 0; d < A.Dh; d += 8) {
+        *reinterpret_cast<int4*>(y + d) = make_int4(0, 0, 0, 0);
+        if (low != nullptr) *reinterpret_cast<int4*>(low + d) = make_int4(0, 0, 0, 0);
+      }
       if (A.lse != nullptr) A.lse[(int64_t)h * A.T + i] = INFINITY;
     }
     return;
@@ -269,11 +277,16 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
       if (i < A.T)
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
-          uint32_t p[4];
+          uint32_t p[4], r[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            p[e] = rm.i < 0 ? 0u : Fmt<T>::pack(__uint_as_float(o[j + 2 * e]) * inv, __uint_as_float(o[j + 2 * e + 1]) * inv);
+          for (int e = 0; e < 4; ++e) {
+            const float v0 = __uint_as_float(o[j + 2 * e]) * inv, v1 = __uint_as_float(o[j + 2 * e + 1]) * inv;
+            p[e] = rm.i < 0 ? 0u : Fmt<T>::pack(v0, v1);
+            const float2 back = Fmt<T>::unpack(p[e]);
+            r[e] = rm.i < 0 ? 0u : Fmt<T>::pack(v0 - back.x, v1 - back.y);
+          }
           *reinterpret_cast<uint4*>(y + d + j) = make_uint4(p[0], p[1], p[2], p[3]);
+          if (low != nullptr) *reinterpret_cast<uint4*>(low + d + j) = make_uint4(r[0], r[1], r[2], r[3]);
         }
     }
     if (i < A.T && A.lse != nullptr) A.lse[(int64_t)h * A.T + i] = rm.i < 0 || l == 0.f ? INFINITY : m * c + log2f(l);

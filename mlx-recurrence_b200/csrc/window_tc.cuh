@@ -19,6 +19,7 @@ template <> struct Fmt<__nv_bfloat16> {
     __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&r);
   }
+  static __device__ float2 unpack(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
 };
 template <> struct Fmt<__half> {
   static constexpr int id = 0;
@@ -26,6 +27,7 @@ template <> struct Fmt<__half> {
     __half2 r = __floats2half2_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&r);
   }
+  static __device__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 };
 
 __device__ __forceinline__ float ex2(float x) {

@@ -94,11 +94,12 @@ def _attend(q, k, v, cu, window, sinks, scale, want_lse):
     T, Hq, Dh = q_.shape
     y = torch.empty((T, Hq, Dh), dtype=dt, device=dev)
     lse = torch.empty((Hq, T), dtype=torch.float32, device=dev) if want_lse else None
+    y_low = torch.empty_like(y) if want_lse and dt != torch.float32 else None  # what rounding y drops
     args = (qt, qh, kt, kh, vt, vh, _lib.addr(cu), S, L, _lib.DTYPE_CODE[dt], T, Hq, k_.shape[1], Dh, window, sinks,
             scale)
     _lib.call_on(dev, "mr_window_attn_fwd", q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), *args, y.data_ptr(),
-                 _lib.addr(lse))
-    return y if packed else y.view(q.shape), args, (q_, k_, v_, cu, y, lse)
+                 _lib.addr(y_low), _lib.addr(lse))
+    return y if packed else y.view(q.shape), args, (q_, k_, v_, cu, y, y_low, lse)
 
 
 class _WindowAttention(torch.autograd.Function):
@@ -112,7 +113,7 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        q_, k_, v_, _, y, lse = ctx.saved_tensors
+        q_, k_, v_, _, y, y_low, lse = ctx.saved_tensors
         dev, dt = q_.device, q_.dtype
         T, Hq, Dh = q_.shape
         Hkv = k_.shape[1]
@@ -121,8 +122,8 @@ class _WindowAttention(torch.autograd.Function):
         gk, gv = (torch.empty((T, Hkv, Dh), dtype=dt, device=dev) for _ in range(2))
         nws = _lib.load().mr_window_attn_bwd_workspace_bytes(_lib.DTYPE_CODE[dt], T, Hq, Hkv, Dh, ctx.args[15])
         ws = torch.empty(max(nws, 16), dtype=torch.uint8, device=dev)
-        _lib.call_on(dev, "mr_window_attn_bwd", gy.data_ptr(), y.data_ptr(), lse.data_ptr(), q_.data_ptr(),
-                     k_.data_ptr(), v_.data_ptr(), *ctx.args, gq.data_ptr(), gk.data_ptr(), gv.data_ptr(),
+        _lib.call_on(dev, "mr_window_attn_bwd", gy.data_ptr(), y.data_ptr(), _lib.addr(y_low), lse.data_ptr(),
+                     q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), *ctx.args, gq.data_ptr(), gk.data_ptr(), gv.data_ptr(),
                      ws.data_ptr(), ws.numel())
         sq, sk = ctx.shapes
         if len(sq) == 4:

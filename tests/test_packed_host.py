@@ -82,7 +82,7 @@ def test_c_abi_status_codes(mr):
 
     def fwd(q=p, ts=64, cu=p, S=1, L=0, dtype=1, T=8, Hq=2, Hkv=1, Dh=64, window=4, sinks=0, scale=0.1, y=p):
         return lib.mr_window_attn_fwd(q, p, p, ts, 64, 64, 64, 64, 64, cu, S, L, dtype, T, Hq, Hkv, Dh, window, sinks,
-                                      scale, y, n, n)
+                                      scale, y, n, n, n)
 
     for change, code in ((dict(dtype=5), m.MR_E_DTYPE), (dict(Hq=3, Hkv=2), m.MR_E_SHAPE), (dict(Dh=48), m.MR_E_SHAPE),
                          (dict(window=0), m.MR_E_SHAPE), (dict(sinks=65), m.MR_E_SHAPE), (dict(scale=0.0), m.MR_E_SHAPE),
@@ -90,7 +90,7 @@ def test_c_abi_status_codes(mr):
                          (dict(cu=n, S=2, L=3), m.MR_E_SHAPE), (dict(T=-1), m.MR_E_SHAPE)):
         assert fwd(**change) == code, change
     assert fwd(T=0) == m.MR_OK
-    rc = lib.mr_window_attn_bwd(p, p, p, p, p, p, 64, 64, 64, 64, 64, 64, p, 1, 0, 1, 8, 2, 1, 64, 4, 0, 0.1, p, p, p, n,
+    rc = lib.mr_window_attn_bwd(p, p, p, p, p, p, p, 64, 64, 64, 64, 64, 64, p, 1, 0, 1, 8, 2, 1, 64, 4, 0, 0.1, p, p, p, n,
                                 0, n)
     assert rc == m.MR_E_WORKSPACE
     assert lib.mr_window_step(p, p, p, p, p, p, 1, 1, 2, 3, 2, 64, 9, 1, 0.1, p, n) == m.MR_E_SHAPE
