@@ -79,6 +79,16 @@ def _dense16(t, dt):
     return t.clone() if t.data_ptr() % 16 else t
 
 
+def _kernel_args(q, k, v, dt, packed_dims, cu, meta):
+    """q, k, v as the kernels read them, and the kernels' shared arguments: strides and addresses are of these very
+    tensors, which the caller keeps until it has launched."""
+    S, L, window, sinks, scale = meta
+    (q, qt, qh), (k, kt, kh), (v, vt, vh) = (_rows(t, dt, packed_dims) for t in (q, k, v))
+    T, Hq, Dh = q.shape
+    return (q, k, v), (qt, qh, kt, kh, vt, vh, _lib.addr(cu), S, L, _lib.DTYPE_CODE[dt], T, Hq, k.shape[1], Dh, window,
+                       sinks, scale)
+
+
 def _attend(q, k, v, cu, window, sinks, scale, want_lse):
     packed = q.dim() == 3
     dev = _lib.require_cuda(q, k, v)
@@ -88,24 +98,21 @@ def _attend(q, k, v, cu, window, sinks, scale, want_lse):
         S, L = cu.numel() - 1, 0
     else:
         S, L = q.shape[:2]
-    q_, qt, qh = _rows(q, dt, packed)
-    k_, kt, kh = _rows(k, dt, packed)
-    v_, vt, vh = _rows(v, dt, packed)
+    meta = S, L, window, sinks, scale
+    (q_, k_, v_), args = _kernel_args(q, k, v, dt, packed, cu, meta)
     T, Hq, Dh = q_.shape
     y = torch.empty((T, Hq, Dh), dtype=dt, device=dev)
     lse = torch.empty((Hq, T), dtype=torch.float32, device=dev) if want_lse else None
     y_low = torch.empty_like(y) if want_lse and dt != torch.float32 else None  # what rounding y drops
-    args = (qt, qh, kt, kh, vt, vh, _lib.addr(cu), S, L, _lib.DTYPE_CODE[dt], T, Hq, k_.shape[1], Dh, window, sinks,
-            scale)
     _lib.call_on(dev, "mr_window_attn_fwd", q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), *args, y.data_ptr(),
                  _lib.addr(y_low), _lib.addr(lse))
-    return y if packed else y.view(q.shape), args, (q_, k_, v_, cu, y, y_low, lse)
+    return y if packed else y.view(q.shape), meta, (q_, k_, v_, cu, y, y_low, lse)
 
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, window, sinks, scale):
-        y, ctx.args, saved = _attend(q, k, v, cu, window, sinks, scale, True)
+        y, ctx.meta, saved = _attend(q, k, v, cu, window, sinks, scale, True)
         ctx.save_for_backward(*saved)
         ctx.shapes = (q.shape, k.shape)
         return y
@@ -113,17 +120,23 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        q_, k_, v_, _, y, y_low, lse = ctx.saved_tensors
+        # Under checkpointing and saved-tensor hooks these are other tensors than the forward's, maybe of other strides:
+        # nothing of the forward's addresses or layout is used here.
+        q_, k_, v_, cu, y, y_low, lse = ctx.saved_tensors
         dev, dt = q_.device, q_.dtype
+        if cu is not None:
+            cu = cu.contiguous()
+        (q_, k_, v_), args = _kernel_args(q_, k_, v_, dt, True, cu, ctx.meta)
         T, Hq, Dh = q_.shape
         Hkv = k_.shape[1]
-        gy = _dense16(gy, dt)
+        gy, y, lse = _dense16(gy, dt), _dense16(y, dt), lse.contiguous()
+        y_low = None if y_low is None else _dense16(y_low, dt)
         gq = torch.empty((T, Hq, Dh), dtype=dt, device=dev)
         gk, gv = (torch.empty((T, Hkv, Dh), dtype=dt, device=dev) for _ in range(2))
-        nws = _lib.load().mr_window_attn_bwd_workspace_bytes(_lib.DTYPE_CODE[dt], T, Hq, Hkv, Dh, ctx.args[15])
+        nws = _lib.load().mr_window_attn_bwd_workspace_bytes(_lib.DTYPE_CODE[dt], T, Hq, Hkv, Dh, ctx.meta[3])
         ws = torch.empty(max(nws, 16), dtype=torch.uint8, device=dev)
         _lib.call_on(dev, "mr_window_attn_bwd", gy.data_ptr(), y.data_ptr(), _lib.addr(y_low), lse.data_ptr(),
-                     q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), *ctx.args, gq.data_ptr(), gk.data_ptr(), gv.data_ptr(),
+                     q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), *args, gq.data_ptr(), gk.data_ptr(), gv.data_ptr(),
                      ws.data_ptr(), ws.numel())
         sq, sk = ctx.shapes
         if len(sq) == 4:
