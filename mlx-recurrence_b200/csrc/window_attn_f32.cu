@@ -190,16 +190,17 @@ __global__ void __launch_bounds__(kThreads, DH <= 64 ? 2 : 1) attn_fwd_f32(const
     for (int x = 8; x > 0; x >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x, 16);
     const int t = q0 + ty * kR + i;
     if (t >= A.T) continue;
+    const bool live = rows[ty * kR + i].i >= 0;  // a row of no sequence is zero whatever its tiles hold
     const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
     float* y = (float*)A.y + ((int64_t)t * A.Hq + h) * A.Dh;
     float odd = 0.f;  // NaN as soon as one element is not finite
 #pragma unroll
     for (int n = 0; n < DH / 16; ++n) {
-      y[tx + 16 * n] = (o[i][n] * inv);
+      y[tx + 16 * n] = live ? o[i][n] * inv : 0.f;
       odd = fmaf(o[i][n], 0.f, odd);
     }
     if (A.lse != nullptr && tx == 0) A.lse[(int64_t)h * A.T + t] = l[i] == 0.f ? INFINITY : m[i] + log2f(l[i]);
-    if (odd != 0.f) again[ty * kR + i] = 1;
+    if (live && odd != 0.f) again[ty * kR + i] = 1;
   }
   __syncthreads();
   for (int r = threadIdx.x >> 5; r < kBT; r += kThreads / 32)
@@ -354,6 +355,7 @@ __global__ void __launch_bounds__(kThreads, DH <= 64 ? 2 : 1) attn_bwd_f32(const
   for (int i = 0; i < kR; ++i) {
     const int t = r0 + ty * kR + i;
     if (t >= A.T) continue;
+    const bool live = KV ? limit[ty * kR + i] > 0 : rows[ty * kR + i].i >= 0;
     const int H = KV ? A.Hkv : A.Hq;
     const int64_t at = ((int64_t)t * H + blockIdx.y) * A.Dh;
     float* g1 = (float*)(KV ? A.gk : A.gq) + at;
@@ -367,11 +369,11 @@ __global__ void __launch_bounds__(kThreads, DH <= 64 ? 2 : 1) attn_bwd_f32(const
         }
 #pragma unroll
     for (int n = 0; n < DH / 16; ++n) {
-      g1[tx + 16 * n] = (o1[i][n] * A.scale);
-      if (KV) ((float*)A.gv + at)[tx + 16 * n] = (o2[i][n]);
+      g1[tx + 16 * n] = live ? o1[i][n] * A.scale : 0.f;
+      if (KV) ((float*)A.gv + at)[tx + 16 * n] = live ? o2[i][n] : 0.f;
       odd = fmaf(o1[i][n], 0.f, fmaf(o2[i][n], 0.f, odd));
     }
-    if (odd != 0.f) again[ty * kR + i] = 1;
+    if (live && odd != 0.f) again[ty * kR + i] = 1;
   }
   __syncthreads();
   for (int r = threadIdx.x >> 5; r < kBT; r += kThreads / 32)

@@ -1,0 +1,49 @@
+"""Sliding-window attention at its edges: rows that belong to no sequence beside
+values that are not finite, rows whose every score is minus infinity, gradients
+of very different sizes in one fp16 batch, mixed types, empty rows, derivatives
+that it does not have."""
+
+import pytest
+import torch
+
+import _packed_oracle as O
+from _window_oracle import Window
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "f32": torch.float32}
+
+
+def _inputs(dev, lens, Hq, Hkv, Dh, dtype, pad=0, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    T = sum(lens) + pad
+    q, gy = (torch.randn(T, Hq, Dh, generator=g) for _ in range(2))
+    k, v = (torch.randn(T, Hkv, Dh, generator=g) for _ in range(2))
+    return [t.to(dtype).to(dev) for t in (q, k, v, gy)] + [O.borders(lens).to(dev)]
+
+
+def _step(mr, q, k, v, gy, cu, window, sinks):
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+    y = mr.window_attention_packed(*leaves, cu, window, sinks=sinks)
+    return [y.detach(), *torch.autograd.grad(y, leaves, gy)]
+
+
+def _check(got, W, names=("y", "gq", "gk", "gv")):
+    for n in names:
+        O.check(n, got[("y", "gq", "gk", "gv").index(n)], getattr(W, n), getattr(W, "tol_" + n))
+
+
+# ---- rows outside every sequence ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", sorted(DT))
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("what", ["k", "v", "q", "gy"])
+def test_rows_outside_are_zero_beside_values_that_are_not_finite(mr, cuda_dev, what, bad, dtype):
+    """Padding before and behind the sequences, in the tiles of tokens that hold infinities or NaN."""
+    q, k, v, gy, _ = _inputs(cuda_dev, [200], 2, 1, 64, DT[dtype], seed=51)
+    cu = torch.tensor([30, 90, 170], device=cuda_dev)
+    t = dict(q=q, k=k, v=v, gy=gy)[what]
+    t[31], t[169] = bad, bad
+    for name, g in zip(("y", "grad_q", "grad_k", "grad_v"), _step(mr, q, k, v, gy, cu, 40, 2)):
+        assert (g[:30] == 0).all() and (g[170:] == 0).all(), name
