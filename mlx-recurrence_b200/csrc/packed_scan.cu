@@ -22,14 +22,18 @@
 // Composed maps need products of gates that stay in float32's range: |a| <= 1
 // always does, larger gates as long as their products along a sequence do.
 //
-// bf16, T=32768, D=2560, 24 sequences: forward 137 us (4.9 TB/s of the 8 bytes an
-// element needs), backward 224 us (4.5 TB/s of 12 bytes). What is left is the wait
-// for the items before (clock stamps: a fold takes 900 cycles, the rest of the work
-// 1,500, the wait some 6,000), so nothing delays an item that others wait for.
-// Measured at that size, forward and backward: tickets taken a stage ahead of the
-// data 182 and 304 us; a plain loop for the steps at borders 227 us; rounds of 4 (8)
-// records of the look-back in place of 1: 160 and 268 us (199 and 343), since they
-// read maps that are not there yet where a state is about to come.
+// bf16, T=32768, D=2560, 24 sequences: forward 140 us (4.8 TB/s of the 8 bytes an
+// element needs), backward 233 us (4.3 TB/s of 12 bytes); fp16, T=131072, D=512, one
+// sequence: 142 and 197 us. What is left is the wait for the items before, so nothing
+// delays an item that others wait for. The look-back keeps the maps it meets and applies
+// them in the items' order; composing them newest first took 138 and 224 us (128 and
+// 186), but its bits varied with the timing, and reading them a second time instead of
+// keeping them took 148 and 232 us (365 and 390). Eight maps kept in the forward instead
+// of sixteen: 140 us (171). Measured before, beside 138 and 224 us at the first size:
+// tickets taken a stage ahead of the data 182 and 304 us; a plain loop for the steps at
+// borders 227 us; rounds of 4 (8) records of the look-back in place of 1: 160 and 268 us
+// (199 and 343), since they read maps that are not there yet where a state is about to
+// come.
 #include "common.cuh"
 #include "launch.cuh"
 #include "tma.cuh"
@@ -41,17 +45,19 @@ constexpr int kWarps = 8;
 constexpr int kSteps = 16;               // steps of a thread
 constexpr int kChunk = kWarps * kSteps;  // steps of an item
 
-// A chunk's map or state for one channel, written and read as one 16-byte access
-// (single-copy atomic), so no flag or fence stands beside it.
+// A chunk's map or state for one channel, written and read as one 16-byte access, so no flag or fence stands beside
+// it. The last word is a function of the others: a read whose words are not of one write (an assembler may narrow a
+// load to the words that are used, which is then no longer one access) counts as not there yet.
 struct alignas(16) Rec {
   float A, B;    // kMap: state out = A state in + B; kState: state out = B
   uint32_t tag;  // 0: not there yet
-  uint32_t pad;
+  uint32_t sum;
 };
 enum : uint32_t { kMap = 1, kState = 2 };
 
 __device__ __forceinline__ void rec_store(Rec* p, float A, float B, uint32_t tag) {
-  const uint64_t lo = (uint64_t)__float_as_uint(B) << 32 | __float_as_uint(A), hi = tag;
+  const uint32_t a = __float_as_uint(A), b = __float_as_uint(B);
+  const uint64_t lo = (uint64_t)b << 32 | a, hi = (uint64_t)(a ^ b ^ tag) << 32 | tag;
   asm volatile("{\n\t.reg .b128 r;\n\tmov.b128 r, {%1, %2};\n\tst.relaxed.gpu.global.b128 [%0], r;\n\t}" ::"l"(p), "l"(lo),
                "l"(hi)
                : "memory");
@@ -62,18 +68,19 @@ __device__ __forceinline__ Rec rec_load(const Rec* p) {
                : "=l"(lo), "=l"(hi)
                : "l"(p)
                : "memory");
-  return {__uint_as_float((uint32_t)lo), __uint_as_float((uint32_t)(lo >> 32)), (uint32_t)hi, 0};
+  const uint32_t a = (uint32_t)lo, b = (uint32_t)(lo >> 32), tag = (uint32_t)hi, sum = (uint32_t)(hi >> 32);
+  return {__uint_as_float(a), __uint_as_float(b), sum == (a ^ b ^ tag) ? tag : 0, sum};
 }
 
-// Polls until the record is there; after 2 s (its writer is always a CTA that
+// Polls until the record's tag is `least` at least; after 2 s (its writer is always a CTA that
 // started earlier, so only a device failure gets here) sets the device error word.
-__device__ __forceinline__ Rec rec_wait(const Rec* p) {
+__device__ __forceinline__ Rec rec_wait(const Rec* p, uint32_t least) {
   Rec r = rec_load(p);
-  if (r.tag != 0) return r;
+  if (r.tag >= least) return r;
   const uint64_t t0 = globaltimer_ns();
   for (uint32_t i = 0; i < kSpinLimit; ++i) {
     r = rec_load(p);
-    if (r.tag != 0) return r;
+    if (r.tag >= least) return r;
     if ((i & 255u) == 255u &&
         (*reinterpret_cast<volatile int*>(&g_device_error) != 0 || globaltimer_ns() - t0 > 2000000000ull))
       break;
@@ -165,9 +172,10 @@ template <typename T, int V> __device__ __forceinline__ void put(T* p, const flo
 }
 
 // What a CTA keeps in shared memory beside the stages.
-template <int V> struct Work {
-  float A[kWarps][32 * V], B[kWarps][32 * V];    // the warps' maps along the chain
-  float fA[kWarps][32 * V], fB[kWarps][32 * V];  // backward: the warps' maps of the forward recurrence
+template <int V, bool BWD> struct Work {
+  static constexpr int kKept = BWD ? kWarps : 2 * kWarps;
+  float map[kKept][2][32 * V];              // the warps' maps A, B along the chain; then the look-back's, newest first
+  float fmap[BWD ? kWarps : 1][2][32 * V];  // backward: the warps' maps of the forward recurrence
   float carry[32 * V];                           // the state entering the item
   int mark[kChunk];                              // per token at a border: its sequence, and which end of it
   uint64_t full;
@@ -187,7 +195,7 @@ constexpr int kStart = 1 << 30, kEnd = INT32_MIN, kSeq = kStart - 1;  // of Work
 template <typename T, bool BWD, bool TMA> struct Feed {
   static constexpr int V = kV<T>, CH = 32 * V;
   unsigned char* stage;
-  Work<V>& sh;
+  Work<V, BWD>& sh;
   const PackedArgs& P;
   const CUtensorMap *ta, *tx, *tg;
   int n = 0;  // items so far
@@ -265,7 +273,8 @@ template <typename T, bool BWD, bool TMA> struct Feed {
 
 // Marks of a chunk that holds borders; all threads call it. A token belongs to
 // one sequence, so one entry serves its start and its end.
-template <int V> __device__ __forceinline__ void mark_borders(Work<V>& sh, const ChunkInfo& c, const PackedArgs& P, int64_t t0, int n) {
+template <int V, bool BWD>
+__device__ __forceinline__ void mark_borders(Work<V, BWD>& sh, const ChunkInfo& c, const PackedArgs& P, int64_t t0, int n) {
   if (threadIdx.x < kChunk) sh.mark[threadIdx.x] = 0;
   __syncthreads();
   for (int s = c.first + threadIdx.x; s <= P.S; s += kWarps * 32) {
@@ -300,20 +309,26 @@ template <int V> __device__ __forceinline__ void begin(const float* state, int s
 
 // The chain. Along it (left to right in the forward, right to left in the
 // backward) item `rank` of a channel tile follows rank - 1. Composes the warps'
-// maps in sh.A, sh.B (bit w of `cut`: warp w's steps hold a border, so its
+// maps in sh.map (bit w of `cut`: warp w's steps hold a border, so its
 // outgoing state is B whatever enters), publishes this item's record, and returns
 // in p, q the map from the state entering the item to the one entering this warp
 // and in carry the former. `need`: whether anything in the item depends on it.
+//
+// The look-back goes to the nearest item whose state is there and applies the maps
+// on the way in the items' order, with the fmaf that the items themselves apply:
+// the bits do not depend on how far the others have come. Maps wait in the place of
+// sh.map, which every warp has read by then; behind kKept of them a state is waited for.
 template <int V, bool BWD>
-__device__ __forceinline__ void chain(Work<V>& sh, const PackedArgs& P, int64_t ch, int live, int rank, uint32_t cut,
+__device__ __forceinline__ void chain(Work<V, BWD>& sh, const PackedArgs& P, int64_t ch, int live, int rank, uint32_t cut,
                                       bool need, float (&carry)[V], float (&p)[V], float (&q)[V]) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = lane * V;
   const bool wait = need && rank > 0, tell = P.counter != nullptr && rank < P.nchunk - 1;
   Rec* recs = P.recs + ch;
+  float tp[V], tq[V];  // warp 0: the item's own map
   auto through = [&](int i) {  // p, q <- the warps' maps up to and including warp i
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const float A = sh.A[i][c + v], B = sh.B[i][c + v];
+      const float A = sh.map[i][0][c + v], B = sh.map[i][1][c + v];
       q[v] = cut >> i & 1 ? B : fmaf(A, q[v], B);
       p[v] = cut >> i & 1 ? 0.f : p[v] * A;
     }
@@ -321,56 +336,69 @@ __device__ __forceinline__ void chain(Work<V>& sh, const PackedArgs& P, int64_t 
 #pragma unroll
   for (int v = 0; v < V; ++v) p[v] = 1.f, q[v] = 0.f;
   if (w == 0) {
-    float tp[V], tq[V];
+    float ep[V], eq[V];  // what enters warp 0, in the backward the last on the chain
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
-      if (BWD && i == kWarps - 1) {
+      if (i == (BWD ? kWarps - 1 : 0)) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) tp[v] = p[v], tq[v] = q[v];  // what enters warp 0, the last on the chain
+        for (int v = 0; v < V; ++v) ep[v] = p[v], eq[v] = q[v];
       }
       through(BWD ? kWarps - 1 - i : i);
     }
-    if (tell)
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (v < live) rec_store(recs + rank * P.D + v, p[v], q[v], cut || !wait ? kState : kMap);
-    if (wait) {
-      float a[V], b[V];  // the composed map of the items looked at so far
-      bool known[V];     // a record may turn from map to state between two reads: each channel stops by itself
-#pragma unroll
-      for (int v = 0; v < V; ++v) a[v] = 1.f, b[v] = 0.f, known[v] = v >= live;
-      bool open = true;
-      for (int at = rank - 1; open; --at) {
-        Rec r[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) r[v] = at >= 0 && !known[v] ? rec_load(recs + at * P.D + v) : Rec{0.f, 0.f, kState, 0};
-        open = false;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          if (!known[v]) {
-            if (r[v].tag == 0) r[v] = rec_wait(recs + at * P.D + v);
-            b[v] = fmaf(a[v], r[v].B, b[v]);
-            a[v] *= r[v].A;
-            known[v] = r[v].tag == kState;
-          }
-          open |= !known[v];
-        }
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        sh.carry[c + v] = b[v];
-        if (tell && !cut && v < live) rec_store(recs + rank * P.D + v, 0.f, fmaf(p[v], b[v], q[v]), kState);
-      }
+    for (int v = 0; v < V; ++v) {
+      tp[v] = p[v], tq[v] = q[v], p[v] = ep[v], q[v] = eq[v];
+      if (tell && v < live) rec_store(recs + rank * P.D + v, tp[v], tq[v], cut || !wait ? kState : kMap);
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v) p[v] = BWD ? tp[v] : 1.f, q[v] = BWD ? tq[v] : 0.f;
   } else {
     if (BWD)
       for (int i = kWarps - 1; i > w; --i) through(i);
     else
       for (int i = 0; i < w; ++i) through(i);
   }
-  if (wait) __syncthreads();
+  if (wait) {
+    __syncthreads();
+    if (w == 0) {
+      float b[V];
+      int kept[V];       // maps between this item and the one whose state is b
+      bool known[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) b[v] = 0.f, kept[v] = 0, known[v] = v >= live;
+      int n = 0;
+      for (bool open = live > 0; open; ++n) {
+        const int at = rank - 1 - n;  // (item 0 always has a state)
+        const uint32_t least = n == Work<V, BWD>::kKept || at == 0 ? kState : kMap;
+        Rec r[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) r[v] = known[v] ? Rec{0.f, 0.f, kState, 0} : rec_load(recs + at * P.D + v);
+        open = false;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          if (known[v]) continue;
+          if (r[v].tag < least) r[v] = rec_wait(recs + at * P.D + v, least);
+          if (r[v].tag == kState) {
+            b[v] = r[v].B, kept[v] = n, known[v] = true;
+          } else {
+            sh.map[n][0][c + v] = r[v].A, sh.map[n][1][c + v] = r[v].B;
+            open = true;
+          }
+        }
+      }
+#pragma unroll 4
+      for (--n; n >= 0; --n)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float A = sh.map[n][0][c + v], B = sh.map[n][1][c + v];
+          if (n < kept[v]) b[v] = fmaf(A, b[v], B);
+        }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        sh.carry[c + v] = b[v];
+        if (tell && !cut && v < live) rec_store(recs + rank * P.D + v, 0.f, fmaf(tp[v], b[v], tq[v]), kState);
+      }
+    }
+    __syncthreads();
+  }
 #pragma unroll
   for (int v = 0; v < V; ++v) carry[v] = wait ? sh.carry[c + v] : 0.f;
 }
@@ -384,7 +412,7 @@ packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
                   const __grid_constant__ CUtensorMap tx) {
   constexpr int V = kV<T>, CH = 32 * V;
   extern __shared__ __align__(128) unsigned char dyn[];
-  __shared__ Work<V> sh;
+  __shared__ Work<V, false> sh;
   Feed<T, false, TMA> feed{dyn, sh, P, &ta, &tx, nullptr};
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, k0 = w * kSteps;
   if constexpr (TMA) {
@@ -424,7 +452,7 @@ packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
       }
     }
 #pragma unroll
-    for (int v = 0; v < V; ++v) sh.A[w][lane * V + v] = A[v], sh.B[w][lane * V + v] = B[v];
+    for (int v = 0; v < V; ++v) sh.map[w][0][lane * V + v] = A[v], sh.map[w][1][lane * V + v] = B[v];
     __syncthreads();
     const bool need = info.lo == 0 && info.hi > 0 && !(info.starts && (sh.mark[0] & kStart));
     float carry[V], p[V], q[V], h[V];
@@ -479,7 +507,7 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
                   const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tg) {
   constexpr int V = kV<T>, CH = 32 * V;
   extern __shared__ __align__(128) unsigned char dyn[];
-  __shared__ Work<V> sh;
+  __shared__ Work<V, true> sh;
   Feed<T, true, TMA> feed{dyn, sh, P, &ta, &tx, &tg};
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, k0 = w * kSteps;
   if constexpr (TMA) {
@@ -541,8 +569,8 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
       }
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        sh.fA[w][lane * V + v] = A[v], sh.fB[w][lane * V + v] = B[v];
-        sh.A[w][lane * V + v] = C[v], sh.B[w][lane * V + v] = Q[v];
+        sh.fmap[w][0][lane * V + v] = A[v], sh.fmap[w][1][lane * V + v] = B[v];
+        sh.map[w][0][lane * V + v] = C[v], sh.map[w][1][lane * V + v] = Q[v];
       }
     }
     __syncthreads();
@@ -554,7 +582,7 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
     for (int v = 0; v < V; ++v) {
       r[v] = enter(p[v], q[v], carry[v], cut);
       for (int i = 0; i < w; ++i) {
-        const float A = sh.fA[i][lane * V + v], B = sh.fB[i][lane * V + v];
+        const float A = sh.fmap[i][0][lane * V + v], B = sh.fmap[i][1][lane * V + v];
         h[v] = info.starts >> i & 1 ? B : fmaf(A, h[v], B);
       }
     }
