@@ -19,21 +19,28 @@
 // uniform. The backward runs the same scheme from the right, and rebuilds h from
 // the states that the forward kept per chunk.
 //
-// Composed maps need products of gates that stay in float32's range: |a| <= 1
-// always does, larger gates as long as their products along a sequence do.
+// A product of gates above one may leave float32's range where the recurrence does not
+// (a state of zero under a = 2). A channel whose composed map is not finite publishes no
+// map, and its state only from the item's last step; a warp whose entering state comes out
+// as not finite computes it again step by step (walk_h, walk_both). Inputs that hold
+// infinities or NaN pay for it too, in their channels: with NaN everywhere the two sizes
+// below take 1.4 and 3.8 ms, 9.3 and 18.5 ms, since their chunks then run one after the
+// other. (Products that fall below float32's smallest number count as zero: what a state
+// contributes 1e38 times smaller than itself is dropped.)
 //
-// bf16, T=32768, D=2560, 24 sequences: forward 140 us (4.8 TB/s of the 8 bytes an
+// bf16, T=32768, D=2560, 24 sequences: forward 144 us (4.7 TB/s of the 8 bytes an
 // element needs), backward 233 us (4.3 TB/s of 12 bytes); fp16, T=131072, D=512, one
-// sequence: 142 and 197 us. What is left is the wait for the items before, so nothing
-// delays an item that others wait for. The look-back keeps the maps it meets and applies
-// them in the items' order; composing them newest first took 138 and 224 us (128 and
-// 186), but its bits varied with the timing, and reading them a second time instead of
-// keeping them took 148 and 232 us (365 and 390). Eight maps kept in the forward instead
-// of sixteen: 140 us (171). Measured before, beside 138 and 224 us at the first size:
-// tickets taken a stage ahead of the data 182 and 304 us; a plain loop for the steps at
-// borders 227 us; rounds of 4 (8) records of the look-back in place of 1: 160 and 268 us
-// (199 and 343), since they read maps that are not there yet where a state is about to
-// come.
+// sequence: 144 and 202 us. What is left is the wait for the items before, so nothing
+// delays an item that others wait for: a branch around the stores of the records instead
+// of a tag that says "not there yet" takes 147 and 235 us (148 and 207). The look-back
+// keeps the maps it meets and applies them in the items' order; composing them newest
+// first took 138 and 224 us (128 and 186), but its bits varied with the timing, and reading
+// them a second time instead of keeping them took 148 and 232 us (365 and 390). Eight maps
+// kept in the forward instead of sixteen: 140 us (171), where sixteen took 140 (142).
+// Measured before, beside 138 and 224 us at the first size: tickets taken a stage ahead of
+// the data 182 and 304 us; a plain loop for the steps at borders 227 us; rounds of 4 (8)
+// records of the look-back in place of 1: 160 and 268 us (199 and 343), since they read
+// maps that are not there yet where a state is about to come.
 #include "common.cuh"
 #include "launch.cuh"
 #include "tma.cuh"
@@ -50,10 +57,10 @@ constexpr int kChunk = kWarps * kSteps;  // steps of an item
 // load to the words that are used, which is then no longer one access) counts as not there yet.
 struct alignas(16) Rec {
   float A, B;    // kMap: state out = A state in + B; kState: state out = B
-  uint32_t tag;  // 0: not there yet
+  uint32_t tag;  // kNone: not there yet
   uint32_t sum;
 };
-enum : uint32_t { kMap = 1, kState = 2 };
+enum : uint32_t { kNone = 0, kMap = 1, kState = 2 };
 
 __device__ __forceinline__ void rec_store(Rec* p, float A, float B, uint32_t tag) {
   const uint32_t a = __float_as_uint(A), b = __float_as_uint(B);
@@ -307,6 +314,67 @@ template <int V> __device__ __forceinline__ void begin(const float* state, int s
   for (int i = 0; i < V; ++i) v[i] = state && i < live ? state[s * D + ch + i] : 0.f;
 }
 
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
+
+// What enters this warp's steps, where the composed maps gave something that is not finite: through the steps of the
+// warps before it, one by one. From the left out of shared memory; from the right with gy from global memory (in
+// shared memory adj takes its place), eight steps ahead. All channels of the lane in one call that finds its data in
+// sh, P and the stages, so that the call costs those that do not make it little.
+template <int V> struct Lane {
+  float v[V];
+};
+template <typename T, int V, bool BWD>
+__device__ __noinline__ Lane<V> walk_h(const Work<V, BWD>& sh, const PackedArgs& P, const unsigned char* stage, Lane<V> from, Lane<V> got) {
+  constexpr int CH = 32 * V;
+  const int c = (threadIdx.x & 31) * V, end = min(sh.info.hi, (int)(threadIdx.x >> 5) * kSteps);
+  const T *a = reinterpret_cast<const T*>(stage) + c, *x = a + kChunk * CH;
+  const int64_t ch = (int64_t)(sh.item % P.ntile) * CH + c;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    if (finite(got.v[v]) || ch + v >= P.D) continue;
+    float h = from.v[v];
+    for (int k = sh.info.lo; k < end; ++k) {
+      if (sh.info.starts != 0 && (sh.mark[k] & kStart)) h = P.h0 ? P.h0[seq_at(sh.mark, k, P.S) * P.D + ch + v] : 0.f;
+      h = fmaf(to_f(a[k * CH + v]), h, to_f(x[k * CH + v]));
+    }
+    got.v[v] = h;
+  }
+  return got;
+}
+template <int V> struct Both {
+  Lane<V> h, r;
+};
+template <typename T, int V>
+__device__ __noinline__ Both<V> walk_both(const Work<V, true>& sh, const PackedArgs& P, const unsigned char* stage, Lane<V> carry, Lane<V> h, Lane<V> r) {
+  constexpr int CH = 32 * V;
+  const int c = (threadIdx.x & 31) * V, beg = max(sh.info.lo, (int)(threadIdx.x >> 5) * kSteps + kSteps);
+  const T* a = reinterpret_cast<const T*>(stage) + c;
+  const int64_t ch = (int64_t)(sh.item % P.ntile) * CH + c, chunk = P.nchunk - 1 - sh.item / P.ntile;
+  Lane<V> ckpt = {};
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    if (ch + v >= P.D) continue;
+    ckpt.v[v] = P.ckpt[chunk * P.D + ch + v];
+    if (finite(r.v[v])) continue;
+    const float* gy = P.gy + chunk * kChunk * P.D + ch + v;
+    float s = carry.v[v];
+    for (int k0 = sh.info.hi; k0 > beg; k0 -= 8) {
+      float g[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[i] = gy[max(k0 - 1 - i, beg) * P.D];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int k = k0 - 1 - i;
+        if (k < beg) break;
+        if (sh.info.ends != 0 && (sh.mark[k] & kEnd)) s = P.gf ? P.gf[seq_at(sh.mark, k, P.S) * P.D + ch + v] : 0.f;
+        s = to_f(a[k * CH + v]) * (g[i] + s);
+      }
+    }
+    r.v[v] = s;
+  }
+  return {walk_h<T, V, true>(sh, P, stage, ckpt, h), r};
+}
+
 // The chain. Along it (left to right in the forward, right to left in the
 // backward) item `rank` of a channel tile follows rank - 1. Composes the warps'
 // maps in sh.map (bit w of `cut`: warp w's steps hold a border, so its
@@ -318,89 +386,111 @@ template <int V> __device__ __forceinline__ void begin(const float* state, int s
 // on the way in the items' order, with the fmaf that the items themselves apply:
 // the bits do not depend on how far the others have come. Maps wait in the place of
 // sh.map, which every warp has read by then; behind kKept of them a state is waited for.
+//
+// The chain's last warp does it, which composes the whole item on its way and ends in
+// the state that the item hands on. A map or state that is not finite is published as not
+// there yet (a store without a branch: the others wait for it): for these channels (bits of
+// `late`, in that warp) publish_late does it.
 template <int V, bool BWD>
 __device__ __forceinline__ void chain(Work<V, BWD>& sh, const PackedArgs& P, int64_t ch, int live, int rank, uint32_t cut,
-                                      bool need, float (&carry)[V], float (&p)[V], float (&q)[V]) {
+                                      bool need, float (&carry)[V], float (&p)[V], float (&q)[V], uint32_t& late) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = lane * V;
+  constexpr int kLast = BWD ? 0 : kWarps - 1;
   const bool wait = need && rank > 0, tell = P.counter != nullptr && rank < P.nchunk - 1;
   Rec* recs = P.recs + ch;
-  float tp[V], tq[V];  // warp 0: the item's own map
-  auto through = [&](int i) {  // p, q <- the warps' maps up to and including warp i
+  float tp[V], tq[V];  // the last warp: the item's own map
+  auto through = [&](int i, const float(&p)[V], const float(&q)[V], float(&op)[V], float(&oq)[V]) {  // and warp i's map
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const float A = sh.map[i][0][c + v], B = sh.map[i][1][c + v];
-      q[v] = cut >> i & 1 ? B : fmaf(A, q[v], B);
-      p[v] = cut >> i & 1 ? 0.f : p[v] * A;
+      oq[v] = cut >> i & 1 ? B : fmaf(A, q[v], B);
+      op[v] = cut >> i & 1 ? 0.f : p[v] * A;
     }
   };
 #pragma unroll
   for (int v = 0; v < V; ++v) p[v] = 1.f, q[v] = 0.f;
-  if (w == 0) {
-    float ep[V], eq[V];  // what enters warp 0, in the backward the last on the chain
+  late = 0;
+  if (w == kLast) {
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      if (i == (BWD ? kWarps - 1 : 0)) {
+    for (int i = 0; i < kWarps - 1; ++i) through(BWD ? kWarps - 1 - i : i, p, q, p, q);
+    through(kLast, p, q, tp, tq);
+    if (tell) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) ep[v] = p[v], eq[v] = q[v];
+      for (int v = 0; v < V; ++v) {
+        const bool state = cut || !wait, good = finite(tq[v]) && (state || finite(tp[v]));
+        if (v < live) rec_store(recs + rank * P.D + v, tp[v], tq[v], !good ? kNone : state ? kState : kMap);
+        late |= (good ? 0u : 1u) << v;
       }
-      through(BWD ? kWarps - 1 - i : i);
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      tp[v] = p[v], tq[v] = q[v], p[v] = ep[v], q[v] = eq[v];
-      if (tell && v < live) rec_store(recs + rank * P.D + v, tp[v], tq[v], cut || !wait ? kState : kMap);
     }
   } else {
     if (BWD)
-      for (int i = kWarps - 1; i > w; --i) through(i);
+      for (int i = kWarps - 1; i > w; --i) through(i, p, q, p, q);
     else
-      for (int i = 0; i < w; ++i) through(i);
+      for (int i = 0; i < w; ++i) through(i, p, q, p, q);
   }
   if (wait) {
     __syncthreads();
-    if (w == 0) {
+    if (w == kLast) {
       float b[V];
-      int kept[V];       // maps between this item and the one whose state is b
-      bool known[V];
+      for (int keep = Work<V, BWD>::kKept;; keep = 0) {
+        int kept[V];  // maps between this item and the one whose state is b
+        bool known[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) b[v] = 0.f, kept[v] = 0, known[v] = v >= live;
-      int n = 0;
-      for (bool open = live > 0; open; ++n) {
-        const int at = rank - 1 - n;  // (item 0 always has a state)
-        const uint32_t least = n == Work<V, BWD>::kKept || at == 0 ? kState : kMap;
-        Rec r[V];
+        for (int v = 0; v < V; ++v) b[v] = 0.f, kept[v] = 0, known[v] = v >= live;
+        int n = 0;
+        for (bool open = live > 0; open; ++n) {
+          const int at = rank - 1 - n;  // (item 0 always has a state)
+          const uint32_t least = n == keep || at == 0 ? kState : kMap;
+          Rec r[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) r[v] = known[v] ? Rec{0.f, 0.f, kState, 0} : rec_load(recs + at * P.D + v);
-        open = false;
+          for (int v = 0; v < V; ++v) r[v] = known[v] ? Rec{0.f, 0.f, kState, 0} : rec_load(recs + at * P.D + v);
+          open = false;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          if (known[v]) continue;
-          if (r[v].tag < least) r[v] = rec_wait(recs + at * P.D + v, least);
-          if (r[v].tag == kState) {
-            b[v] = r[v].B, kept[v] = n, known[v] = true;
-          } else {
-            sh.map[n][0][c + v] = r[v].A, sh.map[n][1][c + v] = r[v].B;
-            open = true;
+          for (int v = 0; v < V; ++v) {
+            if (known[v]) continue;
+            if (r[v].tag < least) r[v] = rec_wait(recs + at * P.D + v, least);
+            if (r[v].tag == kState) {
+              b[v] = r[v].B, kept[v] = n, known[v] = true;
+            } else {
+              sh.map[n][0][c + v] = r[v].A, sh.map[n][1][c + v] = r[v].B;
+              open = true;
+            }
           }
         }
-      }
 #pragma unroll 4
-      for (--n; n >= 0; --n)
+        for (--n; n >= 0; --n)
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float A = sh.map[n][0][c + v], B = sh.map[n][1][c + v];
-          if (n < kept[v]) b[v] = fmaf(A, b[v], B);
-        }
+          for (int v = 0; v < V; ++v) {
+            const float A = sh.map[n][0][c + v], B = sh.map[n][1][c + v];
+            if (n < kept[v]) b[v] = fmaf(A, b[v], B);
+          }
+        bool good = true;
+#pragma unroll
+        for (int v = 0; v < V; ++v) good &= finite(b[v]);
+        if (good || keep == 0) break;  // once not finite, always: then what the item before ended in decides
+      }
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         sh.carry[c + v] = b[v];
-        if (tell && !cut && v < live) rec_store(recs + rank * P.D + v, 0.f, fmaf(tp[v], b[v], tq[v]), kState);
+        const float out = fmaf(tp[v], b[v], tq[v]);
+        if (tell && !cut) {
+          if (v < live) rec_store(recs + rank * P.D + v, 0.f, out, finite(out) ? kState : kNone);
+          late = (late & ~(1u << v)) | (finite(out) ? 0u : 1u) << v;
+        }
       }
     }
     __syncthreads();
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) carry[v] = wait ? sh.carry[c + v] : 0.f;
+}
+
+template <int V>
+__device__ __forceinline__ void publish_late(const PackedArgs& P, int64_t ch, int live, int rank, uint32_t late, const float (&out)[V]) {
+  if (late == 0) return;
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (v < live && (late >> v & 1)) rec_store(P.recs + ch + rank * P.D + v, 0.f, out[v], kState);
 }
 
 // state entering the warp, from the one entering the item; a cut leaves p = 0 and q alone (0 x infinity would not)
@@ -427,6 +517,7 @@ packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
     const int64_t ch = (int64_t)(item % P.ntile) * CH + lane * V, t0 = (int64_t)chunk * kChunk;
     const int n = (int)min((int64_t)kChunk, P.L - t0), live = (int)min((int64_t)V, max((int64_t)0, P.D - ch));
     const ChunkInfo info = TMA ? sh.info : P.info ? P.info[chunk] : chunk_info(P.cu, P.S, t0, n);
+    if (!TMA && threadIdx.x == 0) sh.info = info;
     if (info.starts | info.ends) mark_borders(sh, info, P, t0, n);
     const bool plain = info.plain(w);
     const StepMasks mask = step_masks(sh.mark, info, w);
@@ -456,11 +547,22 @@ packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
     __syncthreads();
     const bool need = info.lo == 0 && info.hi > 0 && !(info.starts && (sh.mark[0] & kStart));
     float carry[V], p[V], q[V], h[V];
-    chain<V, false>(sh, P, ch, live, chunk, info.starts, need, carry, p, q);
+    uint32_t late;
+    chain<V, false>(sh, P, ch, live, chunk, info.starts, need, carry, p, q, late);
     const bool cut = info.starts & ((1u << w) - 1);
+    bool good = true;
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = enter(p[v], q[v], carry[v], cut), good &= finite(h[v]);
+    if (!good) {
+      Lane<V> from, got;
+#pragma unroll
+      for (int v = 0; v < V; ++v) from.v[v] = carry[v], got.v[v] = h[v];
+      got = walk_h<T>(sh, P, dyn, from, got);
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = got.v[v];
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      h[v] = enter(p[v], q[v], carry[v], cut);
       if (P.ckpt != nullptr && w == 0 && v < live && n > 0) P.ckpt[chunk * P.D + ch + v] = h[v];
     }
     float* y = P.y + (t0 + k0) * P.D + ch;
@@ -493,6 +595,7 @@ packed_fwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
         put<float, V>(y, out, P.vec, live);
       }
     }
+    publish_late(P, ch, live, chunk, late, h);
     if (P.fin != nullptr)  // empty sequences, spread over the chunks
       for (int s = (int)((int64_t)chunk * P.S / P.nchunk) + w; s < (int)((int64_t)(chunk + 1) * P.S / P.nchunk); s += kWarps)
         if (P.cu[s + 1] <= P.cu[s])
@@ -522,6 +625,7 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
     const int64_t ch = (int64_t)(item % P.ntile) * CH + lane * V, t0 = (int64_t)chunk * kChunk;
     const int n = (int)min((int64_t)kChunk, P.L - t0), live = (int)min((int64_t)V, max((int64_t)0, P.D - ch));
     const ChunkInfo info = TMA ? sh.info : P.info ? P.info[chunk] : chunk_info(P.cu, P.S, t0, n);
+    if (!TMA && threadIdx.x == 0) sh.info = info;
     float h[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = v < live && n > 0 ? P.ckpt[chunk * P.D + ch + v] : 0.f;
@@ -576,8 +680,10 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
     __syncthreads();
     const bool need = info.hi == n && info.hi > info.lo && !(info.ends && (sh.mark[n - 1] & kEnd));
     float carry[V], p[V], q[V], r[V];
-    chain<V, true>(sh, P, ch, live, rank, info.ends, need, carry, p, q);
+    uint32_t late;
+    chain<V, true>(sh, P, ch, live, rank, info.ends, need, carry, p, q, late);
     const bool cut = info.ends >> (w + 1);
+    bool good = true;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       r[v] = enter(p[v], q[v], carry[v], cut);
@@ -585,6 +691,16 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
         const float A = sh.fmap[i][0][lane * V + v], B = sh.fmap[i][1][lane * V + v];
         h[v] = info.starts >> i & 1 ? B : fmaf(A, h[v], B);
       }
+      good &= finite(r[v]) && finite(h[v]);
+    }
+    if (!good) {
+      Lane<V> from;
+      Both<V> got;
+#pragma unroll
+      for (int v = 0; v < V; ++v) from.v[v] = carry[v], got.h.v[v] = h[v], got.r.v[v] = r[v];
+      got = walk_both<T>(sh, P, dyn, from, got.h, got.r);
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = got.h.v[v], r[v] = got.r.v[v];
     }
     T *ga = (T*)P.ga + (t0 + k0) * P.D + ch, *gx = (T*)P.gx + (t0 + k0) * P.D + ch;
     if (plain) {
@@ -600,6 +716,7 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
         }
         *reinterpret_cast<Vec<float, V>*>(sg + k * CH) = gv;
       }
+      publish_late(P, ch, live, rank, late, r);
 #pragma unroll
       for (int k = 0; k < kSteps; ++k, ga += P.D, gx += P.D) {
         const Vec<T, V> av = ld_vec<T, V>(sa + k * CH), xv = ld_vec<T, V>(sx + k * CH);
@@ -632,6 +749,7 @@ packed_bwd_kernel(const __grid_constant__ PackedArgs P, const __grid_constant__ 
             if (v < live) P.gh0[at + v] = r[v];
         }
       }
+      publish_late(P, ch, live, rank, late, r);
 #pragma unroll
       for (int k = 0; k < kSteps; ++k, ga += P.D, gx += P.D) {
         if (k0 + k >= n) continue;

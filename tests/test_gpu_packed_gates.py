@@ -61,3 +61,76 @@ def test_gates_near_one_against_float64(mr, cuda_dev):
     a = 1 - 0.01 * torch.rand(T, D, generator=g)
     x, gy, h0, gf = (torch.randn(n, D, generator=g) for n in (T, T, 3, 3))
     _check(mr, *(t.to(cuda_dev) for t in (a, x, O.borders(lens), h0, gy, gf)))
+
+
+# ---- gates above one ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("D", [64, 33])  # (33: rows that no 16-byte copy takes)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("gate", [1.25, 3.0, -40.0, 1e4])
+def test_zero_state_under_growing_gates(mr, cuda_dev, gate, dtype, D):
+    """x, h0 and gf are zero and gy too but for the first tokens: everything the gates' products would multiply is
+    zero, so y is, and what little is not zero has the plain bounds."""
+    lens = [700, 130, 0, 900]
+    T, S, cu = sum(lens), len(lens), O.borders(lens).to(cuda_dev)
+    a = torch.full((T, D), gate, device=cuda_dev).to(dtype)
+    x, gy = torch.zeros(T, D, device=cuda_dev).to(dtype), torch.zeros(T, D, device=cuda_dev)
+    for lo in (0, 700, 830):
+        gy[lo:lo + 5] = torch.arange(1.0, 6.0, device=cuda_dev)[:, None]
+    z = torch.zeros(S, D, device=cuda_dev)
+    got = _grads(mr, a, x, cu, z, gy, z)
+    assert (got[0] == 0).all() and (got[1] == 0).all() and (got[2] == 0).all()
+    ga, gx, gh = O.scan_backward(a, x, cu, gy, z, z)
+    _, _, _, tx, th = O.scan_bounds(a, x, cu, gy, z, z)
+    r = 0.0 if dtype == torch.float32 else O.half_step(dtype)
+    O.check("grad_x", got[3], gx, tx + r * (gx.abs() + tx))
+    O.check("grad_h0", got[4], gh, th)
+
+
+@pytest.mark.parametrize("D", [64, 33])
+@pytest.mark.parametrize("start", [0, 60, 128, 200])
+def test_products_out_of_range_and_back(mr, cuda_dev, start, D):
+    """Gates of 2 for 150 tokens, then of 1/2 for 120: their product passes 2^128, the states stay between 2^-100 and
+    2^50, the adjoints between 2^-40 and 2^110. Powers of two: exact in every order. A sequence before it and one
+    behind it are ordinary."""
+    g = torch.Generator().manual_seed(43)
+    lens = [start, 270, 90]
+    T, cu = sum(lens), O.borders(lens)
+    a, x, gy = torch.rand(T, D, generator=g), torch.randn(T, D, generator=g), torch.randn(T, D, generator=g)
+    h0, gf = torch.randn(3, D, generator=g), torch.randn(3, D, generator=g)
+    mid = slice(start, start + 270)
+    a[mid], x[mid], gy[mid] = 0.5, 0.0, 0.0
+    a[start:start + 150] = 2.0
+    h0[1], gf[1] = 2.0 ** -100, 2.0 ** 80
+    # a channel of ordinary gates beside it, and one whose gates are all one
+    a[mid, 3], x[mid, 3], gy[mid, 3], h0[1, 3], gf[1, 3] = 0.9, 1.0, 1.0, 1.0, 1.0
+    a[mid, 5] = 1.0
+    got = _check(mr, *(t.to(cuda_dev) for t in (a, x, cu, h0, gy, gf)))
+    assert (got[1][1, 6:] == 2.0 ** -70).all() and (got[4][1, 6:] == 2.0 ** 110).all()
+    # adj_t h_t is the same for all t where gy and x are zero (2^80 2^-70), and grad_a_t = adj_t h_t / a_t
+    assert (got[2][mid, 6:].cpu() * a[mid, 6:] == 2.0 ** 10).all()
+
+
+def test_late_input_under_growing_gates(mr, cuda_dev):
+    """Zeros for 2800 tokens under gates of 1.05, then input for 200: the gates' product over the zeros, some 1e59,
+    multiplies nothing. The other way round for the adjoint."""
+    g = torch.Generator().manual_seed(44)
+    T, D = 3000, 40
+    a = torch.full((T, D), 1.05)
+    x, gy = torch.randn(T, D, generator=g), torch.randn(T, D, generator=g)
+    x[:2800], gy[200:] = 0.0, 0.0
+    z = torch.zeros(1, D)
+    _check(mr, *(t.to(cuda_dev) for t in (a, x, O.borders([T]), z, gy, z)))
+
+
+def test_states_that_overflow_are_infinite(mr, cuda_dev):
+    """y itself leaves float32's range: infinite from there on, finite and right before."""
+    T, D = 1000, 40
+    a, x = torch.full((T, D), 2.0, device=cuda_dev), torch.zeros(T, D, device=cuda_dev)
+    x[300] = 1.0  # 2^(t - 300) from here on
+    y = mr.rglru_scan_packed(a, x, torch.tensor([0, T], device=cuda_dev))
+    want = torch.zeros(T, dtype=torch.float64)
+    want[300:] = 2.0 ** torch.arange(700, dtype=torch.float64).clamp(max=1000)
+    want = want.float().to(cuda_dev)
+    assert torch.equal(y, want[:, None].expand(T, D))
