@@ -7,6 +7,7 @@ forward + all-gradient parity helper.
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 
@@ -111,6 +112,13 @@ def grad_out(g, shape, device):
     if g is None:
         return torch.zeros(shape, dtype=torch.float32, device=device)
     return g.to(torch.float32).contiguous()
+
+
+def wants_grad(*tensors):
+    """Whether a call on these (None is skipped) has to go through its autograd function: a gradient is wanted, or one
+    carries a forward-mode tangent, which the function refuses and a call past it would drop."""
+    grad = torch.is_grad_enabled()
+    return any(t is not None and ((grad and t.requires_grad) or unpack_dual(t).tangent is not None) for t in tensors)
 
 
 def parity_check(

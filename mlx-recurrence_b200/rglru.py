@@ -19,7 +19,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._chassis import (DEFAULT_SEG, check_segment_shape, common_dtype, grad_out, prep, prep_cu, prep_h0,
-                       step_state)
+                       step_state, wants_grad)
 
 
 class _RGLRUScan(torch.autograd.Function):
@@ -249,7 +249,7 @@ class _RGLRUPacked(torch.autograd.Function):
 
 
 def _packed(a, x, cu_seqlens, h0, want_final):
-    if torch.is_grad_enabled() and (a.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
+    if wants_grad(a, x, h0):
         return _RGLRUPacked.apply(a, x, cu_seqlens, h0, want_final)
     return _packed_forward(a, x, cu_seqlens, h0, want_final, False)[:2]
 

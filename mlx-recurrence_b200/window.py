@@ -21,7 +21,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._chassis import common_dtype, prep, prep_cu
+from ._chassis import common_dtype, prep, prep_cu, wants_grad
 
 MAX_SINKS = 64
 HEAD_DIMS = (32, 64, 96, 128)
@@ -145,7 +145,7 @@ class _WindowAttention(torch.autograd.Function):
 
 
 def _dispatch(q, k, v, cu, window, sinks, scale):
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if wants_grad(q, k, v):
         return _WindowAttention.apply(q, k, v, cu, window, sinks, scale)
     return _attend(q, k, v, cu, window, sinks, scale, False)[0]
 

@@ -5,6 +5,7 @@ that it does not have."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd_ad
 
 import _packed_oracle as O
 from _window_oracle import Window
@@ -47,3 +48,28 @@ def test_rows_outside_are_zero_beside_values_that_are_not_finite(mr, cuda_dev, w
     t[31], t[169] = bad, bad
     for name, g in zip(("y", "grad_q", "grad_k", "grad_v"), _step(mr, q, k, v, gy, cu, 40, 2)):
         assert (g[:30] == 0).all() and (g[170:] == 0).all(), name
+
+
+# ---- derivatives that there are none of --------------------------------------------------------
+
+
+def test_forward_mode_derivatives_are_refused(mr, cuda_dev):
+    """A tangent would be dropped without a word; the other scans refuse it too."""
+    q, k, v, gy, cu = _inputs(cuda_dev, [40], 2, 1, 32, torch.float32, seed=62)
+    a, x, h0 = torch.rand(40, 8, device=cuda_dev), torch.rand(40, 8, device=cuda_dev), torch.rand(1, 8, device=cuda_dev)
+
+    def dual(t):
+        return fwd_ad.make_dual(t, torch.ones_like(t))
+
+    with fwd_ad.dual_level():
+        for call in (lambda: mr.window_attention_packed(dual(q), k, v, cu, 8),
+                     lambda: mr.window_attention_packed(q, k, dual(v), cu, 8),
+                     lambda: mr.window_attention(q[None], dual(k[None]), v[None], 8),
+                     lambda: mr.rglru_scan_packed(dual(a), x, cu), lambda: mr.rglru_scan_packed(a, dual(x), cu),
+                     lambda: mr.rglru_scan_packed_with_state(a, x, cu, h0=dual(h0)),
+                     lambda: mr.rglru_scan(dual(a[None, :32].repeat(1, 1, 4)), x[None, :32].repeat(1, 1, 4))):
+            with pytest.raises(NotImplementedError):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                call()
+        assert mr.rglru_scan_packed(a, x, cu).shape == a.shape  # no tangent, no refusal
