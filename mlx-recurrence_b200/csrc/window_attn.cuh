@@ -197,9 +197,9 @@ template <int SH> int attn_sink_sum_launch(const AttnArgs& A, cudaStream_t st) {
 // ---- exact rows --------------------------------------------------------------
 // The tiled kernels multiply masked terms by zero, which an infinity or a NaN
 // that a row must not see (another sequence's, a later token's) turns into a
-// NaN. A row whose results are not finite is therefore computed again here, one
-// warp per row, from its visible keys (queries) alone: whatever non-finite value
-// then remains is the row's own. Slow (a shuffle reduction per pair), and only
+// NaN. A row whose results are not finite, or whose scores are all -infinity, is
+// therefore computed again here, one warp per row, from its visible keys (queries)
+// alone: whatever non-finite value then remains is the row's own. Slow (a shuffle reduction per pair), and only
 // ever reached by inputs that hold infinities or NaN.
 
 constexpr float kAttnLog2e = 1.4426950408889634f;

@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, DH <= 64 ? 2 : 1) attn_fwd_f32(const
       odd = fmaf(o[i][n], 0.f, odd);
     }
     if (A.lse != nullptr && tx == 0) A.lse[(int64_t)h * A.T + t] = l[i] == 0.f ? INFINITY : m[i] + log2f(l[i]);
-    if (live && odd != 0.f) again[ty * kR + i] = 1;
+    if (live && (odd != 0.f || l[i] == 0.f)) again[ty * kR + i] = 1;  // (l = 0: scores of -infinity alone)
   }
   __syncthreads();
   for (int r = threadIdx.x >> 5; r < kBT; r += kThreads / 32)

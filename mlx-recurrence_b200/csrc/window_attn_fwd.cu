@@ -290,7 +290,8 @@ attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUte
         }
     }
     if (i < A.T && A.lse != nullptr) A.lse[(int64_t)h * A.T + i] = rm.i < 0 || l == 0.f ? INFINITY : m * c + log2f(l);
-    const uint32_t again = __ballot_sync(0xffffffffu, rm.i >= 0 && odd != 0.f);
+    // l = 0: nothing but scores of -infinity, whose softmax is the row's own NaN
+    const uint32_t again = __ballot_sync(0xffffffffu, rm.i >= 0 && (odd != 0.f || l == 0.f));
     __syncwarp();
     for (int r = 0; r < 32 && again; ++r)
       if (again >> r & 1) exact_fwd_row<T>(A, h, q0 + w * 32 + r);

@@ -50,6 +50,43 @@ def test_rows_outside_are_zero_beside_values_that_are_not_finite(mr, cuda_dev, w
         assert (g[:30] == 0).all() and (g[170:] == 0).all(), name
 
 
+# ---- rows that every visible key gives minus infinity ------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", sorted(DT))
+def test_scores_of_minus_infinity_alone_give_nan(mr, cuda_dev, dtype):
+    """softmax of nothing but -inf is NaN: in y, in lse's row of the gradients, and nowhere else."""
+    lens, at = [50, 200], 140
+    q, k, v, gy, cu = _inputs(cuda_dev, lens, 2, 1, 64, DT[dtype], seed=52)
+    W = Window(q, k, v, cu, 1, 0, gy)
+    q[at], k[at] = 1.0, -float("inf")
+    got = _step(mr, q, k, v, gy, cu, 1, 0)
+    rest = torch.arange(250, device=cuda_dev) != at
+    for t in got:
+        assert torch.isnan(t[at]).all() and torch.isfinite(t[rest]).all()
+    O.check("y", got[0][rest], W.y[rest], W.tol_y[rest])
+    # a first token that sees only itself, and rows behind it that give it no weight
+    q, k, v, gy, cu = _inputs(cuda_dev, lens, 2, 1, 64, DT[dtype], seed=53)
+    q.abs_()
+    k[50] = -float("inf")
+    y = mr.window_attention_packed(q, k, v, cu, 3)
+    assert torch.isnan(y[50]).all() and torch.isfinite(y[:50]).all() and torch.isfinite(y[51:]).all()
+    assert torch.equal(y, mr.window_attention_packed(q, k, v, cu, 3, sinks=1)) is False  # (NaN is not equal to itself)
+    # the decode step says the same
+    pos = torch.zeros(1, dtype=torch.long, device=cuda_dev)
+    ck, cv = (torch.zeros(1, 4, 1, 64, dtype=DT[dtype], device=cuda_dev) for _ in range(2))
+    y = mr.window_attention_step(q[50:51], k[50:51], v[50:51], ck, cv, pos)
+    assert torch.isnan(y).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_finite_inputs_whose_scores_overflow(mr, cuda_dev, dtype):
+    q, k, v, gy, cu = _inputs(cuda_dev, [3], 1, 1, 32, DT[dtype], seed=54)
+    q[0], k[0] = 1e25, -1e25
+    y = mr.window_attention_packed(q, k, v, cu, 1)
+    assert torch.isnan(y[0]).all() and torch.equal(y[1:], v[1:])
+
+
 # ---- derivatives that there are none of --------------------------------------------------------
 
 
