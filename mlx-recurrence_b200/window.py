@@ -180,10 +180,9 @@ def window_attention_packed(q, k, v, cu_seqlens, window, sinks=0, scale=None):
     return _dispatch(q, k, v, cu_seqlens, window, sinks, scale)
 
 
-def _caches(k, v, cu, window, sinks):
+def _caches(k, v, dt, cu, window, sinks):
     packed = k.dim() == 3
     dev = k.device
-    dt = common_dtype(k, v)
     S, L = (cu.numel() - 1, 0) if packed else k.shape[:2]
     (k_, *ks), (v_, *vs) = (_rows(t.detach(), dt, packed) for t in (k, v))
     T, Hkv, Dh = k_.shape
@@ -197,18 +196,18 @@ def _caches(k, v, cu, window, sinks):
 
 def window_attention_with_state(q, k, v, window, sinks=0, scale=None):
     """:func:`window_attention` that also returns the caches a decode loop
-    starts from: cache_k, cache_v [B, sinks + window, Hkv, Dh] in the inputs'
-    dtype. Token t lies in slot t (t < sinks) or sinks + (t - sinks) % window;
-    unused slots are zero. The caches are state, not differentiable."""
+    starts from: cache_k, cache_v [B, sinks + window, Hkv, Dh] in y's dtype.
+    Token t lies in slot t (t < sinks) or sinks + (t - sinks) % window; unused
+    slots are zero. The caches are state, not differentiable."""
     y = window_attention(q, k, v, window, sinks, scale)
-    return (y, *_caches(k, v, None, operator.index(window), operator.index(sinks)))
+    return (y, *_caches(k, v, y.dtype, None, operator.index(window), operator.index(sinks)))
 
 
 def window_attention_packed_with_state(q, k, v, cu_seqlens, window, sinks=0, scale=None):
     """:func:`window_attention_packed` that also returns every sequence's caches
     [S, sinks + window, Hkv, Dh] (see :func:`window_attention_with_state`)."""
     y = window_attention_packed(q, k, v, cu_seqlens, window, sinks, scale)
-    return (y, *_caches(k, v, cu_seqlens, operator.index(window), operator.index(sinks)))
+    return (y, *_caches(k, v, y.dtype, cu_seqlens, operator.index(window), operator.index(sinks)))
 
 
 def window_attention_step(q, k, v, cache_k, cache_v, pos, sinks=0, scale=None):

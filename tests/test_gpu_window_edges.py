@@ -87,6 +87,20 @@ def test_finite_inputs_whose_scores_overflow(mr, cuda_dev, dtype):
     assert torch.isnan(y[0]).all() and torch.equal(y[1:], v[1:])
 
 
+# ---- mixed types -------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("qd,kd", [("f32", "bf16"), ("bf16", "f32"), ("fp16", "bf16")])
+def test_caches_of_mixed_types_serve_the_step(mr, cuda_dev, qd, kd):
+    """Caches come in the common dtype of q, k and v, which is what the step asks for."""
+    q, k, v, _, cu = _inputs(cuda_dev, [9, 30], 4, 2, 32, torch.float32, seed=61)
+    q, k, v = q.to(DT[qd]), k.to(DT[kd]), v.to(DT[kd])
+    y, ck, cv = mr.window_attention_packed_with_state(q, k, v, cu, 12, sinks=2)
+    assert ck.dtype == cv.dtype == y.dtype == torch.promote_types(DT[qd], DT[kd])
+    pos = torch.tensor([9, 30], device=cuda_dev)
+    assert mr.window_attention_step(q[:2], k[:2], v[:2], ck, cv, pos, sinks=2).dtype == y.dtype
+
+
 # ---- derivatives that there are none of --------------------------------------------------------
 
 
