@@ -451,7 +451,7 @@ int mr_window_cache(const void* k, const void* v, int64_t k_ts, int64_t k_hs, in
   if (S < 0 || T < 0 || T > INT32_MAX / 2 || S > INT32_MAX / 2 || Hkv <= 0 || Dh <= 0 || Dh % 32 != 0 ||
       sinks < 0 || slots <= sinks || slots > (1 << 30))
     return set_error(MR_E_SHAPE, "%s: bad shape (Dh a multiple of 32, slots > sinks >= 0)", what);
-  if (cu_seqlens == nullptr && (L <= 0 || S * L != T))
+  if (cu_seqlens == nullptr && (L < 0 || S * L != T))
     return set_error(MR_E_SHAPE, "%s: without cu_seqlens T must be S * L", what);
   if (S == 0) return MR_OK;
   for (const void* p : {k, v, (const void*)cache_k, (const void*)cache_v})

@@ -101,6 +101,18 @@ def test_caches_of_mixed_types_serve_the_step(mr, cuda_dev, qd, kd):
     assert mr.window_attention_step(q[:2], k[:2], v[:2], ck, cv, pos, sinks=2).dtype == y.dtype
 
 
+# ---- empty rows --------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_dense_batch_of_empty_rows(mr, cuda_dev, dtype):
+    z = torch.zeros(3, 0, 2, 64, dtype=DT[dtype], device=cuda_dev)
+    y, ck, cv = mr.window_attention_with_state(z, z, z, 7, sinks=2)
+    assert y.shape == z.shape and ck.shape == cv.shape == (3, 9, 2, 64) and (ck == 0).all() and (cv == 0).all()
+    none = torch.zeros(0, 5, 2, 64, dtype=DT[dtype], device=cuda_dev)
+    assert mr.window_attention_with_state(none, none, none, 7)[1].shape == (0, 7, 2, 64)
+
+
 # ---- derivatives that there are none of --------------------------------------------------------
 
 
