@@ -122,8 +122,11 @@ __global__ void __launch_bounds__(32 * kF32Warps) window_step_f32(const __grid_c
 // memory by asynchronous copies kRing tiles ahead; a warp takes 16 slots of a tile
 // with its own online softmax. Warps, then CTAs (over distributed shared memory)
 // join their maxima, sums and outputs in a fixed order; one launch, no workspace.
-// B=96, 16 heads of 128 on 4, 2052 slots: 66 us, 6.1 TB/s of the caches' bytes; B=1,
-// 8 heads of 64 on 2, 516 slots: 6 us, a launch and a few dependent loads.
+// P goes into its product in two parts, rounded to the inputs' type and what that
+// drops, so its rounding is squared (y's error was 1.2 times that of rounding y alone).
+// B=96, 16 heads of 128 on 4, 2052 slots: 67 us, 6.0 TB/s of the caches' bytes (66 with
+// the first part alone); B=1, 8 heads of 64 on 2, 516 slots: 6.3 us (6.1), a launch and a
+// few dependent loads.
 
 constexpr int kTile = 64, kRing = 2;
 
@@ -138,6 +141,7 @@ template <> struct Mma<__nv_bfloat16> {
     __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&r);
   }
+  static __device__ float2 unpack(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
 };
 template <> struct Mma<__half> {
   static __device__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -149,6 +153,7 @@ template <> struct Mma<__half> {
     __half2 r = __floats2half2_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&r);
   }
+  static __device__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 };
 
 template <bool TRANS> __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -244,7 +249,7 @@ __global__ void __launch_bounds__(128) window_step_mma(const __grid_constant__ S
       Mma<T>::run(s[0], q[k], f[0], f[1]);
       Mma<T>::run(s[1], q[k], f[2], f[3]);
     }
-    uint32_t pa[4];
+    uint32_t pa[4], pb[4];  // P in the inputs' type, and what that rounding drops
 #pragma unroll
     for (int r = 0; r < 2; ++r) {  // rows lane / 4 and + 8
       float mx = m[r];
@@ -266,17 +271,26 @@ __global__ void __launch_bounds__(128) window_step_mma(const __grid_constant__ S
         v = exp2f(v - to);
         l[r] += v;
       }
-      pa[r] = Mma<T>::pack(s[0][r * 2], s[0][r * 2 + 1]);
-      pa[r + 2] = Mma<T>::pack(s[1][r * 2], s[1][r * 2 + 1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float p0 = s[i][r * 2], p1 = s[i][r * 2 + 1];
+        pa[r + 2 * i] = Mma<T>::pack(p0, p1);
+        const float2 back = Mma<T>::unpack(pa[r + 2 * i]);
+        pb[r + 2 * i] = Mma<T>::pack(p0 - back.x, p1 - back.y);
+      }
 #pragma unroll
       for (int i = 0; i < NC; ++i) o[i][r * 2] *= keep, o[i][r * 2 + 1] *= keep;
     }
 #pragma unroll
-    for (int i = 0; i < NC; i += 2) {
-      uint32_t f[4];
-      ldmatrix4<true>(f, sv + chunk_at<DH>(s0 + (lane >> 3 & 1) * 8 + (lane & 7), i + (lane >> 4)) * 16);
-      Mma<T>::run(o[i], pa, f[0], f[1]);
-      Mma<T>::run(o[i + 1], pa, f[2], f[3]);
+    for (int i = 0; i < NC; i += 4) {
+      uint32_t f[2][4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        ldmatrix4<true>(f[x], sv + chunk_at<DH>(s0 + (lane >> 3 & 1) * 8 + (lane & 7), i + 2 * x + (lane >> 4)) * 16);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) Mma<T>::run(o[i + x], pa, f[x >> 1][(x & 1) * 2], f[x >> 1][(x & 1) * 2 + 1]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) Mma<T>::run(o[i + x], pb, f[x >> 1][(x & 1) * 2], f[x >> 1][(x & 1) * 2 + 1]);
     }
   }
   // join the warps: the ring's memory is free
@@ -338,7 +352,7 @@ template <typename T, int DH> static int step_mma_dh(const StepArgs& A, cudaStre
   const int G = A.Hq / A.Hkv, head_tiles = (G + 15) / 16, tiles = (A.slots + kTile - 1) / kTile;
   const int64_t units = (int64_t)A.B * A.Hkv * head_tiles;
   // CTAs for two on every SM (three fit: one wave), each with two tiles at least. At B=96, Hkv=4, Dh=128, 2052 slots:
-  // 66 us unsplit, 76 in two, 85 in four (later waves leave SMs idle); at B=8: 12 us in eight
+  // 66 us unsplit, 76 in two, 85 in four (later waves leave SMs idle); at B=8: 13 us in eight
   int splits = 1;
   while (splits < 8 && units * splits < 148 * 2 && splits * 4 <= tiles) splits *= 2;
   auto kernel = window_step_mma<T, DH>;

@@ -164,7 +164,9 @@ def window_attention(q, k, v, window, sinks=0, scale=None):
     Returns:
         y: [B, L, Hq, Dh] in the inputs' common dtype (float32, bfloat16 or
         float16); differentiable in q, k, v. Scores, softmax statistics and
-        sums are float32. A key that a query does not see has no influence on
+        sums are float32; for 16-bit inputs the probabilities, and in the
+        backward the scores' gradients, are rounded to the inputs' dtype for
+        the tensor cores' products. A key that a query does not see has no influence on
         its row, even if it holds infinities or NaN. Slices of a fused
         projection are read in place.
     """
@@ -225,7 +227,8 @@ def window_attention_step(q, k, v, cache_k, cache_v, pos, sinks=0, scale=None):
         sinks, scale: as in :func:`window_attention`.
 
     Returns:
-        y: [B, Hq, Dh] in the inputs' dtype. Not differentiable.
+        y: [B, Hq, Dh] in the inputs' dtype. Not differentiable. (Its products
+        take the probabilities' rounding along, unlike the other forms'.)
     """
     dims = "[B, H, Dh]"
     B, Hq, Dh = q.shape if q.dim() == 3 else (0, 0, 0)

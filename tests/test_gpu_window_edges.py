@@ -87,6 +87,27 @@ def test_finite_inputs_whose_scores_overflow(mr, cuda_dev, dtype):
     assert torch.isnan(y[0]).all() and torch.equal(y[1:], v[1:])
 
 
+# ---- the decode step's own precision -----------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("Hq,Hkv,Dh", [(4, 2, 64), (5, 1, 128), (2, 2, 96)])
+def test_step_does_not_round_the_probabilities(mr, cuda_dev, Hq, Hkv, Dh, dtype):
+    """The probabilities' rounding is carried along: what is left is its square and the rounding of y."""
+    B, n, dt = 3, 300, DT[dtype]
+    g = torch.Generator().manual_seed(60)
+    q, k, v = (torch.randn(B, h, Dh, generator=g).to(dt).to(cuda_dev) for h in (Hq, Hkv, Hkv))
+    ck, cv = (torch.randn(B, n, Hkv, Dh, generator=g).to(dt).to(cuda_dev) for _ in range(2))
+    pos = torch.tensor([n - 1, 200, 5 * n], device=cuda_dev)
+    y = mr.window_attention_step(q, k, v, ck, cv, pos)
+    for b, p in enumerate(pos.tolist()):
+        m = min(p + 1, n)
+        qq = torch.zeros(m, Hq, Dh, dtype=dt, device=cuda_dev)
+        qq[-1] = q[b]
+        W = Window(qq, ck[b, :m], cv[b, :m], torch.tensor([0, m]), m, 0, r=O.half_step(dt) ** 2)
+        O.check(f"y at position {p}", y[b], W.y[-1], W.tol_y[-1])
+
+
 # ---- mixed types -------------------------------------------------------------------------------
 
 
