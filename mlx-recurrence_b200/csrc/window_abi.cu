@@ -9,7 +9,7 @@ int attn_bwd_f32_launch(const AttnArgs&, void* ws, cudaStream_t);
 size_t attn_bwd_f32_ws_bytes(int64_t T, int64_t Hq, int64_t Dh, int64_t sinks);
 template <typename T> int attn_fwd_launch(const AttnArgs&, cudaStream_t);
 template <typename T> int attn_bwd_launch(const AttnArgs&, void*, cudaStream_t);
-size_t attn_bwd_ws_bytes(int64_t T, int64_t Hq, int64_t Dh, int64_t sinks);
+size_t attn_bwd_ws_bytes(bool half, int64_t T, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t sinks);
 
 static int attn_check(const char* what, const AttnArgs& A, int64_t S, int64_t L, int dtype, int64_t T, int64_t Hq,
                       int64_t Hkv, int64_t Dh, int64_t window, int64_t sinks) {
@@ -84,7 +84,7 @@ int mr_window_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ts
 
 size_t mr_window_attn_bwd_workspace_bytes(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t sinks) {
   if (T <= 0 || Hq <= 0 || Hkv <= 0 || Dh <= 0 || sinks < 0) return 0;
-  return dtype == MR_F32 ? attn_bwd_f32_ws_bytes(T, Hq, Dh, sinks) : attn_bwd_ws_bytes(T, Hq, Dh, sinks);
+  return dtype == MR_F32 ? attn_bwd_f32_ws_bytes(T, Hq, Dh, sinks) : attn_bwd_ws_bytes(dtype == MR_F16, T, Hq, Hkv, Dh, sinks);
 }
 
 int mr_window_attn_bwd(const void* grad_y, const void* y, const void* y_low, const float* lse, const void* q,

@@ -21,9 +21,11 @@
 // under the dS arithmetic, the next S follows as soon as P (KV = false: S) has
 // been read, the next dP after dS C1.
 //
-// P and dS are rounded to the inputs' type, which the products take (fp16: dS at a
-// power-of-two scale of max |gy|, so that neither large nor small loss scales leave
-// its range); lse, delta and the sums are float32.
+// P and dS are rounded to the inputs' type, which the products take; lse, delta and the
+// sums are float32. In fp16 dS goes in at a power of two of each row's own (a query's, or
+// a key's), taken from a bound of what the row can meet, |dS_ij| <= |gy_i| |v_j| + |delta_i|
+// over the j it sees (the i that see it): nothing leaves fp16's range whatever the loss
+// scale, and no other sequence, head or token out of reach costs it precision.
 //
 // bf16, 16384 tokens, 32 heads of 64, window 1024: 824 us (391 TFLOP/s of the 5
 // products); 16 heads of 128 on 4, window 2048, 4 sinks: 772 us (480). Measured and
@@ -46,20 +48,13 @@ template <int NB> constexpr int kBwdThreads = kNS<NB> * 128 + 32;
 
 struct BwdArgs {
   AttnArgs a;
-  const uint32_t* amax;  // fp16: the largest finite |gy| as float bits
+  const float *fq, *fk;  // fp16: [Hq, T], [Hkv, T], dS's scale per query and per key
 };
-
-// fp16 keeps dS near one: a power of two of the size of gy comes out of it and back in at the end
-template <typename T> __device__ __forceinline__ float ds_factor(const uint32_t*) { return 1.f; }
-template <> __device__ __forceinline__ float ds_factor<__half>(const uint32_t* amax) {
-  const uint32_t e = *amax >> 23;  // 0 for gy = 0
-  return e == 0 || e > 250 ? 1.f : __uint_as_float((254 - e) << 23);
-}
 
 struct BwdShared {
   uint64_t r_full, c_full[kStages], s_done[2], dp_done[2], p_ready[2], ds_ready[2], acc2_done, acc1_done, all_done, sink_done, sink_read;
   uint32_t tmem;
-  int lo_max, lim_min;
+  int lo_max, lim_min, f_min;
   int again[128];
   alignas(16) float lse[2][kNC], delta[2][kNC];  // negated, of the column tile's queries
 };
@@ -115,7 +110,7 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
     mbar_init(&sh.acc1_done, 1), mbar_init(&sh.acc2_done, 1), mbar_init(&sh.all_done, 1);
     mbar_init(&sh.sink_done, 1), mbar_init(&sh.sink_read, 128);
     fence_mbar_init();
-    sh.lo_max = 0, sh.lim_min = INT32_MAX;
+    sh.lo_max = 0, sh.lim_min = INT32_MAX, sh.f_min = 0x7f000000;
   }
   if (tid < 128) sh.again[tid] = 0;
   if (w == 4 * NS) {
@@ -240,7 +235,8 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
   } else {
     const int wg = w >> 2, row = tid & 127, r = r0 + row;
     const uint32_t trow = tm + ((uint32_t)((w & 3) * 32) << 16);
-    const float c = A.scale * kAttnLog2e, f = ds_factor<T>(P.amax);
+    const float c = A.scale * kAttnLog2e;
+    float f = 1.f;  // dS's scale
     // what the row sees: columns [lo, hi) and (queries) sinks [s_lo, s_hi)
     int lo = INT32_MAX, hi = 0, s_lo = INT32_MAX, s_hi = 0;
     float lse_r = INFINITY, delta_r = 0.f;
@@ -251,6 +247,7 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
       if (alive) {
         lo = r;
         atomicMin(&sh.lim_min, hi);
+        if (Fmt<T>::id == 0) f = P.fk[(int64_t)hr * A.T + r];
       }
     } else {
       const RowMask m = row_mask(A, r);
@@ -259,10 +256,16 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
         lo = m.lo, hi = r + 1, s_lo = m.start, s_hi = min(m.sink_end, r + 1);
         lse_r = A.lse[(int64_t)hr * A.T + r], delta_r = A.delta[(int64_t)hr * A.T + r];
         atomicMax(&sh.lo_max, lo);
+        if (Fmt<T>::id == 0) {
+          f = P.fq[(int64_t)hr * A.T + r];
+          if (nsink && m.start == s0) atomicMin(&sh.f_min, __float_as_int(f));
+        }
       }
     }
     asm volatile("bar.sync 1, %0;" ::"n"(NS * 128) : "memory");
     const int lo_max = sh.lo_max, lim_min = sh.lim_min;
+    // the sinks' sums need one scale for all queries that see them
+    auto f_sink = [&] { return Fmt<T>::id == 0 ? __int_as_float(*reinterpret_cast<volatile int*>(&sh.f_min)) : 1.f; };
     if (!KV && nsink && r0 + 128 > end) {
       // queries behind the last sequence may hold anything: they must not reach the sinks' sums as 0 x NaN
       mbar_wait(&sh.r_full, 0);
@@ -326,6 +329,7 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
       };
       auto to_ds = [&](auto masked) {
         ulonglong2 d4 = {};
+        [[maybe_unused]] uint32_t to_sink[4];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           uint32_t dp[32];
@@ -336,8 +340,18 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
             if (KV && j % 2 == 0) d4 = *reinterpret_cast<const ulonglong2*>(&sh.delta[wg][x * 32 + 2 * j]);
             const uint64_t d = KV ? (j % 2 ? d4.y : d4.x) : d2;
             uint64_t g = mul2(pair(s[x][2 * j], s[x][2 * j + 1]), add2(pair(dp[2 * j], dp[2 * j + 1]), d));
-            if (Fmt<T>::id == 0) g = mul2(g, f2);
             float g0, g1;
+            if constexpr (Fmt<T>::id == 0) {
+              if (!KV && masked && sink) {  // at the sinks' scale, to shared memory
+                const float fs = f_sink();
+                unpair(mul2(g, pair(fs, fs)), g0, g1);
+                to_sink[j & 3] = Fmt<T>::pack(see[x] >> (2 * j) & 1 ? g0 : 0.f, see[x] >> (2 * j + 1) & 1 ? g1 : 0.f);
+                if ((j & 3) == 3)
+                  *reinterpret_cast<uint4*>(sC + kStageBytes + kTileBytes + umma::sw128_off(row, x * 32 + (j & ~3) * 2)) =
+                      make_uint4(to_sink[0], to_sink[1], to_sink[2], to_sink[3]);
+              }
+              g = mul2(g, f2);
+            }
             unpair(g, g0, g1);
             if (masked) {  // not 0 x NaN of what the row does not see
               g0 = see[x] >> (2 * j) & 1 ? g0 : 0.f;
@@ -386,7 +400,8 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
           *reinterpret_cast<uint4*>(sp + umma::sw128_off(row, x * 8)) = make_uint4(p[x * 4], p[x * 4 + 1], p[x * 4 + 2], p[x * 4 + 3]);
-          *reinterpret_cast<uint4*>(sd + umma::sw128_off(row, x * 8)) = make_uint4(ds[x * 4], ds[x * 4 + 1], ds[x * 4 + 2], ds[x * 4 + 3]);
+          if (Fmt<T>::id != 0)
+            *reinterpret_cast<uint4*>(sd + umma::sw128_off(row, x * 8)) = make_uint4(ds[x * 4], ds[x * 4 + 1], ds[x * 4 + 2], ds[x * 4 + 3]);
         }
         fence_proxy_async_smem();
       }
@@ -405,13 +420,15 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
             umma::tmem_ld32(trow + kAcc2 + d, gv);
             umma::tmem_wait_ld(gk);
             umma::tmem_wait_ld(gv);
-            if (row < send - s0)
+            if (row < send - s0) {
+              const float back = 1.f / f_sink();
 #pragma unroll
               for (int j = 0; j < 32; j += 4) {
-                *reinterpret_cast<float4*>(pk + d + j) = make_float4(
-                    __uint_as_float(gk[j]) / f, __uint_as_float(gk[j + 1]) / f, __uint_as_float(gk[j + 2]) / f, __uint_as_float(gk[j + 3]) / f);
+                *reinterpret_cast<float4*>(pk + d + j) = make_float4(__uint_as_float(gk[j]) * back, __uint_as_float(gk[j + 1]) * back,
+                                                                     __uint_as_float(gk[j + 2]) * back, __uint_as_float(gk[j + 3]) * back);
                 *reinterpret_cast<uint4*>(pv + d + j) = make_uint4(gv[j], gv[j + 1], gv[j + 2], gv[j + 3]);
               }
+            }
           }
         }
         umma::fence_before_sync();
@@ -467,14 +484,12 @@ attn_bwd_kernel(const __grid_constant__ BwdArgs P, const __grid_constant__ CUten
 }
 
 // delta[h][t] = sum_d gy y with y and what its rounding dropped (from the rounded y alone the gradients' error is 1.55
-// times the output rounding's, so 1.4), zero for rows outside every sequence; fp16: the
-// largest finite |gy| (the order of an integer maximum does not matter). 8 lanes
-// per row, 16 bytes each at a time.
-template <typename T> __global__ void __launch_bounds__(256) attn_delta_kernel(const __grid_constant__ AttnArgs A, uint32_t* amax) {
+// times the output rounding's, so 1.4), zero for rows outside every sequence; fp16: norm[h][t] = |gy| over its finite
+// elements. 8 lanes per row, 16 bytes each at a time.
+template <typename T> __global__ void __launch_bounds__(256) attn_delta_kernel(const __grid_constant__ AttnArgs A, float* norm) {
   const int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
   const int sub = threadIdx.x & 7;
-  float s = 0.f;
-  uint32_t big = 0;
+  float s = 0.f, sq = 0.f;
   if (row < (int64_t)A.T * A.Hq) {
     const int64_t t = row / A.Hq, h = row % A.Hq;
     const bool in = A.lse[h * A.T + t] != INFINITY;
@@ -486,22 +501,118 @@ template <typename T> __global__ void __launch_bounds__(256) attn_delta_kernel(c
         for (int j = 0; j < 8; ++j) {
           const float x = to_f(g.v[j]);
           s = fmaf(x, to_f(y.v[j]) + to_f(r.v[j]), s);
-          const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-          if (b < 0x7f800000u) big = max(big, b);
+          if (fabsf(x) < INFINITY) sq = fmaf(x, x, sq);
         }
       }
   }
 #pragma unroll
-  for (int x = 4; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x, 8);
-  if (sub == 0 && row < (int64_t)A.T * A.Hq) A.delta[row % A.Hq * A.T + row / A.Hq] = s;
-  if (amax != nullptr) {
-    big = __reduce_max_sync(0xffffffffu, big);
-    if ((threadIdx.x & 31) == 0 && big != 0) atomicMax(amax, big);
+  for (int x = 4; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x, 8), sq += __shfl_xor_sync(0xffffffffu, sq, x, 8);
+  if (sub == 0 && row < (int64_t)A.T * A.Hq) {
+    const int64_t at = row % A.Hq * A.T + row / A.Hq;
+    A.delta[at] = s;
+    if (norm != nullptr) norm[at] = sqrtf(sq);
   }
 }
 
-size_t attn_bwd_ws_bytes(int64_t T, int64_t Hq, int64_t Dh, int64_t sinks) {
-  return 16 + (size_t)((T * Hq + 3) / 4 * 16) + part_bytes<7>(T, Hq, Dh, sinks);
+// ---- fp16: dS's scales ------------------------------------------------------------
+// A row's bound is a maximum over the window of tokens around it, so norms are kept per token and, for whole runs of
+// kRun tokens, as the run's maximum.
+constexpr int kRun = 64;
+struct ScaleArgs {
+  float* fq;            // [Hq, T]: |gy|, then the queries' scales
+  float *g, *d, *v;     // [Hkv, T]: |gy| and |delta|, the largest of the key head's query heads, and |v|
+  float *rg, *rd, *rv;  // [Hkv, runs]: their maxima
+  float* fk;            // [Hkv, T]: the keys' scales
+};
+
+// g, d, v and the runs' maxima: a CTA per run and key head, 4 lanes per token. Values that are not finite are left out
+// (what they reach is not finite whatever the scale), tokens of no sequence count as zero.
+template <typename T>
+__global__ void __launch_bounds__(4 * kRun) attn_norm_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ ScaleArgs W) {
+  __shared__ uint32_t top[3][4 * kRun / 32];
+  const int hk = blockIdx.y, G = A.Hq / A.Hkv, t = blockIdx.x * kRun + (threadIdx.x >> 2), sub = threadIdx.x & 3;
+  float sq = 0.f, g = 0.f, d = 0.f;
+  if (t < A.T && A.lse[(int64_t)hk * G * A.T + t] != INFINITY) {
+    const T* v = (const T*)A.v + t * A.v_ts + hk * A.v_hs;
+    for (int e = sub * 8; e < A.Dh; e += 32) {
+      const Vec<T, 8> x = ld_vec<T, 8>(v + e);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (fabsf(to_f(x.v[j])) < INFINITY) sq = fmaf(to_f(x.v[j]), to_f(x.v[j]), sq);
+    }
+    for (int h = hk * G + sub; h < (hk + 1) * G; h += 4) {
+      const float dl = fabsf(A.delta[(int64_t)h * A.T + t]);
+      g = fmaxf(g, W.fq[(int64_t)h * A.T + t]);
+      if (dl < INFINITY) d = fmaxf(d, dl);
+    }
+  }
+#pragma unroll
+  for (int x = 1; x < 4; x *= 2) {
+    sq += __shfl_xor_sync(0xffffffffu, sq, x);
+    g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, x));
+    d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, x));
+  }
+  const float n = sqrtf(sq);
+  if (sub == 0 && t < A.T) {
+    const int64_t at = (int64_t)hk * A.T + t;
+    W.g[at] = g, W.d[at] = d, W.v[at] = n;
+  }
+  // (the bits of floats that are not negative have the floats' order)
+  const uint32_t m[3] = {__reduce_max_sync(0xffffffffu, __float_as_uint(g)), __reduce_max_sync(0xffffffffu, __float_as_uint(d)),
+                         __reduce_max_sync(0xffffffffu, __float_as_uint(n))};
+  if ((threadIdx.x & 31) == 0)
+#pragma unroll
+    for (int i = 0; i < 3; ++i) top[i][threadIdx.x >> 5] = m[i];
+  __syncthreads();
+  if (threadIdx.x < 3) {
+    uint32_t x = 0;
+    for (int i = 0; i < 4 * kRun / 32; ++i) x = max(x, top[threadIdx.x][i]);
+    float* r = threadIdx.x == 0 ? W.rg : threadIdx.x == 1 ? W.rd : W.rv;
+    r[(int64_t)hk * gridDim.x + blockIdx.x] = __uint_as_float(x);
+  }
+}
+
+// the largest of x[a .. b-1], whole runs by their maxima
+__device__ __forceinline__ float range_max(const float* x, const float* runs, int a, int b) {
+  float m = 0.f;
+  const int a1 = min((a + kRun - 1) / kRun * kRun, b), b0 = max(b / kRun * kRun, a1);
+  for (int i = a; i < a1; ++i) m = fmaxf(m, x[i]);
+  for (int i = a1 / kRun; i < b0 / kRun; ++i) m = fmaxf(m, runs[i]);
+  for (int i = b0; i < b; ++i) m = fmaxf(m, x[i]);
+  return m;
+}
+// a power of two that takes the bound to 2^14 .. 2^15, below fp16's largest number (1 for zero)
+__device__ __forceinline__ float ds_scale(float bound) {
+  if (bound == 0.f) return 1.f;
+  const int e = max((int)(__float_as_uint(bound) >> 23) - 127, -86);
+  return __int_as_float((127 + 14 - e) << 23);
+}
+// Grid: tokens, key heads. T=16384, 32 heads of 64, window 1024: 34 us, and 24 for the norms, of a backward of 953 us
+// (bf16, which needs neither: 820); 16 heads of 128 on 4, window 2048: 838 us (775).
+__global__ void __launch_bounds__(128) attn_scale_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ ScaleArgs W, int runs) {
+  const int t = blockIdx.x * 128 + threadIdx.x, hk = blockIdx.y, G = A.Hq / A.Hkv;
+  if (t >= A.T) return;
+  const int64_t at = (int64_t)hk * A.T, rat = (int64_t)hk * runs;
+  const RowMask m = row_mask(A, t);
+  float v = 0.f;
+  if (m.i >= 0) {
+    v = range_max(W.v + at, W.rv + rat, m.lo, t + 1);
+    if (m.start < min(m.sink_end, m.lo)) v = fmaxf(v, range_max(W.v + at, W.rv + rat, m.start, min(m.sink_end, m.lo)));
+  }
+  for (int h = hk * G; h < (hk + 1) * G; ++h) {  // |delta| <= |gy| max |v|
+    float* f = W.fq + (int64_t)h * A.T + t;
+    *f = ds_scale(2.f * *f * v);
+  }
+  const int end = key_limit(A, t);
+  float g = 0.f, d = 0.f;
+  if (end > 0) g = range_max(W.g + at, W.rg + rat, t, end), d = range_max(W.d + at, W.rd + rat, t, end);
+  W.fk[at + t] = ds_scale(fmaf(g, W.v[at + t], d));
+}
+
+static int64_t delta_floats(int64_t T, int64_t Hq) { return (T * Hq + 3) / 4 * 4; }
+size_t attn_bwd_ws_bytes(bool half, int64_t T, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t sinks) {
+  const int64_t scales = half ? T * Hq + 4 * T * Hkv + 3 * Hkv * ((T + kRun - 1) / kRun) : 0;
+  return (size_t)((delta_floats(T, Hq) + scales) * 4) + part_bytes<7>(T, Hq, Dh, sinks);
 }
 
 template <typename T, int NB, bool KV>
@@ -527,21 +638,31 @@ template <typename T, int NB> static int bwd_nb(const BwdArgs& P, cudaStream_t s
   return bwd_one<T, NB, true>(P, st);
 }
 
-// ws: attn_bwd_ws_bytes, 16-byte aligned
+// ws: attn_bwd_ws_bytes, 16-byte aligned: delta, the sinks' partials, the scales
 template <typename T> int attn_bwd_launch(const AttnArgs& A0, void* ws, cudaStream_t st) {
-  BwdArgs P{A0, nullptr};
-  uint32_t* amax = (uint32_t*)ws;
-  P.a.delta = (float*)((char*)ws + 16);
-  if (has_far(A0)) P.a.part = P.a.delta + ((int64_t)A0.T * A0.Hq + 3) / 4 * 4;
+  BwdArgs P{A0, nullptr, nullptr};
+  AttnArgs& A = P.a;
+  A.delta = (float*)ws;
+  float* rest = A.delta + delta_floats(A.T, A.Hq);
+  if (has_far(A)) A.part = rest;
+  rest += part_bytes<7>(A.T, A.Hq, A.Dh, A.sinks) / 4;
   const bool half = Fmt<T>::id == 0;
-  if (half) {
-    P.amax = amax;
-    const cudaError_t e = cudaMemsetAsync(amax, 0, 4, st);
-    if (e != cudaSuccess) return set_error(MR_E_LAUNCH, "cudaMemsetAsync: %s", cudaGetErrorString(e));
-  }
-  attn_delta_kernel<T><<<(unsigned)(((int64_t)A0.T * A0.Hq + 31) / 32), 256, 0, st>>>(P.a, half ? amax : nullptr);
+  attn_delta_kernel<T><<<(unsigned)(((int64_t)A.T * A.Hq + 31) / 32), 256, 0, st>>>(A, half ? rest : nullptr);
   if (int rc = check_launch("attn_delta_kernel")) return rc;
-  return A0.Dh <= 64 ? bwd_nb<T, 1>(P, st) : bwd_nb<T, 2>(P, st);
+  if (half) {
+    const int runs = (A.T + kRun - 1) / kRun;
+    const int64_t n = (int64_t)A.Hkv * A.T, r = (int64_t)A.Hkv * runs;
+    ScaleArgs W;
+    W.fq = rest;
+    W.g = W.fq + (int64_t)A.Hq * A.T, W.d = W.g + n, W.v = W.d + n, W.fk = W.v + n;
+    W.rg = W.fk + n, W.rd = W.rg + r, W.rv = W.rd + r;
+    P.fq = W.fq, P.fk = W.fk;
+    attn_norm_kernel<T><<<dim3(runs, A.Hkv), 4 * kRun, 0, st>>>(A, W);
+    if (int rc = check_launch("attn_norm_kernel")) return rc;
+    attn_scale_kernel<<<dim3((A.T + 127) / 128, A.Hkv), 128, 0, st>>>(A, W, runs);
+    if (int rc = check_launch("attn_scale_kernel")) return rc;
+  }
+  return A.Dh <= 64 ? bwd_nb<T, 1>(P, st) : bwd_nb<T, 2>(P, st);
 }
 template int attn_bwd_launch<__nv_bfloat16>(const AttnArgs&, void*, cudaStream_t);
 template int attn_bwd_launch<__half>(const AttnArgs&, void*, cudaStream_t);

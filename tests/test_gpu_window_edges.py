@@ -87,6 +87,41 @@ def test_finite_inputs_whose_scores_overflow(mr, cuda_dev, dtype):
     assert torch.isnan(y[0]).all() and torch.equal(y[1:], v[1:])
 
 
+# ---- fp16 gradients of very different sizes in one batch ---------------------------------------
+
+
+@pytest.mark.parametrize("Dh", [64, 128])
+@pytest.mark.parametrize("sinks", [0, 4])
+def test_fp16_gradients_of_one_sequence_beside_anothers(mr, cuda_dev, sinks, Dh):
+    """grad_y of one sequence 10^5 times the other's: each keeps the precision of its own size."""
+    lens = [100, 300, 190]
+    q, k, v, gy, cu = _inputs(cuda_dev, lens, 2, 1, Dh, torch.float16, seed=55)
+    gy *= 0.05
+    gy[100:400] = (gy[100:400].double() * 1e5).to(torch.float16)
+    got = _step(mr, q, k, v, gy, cu, 120, sinks)
+    _check(got, Window(q, k, v, cu, 120, sinks, gy))
+
+
+@pytest.mark.parametrize("Dh", [32, 96])
+def test_fp16_gradients_of_one_head_and_token_beside_others(mr, cuda_dev, Dh):
+    q, k, v, gy, cu = _inputs(cuda_dev, [150, 333], 4, 2, Dh, torch.float16, seed=56)
+    gy *= 0.02
+    gy[:, 2:] = (gy[:, 2:].double() * 1e5).to(torch.float16)  # the second key head's
+    gy[300, 0] = (gy[300, 0].double() * 1e6).to(torch.float16)
+    got = _step(mr, q, k, v, gy, cu, 100, 3)
+    _check(got, Window(q, k, v, cu, 100, 3, gy))
+
+
+@pytest.mark.parametrize("vscale", [1e-3, 30.0, 2000.0])
+def test_fp16_gradients_with_values_of_any_size(mr, cuda_dev, vscale):
+    """|dS| itself may pass fp16's range where neither gy, v nor the gradients do."""
+    q, k, v, gy, cu = _inputs(cuda_dev, [260, 40], 2, 1, 64, torch.float16, seed=57)
+    v = (v * vscale).to(torch.float16)
+    q, k = q * 0.05, k * 0.05
+    got = _step(mr, q, k, v, gy, cu, 90, 2)
+    _check(got, Window(q, k, v, cu, 90, 2, gy))
+
+
 # ---- the decode step's own precision -----------------------------------------------------------
 
 
