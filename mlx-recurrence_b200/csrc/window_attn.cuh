@@ -258,10 +258,13 @@ template <typename T> __device__ __noinline__ void exact_fwd_row(const AttnArgs&
     if (j >= w.sink_end && j < w.lo) j = w.lo;
   }
   const int64_t at = ((int64_t)i * A.Hq + h) * A.Dh;
-  row_store((T*)A.y + at, o, 1.f / l, A.Dh, lane);
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) o.v[n] *= inv;
+  row_store((T*)A.y + at, o, 1.f, A.Dh, lane);
   if (A.y_low != nullptr) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n) o.v[n] = o.v[n] / l - to_f(from_f<T>(o.v[n] / l));
+    for (int n = 0; n < 4; ++n) o.v[n] -= to_f(from_f<T>(o.v[n]));
     row_store((T*)A.y_low + at, o, 1.f, A.Dh, lane);
   }
   if (A.lse != nullptr && lane == 0) A.lse[(int64_t)h * A.T + i] = m + log2f(l);

@@ -3,6 +3,8 @@ values that are not finite, rows whose every score is minus infinity, gradients
 of very different sizes in one fp16 batch, mixed types, empty rows, derivatives
 that it does not have."""
 
+import importlib
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd_ad
@@ -120,6 +122,35 @@ def test_fp16_gradients_with_values_of_any_size(mr, cuda_dev, vscale):
     q, k = q * 0.05, k * 0.05
     got = _step(mr, q, k, v, gy, cu, 90, 2)
     _check(got, Window(q, k, v, cu, 90, 2, gy))
+
+
+# ---- what the backward gets beside y -----------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("Dh", [64, 128])
+def test_y_low_is_what_rounding_dropped(mr, cuda_dev, Dh, dtype):
+    """Through the C entry point: y + y_low is y before it was rounded, in ragged tiles, in padding and in rows that
+    are computed again because of a value that they do not see. With q = 0 every probability is one over the count of
+    the row's keys, which the kernels hold without rounding (1, and the sum that divides): y's rounding is all there is."""
+    lib = importlib.import_module("mlx-recurrence_b200._lib")
+    lens, pad, H, window, sinks = [140, 0, 203], 27, 2, 60, 2
+    q, k, v, _, cu = _inputs(cuda_dev, lens, H, 1, Dh, DT[dtype], pad=pad, seed=59)
+    q.zero_()
+    W = Window(q, k, v, cu, window, sinks, r=0.0)
+    at, T = 200, sum(lens) + pad
+    v = v.clone()
+    v[at] = float("nan")
+    clean = ~O.visible(T, cu, window, sinks, cuda_dev)[:, at]
+    y, low = torch.empty_like(q), torch.empty_like(q)
+    lse, cu32 = torch.empty(H, T, device=cuda_dev), cu.int()
+    lib.call_on(cuda_dev, "mr_window_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), H * Dh, Dh, Dh, Dh, Dh, Dh,
+                cu32.data_ptr(), len(lens), 0, lib.DTYPE_CODE[DT[dtype]], T, H, 1, Dh, window, sinks, Dh ** -0.5,
+                y.data_ptr(), low.data_ptr(), lse.data_ptr())
+    O.check("y", y[clean], W.y[clean], W.tol_y[clean])
+    O.check("y + y_low", (y.double() + low.double())[clean], W.y[clean], W.tol_sum[clean])
+    assert ((y.double() - W.y).abs() > W.tol_sum)[clean].double().mean() > 0.5  # (y alone is not within that bound)
+    assert (y[sum(lens):] == 0).all() and (low[sum(lens):] == 0).all()
 
 
 # ---- the decode step's own precision -----------------------------------------------------------
