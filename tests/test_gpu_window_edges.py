@@ -124,6 +124,16 @@ def test_fp16_gradients_with_values_of_any_size(mr, cuda_dev, vscale):
     _check(got, Window(q, k, v, cu, 90, 2, gy))
 
 
+# ---- layouts ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "f32"])
+@pytest.mark.parametrize("Dh,sinks", [(32, 64), (96, 5), (96, 64), (128, 0), (128, 4), (128, 64)])
+def test_head_sizes_and_sinks(mr, cuda_dev, Dh, sinks, dtype):
+    q, k, v, gy, cu = _inputs(cuda_dev, [333, 1, 210], 4, 2, Dh, DT[dtype], seed=58)
+    _check(_step(mr, q, k, v, gy, cu, 100, sinks), Window(q, k, v, cu, 100, sinks, gy))
+
+
 # ---- what the backward gets beside y -----------------------------------------------------------
 
 
