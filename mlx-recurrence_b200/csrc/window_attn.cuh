@@ -199,14 +199,25 @@ template <int SH> int attn_sink_sum_launch(const AttnArgs& A, cudaStream_t st) {
 // that a row must not see (another sequence's, a later token's) turns into a
 // NaN. A row whose results are not finite, or whose scores are all -infinity, is
 // therefore computed again here, one warp per row, from its visible keys (queries)
-// alone: whatever non-finite value then remains is the row's own. Slow (a shuffle reduction per pair), and only
-// ever reached by inputs that hold infinities or NaN.
+// alone: whatever non-finite value then remains is the row's own. Only ever reached by
+// inputs that hold infinities or NaN, which pay for it (fp16 loss scaling's probes
+// among them). T=16384, fp16, 32 heads of 64, window 1024: one infinity in grad_y 5.5
+// ms of backward in place of 1.0 (18 with a shuffle reduction per term), one token of v
+// that is NaN 4.2 ms of forward in place of 0.27 (16), everything infinite or NaN 149
+// and 46 ms (543, 200); bf16, 16 heads of 128 on 4, window 2048, 4 sinks: 40 and 10 ms
+// (92, 32), everything 230 and 62 (656, 205).
 
 constexpr float kAttnLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float attn_warp_sum(float v) {
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
+  return v;
+}
+
+__device__ __forceinline__ float attn_warp_max(float v) {
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
   return v;
 }
 
@@ -224,47 +235,67 @@ template <typename T> __device__ __forceinline__ void row_store(T* p, const RowV
   for (int n = 0; n < 4; ++n)
     if (32 * n < Dh) p[lane + 32 * n] = from_f<T>(r.v[n] * f);
 }
-__device__ __forceinline__ float row_dot(const RowVec& a, const RowVec& b, int Dh) {
-  float s = 0.f;
-#pragma unroll
-  for (int n = 0; n < 4; ++n)
-    if (32 * n < Dh) s = fmaf(a.v[n], b.v[n], s);
-  return attn_warp_sum(s);
-}
 __device__ __forceinline__ void row_axpy(RowVec& a, float f, const RowVec& b) {
 #pragma unroll
   for (int n = 0; n < 4; ++n) a.v[n] = fmaf(f, b.v[n], a.v[n]);
 }
+// A lane's own product of two rows (16-byte aligned).
+template <typename T> __device__ __forceinline__ float lane_dot(const T* a, const T* b, int Dh) {
+  constexpr int N = 16 / sizeof(T);
+  float s = 0.f;
+#pragma unroll 4
+  for (int d = 0; d < Dh; d += N) {
+    const Vec<T, N> x = ld_vec<T, N>(a + d), y = ld_vec<T, N>(b + d);
+#pragma unroll
+    for (int j = 0; j < N; ++j) s = fmaf(to_f(x.v[j]), to_f(y.v[j]), s);
+  }
+  return s;
+}
+// a += sum over the warp's first `n` lanes of f x row(j), the rows' loads eight ahead
+template <typename T>
+__device__ __forceinline__ void rows_axpy(RowVec& a, float f, int j, int n, const T* p, int64_t ts, int Dh, int lane) {
+  for (int x = 0; x < n; x += 8) {
+    RowVec r[8];
+#pragma unroll
+    for (int y = 0; y < 8; ++y) r[y] = row_load(p + __shfl_sync(0xffffffffu, j, min(x + y, n - 1)) * ts, Dh, lane);
+#pragma unroll
+    for (int y = 0; y < 8; ++y) {
+      const float fy = __shfl_sync(0xffffffffu, f, min(x + y, n - 1));
+      if (x + y < n) row_axpy(a, fy, r[y]);
+    }
+  }
+}
 
+// A row's visible terms, 32 at a time: each lane the scores of one, then all lanes the sums over them, term by term.
 template <typename T> __device__ __noinline__ void exact_fwd_row(const AttnArgs& A, int h, int i) {
   const int lane = threadIdx.x & 31, hk = h / (A.Hq / A.Hkv);
   const RowMask w = row_mask(A, i);
   if (w.i < 0) return;
   const T* k = (const T*)A.k + hk * A.k_hs;
   const T* v = (const T*)A.v + hk * A.v_hs;
-  const RowVec q = row_load((const T*)A.q + i * A.q_ts + h * A.q_hs, A.Dh, lane);
+  const T* q = (const T*)A.q + i * A.q_ts + h * A.q_hs;
   RowVec o = {};
   float m = -INFINITY, l = 0.f;
-  int j = w.start < min(w.sink_end, w.lo) ? w.start : w.lo;
-  while (j <= i) {
-    const float s = row_dot(q, row_load(k + j * A.k_ts, A.Dh, lane), A.Dh) * (A.scale * kAttnLog2e);
-    const float mx = fmaxf(m, s), base = mx == -INFINITY ? 0.f : mx, keep = exp2f(m - base), e = exp2f(s - base);
+  const int sinks = max(0, min(w.sink_end, w.lo) - w.start), n = sinks + i - w.lo + 1;
+  for (int b = 0; b < n; b += 32) {
+    const int x = min(b + lane, n - 1), j = x < sinks ? w.start + x : w.lo + x - sinks;
+    const float d = lane_dot(q, k + j * A.k_ts, A.Dh) * (A.scale * kAttnLog2e), s = b + lane < n ? d : -INFINITY;
+    const float mx = fmaxf(m, attn_warp_max(s)), base = mx == -INFINITY ? 0.f : mx, keep = exp2f(m - base);
+    const float e = b + lane < n ? exp2f(s - base) : 0.f;
     m = mx;
-    l = l * keep + e;
+    l = l * keep + attn_warp_sum(e);
 #pragma unroll
-    for (int n = 0; n < 4; ++n) o.v[n] *= keep;
-    row_axpy(o, e, row_load(v + j * A.v_ts, A.Dh, lane));
-    ++j;
-    if (j >= w.sink_end && j < w.lo) j = w.lo;
+    for (int c = 0; c < 4; ++c) o.v[c] *= keep;
+    rows_axpy(o, e, j, min(32, n - b), v, A.v_ts, A.Dh, lane);
   }
   const int64_t at = ((int64_t)i * A.Hq + h) * A.Dh;
   const float inv = 1.f / l;
 #pragma unroll
-  for (int n = 0; n < 4; ++n) o.v[n] *= inv;
+  for (int c = 0; c < 4; ++c) o.v[c] *= inv;
   row_store((T*)A.y + at, o, 1.f, A.Dh, lane);
   if (A.y_low != nullptr) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n) o.v[n] -= to_f(from_f<T>(o.v[n]));
+    for (int c = 0; c < 4; ++c) o.v[c] -= to_f(from_f<T>(o.v[c]));
     row_store((T*)A.y_low + at, o, 1.f, A.Dh, lane);
   }
   if (A.lse != nullptr && lane == 0) A.lse[(int64_t)h * A.T + i] = m + log2f(l);
@@ -277,17 +308,15 @@ template <typename T> __device__ __noinline__ void exact_gq_row(const AttnArgs& 
   const T* k = (const T*)A.k + hk * A.k_hs;
   const T* v = (const T*)A.v + hk * A.v_hs;
   const int64_t at = ((int64_t)i * A.Hq + h) * A.Dh;
-  const RowVec q = row_load((const T*)A.q + i * A.q_ts + h * A.q_hs, A.Dh, lane);
-  const RowVec g = row_load((const T*)A.gy + at, A.Dh, lane);
+  const T *q = (const T*)A.q + i * A.q_ts + h * A.q_hs, *g = (const T*)A.gy + at;
   const float lse = A.lse[(int64_t)h * A.T + i], delta = A.delta[(int64_t)h * A.T + i];
   RowVec o = {};
-  int j = w.start < min(w.sink_end, w.lo) ? w.start : w.lo;
-  while (j <= i) {
-    const RowVec kj = row_load(k + j * A.k_ts, A.Dh, lane);
-    const float p = exp2f(row_dot(q, kj, A.Dh) * (A.scale * kAttnLog2e) - lse);
-    row_axpy(o, p * (row_dot(g, row_load(v + j * A.v_ts, A.Dh, lane), A.Dh) - delta), kj);
-    ++j;
-    if (j >= w.sink_end && j < w.lo) j = w.lo;
+  const int sinks = max(0, min(w.sink_end, w.lo) - w.start), n = sinks + i - w.lo + 1;
+  for (int b = 0; b < n; b += 32) {
+    const int x = min(b + lane, n - 1), j = x < sinks ? w.start + x : w.lo + x - sinks;
+    const float p = exp2f(lane_dot(q, k + j * A.k_ts, A.Dh) * (A.scale * kAttnLog2e) - lse);
+    const float f = p * (lane_dot(g, v + j * A.v_ts, A.Dh) - delta);
+    rows_axpy(o, f, j, min(32, n - b), k, A.k_ts, A.Dh, lane);
   }
   row_store((T*)A.gq + at, o, A.scale, A.Dh, lane);
 }
@@ -295,17 +324,21 @@ template <typename T> __device__ __noinline__ void exact_gq_row(const AttnArgs& 
 template <typename T> __device__ __noinline__ void exact_gkv_row(const AttnArgs& A, int hk, int j) {
   const int lane = threadIdx.x & 31, G = A.Hq / A.Hkv, end = key_limit(A, j);
   if (end == 0) return;
-  const RowVec k = row_load((const T*)A.k + j * A.k_ts + hk * A.k_hs, A.Dh, lane);
-  const RowVec v = row_load((const T*)A.v + j * A.v_ts + hk * A.v_hs, A.Dh, lane);
+  const T* k = (const T*)A.k + j * A.k_ts + hk * A.k_hs;
+  const T* v = (const T*)A.v + j * A.v_ts + hk * A.v_hs;
+  const int64_t gts = (int64_t)A.Hq * A.Dh;
   RowVec gk = {}, gv = {};
-  for (int h = hk * G; h < (hk + 1) * G; ++h)
-    for (int i = j; i < end; ++i) {
-      const RowVec q = row_load((const T*)A.q + i * A.q_ts + h * A.q_hs, A.Dh, lane);
-      const RowVec g = row_load((const T*)A.gy + ((int64_t)i * A.Hq + h) * A.Dh, A.Dh, lane);
-      const float p = exp2f(row_dot(q, k, A.Dh) * (A.scale * kAttnLog2e) - A.lse[(int64_t)h * A.T + i]);
-      row_axpy(gv, p, g);
-      row_axpy(gk, p * (row_dot(g, v, A.Dh) - A.delta[(int64_t)h * A.T + i]), q);
+  for (int h = hk * G; h < (hk + 1) * G; ++h) {
+    const T *q = (const T*)A.q + h * A.q_hs, *g = (const T*)A.gy + (int64_t)h * A.Dh;
+    const float *lse = A.lse + (int64_t)h * A.T, *delta = A.delta + (int64_t)h * A.T;
+    for (int b = j; b < end; b += 32) {
+      const int i = min(b + lane, end - 1), n = min(32, end - b);
+      const float p = exp2f(lane_dot(k, q + i * A.q_ts, A.Dh) * (A.scale * kAttnLog2e) - lse[i]);
+      const float f = p * (lane_dot(v, g + i * gts, A.Dh) - delta[i]);
+      rows_axpy(gv, p, i, n, g, gts, A.Dh, lane);
+      rows_axpy(gk, f, i, n, q, A.q_ts, A.Dh, lane);
     }
+  }
   const int64_t at = ((int64_t)j * A.Hkv + hk) * A.Dh;
   row_store((T*)A.gk + at, gk, A.scale, A.Dh, lane);
   row_store((T*)A.gv + at, gv, 1.f, A.Dh, lane);
