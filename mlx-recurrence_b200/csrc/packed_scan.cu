@@ -118,11 +118,17 @@ __device__ __forceinline__ ChunkInfo chunk_info(const int* __restrict__ cu, int 
   }
   ChunkInfo c = {};
   c.first = l;
-  for (int s = l; s <= S; ++s) {
+  for (int s = l, next; s <= S; s = next) {  // from the first border of a run of equal ones to the next run's
     const int64_t at = cu[s] - t0;
     if (at > n) break;
-    if (at >= 0 && at < n && s < S && cu[s + 1] > cu[s]) c.starts |= 1u << (at / kSteps);
-    if (at >= 1 && s > 0 && cu[s] > cu[s - 1]) c.ends |= 1u << ((at - 1) / kSteps);
+    next = s + 1;
+    if (next <= S && cu[next] <= cu[s])  // empty sequences, however many
+      for (int r = S + 1; next < r;) {
+        const int m = next + ((r - next) >> 1);
+        if (cu[m] <= cu[s]) next = m + 1; else r = m;
+      }
+    if (at >= 0 && at < n && next <= S) c.starts |= 1u << (at / kSteps);
+    if (at >= 1 && s > 0) c.ends |= 1u << ((at - 1) / kSteps);
   }
   c.lo = (int)min(max((int64_t)cu[0] - t0, (int64_t)0), (int64_t)n);
   c.hi = (int)min(max((int64_t)cu[S] - t0, (int64_t)0), (int64_t)n);

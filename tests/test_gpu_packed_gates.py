@@ -134,3 +134,27 @@ def test_states_that_overflow_are_infinite(mr, cuda_dev):
     want[300:] = 2.0 ** torch.arange(700, dtype=torch.float64).clamp(max=1000)
     want = want.float().to(cuda_dev)
     assert torch.equal(y, want[:, None].expand(T, D))
+
+
+# ---- many borders at one place -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("many", [1000, 70000])
+def test_many_empty_sequences(mr, cuda_dev, many):
+    """Borders padded to a fixed count (a captured graph's): whole runs of empty sequences in front, at a chunk's
+    border, inside a chunk and behind the last token change nothing, and each hands on its own state."""
+    g = torch.Generator().manual_seed(45)
+    T, D, at = 700, 48, [0, 128, 300, 700]
+    a, x, gy = torch.rand(T, D, generator=g), torch.randn(T, D, generator=g), torch.randn(T, D, generator=g)
+    a, x, gy = a.to(cuda_dev), x.to(cuda_dev), gy.to(cuda_dev)
+    cu = torch.tensor([b for b in at for _ in range(many)], device=cuda_dev)
+    S = cu.numel() - 1
+    h0, gf = torch.randn(S, D, generator=g).to(cuda_dev), torch.randn(S, D, generator=g).to(cuda_dev)
+    real = torch.tensor([many - 1, 2 * many - 1, 3 * many - 1], device=cuda_dev)  # the sequences that hold tokens
+    got = _grads(mr, a, x, cu, h0, gy, gf)
+    want = _grads(mr, a, x, torch.tensor(at, device=cuda_dev), h0[real], gy, gf[real])
+    for i in (0, 2, 3):
+        assert torch.equal(got[i], want[i])
+    for i, own in ((1, h0), (4, gf)):
+        own[real] = want[i]
+        assert torch.equal(got[i], own)
