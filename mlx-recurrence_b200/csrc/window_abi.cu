@@ -25,8 +25,8 @@ static int attn_check(const char* what, const AttnArgs& A, int64_t S, int64_t L,
   if (window <= 0 || sinks < 0 || sinks > 64)
     return set_error(MR_E_SHAPE, "%s: window=%lld must be positive and sinks=%lld in 0..64", what, (long long)window,
                      (long long)sinks);
-  if (!(A.scale > 0.f) || A.scale > 3e38f)
-    return set_error(MR_E_SHAPE, "%s: scale must be positive and finite", what);
+  if (!(A.scale > 0.f) || A.scale > 2e38f)
+    return set_error(MR_E_SHAPE, "%s: scale must be positive and at most 2e38", what);
   if (A.cu == nullptr && T > 0 && (L <= 0 || L > T || S * L != T))
     return set_error(MR_E_SHAPE, "%s: without cu_seqlens T must be S * L", what);
   const int64_t n = dtype == MR_F32 ? 4 : 8;

@@ -440,7 +440,7 @@ int mr_window_step(const void* q, const void* k, const void* v, void* cache_k, v
   if (sinks < 0 || slots <= sinks || slots > (1 << 30))
     return set_error(MR_E_SHAPE, "%s: slots=%lld must exceed sinks=%lld >= 0", what, (long long)slots,
                      (long long)sinks);
-  if (!(scale > 0.f) || scale > 3e38f) return set_error(MR_E_SHAPE, "%s: scale must be positive and finite", what);
+  if (!(scale > 0.f) || scale > 2e38f) return set_error(MR_E_SHAPE, "%s: scale must be positive and at most 2e38", what);
   if (batch == 0) return MR_OK;
   for (const void* p : {q, k, v, (const void*)cache_k, (const void*)cache_v, (const void*)y})
     if (p == nullptr || ((uintptr_t)p & 15u))

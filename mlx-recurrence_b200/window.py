@@ -43,8 +43,8 @@ def _check(q, k, v, window, sinks, scale, dims, layout):
     if not 0 <= sinks <= MAX_SINKS:
         raise ValueError(f"sinks must be in 0..{MAX_SINKS}, got {sinks}")
     scale = Dh ** -0.5 if scale is None else float(scale)
-    if not (0.0 < scale < 3e38):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not (0.0 < scale <= 2e38):  # times log2(e) it must stay finite
+        raise ValueError(f"scale must be positive and at most 2e38, got {scale}")
     return window, sinks, scale
 
 
