@@ -646,10 +646,10 @@ template <typename T> int attn_bwd_launch(const AttnArgs& A0, void* ws, cudaStre
   float* rest = A.delta + delta_floats(A.T, A.Hq);
   if (has_far(A)) A.part = rest;
   rest += part_bytes<7>(A.T, A.Hq, A.Dh, A.sinks) / 4;
-  const bool half = Fmt<T>::id == 0;
+  constexpr bool half = Fmt<T>::id == 0;
   attn_delta_kernel<T><<<(unsigned)(((int64_t)A.T * A.Hq + 31) / 32), 256, 0, st>>>(A, half ? rest : nullptr);
   if (int rc = check_launch("attn_delta_kernel")) return rc;
-  if (half) {
+  if constexpr (half) {
     const int runs = (A.T + kRun - 1) / kRun;
     const int64_t n = (int64_t)A.Hkv * A.T, r = (int64_t)A.Hkv * runs;
     ScaleArgs W;
