@@ -366,7 +366,7 @@ MR_API int mr_rotlru_step(const void* a, const void* cs, const void* sn, const v
  * zeros, in outputs and gradients. T may be 0.
  *
  * RG-LRU recurrence h_t = a_t h_{t-1} + x_t per sequence: a, x [T,D] in `dtype`
- * (any T, D >= 1; element-aligned pointers), y [T,D] f32, h0 [S,D] f32 or NULL
+ * (any T, D >= 1, gates of any value; element-aligned pointers), y [T,D] f32, h0 [S,D] f32 or NULL
  * (zero), final_state [S,D] f32 or NULL (h0 for an empty sequence). ckpt
  * [ceil(T / mr_rglru_packed_chunk()), D] f32 receives what the backward needs
  * (NULL when none follows). grad_final [S,D] and grad_h0 [S,D] may be NULL. */
@@ -389,7 +389,7 @@ MR_API int mr_rglru_packed_bwd(const float* grad_y, const float* grad_final, con
  * cu_seqlens NULL: S sequences of L tokens (T = S L). y and the gradients are
  * dense and in `dtype`; lse [Hq,T] f32 and (not for f32) y_low, like y, hold
  * what the backward needs: the rows' sums and what rounding y dropped. Both NULL
- * when no backward follows. */
+ * when no backward follows. 0 < scale <= 2e38. */
 MR_API int mr_window_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ts, int64_t q_hs, int64_t k_ts,
                               int64_t k_hs, int64_t v_ts, int64_t v_hs, const int32_t* cu_seqlens, int64_t S,
                               int64_t L, int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t window,
