@@ -262,7 +262,8 @@ def rglru_scan_packed(a, x, cu_seqlens, h0=None):
     one or anything else, and D may be any size.
 
     Args:
-        a:   [T, D] per-channel recurrent gate (any real value).
+        a:   [T, D] per-channel recurrent gate (any real value; channels where
+             products of gates, states or inputs are not finite take longer).
         x:   [T, D] the already-gated input.
         cu_seqlens: [S + 1] int32 or int64 borders on the same device,
              nondecreasing, starting at 0: sequence s holds the rows

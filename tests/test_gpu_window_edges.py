@@ -73,7 +73,6 @@ def test_scores_of_minus_infinity_alone_give_nan(mr, cuda_dev, dtype):
     k[50] = -float("inf")
     y = mr.window_attention_packed(q, k, v, cu, 3)
     assert torch.isnan(y[50]).all() and torch.isfinite(y[:50]).all() and torch.isfinite(y[51:]).all()
-    assert torch.equal(y, mr.window_attention_packed(q, k, v, cu, 3, sinks=1)) is False  # (NaN is not equal to itself)
     # the decode step says the same
     pos = torch.zeros(1, dtype=torch.long, device=cuda_dev)
     ck, cv = (torch.zeros(1, 4, 1, 64, dtype=DT[dtype], device=cuda_dev) for _ in range(2))
