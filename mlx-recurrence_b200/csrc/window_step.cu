@@ -123,10 +123,12 @@ __global__ void __launch_bounds__(32 * kF32Warps) window_step_f32(const __grid_c
 // with its own online softmax. Warps, then CTAs (over distributed shared memory)
 // join their maxima, sums and outputs in a fixed order; one launch, no workspace.
 // P goes into its product in two parts, rounded to the inputs' type and what that
-// drops, so its rounding is squared (y's error was 1.2 times that of rounding y alone).
-// B=96, 16 heads of 128 on 4, 2052 slots: 67 us, 6.0 TB/s of the caches' bytes (66 with
-// the first part alone); B=1, 8 heads of 64 on 2, 516 slots: 6.3 us (6.1), a launch and a
-// few dependent loads.
+// drops, so its rounding is squared (y's error was 1.2 times that of rounding y alone):
+// as rows of their own where the group leaves half of the sixteen, or in a second product.
+// B=96, 16 heads of 128 on 4, 2052 slots: 66 us, 6.1 TB/s of the caches' bytes (67 by
+// second products, 66 without the second part); B=33, 10 heads of 64 on 1, 1024 slots: 7.5
+// us (7.1 without); B=1, 8 heads of 64 on 2, 516 slots: 6.3 us, a launch and a few
+// dependent loads.
 
 constexpr int kTile = 64, kRing = 2;
 
@@ -185,6 +187,7 @@ __global__ void __launch_bounds__(128) window_step_mma(const __grid_constant__ S
   const int rank = blockIdx.x % splits, unit = blockIdx.x / splits;
   const int b = blockIdx.y, hk = unit / head_tiles, h0 = unit % head_tiles * 16, G = A.Hq / A.Hkv;
   const int rows = min(16, G - h0);
+  const bool paired = rows <= 8;  // P's second part takes the place of rows 8 .. 15
   const int64_t qat = ((int64_t)b * A.Hq + hk * G + h0) * DH;
   T* y = (T*)A.y + qat;
   const int64_t p = step_pos(A, b);
@@ -250,8 +253,13 @@ __global__ void __launch_bounds__(128) window_step_mma(const __grid_constant__ S
       Mma<T>::run(s[1], q[k], f[2], f[3]);
     }
     uint32_t pa[4], pb[4];  // P in the inputs' type, and what that rounding drops
+    float keep[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {  // rows lane / 4 and + 8
+      if (r == 1 && paired) {
+        pa[1] = pb[0], pa[3] = pb[2], keep[1] = keep[0];
+        break;
+      }
       float mx = m[r];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -262,9 +270,10 @@ __global__ void __launch_bounds__(128) window_step_mma(const __grid_constant__ S
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float to = mx == -INFINITY ? 0.f : mx, keep = exp2f(m[r] - to);
+      const float to = mx == -INFINITY ? 0.f : mx;
+      keep[r] = exp2f(m[r] - to);
       m[r] = mx;
-      l[r] *= keep;
+      l[r] *= keep[r];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float& v = s[i >> 1][r * 2 + (i & 1)];
@@ -278,9 +287,9 @@ __global__ void __launch_bounds__(128) window_step_mma(const __grid_constant__ S
         const float2 back = Mma<T>::unpack(pa[r + 2 * i]);
         pb[r + 2 * i] = Mma<T>::pack(p0 - back.x, p1 - back.y);
       }
-#pragma unroll
-      for (int i = 0; i < NC; ++i) o[i][r * 2] *= keep, o[i][r * 2 + 1] *= keep;
     }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) o[i][0] *= keep[0], o[i][1] *= keep[0], o[i][2] *= keep[1], o[i][3] *= keep[1];
 #pragma unroll
     for (int i = 0; i < NC; i += 4) {
       uint32_t f[2][4];
@@ -289,10 +298,14 @@ __global__ void __launch_bounds__(128) window_step_mma(const __grid_constant__ S
         ldmatrix4<true>(f[x], sv + chunk_at<DH>(s0 + (lane >> 3 & 1) * 8 + (lane & 7), i + 2 * x + (lane >> 4)) * 16);
 #pragma unroll
       for (int x = 0; x < 4; ++x) Mma<T>::run(o[i + x], pa, f[x >> 1][(x & 1) * 2], f[x >> 1][(x & 1) * 2 + 1]);
+      if (!paired)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) Mma<T>::run(o[i + x], pb, f[x >> 1][(x & 1) * 2], f[x >> 1][(x & 1) * 2 + 1]);
+        for (int x = 0; x < 4; ++x) Mma<T>::run(o[i + x], pb, f[x >> 1][(x & 1) * 2], f[x >> 1][(x & 1) * 2 + 1]);
     }
   }
+  if (paired)
+#pragma unroll
+    for (int i = 0; i < NC; ++i) o[i][0] += o[i][2], o[i][1] += o[i][3];
   // join the warps: the ring's memory is free
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
@@ -352,7 +365,7 @@ template <typename T, int DH> static int step_mma_dh(const StepArgs& A, cudaStre
   const int G = A.Hq / A.Hkv, head_tiles = (G + 15) / 16, tiles = (A.slots + kTile - 1) / kTile;
   const int64_t units = (int64_t)A.B * A.Hkv * head_tiles;
   // CTAs for two on every SM (three fit: one wave), each with two tiles at least. At B=96, Hkv=4, Dh=128, 2052 slots:
-  // 66 us unsplit, 76 in two, 85 in four (later waves leave SMs idle); at B=8: 13 us in eight
+  // 66 us unsplit, 76 in two, 85 in four (later waves leave SMs idle); at B=8: 12.5 us in eight
   int splits = 1;
   while (splits < 8 && units * splits < 148 * 2 && splits * 4 <= tiles) splits *= 2;
   auto kernel = window_step_mma<T, DH>;
